@@ -19,7 +19,8 @@ BUILD = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libgfl_moe.so")
 ARCH = os.environ.get("GFL_ARCH", "gfx950")
 
-SOURCES = ["k_moe.hip", "k_split.hip", "k_prefill.hip", "gfl_api.cpp"]
+SOURCES = ["k_moe.hip", "k_split.hip", "k_prefill.hip", "k_dense_bf16.hip", "k_dense_f16.hip", "k_dense_i8.hip",
+           "k_quant.hip", "k_sample.hip", "gfl_api.cpp", "gfl_dense.cpp"]
 
 CFLAGS = ["--offload-arch=" + ARCH, "-O3", "-fPIC", "-std=c++17", "-ffp-contract=off",
           "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",

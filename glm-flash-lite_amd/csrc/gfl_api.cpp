@@ -30,6 +30,15 @@ int hip_fail(hipError_t e, const char* what)
     return fail(GFL_ERUNTIME, std::string(what) + ": " + hipGetErrorString(e));
 }
 
+}  // namespace
+
+namespace gfl {
+int api_fail(int code, const char* msg) { return fail(code, msg); }
+int api_hip_fail(hipError_t e, const char* what) { return hip_fail(e, what); }
+}  // namespace gfl
+
+namespace {
+
 #define GFL_HIP(call)                                       \
     do                                                      \
     {                                                       \

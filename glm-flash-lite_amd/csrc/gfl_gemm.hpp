@@ -1,0 +1,587 @@
+// The tile GEMM of the dense operators (gated feed-forward block and its gradients, 8-bit integer product):
+//   D[m][n] = sum_k A(m, k) * B(n, k), in fp32 (f16, bf16 inputs) or int32 (i8).
+//
+// A workgroup of WM x WN waves forms a TM x TN tile over K steps of 128 bytes a row (64 16-bit elements, 128 bytes of
+// i8). Each operand is stored either with K contiguous ("KC": [rows][K], as activations and nn.Linear weights are) or
+// with K as the rows ("KS": [K][cols], the transposed products of the gradients):
+//   KC tiles lie in LDS as [rows][8 chunks of 16 bytes], chunk c of row r at place c ^ ((r >> 1) & 7); a fragment is one
+//   ds_read_b128 per lane;
+//   KS tiles (16-bit types) lie as [64 k][cols], chunk c of row k at place c ^ ks_swz(k); a fragment is two
+//   ds_read_b64_tr_b16, which hand lane i of each 16 the 4 k values of column i.
+// MFMA operands are (B rows, A rows), so that a lane's 4 accumulators are 4 neighbouring n of one m: vector stores.
+//
+// AL = 1 (every chunk of 16 bytes aligned and whole) loads tiles by LDS-direct buffer loads, NST - 1 steps ahead; rows past
+// the matrix are clamped to its last (their results are not stored), k past the end is read as zero through the
+// buffer's bounds. AL = 0 takes any strides and sizes: chunks go through registers, masked per element.
+#pragma once
+#include "gfl_internal.hpp"
+
+namespace gfl {
+
+typedef __attribute__((address_space(3))) void gm_lds_void;
+typedef int gm_i4 __attribute__((ext_vector_type(4)));
+typedef float gm_f4 __attribute__((ext_vector_type(4)));
+typedef _Float16 gm_h8 __attribute__((ext_vector_type(8)));
+typedef __bf16 gm_b8 __attribute__((ext_vector_type(8)));
+typedef short gm_s4 __attribute__((ext_vector_type(4)));
+
+struct GmF16
+{
+    typedef _Float16 elem;
+    typedef gm_f4 acc;
+    typedef float scalar;
+    static __device__ __forceinline__ acc mfma(gm_i4 a, gm_i4 b, acc c)
+    {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(gm_h8, a), __builtin_bit_cast(gm_h8, b), c, 0, 0,
+                                                      0);
+    }
+};
+struct GmBF16
+{
+    typedef __bf16 elem;
+    typedef gm_f4 acc;
+    typedef float scalar;
+    static __device__ __forceinline__ acc mfma(gm_i4 a, gm_i4 b, acc c)
+    {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(gm_b8, a), __builtin_bit_cast(gm_b8, b), c, 0,
+                                                       0, 0);
+    }
+};
+struct GmI8
+{
+    typedef int8_t elem;
+    typedef gm_i4 acc;
+    typedef int scalar;
+    static __device__ __forceinline__ acc mfma(gm_i4 a, gm_i4 b, acc c)
+    {
+        return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0);
+    }
+};
+
+template <int N>
+__device__ __forceinline__ void gm_wait_vmcnt()
+{
+    static_assert(N <= 63, "vmcnt has 6 bits");
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void gm_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+__device__ __forceinline__ const char* gm_uniform(const char* p)
+{
+    const uint64_t v = reinterpret_cast<uint64_t>(p);
+    const uint32_t lo = __builtin_amdgcn_readfirstlane((int)(uint32_t)v);
+    const uint32_t hi = __builtin_amdgcn_readfirstlane((int)(uint32_t)(v >> 32));
+    return reinterpret_cast<const char*>(((uint64_t)hi << 32) | lo);
+}
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t gm_rsrc(const char* p)
+{
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(p), (short)0, 0x7FFFFFFF, 0x00020000);
+}
+constexpr uint32_t GM_OUT = 0x80000000u;   // a lane offset past every buffer: reads as zero
+
+// the 16 bytes at p of which the first nb (a multiple of ES, at most 16; may be <= 0) exist; the rest is zero
+template <int ES>
+__device__ __forceinline__ gm_i4 gm_masked(const char* p, int nb)
+{
+    gm_i4 r = { 0, 0, 0, 0 };
+    if (nb >= 16)
+    {
+        __builtin_memcpy(&r, p, 16);
+        return r;
+    }
+    uint32_t w[4] = { 0, 0, 0, 0 };
+#pragma unroll
+    for (int i = 0; i < 16 / ES; ++i)
+        if (i * ES < nb)
+        {
+            const uint32_t e = ES == 2 ? (uint32_t)*reinterpret_cast<const uint16_t*>(p + i * ES)
+                                       : (uint32_t)*reinterpret_cast<const uint8_t*>(p + i * ES);
+            w[i * ES / 4] |= e << (i * ES % 4 * 8);
+        }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = (int)w[i];
+    return r;
+}
+
+__device__ __forceinline__ int gm_ks_swz(int k, int chunks) { return (2 * ((k & 3) | ((k >> 1) & 4))) & (chunks - 1); }
+
+// One operand of a tile: R rows (KC) or columns (KS) from r0 on of a matrix with `rows` of them.
+// p points at the tile's first k; advance by step() bytes per K step.
+template <typename T, int R, bool KS, bool DUAL, int NW>
+struct GmSide
+{
+    static constexpr int ES = sizeof(typename T::elem);
+    static constexpr int BK = 128 / ES;                  // elements per K step
+    static constexpr int CH = KS ? R * ES / 16 : 8;      // chunks of 16 bytes per LDS row
+    static constexpr int LROWS = 64 / CH;                // LDS rows per load of a wave
+    static constexpr int NI = R * 128 / 1024;            // wave loads per K step
+    static constexpr int NV = (NI + NW - 1) / NW;        // per wave (waves past NI repeat others' loads)
+    static constexpr int BYTES = R * 128;
+    static_assert(CH <= 64, "an LDS row is at most one wave load");
+
+    int lrow[NV], chunk[NV];                             // this lane's LDS row and source chunk
+    uint32_t voff[NV];                                   // AL: byte offset from the base
+    const char* p0;
+    const char* p1;                                      // DUAL: the second matrix (rows 16..31 of every 32)
+    int64_t ld;
+    int nrow;                                            // rows (KC) or columns (KS) from r0 to the matrix's end
+
+    __device__ __forceinline__ void init(int wave, int lane, const char* a, const char* b, int64_t ld_, int r0, int rows)
+    {
+        ld = ld_;
+        nrow = rows - r0;
+        p0 = gm_uniform(KS ? a + (int64_t)r0 * ES : a + (int64_t)r0 * ld);
+        p1 = DUAL ? gm_uniform(b + (int64_t)r0 * ld) : p0;
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+        {
+            const int ii = (wave + NW * j) % NI;
+            const int r = ii * LROWS + lane / CH;
+            lrow[j] = r;
+            chunk[j] = KS ? (lane % CH) ^ gm_ks_swz(r, CH) : (lane % CH) ^ ((r >> 1) & 7);
+            if constexpr (KS)
+                voff[j] = (uint32_t)(r * (int)ld + min(chunk[j] * 16, ((nrow + 7) / 8 - 1) * 16));
+            else
+                voff[j] = (uint32_t)(min(src_row(r), nrow - 1) * (int)ld + chunk[j] * 16);
+        }
+    }
+    // row of the matrix that LDS row r holds (DUAL: rows 16..31 of every 32 come from the second matrix)
+    static __device__ __forceinline__ int src_row(int r) { return DUAL ? (r >> 5) * 16 + (r & 15) : r; }
+    static __device__ __forceinline__ bool second(int wave, int j) { return DUAL && ((((wave + NW * j) % NI) >> 1) & 1); }
+    __device__ __forceinline__ int64_t step() const { return KS ? (int64_t)BK * ld : 128; }
+    __device__ __forceinline__ void advance(int64_t n)
+    {
+        p0 += n * step();
+        if (DUAL) p1 += n * step();
+    }
+
+    // LDS-direct loads of one K step of which `rem` elements exist
+    __device__ __forceinline__ void issue(char* lds, int wave, int rem) const
+    {
+        const __amdgpu_buffer_rsrc_t r0 = gm_rsrc(p0);
+        const __amdgpu_buffer_rsrc_t r1 = DUAL ? gm_rsrc(p1) : r0;
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+        {
+            const int ii = (wave + NW * j) % NI;
+            uint32_t v = voff[j];
+            if (rem < BK) v = (KS ? lrow[j] : chunk[j] * (16 / ES)) < rem ? v : GM_OUT;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(second(wave, j) ? r1 : r0, (gm_lds_void*)(lds + ii * 1024), 16, v, 0, 0,
+                                                     0);
+        }
+    }
+    // the same chunks through registers
+    __device__ __forceinline__ void fetch(gm_i4 (&b)[NV], int wave, int rem) const
+    {
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+        {
+            const char* base = second(wave, j) ? p1 : p0;
+            if constexpr (KS)
+            {
+                const int c = chunk[j] * (16 / ES);
+                b[j] = gm_masked<ES>(base + lrow[j] * ld + c * ES, lrow[j] < rem ? (nrow - c) * ES : 0);
+            }
+            else
+            {
+                const int c = chunk[j] * (16 / ES);
+                b[j] = gm_masked<ES>(base + (int64_t)min(src_row(lrow[j]), nrow - 1) * ld + c * ES, (rem - c) * ES);
+            }
+        }
+    }
+    __device__ __forceinline__ void commit(const gm_i4 (&b)[NV], char* lds, int wave, int lane) const
+    {
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+            *reinterpret_cast<gm_i4*>(lds + (wave + NW * j) % NI * 1024 + lane * 16) = b[j];
+    }
+
+    // fragment f (rows 16f..16f+15), half kk (0, 1) of the K step
+    static __device__ __forceinline__ gm_i4 frag(const char* lds, int lane, int f, int kk)
+    {
+        const int i = lane & 15, q = lane >> 4;
+        if constexpr (!KS)
+            return *reinterpret_cast<const gm_i4*>(lds + f * 2048 + i * 128 + (((kk * 4 + q) ^ ((i >> 1) & 7)) << 4));
+        else
+        {
+            union { gm_i4 v; gm_s4 h[2]; } r;
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+            {
+                const int k = kk * 32 + q * 8 + j * 4 + (i >> 2);
+                const int off = k * (CH * 16) + (((f * 2 + ((i & 3) >> 1)) ^ gm_ks_swz(k, CH)) << 4) + (i & 1) * 8;
+                r.h[j] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((gm_s4 __attribute__((address_space(3)))*)(lds + off));
+            }
+            return r.v;
+        }
+    }
+};
+
+template <typename E>
+__device__ __forceinline__ float gm_silu(float g, float& s)
+{
+    s = __builtin_amdgcn_rcpf(1.0f + __expf(-g));
+    return g * s;
+}
+
+// v = 4 neighbouring elements at p of which the first n exist
+template <typename E>
+__device__ __forceinline__ void gm_store4(E* p, const float (&v)[4], int n)
+{
+    typedef E vec __attribute__((ext_vector_type(4)));
+    if (n >= 4 && (reinterpret_cast<uintptr_t>(p) & (4 * sizeof(E) - 1)) == 0)
+    {
+        vec o;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[i] = static_cast<E>(v[i]);
+        *reinterpret_cast<vec*>(p) = o;
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (i < n) p[i] = static_cast<E>(v[i]);
+}
+template <typename E>
+__device__ __forceinline__ void gm_load4(const E* p, float (&v)[4], int n)
+{
+    typedef E vec __attribute__((ext_vector_type(4)));
+    if (n >= 4 && (reinterpret_cast<uintptr_t>(p) & (4 * sizeof(E) - 1)) == 0)
+    {
+        const vec o = *reinterpret_cast<const vec*>(p);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = static_cast<float>(o[i]);
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = i < n ? static_cast<float>(p[i]) : 0.f;
+}
+
+__device__ __forceinline__ void gm_put4(void* out, int odt, int64_t at, const float (&v)[4], int n, int accumulate)
+{
+    if (odt == 2)
+    {
+        float* p = static_cast<float*>(out) + at;
+        if (accumulate)
+        {
+            float o[4];
+            gm_load4(p, o, n);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[i] += v[i];
+            gm_store4(p, o, n);
+        }
+        else gm_store4(p, v, n);
+    }
+    else if (odt == 1) gm_store4(static_cast<__bf16*>(out) + at, v, n);
+    else gm_store4(static_cast<_Float16*>(out) + at, v, n);
+}
+
+// the block's forward epilogue for 4 neighbouring columns: h, and the 16-bit g and u of a training pass. A stored value stays
+// on its own side of the clamp, so that the backward pass masks the gradients of the values that were clamped.
+template <typename E>
+__device__ __forceinline__ E gm_keep_side(float v, float limit, bool beyond, bool gate)
+{
+    E r = static_cast<E>(v);
+    if (limit != 0.f)
+    {
+        auto over = [&](E x) {
+            float s;
+            const float f = static_cast<float>(x);
+            return gate ? gm_silu<E>(f, s) > limit : fabsf(f) > limit;
+        };
+        uint16_t b = __builtin_bit_cast(uint16_t, r);
+        if (beyond && !over(r)) b += 1;            // away from zero: the next magnitude lies past the clamp
+        if (!beyond && over(r)) b -= 1;
+        r = __builtin_bit_cast(E, b);
+    }
+    return r;
+}
+
+template <typename E>
+__device__ __forceinline__ void gm_gate4(const GmArgs& a, int m, int n, const float (&g)[4], const float (&u)[4])
+{
+    const int left = a.N - n;
+    float h[4];
+    E kg[4], ku[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+    {
+        float s, t = gm_silu<E>(g[i], s), v = u[i];
+        if (a.g)
+        {
+            kg[i] = gm_keep_side<E>(g[i], a.limit, t > a.limit, true);
+            ku[i] = gm_keep_side<E>(u[i], a.limit, fabsf(v) > a.limit, false);
+        }
+        if (a.limit != 0.f)
+        {
+            t = fminf(t, a.limit);
+            v = fminf(fmaxf(v, -a.limit), a.limit);
+        }
+        h[i] = t * v;
+    }
+    gm_store4(static_cast<E*>(a.out[0]) + (int64_t)m * a.ldo + n, h, left);
+    if (a.g)
+    {
+        E* pg = static_cast<E*>(a.g) + (int64_t)m * a.ldg + n;
+        E* pu = static_cast<E*>(a.u) + (int64_t)m * a.ldg + n;
+        float vg[4], vu[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) vg[i] = static_cast<float>(kg[i]), vu[i] = static_cast<float>(ku[i]);
+        gm_store4(pg, vg, left);
+        gm_store4(pu, vu, left);
+    }
+}
+
+// dh -> dg = dh * clamp(u) * [silu(g) <= L] * silu'(g), du = dh * min(silu(g), L) * [|u| <= L], h
+template <typename E>
+__device__ __forceinline__ void gm_dact4(const GmArgs& a, int m, int n, const float (&dh)[4])
+{
+    const int left = a.N - n;
+    float g[4], u[4], dg[4], du[4], h[4];
+    gm_load4(static_cast<const E*>(a.g) + (int64_t)m * a.ldg + n, g, left);
+    gm_load4(static_cast<const E*>(a.u) + (int64_t)m * a.ldg + n, u, left);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+    {
+        float s, t = gm_silu<E>(g[i], s), v = u[i];
+        float kg = s + t * (1.0f - s), ku = 1.0f;
+        if (a.limit != 0.f)
+        {
+            if (t > a.limit) kg = 0.f;
+            if (fabsf(v) > a.limit) ku = 0.f;
+            t = fminf(t, a.limit);
+            v = fminf(fmaxf(v, -a.limit), a.limit);
+        }
+        dg[i] = dh[i] * v * kg;
+        du[i] = dh[i] * t * ku;
+        h[i] = t * v;
+    }
+    const int64_t at = (int64_t)m * a.ldo + n;
+    gm_store4(static_cast<E*>(a.dg) + at, dg, left);
+    gm_store4(static_cast<E*>(a.du) + at, du, left);
+    gm_store4(static_cast<E*>(a.out[0]) + at, h, left);
+}
+
+// Tile of a workgroup: consecutive workgroups go to the 8 XCDs in turn, each XCD takes a run of neighbouring tiles, in
+// groups of GM_GROUP tile rows, so that the tiles an XCD's CUs work on at once share their operands in its L2.
+constexpr int GM_GROUP = 4;
+__device__ __forceinline__ void gm_tile(int b, int tm, int tn, int& im, int& in)
+{
+    const int total = tm * tn, per = total / 8, extra = total % 8;
+    const int x = b % 8, s = b / 8;
+    const int p = x * per + min(x, extra) + s;
+    const int wide = GM_GROUP * tn, grp = p / wide, first = grp * GM_GROUP;
+    const int rows = min(GM_GROUP, tm - first), r = p - grp * wide;
+    im = first + r % rows;
+    in = r / rows;
+}
+
+template <typename T, int TM, int TN, int WM, int WN, bool AKS, bool BKS, bool DUAL, int NST, bool AL, int EP>
+__global__ __launch_bounds__(WM* WN * 64, (WM * WN + 3) / 4) void gm_kernel(GmArgs a)
+{
+    constexpr int NW = WM * WN;
+    typedef GmSide<T, TM, AKS, false, NW> SA;
+    typedef GmSide<T, TN, BKS, DUAL, NW> SB;
+    constexpr int MI = TM / WM / 16, NI = TN / WN / 16;
+    constexpr int STAGE = SA::BYTES + SB::BYTES;
+    constexpr int BK = SA::BK;
+    static_assert(!DUAL || NI % 2 == 0, "gate and up fragments alternate");
+    extern __shared__ __align__(16) char gm_lds[];
+
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / 64), lane = threadIdx.x % 64;
+    const int wm = wave / WN, wn = wave % WN;
+    int im, in;
+    gm_tile(blockIdx.x, a.tm, a.tn, im, in);
+    constexpr int TNC = DUAL ? TN / 2 : TN;   // columns of a tile
+    const int m0 = im * TM, n0 = in * TNC;
+    const int z = blockIdx.z;
+
+    // K steps of this part, over the segments
+    const int steps1 = (a.K + BK - 1) / BK;
+    int t0 = 0, t1 = steps1 * a.segs;
+    if (a.parts > 1)
+    {
+        t0 = (int)((int64_t)steps1 * blockIdx.y / a.parts);
+        t1 = (int)((int64_t)steps1 * (blockIdx.y + 1) / a.parts);
+    }
+    SA sa;
+    SB sb;
+    sa.init(wave, lane, a.A[z], a.A[z], a.lda, m0, a.M);
+    sb.init(wave, lane, DUAL ? a.B[0] : a.B[z], a.B[1], a.ldb, n0, a.N);
+    sa.advance(t0);
+    sb.advance(t0);
+    // the step whose loads are issued next
+    int ti = t0;
+    auto rem_of = [&](int t) { return a.K - (t < steps1 ? t : t - steps1) * BK; };
+    auto next = [&]() {
+        ++ti;
+        if (a.segs > 1 && ti == steps1)   // the second segment from its start
+        {
+            sa.p0 = gm_uniform(AKS ? a.A[1] + (int64_t)m0 * SA::ES : a.A[1] + (int64_t)m0 * a.lda);
+            sb.p0 = gm_uniform(BKS ? a.B[1] + (int64_t)n0 * SB::ES : a.B[1] + (int64_t)n0 * a.ldb);
+        }
+        else
+        {
+            sa.advance(1);
+            sb.advance(1);
+        }
+    };
+
+    typename T::acc acc[NI][MI];
+#pragma unroll
+    for (int i = 0; i < NI; ++i)
+#pragma unroll
+        for (int j = 0; j < MI; ++j) acc[i][j] = typename T::acc{ 0, 0, 0, 0 };
+
+    auto compute = [&](const char* st) {
+        const char* la = st + (AKS ? 0 : wm * (TM / WM) * 128);
+        const char* lb = st + SA::BYTES + (BKS ? 0 : wn * (TN / WN) * 128);
+        const int fa = AKS ? wm * MI : 0, fb = BKS ? wn * NI : 0;
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk)
+        {
+            gm_i4 fa_[MI], fb_[NI];
+#pragma unroll
+            for (int i = 0; i < NI; ++i) fb_[i] = SB::frag(lb, lane, fb + i, kk);
+#pragma unroll
+            for (int j = 0; j < MI; ++j) fa_[j] = SA::frag(la, lane, fa + j, kk);
+#pragma unroll
+            for (int j = 0; j < MI; ++j)
+#pragma unroll
+                for (int i = 0; i < NI; ++i) acc[i][j] = T::mfma(fb_[i], fa_[j], acc[i][j]);
+        }
+    };
+
+    if constexpr (AL)
+    {
+        constexpr int NV = SA::NV + SB::NV;
+        auto issue = [&](int slot) {
+            char* st = gm_lds + slot * STAGE;
+            sa.issue(st, wave, rem_of(ti));
+            sb.issue(st + SA::BYTES, wave, rem_of(ti));
+            next();
+        };
+        for (int s = 0; s < NST - 1; ++s)
+            if (ti < t1) issue(s);
+        int cur = 0, fill = NST - 1;
+        for (int t = t0; t < t1; ++t)
+        {
+            if (t + NST - 2 < t1) gm_wait_vmcnt<(NST - 2) * NV>();   // this wave's loads of step t have landed
+            else gm_wait_vmcnt<0>();
+            gm_barrier();                     // every wave's have, and every wave is done with step t - 1
+            if (ti < t1) issue(fill);         // into the slot of step t - 1
+            compute(gm_lds + cur * STAGE);
+            cur = cur + 1 == NST ? 0 : cur + 1;
+            fill = fill + 1 == NST ? 0 : fill + 1;
+        }
+    }
+    else
+    {
+        gm_i4 ba[SA::NV], bb[SB::NV];
+        if (ti < t1)
+        {
+            sa.fetch(ba, wave, rem_of(ti));
+            sb.fetch(bb, wave, rem_of(ti));
+            next();
+        }
+        for (int t = t0; t < t1; ++t)
+        {
+            __syncthreads();   // every wave is done with step t - 1
+            sa.commit(ba, gm_lds, wave, lane);
+            sb.commit(bb, gm_lds + SA::BYTES, wave, lane);
+            __syncthreads();
+            if (ti < t1)
+            {
+                sa.fetch(ba, wave, rem_of(ti));
+                sb.fetch(bb, wave, rem_of(ti));
+                next();
+            }
+            compute(gm_lds);
+        }
+    }
+
+    const int i16 = lane & 15, q = lane >> 4;
+#pragma unroll
+    for (int j = 0; j < MI; ++j)
+    {
+        const int m = m0 + wm * (TM / WM) + j * 16 + i16;
+        if (m >= a.M) continue;
+#pragma unroll
+        for (int i = 0; i < NI; i += DUAL ? 2 : 1)
+        {
+            const int n = n0 + wn * (TNC / WN) + (DUAL ? i / 2 : i) * 16 + q * 4;
+            if (n >= a.N) continue;
+            if constexpr (EP == EP_PART)
+            {
+                typename T::scalar* p = static_cast<typename T::scalar*>(a.out[0]) +
+                                        ((int64_t)blockIdx.y * (DUAL ? 2 : 1) * a.M + m) * a.ldo + n;
+                // ldo is a multiple of 4 and rows are padded to it: whole vectors
+                *reinterpret_cast<typename T::acc*>(p) = acc[i][j];
+                if (DUAL) *reinterpret_cast<typename T::acc*>(p + (int64_t)a.M * a.ldo) = acc[i + 1 < NI ? i + 1 : i][j];
+            }
+            else
+            {
+                float v[4];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) v[r] = static_cast<float>(acc[i][j][r]);
+                if constexpr (EP == EP_GATE)
+                {
+                    float w[4];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) w[r] = static_cast<float>(acc[i + 1 < NI ? i + 1 : i][j][r]);
+                    gm_gate4<typename T::elem>(a, m, n, v, w);
+                }
+                else if constexpr (EP == EP_DACT) gm_dact4<typename T::elem>(a, m, n, v);
+                else
+                {
+                    if constexpr (EP == EP_I8)
+                    {
+                        float sn[4];
+                        gm_load4(a.sb + n, sn, a.N - n);
+                        const float sm = a.sa[m];
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) v[r] = v[r] * sm * sn[r];
+                    }
+                    gm_put4(a.out[z], a.odt, (int64_t)m * a.ldo + n, v, a.N - n, a.accumulate);
+                }
+            }
+        }
+    }
+}
+
+// Joins the K parts of a split product and runs its epilogue: a thread per 4 neighbouring columns.
+template <typename T, bool DUAL, int EP>
+__global__ __launch_bounds__(256) void gm_join_kernel(GmArgs a, const void* part, int64_t ldp, int parts)
+{
+    const int cols = (a.N + 3) / 4;
+    const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (at >= (int64_t)a.M * cols) return;
+    const int m = (int)(at / cols), n = (int)(at % cols) * 4;
+    const typename T::scalar* p = static_cast<const typename T::scalar*>(part) + (int64_t)m * ldp + n;
+    typename T::acc s0 = { 0, 0, 0, 0 }, s1 = { 0, 0, 0, 0 };
+    const int64_t mat = (int64_t)a.M * ldp;
+    for (int k = 0; k < parts; ++k)
+    {
+        s0 += *reinterpret_cast<const typename T::acc*>(p);
+        if (DUAL) s1 += *reinterpret_cast<const typename T::acc*>(p + mat);
+        p += (DUAL ? 2 : 1) * mat;
+    }
+    float v[4], w[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) v[r] = static_cast<float>(s0[r]), w[r] = static_cast<float>(s1[r]);
+    if constexpr (EP == EP_GATE) gm_gate4<typename T::elem>(a, m, n, v, w);
+    else
+    {
+        if constexpr (EP == EP_I8)
+        {
+            float sn[4];
+            gm_load4(a.sb + n, sn, a.N - n);
+            const float sm = a.sa[m];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) v[r] = v[r] * sm * sn[r];
+        }
+        gm_put4(a.out[0], a.odt, (int64_t)m * a.ldo + n, v, a.N - n, a.accumulate);
+    }
+}
+
+}  // namespace gfl

@@ -170,4 +170,79 @@ int launch_route_split(const float* logits, int M, int ER, int topk, int64_t* se
                        int64_t* sel_out, uint16_t* w_out, int64_t* dflag, int64_t* stats, const int32_t* rres,
                        hipStream_t st);
 
+// ---- the dense operators (gfl_dense.cpp, k_dense_*.hip, k_quant.hip) ----
+
+// records msg as the thread's last error and returns code (gfl_api.cpp)
+int api_fail(int code, const char* msg);
+int api_hip_fail(hipError_t e, const char* what);
+
+// What a tile's results become.
+enum
+{
+    EP_OUT = 0,    // out[m][n] in 16 bits or fp32, or out += (fp32)
+    EP_GATE = 1,   // DUAL: h = act(g, u) in 16 bits, and g, u themselves where asked for
+    EP_DACT = 2,   // acc = dh: dg, du, h from it and the stored g, u
+    EP_I8 = 3,     // acc * sa[m] * sb[n]
+    EP_PART = 4,   // a K part's accumulators, [part][DUAL matrix][M][N], joined by a second launch
+};
+
+struct GmArgs
+{
+    const char* A[2] = { nullptr, nullptr };   // K segment 0, 1 (or output 0, 1: zmode)
+    const char* B[2] = { nullptr, nullptr };   // the same; DUAL: gate, up
+    int64_t lda = 0, ldb = 0;                  // bytes
+    int M = 0, N = 0, K = 0;                   // K of one segment, elements
+    int segs = 1;                              // K segments (dx: dg Wg + du Wu)
+    int parts = 1;                             // K split over grid y (segs = 1)
+    int tm = 0, tn = 0;                        // tiles along M and N
+    void* out[2] = { nullptr, nullptr };       // out / h / part; by grid z for two outputs (dWg, dWu)
+    int64_t ldo = 0;                           // elements
+    int odt = 0;                               // GFL_F16 / GFL_BF16 / GFL_F32
+    int accumulate = 0;                        // EP_OUT, fp32: out += D
+    float limit = 0.f;                         // SwiGLU clamp, 0 = off
+    void* g = nullptr;                         // [M][N] 16-bit: EP_GATE written (may be NULL), EP_DACT read
+    void* u = nullptr;
+    int64_t ldg = 0;
+    void* dg = nullptr;                        // EP_DACT outputs, [M][ldo]
+    void* du = nullptr;
+    const float* sa = nullptr;                 // EP_I8 scales
+    const float* sb = nullptr;
+};
+
+
+// Storage of the operands of a tile product: NT = A [M][K], B [N][K]; NN = A [M][K], B [K][N]; TN = A [K][M], B [K][N].
+enum
+{
+    GM_NT = 0,
+    GM_NN = 1,
+    GM_TN = 2,
+};
+// One tile product with its epilogue, aligned = every chunk of 16 bytes of both operands is whole and aligned. ws / ws_bytes:
+// room for K parts (gm_plan of the same sizes); 0 on success, -1 for a form that is not built.
+int launch_gemm_f16(int form, int ep, int dual, int aligned, GmArgs& a, void* ws, size_t ws_bytes, int nz, hipStream_t st);
+int launch_gemm_bf16(int form, int ep, int dual, int aligned, GmArgs& a, void* ws, size_t ws_bytes, int nz, hipStream_t st);
+int launch_gemm_i8(int form, int ep, int dual, int aligned, GmArgs& a, void* ws, size_t ws_bytes, int nz, hipStream_t st);
+
+// int8 rows of x [M][K] (16-bit, ldx elements between rows): q [M][ldq], scale [M] (k_quant.hip)
+void launch_quant_i8(const void* x, int64_t ldx, int bf16, int M, int K, int8_t* q, int64_t ldq, float* scale, hipStream_t st);
+
+// token selection (k_sample.hip)
+constexpr int MAX_VOCAB = 1 << 20;
+struct SampleArgs
+{
+    const void* logits = nullptr;
+    int64_t ld = 0;
+    int dtype = 0, B = 0, V = 0;
+    const float* temperature = nullptr;   // [B] each, NULL = off
+    const int32_t* top_k = nullptr;
+    const float* top_p = nullptr;
+    const float* min_p = nullptr;
+    const float* u = nullptr;
+    int64_t* token = nullptr;
+    float* prob = nullptr;
+    void* ws = nullptr;
+};
+size_t sample_ws_bytes(int B, int V);
+void launch_sample(const SampleArgs& a, hipStream_t st);
+
 }  // namespace gfl

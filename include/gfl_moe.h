@@ -253,6 +253,78 @@ int gfl_grouped_rows(const int64_t* sel, const float* w, int T, int K, const uin
  * E <= 1024, topk <= min(E, 64). One wave per token, stream-ordered. */
 int gfl_route(const float* logits, int M, int E, int topk, int64_t* sel, uint16_t* w, gfl_stream stream);
 
+/* ---- Dense operators: what a served model computes beside its EXL3 experts (no counterpart in the reference, whose model
+ * runtime runs them). Stateless: matrices are row-major with a row stride in elements (ld), on the stream's device, and the
+ * caller gives the workspace (16-byte aligned device memory; its size from the *_workspace calls, which depend on the
+ * arguments alone). Calls that may overlap need workspaces of their own, two captured graphs among them. Outputs must
+ * not overlap inputs. Any sizes and strides are taken; matrices whose row strides and addresses are multiples of 16 bytes
+ * and whose widths are multiples of 8 (16-bit) or 16 (int8) elements run on the direct tile loads. Row strides stay below
+ * 2^22 elements. Empty calls (M = 0) launch nothing, but gfl_ffn_backward then writes zeros to the weights' gradients. */
+enum
+{
+    GFL_F16 = 0,
+    GFL_BF16 = 1,
+    GFL_F32 = 2, /* outputs only */
+};
+#define GFL_MAX_LD 4194304
+
+/* Gated feed-forward block, unquantised: g = x Wg^T, u = x Wu^T, h = min(silu(g), L) * clamp(u, -L, L),
+ * y = h Wd^T, with the experts' clamp L = act_limit (0 = off). x [M, H], Wg and Wu [I, H], Wd [H, I] contiguous (as
+ * nn.Linear keeps them), all of one type dtype (GFL_F16 or GFL_BF16); out [M, H] of out_dtype: dtype or GFL_F32. accumulate
+ * (GFL_F32 only): out += y, the shared expert's join. Sums are fp32; h is rounded to dtype before the down product (for
+ * GFL_F16 its range is fp16's), everything else once at the end.
+ * g, u [M, I] contiguous (both or neither): the 16-bit values the backward pass needs. */
+int gfl_ffn_forward(const void* x, int64_t ldx, const void* wg, const void* wu, const void* wd, int dtype, int M, int H,
+                    int I, float act_limit, void* g, void* u, void* out, int64_t ldo, int out_dtype, int accumulate,
+                    void* ws, size_t ws_bytes, gfl_stream stream);
+
+/* Gradients of the block for dy [M, H]: dx [M, H], dwg and dwu [I, H], dwd [H, I] contiguous, all of dtype, each of which
+ * may be NULL (not wanted). x, the weights, act_limit as in the forward call, g and u as it stored them. The clamps pass the
+ * gradient where silu(g) <= L and |u| <= L. dg, du and h are rounded to dtype between the products; sums are fp32. */
+int gfl_ffn_backward(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* g, const void* u,
+                     const void* wg, const void* wu, const void* wd, int dtype, int M, int H, int I, float act_limit,
+                     void* dx, int64_t lddx, void* dwg, void* dwu, void* dwd, void* ws, size_t ws_bytes,
+                     gfl_stream stream);
+
+/* Bytes of workspace: *forward for gfl_ffn_forward, *backward for gfl_ffn_backward (either may be NULL). */
+int gfl_ffn_workspace(int dtype, int M, int H, int I, size_t* forward, size_t* backward);
+
+/* Rows to 8 bits: scale[m] = max_k |x[m][k]| / 127, q[m][k] = x[m][k] * 127 / max rounded to the nearest whole number (ties
+ * to even), for x [M, K] fp16 or bf16. A row of zeros has scale 0 and q 0; a row holding an infinity or a NaN has a scale
+ * that is not finite and q 0, so that its products are NaN. q [M, K] contiguous. */
+int gfl_quant_i8(const void* x, int64_t ldx, int dtype, int M, int K, int8_t* q, float* scale, gfl_stream stream);
+
+/* out[m][n] = (sum_k a[m][k] * b[n][k]) * sa[m] * sb[n]: a int8 [M, K], b int8 [N, K] (a weight as nn.Linear keeps it), a
+ * scale for each token and channel. The sum is exact (int32, K <= 131071); out fp16, bf16 or fp32. */
+int gfl_gemm_i8(const int8_t* a, int64_t lda, const float* sa, const int8_t* b, int64_t ldb, const float* sb, int M, int N,
+                int K, void* out, int64_t ldo, int out_dtype, void* ws, size_t ws_bytes, gfl_stream stream);
+
+/* gfl_quant_i8 of x [M, K] (fp16 or bf16), then gfl_gemm_i8: a linear layer with an 8-bit weight. */
+int gfl_linear_i8(const void* x, int64_t ldx, int dtype, const int8_t* b, int64_t ldb, const float* sb, int M, int N, int K,
+                  void* out, int64_t ldo, int out_dtype, void* ws, size_t ws_bytes, gfl_stream stream);
+
+/* Bytes of workspace: *gemm for gfl_gemm_i8, *linear for gfl_linear_i8 (either may be NULL). */
+int gfl_i8_workspace(int M, int N, int K, size_t* gemm, size_t* linear);
+
+/* Draws a token for each row of logits [B, V] (fp32, fp16 or bf16) from given uniform numbers u [B] in [0, 1).
+ * Per row, each array fp32 [B] (top_k int32), NULL = off for every row:
+ *   temperature  weight of token i = exp((logit_i - max) / T); not above 0: the row is greedy (its largest logit)
+ *   top_k        the k largest logits; not above 0: off
+ *   top_p        the smallest number of largest logits (of the top-k) that hold at least p of the top-k's weight; at
+ *                least one; 1 and above: off
+ *   min_p        the logits whose weight is at least min_p of the largest's; the largest stays; not above 0: off
+ * Equal logits are ordered by index, lowest first. token = the lowest index i (in index order, among the kept) at which the
+ * kept weights summed up to i exceed u * their sum; prob (fp32 [B], may be NULL) = its weight / that sum. -inf and NaN logits
+ * are never drawn; a row with nothing else gives token -1 and prob 0. With +inf logits only they are drawn. Weights are
+ * computed in fp64 and summed as integers in units of 2^-43 of the largest, so results do not depend on the order of
+ * sums. V <= 2^20. */
+int gfl_sample(const void* logits, int64_t ld, int dtype, int B, int V, const float* temperature, const int32_t* top_k,
+               const float* top_p, const float* min_p, const float* u, int64_t* token, float* prob, void* ws,
+               size_t ws_bytes, gfl_stream stream);
+
+/* Bytes of workspace for gfl_sample. */
+int gfl_sample_workspace(int B, int V, size_t* bytes);
+
 /* Fill nbytes of device memory with the splitmix64 stream of `seed` (synthetic trellis for tests and benchmarks;
  * any bit stream is a valid EXL3 tile). Byte b = byte (b % 8) of output b/8. */
 int gfl_synth_trellis(void* dst, size_t nbytes, uint64_t seed, gfl_stream stream);
