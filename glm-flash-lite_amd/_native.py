@@ -473,8 +473,8 @@ def _ffn_weights(name, x, wg, wu, wd):
 def ffn_forward(x, wg, wu, wd, out=None, act_limit=0.0, save=False, accumulate=False):
     """Gated feed-forward block (gfl_ffn_forward): (min(silu(x wg^T), L) * clamp(x wu^T, -L, L)) wd^T, L = act_limit, 0 = off.
     x fp16 or bf16 [..., H] (rows may have a stride), wg and wu [I, H], wd [H, I] as nn.Linear keeps them. out: of x's type
-    (the default) or fp32; accumulate (fp32 out): out += the block. save=True returns (out, g, u) with the 16-bit g and u [M,
-    I] that ffn_backward takes."""
+    (the default) or fp32; accumulate (fp32 out): out += the block. save=True returns (out, g, u) with the fp32 g and u [M, I] that
+    ffn_backward takes."""
     import torch
     H, I = _ffn_weights("ffn_forward", x, wg, wu, wd)
     M, ldx = _rows("ffn_forward: x", x, H)
@@ -488,8 +488,8 @@ def ffn_forward(x, wg, wu, wd, out=None, act_limit=0.0, save=False, accumulate=F
         raise ValueError("ffn_forward: out must have x's shape and be of its type or fp32")
     mo, ldo = _rows("ffn_forward: out", out, H)
     _check_rows("ffn_forward: out", mo, ldo, H)
-    g = torch.empty((M, I), dtype=x.dtype, device=dev) if save else None
-    u = torch.empty((M, I), dtype=x.dtype, device=dev) if save else None
+    g = torch.empty((M, I), dtype=torch.float32, device=dev) if save else None
+    u = torch.empty((M, I), dtype=torch.float32, device=dev) if save else None
     L, need = load(), C.c_size_t()
     code = _dtype_code(x.dtype)
     check(L.gfl_ffn_workspace(code, M, H, I, C.byref(need), None))
@@ -513,8 +513,8 @@ def ffn_backward(dy, x, g, u, wg, wu, wd, act_limit=0.0, need=(True, True, True,
     _check_rows("ffn_backward: x", M, ldx, H)
     _check_rows("ffn_backward: dy", my, ldy, H)
     for n, t in (("g", g), ("u", u)):
-        if tuple(t.shape) != (M, I) or t.dtype != x.dtype or not t.is_contiguous():
-            raise ValueError(f"ffn_backward: {n} must be contiguous [{M}, {I}], of x's type")
+        if tuple(t.shape) != (M, I) or t.dtype != torch.float32 or not t.is_contiguous():
+            raise ValueError(f"ffn_backward: {n} must be contiguous fp32 [{M}, {I}]")
     dev = _on_device("ffn_backward", x, dy, g, u, wg, wu, wd)
     dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need[0] else None
     dw = [torch.empty_like(t) if n else None for t, n in zip((wg, wu, wd), need[1:])]

@@ -77,7 +77,7 @@ int gfl_ffn_workspace(int dtype, int M, int H, int I, size_t* forward, size_t* b
 }
 
 int gfl_ffn_forward(const void* x, int64_t ldx, const void* wg, const void* wu, const void* wd, int dtype, int M, int H,
-                    int I, float act_limit, void* g, void* u, void* out, int64_t ldo, int out_dtype, int accumulate,
+                    int I, float act_limit, float* g, float* u, void* out, int64_t ldo, int out_dtype, int accumulate,
                     void* ws, size_t ws_bytes, gfl_stream stream)
 {
     if (int rc = ffn_check("gfl_ffn_forward", dtype, M, H, I)) return rc;
@@ -127,7 +127,7 @@ int gfl_ffn_forward(const void* x, int64_t ldx, const void* wg, const void* wu, 
     return gemm16("gfl_ffn_forward: down product", dtype, gfl::GM_NT, gfl::EP_OUT, 0, al, b, part, z.part, 1, st);
 }
 
-int gfl_ffn_backward(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* g, const void* u,
+int gfl_ffn_backward(const void* dy, int64_t lddy, const void* x, int64_t ldx, const float* g, const float* u,
                      const void* wg, const void* wu, const void* wd, int dtype, int M, int H, int I, float act_limit,
                      void* dx, int64_t lddx, void* dwg, void* dwu, void* dwd, void* ws, size_t ws_bytes, gfl_stream stream)
 {
@@ -154,7 +154,7 @@ int gfl_ffn_backward(const void* dy, int64_t lddy, const void* x, int64_t ldx, c
         a.dg = dg; a.du = du;
         a.ldo = z.ldh;
         a.limit = act_limit;
-        a.g = const_cast<void*>(g); a.u = const_cast<void*>(u); a.ldg = I;
+        a.g = const_cast<float*>(g); a.u = const_cast<float*>(u); a.ldg = I;
         const int al = wide(dy, a.lda) && wide(wd, a.ldb) && H % 8 == 0 && I % 8 == 0;
         if (int rc = gemm16("gfl_ffn_backward: dh", dtype, gfl::GM_NN, gfl::EP_DACT, 0, al, a, nullptr, 0, 1, st)) return rc;
         if (dx)
@@ -311,7 +311,8 @@ int gfl_linear_i8(const void* x, int64_t ldx, int dtype, const int8_t* b, int64_
 
 int gfl_sample_workspace(int B, int V, size_t* bytes)
 {
-    if (B < 0 || V < 1 || V > gfl::MAX_VOCAB) return api_fail(GFL_EINVAL, "gfl_sample: need B >= 0 and 1 <= V <= 2^20");
+    if (B < 0 || B > 65535 || V < 1 || V > gfl::MAX_VOCAB)
+        return api_fail(GFL_EINVAL, "gfl_sample: need 0 <= B <= 65535 (grid) and 1 <= V <= 2^20");
     if (bytes) *bytes = gfl::sample_ws_bytes(B, V);
     return GFL_OK;
 }

@@ -276,42 +276,17 @@ __device__ __forceinline__ void gm_put4(void* out, int odt, int64_t at, const fl
     else gm_store4(static_cast<_Float16*>(out) + at, v, n);
 }
 
-// the block's forward epilogue for 4 neighbouring columns: h, and the 16-bit g and u of a training pass. A stored value stays
-// on its own side of the clamp, so that the backward pass masks the gradients of the values that were clamped.
-template <typename E>
-__device__ __forceinline__ E gm_keep_side(float v, float limit, bool beyond, bool gate)
-{
-    E r = static_cast<E>(v);
-    if (limit != 0.f)
-    {
-        auto over = [&](E x) {
-            float s;
-            const float f = static_cast<float>(x);
-            return gate ? gm_silu<E>(f, s) > limit : fabsf(f) > limit;
-        };
-        uint16_t b = __builtin_bit_cast(uint16_t, r);
-        if (beyond && !over(r)) b += 1;            // away from zero: the next magnitude lies past the clamp
-        if (!beyond && over(r)) b -= 1;
-        r = __builtin_bit_cast(E, b);
-    }
-    return r;
-}
-
+// the block's forward epilogue for 4 neighbouring columns: h, and g and u of a training pass in fp32 (16-bit ones doubled the
+// gradients' error: 2.0 against 1.4 roundings in the root mean square; their traffic is 2% of a training step)
 template <typename E>
 __device__ __forceinline__ void gm_gate4(const GmArgs& a, int m, int n, const float (&g)[4], const float (&u)[4])
 {
     const int left = a.N - n;
     float h[4];
-    E kg[4], ku[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i)
     {
         float s, t = gm_silu<E>(g[i], s), v = u[i];
-        if (a.g)
-        {
-            kg[i] = gm_keep_side<E>(g[i], a.limit, t > a.limit, true);
-            ku[i] = gm_keep_side<E>(u[i], a.limit, fabsf(v) > a.limit, false);
-        }
         if (a.limit != 0.f)
         {
             t = fminf(t, a.limit);
@@ -322,13 +297,8 @@ __device__ __forceinline__ void gm_gate4(const GmArgs& a, int m, int n, const fl
     gm_store4(static_cast<E*>(a.out[0]) + (int64_t)m * a.ldo + n, h, left);
     if (a.g)
     {
-        E* pg = static_cast<E*>(a.g) + (int64_t)m * a.ldg + n;
-        E* pu = static_cast<E*>(a.u) + (int64_t)m * a.ldg + n;
-        float vg[4], vu[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) vg[i] = static_cast<float>(kg[i]), vu[i] = static_cast<float>(ku[i]);
-        gm_store4(pg, vg, left);
-        gm_store4(pu, vu, left);
+        gm_store4(a.g + (int64_t)m * a.ldg + n, g, left);
+        gm_store4(a.u + (int64_t)m * a.ldg + n, u, left);
     }
 }
 
@@ -338,8 +308,8 @@ __device__ __forceinline__ void gm_dact4(const GmArgs& a, int m, int n, const fl
 {
     const int left = a.N - n;
     float g[4], u[4], dg[4], du[4], h[4];
-    gm_load4(static_cast<const E*>(a.g) + (int64_t)m * a.ldg + n, g, left);
-    gm_load4(static_cast<const E*>(a.u) + (int64_t)m * a.ldg + n, u, left);
+    gm_load4(a.g + (int64_t)m * a.ldg + n, g, left);
+    gm_load4(a.u + (int64_t)m * a.ldg + n, u, left);
 #pragma unroll
     for (int i = 0; i < 4; ++i)
     {

@@ -180,7 +180,7 @@ int api_hip_fail(hipError_t e, const char* what);
 enum
 {
     EP_OUT = 0,    // out[m][n] in 16 bits or fp32, or out += (fp32)
-    EP_GATE = 1,   // DUAL: h = act(g, u) in 16 bits, and g, u themselves where asked for
+    EP_GATE = 1,   // DUAL: h = act(g, u) in 16 bits, and g, u in fp32 where asked for
     EP_DACT = 2,   // acc = dh: dg, du, h from it and the stored g, u
     EP_I8 = 3,     // acc * sa[m] * sb[n]
     EP_PART = 4,   // a K part's accumulators, [part][DUAL matrix][M][N], joined by a second launch
@@ -200,8 +200,8 @@ struct GmArgs
     int odt = 0;                               // GFL_F16 / GFL_BF16 / GFL_F32
     int accumulate = 0;                        // EP_OUT, fp32: out += D
     float limit = 0.f;                         // SwiGLU clamp, 0 = off
-    void* g = nullptr;                         // [M][N] 16-bit: EP_GATE written (may be NULL), EP_DACT read
-    void* u = nullptr;
+    float* g = nullptr;                        // [M][N]: EP_GATE written (may be NULL), EP_DACT read
+    float* u = nullptr;
     int64_t ldg = 0;
     void* dg = nullptr;                        // EP_DACT outputs, [M][ldo]
     void* du = nullptr;

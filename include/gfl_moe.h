@@ -273,15 +273,15 @@ enum
  * nn.Linear keeps them), all of one type dtype (GFL_F16 or GFL_BF16); out [M, H] of out_dtype: dtype or GFL_F32. accumulate
  * (GFL_F32 only): out += y, the shared expert's join. Sums are fp32; h is rounded to dtype before the down product (for
  * GFL_F16 its range is fp16's), everything else once at the end.
- * g, u [M, I] contiguous (both or neither): the 16-bit values the backward pass needs. */
+ * g, u fp32 [M, I] contiguous (both or neither): what the backward pass needs. */
 int gfl_ffn_forward(const void* x, int64_t ldx, const void* wg, const void* wu, const void* wd, int dtype, int M, int H,
-                    int I, float act_limit, void* g, void* u, void* out, int64_t ldo, int out_dtype, int accumulate,
+                    int I, float act_limit, float* g, float* u, void* out, int64_t ldo, int out_dtype, int accumulate,
                     void* ws, size_t ws_bytes, gfl_stream stream);
 
 /* Gradients of the block for dy [M, H]: dx [M, H], dwg and dwu [I, H], dwd [H, I] contiguous, all of dtype, each of which
  * may be NULL (not wanted). x, the weights, act_limit as in the forward call, g and u as it stored them. The clamps pass the
  * gradient where silu(g) <= L and |u| <= L. dg, du and h are rounded to dtype between the products; sums are fp32. */
-int gfl_ffn_backward(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* g, const void* u,
+int gfl_ffn_backward(const void* dy, int64_t lddy, const void* x, int64_t ldx, const float* g, const float* u,
                      const void* wg, const void* wu, const void* wd, int dtype, int M, int H, int I, float act_limit,
                      void* dx, int64_t lddx, void* dwg, void* dwu, void* dwd, void* ws, size_t ws_bytes,
                      gfl_stream stream);
@@ -317,7 +317,7 @@ int gfl_i8_workspace(int M, int N, int K, size_t* gemm, size_t* linear);
  * kept weights summed up to i exceed u * their sum; prob (fp32 [B], may be NULL) = its weight / that sum. -inf and NaN logits
  * are never drawn; a row with nothing else gives token -1 and prob 0. With +inf logits only they are drawn. Weights are
  * computed in fp64 and summed as integers in units of 2^-43 of the largest, so results do not depend on the order of
- * sums. V <= 2^20. */
+ * sums. B <= 65535, V <= 2^20. */
 int gfl_sample(const void* logits, int64_t ld, int dtype, int B, int V, const float* temperature, const int32_t* top_k,
                const float* top_p, const float* min_p, const float* u, int64_t* token, float* prob, void* ws,
                size_t ws_bytes, gfl_stream stream);

@@ -61,9 +61,7 @@ class FFN:
         pass_g, pass_u = self.raw <= L, self.u.abs() <= L
         dg = torch.where(pass_g, dh * self.v * k, 0.0)
         du = torch.where(pass_u, dh * self.t, 0.0)
-        # the stored 16-bit g, u: a rounding, or a step to the value's own side of the clamp
-        eg = self.eg + 2 * u * (self.g.abs() + self.eg) + tiny(dt)
-        eu = self.eu + 2 * u * (self.u.abs() + self.eu) + tiny(dt)
+        eg, eu = self.eg, self.eu
         ek = 0.5 * eg + (8 + 2 * self.g.abs()) * U32 * (2 + self.g.abs())
         et = 1.1 * eg + (8 + 2 * self.g.abs()) * U32 * self.raw.abs()
         a, b, c = dh.abs() + edh, self.v.abs() + eu, k.abs() + ek
@@ -127,7 +125,7 @@ def sample(logits, u, temperature=None, top_k=None, top_p=None, min_p=None):
             out.append((int(idx[0]), 1.0, 1.0))
             continue
         e = torch.where(val == val[0], 1.0, torch.where((val == -math.inf) | (val[0] == math.inf), 0.0,
-                                                        torch.exp((val - val[0]) / T)))
+                                                        torch.exp((val - val[0]) / T)))   # T = inf: all the finite ones weigh 1
         n, margin = len(x), 1.0
         if top_k is not None and int(top_k[b]) > 0:
             n = min(n, int(top_k[b]))

@@ -383,6 +383,26 @@ def test_sample_extremes(gpu):
     assert tok.cpu().tolist() == [int(keep[b, c]) for b, c in enumerate((0, 0, 2, 2, 0, 0, 2, 0))]
 
 
+@pytest.mark.parametrize("dt", [F32, BF16])
+def test_sample_large_k_and_low_temperature(gpu, dt):
+    """A top-k larger than a row's list, one that ends below where weights round to zero, temperatures from near greedy to flat,
+    finite masks of the type's lowest value, logits that span the type's range."""
+    g = _rng(17)
+    V = 70000
+    x = (torch.randn((6, V), generator=g) * 2.5).to(dt)
+    x[2, torch.rand(V, generator=g) < 0.9] = torch.finfo(dt).min
+    x[3] = (torch.rand(V, generator=g) * 2 - 1).to(dt) * (torch.finfo(dt).max / 2)
+    x[4, 1000:] = -math.inf
+    u = torch.rand(6, generator=g)
+    for t in (0.02, 0.7, 50.0, math.inf):
+        for k in (3, 900, 1500, 5000, 69999):
+            _check_draw(x, u, temperature=[t] * 6, top_k=[k] * 6, skip=1)
+            _check_draw(x, u, temperature=[t] * 6, top_k=[k] * 6, top_p=[0.93] * 6, min_p=[1e-4] * 6, skip=1)
+        _check_draw(x, u, temperature=[t] * 6, top_p=[0.8] * 6, skip=1)
+        _check_draw(x, u, temperature=[t] * 6, top_p=[0.999] * 6, min_p=[0.02] * 6, skip=1)
+        _check_draw(x, u, temperature=[t] * 6, min_p=[0.02] * 6, skip=1)
+
+
 def test_sample_strided_rows(gpu):
     x = torch.randn((5, 1003), generator=_rng(2))
     buf = torch.full((5, 1100), 1e30, device="cuda")
