@@ -11,7 +11,12 @@ using gfl::api_fail;
 
 constexpr size_t up256(size_t x) { return (x + 255) & ~size_t(255); }
 
-bool wide(const void* p, int64_t ld_bytes) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld_bytes % 16 == 0; }
+// rows of whole 4-byte words, which the direct tile loads need
+bool words(const void* p, int64_t ld_bytes)
+{
+    // at least a chunk long: what a chunk reads past its row then lies in the next one
+    return reinterpret_cast<uintptr_t>(p) % 4 == 0 && ld_bytes % 4 == 0 && ld_bytes >= 16;
+}
 
 int check_launch(const char* what)
 {
@@ -109,7 +114,8 @@ int gfl_ffn_forward(const void* x, int64_t ldx, const void* wg, const void* wu, 
     a.ldo = z.ldh;
     a.limit = act_limit;
     a.g = g; a.u = u; a.ldg = I;
-    int al = wide(x, a.lda) && wide(wg, a.ldb) && wide(wu, a.ldb) && H % 8 == 0;
+    int al = words(x, a.lda) && words(wg, a.ldb) && words(wu, a.ldb);
+    a.ragged = H % 8 != 0;
     if (int rc = gemm16("gfl_ffn_forward: gate and up product", dtype, gfl::GM_NT, gfl::EP_GATE, 1, al, a, part, z.part, 1, st))
         return rc;
 
@@ -123,7 +129,8 @@ int gfl_ffn_forward(const void* x, int64_t ldx, const void* wg, const void* wu, 
     b.ldo = ldo;
     b.odt = out_dtype;
     b.accumulate = accumulate;
-    al = wide(wd, b.ldb) && I % 8 == 0;
+    al = words(wd, b.ldb);
+    b.ragged = I % 8 != 0;
     return gemm16("gfl_ffn_forward: down product", dtype, gfl::GM_NT, gfl::EP_OUT, 0, al, b, part, z.part, 1, st);
 }
 
@@ -155,7 +162,8 @@ int gfl_ffn_backward(const void* dy, int64_t lddy, const void* x, int64_t ldx, c
         a.ldo = z.ldh;
         a.limit = act_limit;
         a.g = const_cast<float*>(g); a.u = const_cast<float*>(u); a.ldg = I;
-        const int al = wide(dy, a.lda) && wide(wd, a.ldb) && H % 8 == 0 && I % 8 == 0;
+        const int al = words(dy, a.lda) && words(wd, a.ldb);
+        a.ragged = H % 8 != 0 || I % 8 != 0;
         if (int rc = gemm16("gfl_ffn_backward: dh", dtype, gfl::GM_NN, gfl::EP_DACT, 0, al, a, nullptr, 0, 1, st)) return rc;
         if (dx)
         {
@@ -169,12 +177,13 @@ int gfl_ffn_backward(const void* dy, int64_t lddy, const void* x, int64_t ldx, c
             b.out[0] = dx;
             b.ldo = lddx;
             b.odt = dtype;
-            const int bl = wide(wg, b.ldb) && wide(wu, b.ldb) && I % 8 == 0 && H % 8 == 0;
+            const int bl = words(wg, b.ldb) && words(wu, b.ldb);
+            b.ragged = H % 8 != 0 || I % 8 != 0;
             if (int rc = gemm16("gfl_ffn_backward: dx", dtype, gfl::GM_NN, gfl::EP_OUT, 0, bl, b, nullptr, 0, 1, st)) return rc;
         }
     }
     // the weights' gradients: [dg | du]^T x and dy^T h (zeros at M = 0: no K step)
-    const int hw = H % 8 == 0 && I % 8 == 0;
+    const int ragged = H % 8 != 0 || I % 8 != 0;
     if (dwg || dwu)
     {
         gfl::GmArgs b;
@@ -187,7 +196,8 @@ int gfl_ffn_backward(const void* dy, int64_t lddy, const void* x, int64_t ldx, c
         b.out[0] = dwg ? dwg : dwu; b.out[1] = dwu;
         b.ldo = H;
         b.odt = dtype;
-        const int al = M == 0 || (hw && wide(x, b.ldb));
+        b.ragged = ragged;
+        const int al = M == 0 || words(x, b.ldb);
         if (int rc = gemm16("gfl_ffn_backward: dWg, dWu", dtype, gfl::GM_TN, gfl::EP_OUT, 0, al, b, nullptr, 0, both ? 2 : 1, st))
             return rc;
     }
@@ -202,7 +212,8 @@ int gfl_ffn_backward(const void* dy, int64_t lddy, const void* x, int64_t ldx, c
         b.out[0] = dwd;
         b.ldo = I;
         b.odt = dtype;
-        const int al = M == 0 || (hw && wide(dy, b.lda));
+        b.ragged = ragged;
+        const int al = M == 0 || words(dy, b.lda);
         if (int rc = gemm16("gfl_ffn_backward: dWd", dtype, gfl::GM_TN, gfl::EP_OUT, 0, al, b, nullptr, 0, 1, st)) return rc;
     }
     return GFL_OK;
@@ -256,7 +267,8 @@ static int i8_product(const char* what, const int8_t* a, int64_t lda, const floa
     g.ldo = ldo;
     g.odt = out_dtype;
     g.sa = sa; g.sb = sb;
-    const int al = wide(a, lda) && wide(b, ldb) && K % 16 == 0;
+    g.ragged = K % 16 != 0;
+    const int al = words(a, lda) && words(b, ldb);
     if (gfl::launch_gemm_i8(gfl::GM_NT, gfl::EP_I8, 0, al, g, part, part_bytes, 1, st)) return api_fail(GFL_EINVAL, what);
     return check_launch(what);
 }

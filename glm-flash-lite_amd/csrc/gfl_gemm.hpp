@@ -10,9 +10,11 @@
 //   ds_read_b64_tr_b16, which hand lane i of each 16 the 4 k values of column i.
 // MFMA operands are (B rows, A rows), so that a lane's 4 accumulators are 4 neighbouring n of one m: vector stores.
 //
-// AL = 1 (every chunk of 16 bytes aligned and whole) loads tiles by LDS-direct buffer loads, NST - 1 steps ahead; rows past
+// AL = 1 (rows start at multiples of 4 bytes) loads tiles by LDS-direct buffer loads, NST - 1 steps ahead; rows past
 // the matrix are clamped to its last (their results are not stored), k past the end is read as zero through the
-// buffer's bounds. AL = 0 takes any strides and sizes: chunks go through registers, masked per element.
+// buffer's bounds. Where rows end inside a chunk of 16 bytes (GmArgs::ragged) the last K step, whose chunks may reach past
+// the matrix, goes through registers, masked per element: what other steps read past a row is the next row's, in
+// columns that are not stored. AL = 0 takes any strides and alignment: every chunk goes through registers.
 #pragma once
 #include "gfl_internal.hpp"
 
@@ -189,6 +191,13 @@ struct GmSide
                 b[j] = gm_masked<ES>(base + (int64_t)min(src_row(lrow[j]), nrow - 1) * ld + c * ES, (rem - c) * ES);
             }
         }
+    }
+    // one K step through registers at once
+    __device__ __forceinline__ void carry(char* lds, int wave, int lane, int rem) const
+    {
+        gm_i4 b[NV];
+        fetch(b, wave, rem);
+        commit(b, lds, wave, lane);
     }
     __device__ __forceinline__ void commit(const gm_i4 (&b)[NV], char* lds, int wave, int lane) const
     {
@@ -427,8 +436,18 @@ __global__ __launch_bounds__(WM* WN * 64, (WM * WN + 3) / 4) void gm_kernel(GmAr
         constexpr int NV = SA::NV + SB::NV;
         auto issue = [&](int slot) {
             char* st = gm_lds + slot * STAGE;
-            sa.issue(st, wave, rem_of(ti));
-            sb.issue(st + SA::BYTES, wave, rem_of(ti));
+            const int rem = rem_of(ti);
+            if (a.ragged && rem <= BK)
+            {
+                // (its loads are waited for here, and with them all earlier ones: the counted waits below stay true)
+                sa.carry(st, wave, lane, rem);
+                sb.carry(st + SA::BYTES, wave, lane, rem);
+            }
+            else
+            {
+                sa.issue(st, wave, rem);
+                sb.issue(st + SA::BYTES, wave, rem);
+            }
             next();
         };
         for (int s = 0; s < NST - 1; ++s)
@@ -549,6 +568,90 @@ __global__ __launch_bounds__(256) void gm_join_kernel(GmArgs a, const void* part
             const float sm = a.sa[m];
 #pragma unroll
             for (int r = 0; r < 4; ++r) v[r] = v[r] * sm * sn[r];
+        }
+        gm_put4(a.out[0], a.odt, (int64_t)m * a.ldo + n, v, a.N - n, a.accumulate);
+    }
+}
+
+// Few tokens (M <= 16): D of 16 rows of B by a workgroup of NW waves, which take the K steps of 64 bytes a row in turn. An MFMA
+// fragment's 16 bytes a lane come straight from memory (16 rows x 64 bytes a load, U loads in flight per wave), so there is no
+// LDS staging and no barrier until the waves' partial sums meet in LDS. DUAL: 8 rows of each matrix. Bound by the weights'
+// bytes: 5120 x 1536 x 2 fp16 in one launch, against a split over workgroups whose parts a second launch joined.
+template <typename T, bool DUAL, int EP, int NW>
+__global__ __launch_bounds__(NW * 64) void gm_skinny_kernel(GmArgs a)
+{
+    constexpr int ES = sizeof(typename T::elem), U = 8;
+    typedef typename T::acc acc_t;
+    __shared__ acc_t red[NW][16][4];   // [wave][token][4 rows]
+    const int wave = threadIdx.x / 64, lane = threadIdx.x % 64, i = lane & 15, q = lane >> 4;
+    constexpr int NR = DUAL ? 8 : 16;
+    const int n0 = blockIdx.x * NR;
+    const char* w = DUAL && i >= 8 ? a.B[1] : a.B[0];
+    w += (int64_t)min(n0 + (DUAL ? i & 7 : i), a.N - 1) * a.ldb + q * 16;
+    const char* x = a.A[0] + (int64_t)min(i, a.M - 1) * a.lda + q * 16;
+    const bool live = i < a.M;
+    const int kb = a.K * ES, whole = kb / 64;   // whole steps
+    acc_t acc = { 0, 0, 0, 0 };
+    auto ld = [](const char* p) {
+        gm_i4 v;
+        __builtin_memcpy(&v, p, 16);
+        return v;
+    };
+    int t = wave;
+    for (; t + (U - 1) * NW < whole; t += U * NW)
+    {
+        gm_i4 fw[U], fx[U];
+#pragma unroll
+        for (int j = 0; j < U; ++j) fw[j] = ld(w + (int64_t)(t + j * NW) * 64);
+#pragma unroll
+        for (int j = 0; j < U; ++j) fx[j] = live ? ld(x + (int64_t)(t + j * NW) * 64) : gm_i4{ 0, 0, 0, 0 };
+#pragma unroll
+        for (int j = 0; j < U; ++j) acc = T::mfma(fw[j], fx[j], acc);
+    }
+    if (t < whole)
+    {
+        gm_i4 fw[U], fx[U];
+#pragma unroll
+        for (int j = 0; j < U; ++j)
+        {
+            const bool in = t + j * NW < whole;
+            fw[j] = in ? ld(w + (int64_t)(t + j * NW) * 64) : gm_i4{ 0, 0, 0, 0 };
+            fx[j] = in && live ? ld(x + (int64_t)(t + j * NW) * 64) : gm_i4{ 0, 0, 0, 0 };
+        }
+#pragma unroll
+        for (int j = 0; j < U; ++j) acc = T::mfma(fw[j], fx[j], acc);
+    }
+    if (kb % 64 && wave == whole % NW)
+    {
+        const int nb = kb - whole * 64 - q * 16;
+        acc = T::mfma(gm_masked<ES>(w + (int64_t)whole * 64, nb), gm_masked<ES>(x + (int64_t)whole * 64, live ? nb : 0), acc);
+    }
+    red[wave][i][q] = acc;
+    __syncthreads();
+    if (wave) return;
+    const int m = lane / 4, r = lane % 4;
+    acc_t sum = red[0][m][r];
+#pragma unroll
+    for (int k = 1; k < NW; ++k) sum += red[k][m][r];
+    float v[4], up[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+    {
+        v[k] = static_cast<float>(sum[k]);
+        if (DUAL) up[k] = __shfl_down(v[k], 2);
+    }
+    const int n = n0 + r * 4;
+    if (m >= a.M || (DUAL && r >= 2) || n >= a.N) return;
+    if constexpr (EP == EP_GATE) gm_gate4<typename T::elem>(a, m, n, v, up);
+    else
+    {
+        if constexpr (EP == EP_I8)
+        {
+            float sn[4];
+            gm_load4(a.sb + n, sn, a.N - n);
+            const float sm = a.sa[m];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[k] = v[k] * sm * sn[k];
         }
         gm_put4(a.out[0], a.odt, (int64_t)m * a.ldo + n, v, a.N - n, a.accumulate);
     }

@@ -26,10 +26,12 @@ static int gm_tiles(GmArgs& a, const GmPlan& p, int aligned, int nz, hipStream_t
     a.tn = (a.N + p.tn - 1) / p.tn;
     if (!aligned)
     {
-        if (p.tm == 16) return gm_go<T, 16, 128, 1, 4, AKS, BKS, DUAL, 2, false, EP>(a, nz, st);
+        if constexpr (BKS && !AKS)
+            if (p.tm == 16) return gm_go<T, 16, 128, 1, 4, AKS, BKS, DUAL, 2, false, EP>(a, nz, st);
         return gm_go<T, 128, 128, 2, 2, AKS, BKS, DUAL, 2, false, EP>(a, nz, st);
     }
-    if (p.tm == 16) return gm_go<T, 16, 128, 1, 4, AKS, BKS, DUAL, 4, true, EP>(a, nz, st);
+    if constexpr (BKS && !AKS)
+        if (p.tm == 16) return gm_go<T, 16, 128, 1, 4, AKS, BKS, DUAL, 4, true, EP>(a, nz, st);
     if (p.tm == 64) return gm_go<T, 64, 128, 1, 4, AKS, BKS, DUAL, 3, true, EP>(a, nz, st);
     if (p.tm == 128) return gm_go<T, 128, 128, 2, 2, AKS, BKS, DUAL, 2, true, EP>(a, nz, st);
     return gm_go<T, 256, 256, 2, 4, AKS, BKS, DUAL, 2, true, EP>(a, nz, st);
@@ -38,6 +40,16 @@ static int gm_tiles(GmArgs& a, const GmPlan& p, int aligned, int nz, hipStream_t
 template <typename T, bool AKS, bool BKS, bool DUAL, int EP>
 static int gm_run(int form, int ep, int aligned, GmArgs& a, void* ws, size_t ws_bytes, int nz, hipStream_t st)
 {
+    if constexpr (!AKS && !BKS && EP != EP_PART)
+        if (a.M <= 16)
+        {
+            const int per = DUAL ? 8 : 16, wg = (a.N + per - 1) / per;
+            // waves of a workgroup: enough loads in flight over the card's CUs, few workgroups taking more waves each
+            if (wg <= 768) hipLaunchKernelGGL((gm_skinny_kernel<T, DUAL, EP, 16>), dim3(wg), dim3(1024), 0, st, a);
+            else if (wg <= 2048) hipLaunchKernelGGL((gm_skinny_kernel<T, DUAL, EP, 8>), dim3(wg), dim3(512), 0, st, a);
+            else hipLaunchKernelGGL((gm_skinny_kernel<T, DUAL, EP, 4>), dim3(wg), dim3(256), 0, st, a);
+            return 0;
+        }
     GmPlan p = gm_plan(form, ep, DUAL, aligned, a.M, a.N, a.K, a.segs);
     if (p.parts > 1 && (!ws || ws_bytes < p.part_bytes)) return -2;
     if (p.parts == 1) return gm_tiles<T, AKS, BKS, DUAL, EP>(a, p, aligned, nz, st);

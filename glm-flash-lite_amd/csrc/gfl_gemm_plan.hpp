@@ -21,7 +21,12 @@ inline GmPlan gm_plan(int form, int ep, int dual, int aligned, int M, int N, int
     const int64_t cu = 256;
     auto tiles = [&](int64_t tm, int64_t tn) { return ((M + tm - 1) / tm) * ((N + tn - 1) / tn); };
     const int d = dual ? 2 : 1;
-    if (M <= 16 && form != GM_TN) p.tm = 16, p.tn = 128 / d;
+    if (M <= 16 && form == GM_NT)   // gm_skinny_kernel
+    {
+        p.tm = 16, p.tn = 16 / d, p.parts = 1, p.ldp = 0, p.part_bytes = 0;
+        return p;
+    }
+    if (M <= 16 && form == GM_NN) p.tm = 16, p.tn = 128 / d;
     else if (!aligned) p.tm = 128, p.tn = 128 / d;
     else if (M <= 64) p.tm = 64, p.tn = 128 / d;
     else if (tiles(256, 256 / d) >= cu * 3 / 4) p.tm = 256, p.tn = 256 / d;

@@ -193,6 +193,7 @@ struct GmArgs
     int64_t lda = 0, ldb = 0;                  // bytes
     int M = 0, N = 0, K = 0;                   // K of one segment, elements
     int segs = 1;                              // K segments (dx: dg Wg + du Wu)
+    int ragged = 0;                            // rows end inside a chunk of 16 bytes (AL tiles)
     int parts = 1;                             // K split over grid y (segs = 1)
     int tm = 0, tn = 0;                        // tiles along M and N
     void* out[2] = { nullptr, nullptr };       // out / h / part; by grid z for two outputs (dWg, dWu)
@@ -217,7 +218,7 @@ enum
     GM_NN = 1,
     GM_TN = 2,
 };
-// One tile product with its epilogue, aligned = every chunk of 16 bytes of both operands is whole and aligned. ws / ws_bytes:
+// One tile product with its epilogue, aligned = the rows of both operands start at multiples of 4 bytes. ws / ws_bytes:
 // room for K parts (gm_plan of the same sizes); 0 on success, -1 for a form that is not built.
 int launch_gemm_f16(int form, int ep, int dual, int aligned, GmArgs& a, void* ws, size_t ws_bytes, int nz, hipStream_t st);
 int launch_gemm_bf16(int form, int ep, int dual, int aligned, GmArgs& a, void* ws, size_t ws_bytes, int nz, hipStream_t st);

@@ -257,9 +257,8 @@ int gfl_route(const float* logits, int M, int E, int topk, int64_t* sel, uint16_
  * runtime runs them). Stateless: matrices are row-major with a row stride in elements (ld), on the stream's device, and the
  * caller gives the workspace (16-byte aligned device memory; its size from the *_workspace calls, which depend on the
  * arguments alone). Calls that may overlap need workspaces of their own, two captured graphs among them. Outputs must
- * not overlap inputs. Any sizes and strides are taken; matrices whose row strides and addresses are multiples of 16 bytes
- * and whose widths are multiples of 8 (16-bit) or 16 (int8) elements run on the direct tile loads. Row strides stay below
- * 2^22 elements. Empty calls (M = 0) launch nothing, but gfl_ffn_backward then writes zeros to the weights' gradients. */
+ * not overlap inputs. Any sizes and strides are taken; above 16 tokens matrices whose addresses and row strides are
+ * multiples of 4 bytes run faster than others. Row strides stay below 2^22 elements. Empty calls (M = 0) launch nothing, but gfl_ffn_backward then writes zeros to the weights' gradients. */
 enum
 {
     GFL_F16 = 0,
