@@ -397,95 +397,16 @@ def grouped_rows(sel, w, take, E):
 # dense operators: the gated feed-forward block, the 8-bit integer product, sampling
 # ---------------------------------------------------------------------------------------------------------------
 
-_T = None          # torch, imported by the first call
-_CODES = {}        # torch dtype -> GFL_F16 / GFL_BF16 / GFL_F32
+_EXT = None
 
 
-def _torch():
-    global _T
-    if _T is None:
-        import torch
-        load()
-        _CODES.update({torch.float16: 0, torch.bfloat16: 1, torch.float32: 2})
-        _T = torch
-    return _T
-
-
-def _device_of(name, ref, *tensors):
-    """The index of the device that all tensors are on."""
-    dev = ref.get_device()
-    if dev < 0:
-        raise ValueError(f"{name}: tensors must be on the device")
-    for t in tensors:
-        if t is not None and t.get_device() != dev:
-            raise ValueError(f"{name}: all tensors must be on {ref.device}")
-    return dev
-
-
-def _launch(dev, fn, *args):
-    """fn(*args, stream) on device dev's current stream. The C calls launch on the current device, so another one is made
-    current for the call."""
-    T = _T
-    st = T.cuda.current_stream(dev).cuda_stream
-    if T.cuda.current_device() == dev:
-        rc = fn(*args, st)
-    else:
-        with T.cuda.device(dev):
-            rc = fn(*args, st)
-    if rc:
-        check(rc)
-
-
-def _rows(name, t, cols):
-    """t [..., cols] as rows with one stride between them: (rows, stride)."""
-    shape = t.shape
-    d = len(shape)
-    if d < 1 or shape[-1] != cols:
-        raise ValueError(f"{name} must be [..., {cols}]")
-    if t.is_contiguous():
-        return (shape[0] if d == 2 else t.numel() // cols), cols
-    if d > 2:
-        raise ValueError(f"{name} with more than two dimensions must be contiguous")
-    st = t.stride()
-    if cols > 1 and st[-1] != 1:
-        raise ValueError(f"{name} must have contiguous rows")
-    if d == 1 or shape[0] <= 1:
-        return (1 if d == 1 else shape[0]), cols
-    if st[0] < cols:
-        raise ValueError(f"{name}: rows overlap (row stride {st[0]}, width {cols})")
-    return shape[0], st[0]
-
-
-def _need(query, *args):
-    """What a *_workspace call says of its last argument but those given as None: bytes."""
-    n = C.c_size_t()
-    rc = query(*(C.byref(n) if a is _need else a for a in args))
-    if rc:
-        check(rc)
-    return n.value
-
-
-def _workspace(nbytes, ref):
-    return _T.empty(nbytes, dtype=_T.uint8, device=ref.device) if nbytes else None
-
-
-def _addr(t):
-    return None if t is None else t.data_ptr()
-
-
-def _ffn_sizes(name, x, wg, wu, wd):
-    dt, H = x.dtype, x.shape[-1] if x.dim() else 0
-    if _CODES.get(dt, 2) > 1:
-        raise ValueError(f"{name}: x must be fp16 or bf16")
-    if wg.dim() != 2 or wg.shape[1] != H or H < 1:
-        raise ValueError(f"{name}: wg must be [I, {H}]")
-    I = wg.shape[0]
-    if wu.shape != wg.shape or wd.shape != (H, I):
-        raise ValueError(f"{name}: wu must be [{I}, {H}] and wd [{H}, {I}]")
-    for t in (wg, wu, wd):
-        if t.dtype != dt or not t.is_contiguous():
-            raise ValueError(f"{name}: the weights must be contiguous, of x's type")
-    return H, I
+def _ext():
+    """The torch extension, which checks these calls' tensors, allocates and launches (csrc/torch_dense.cpp)."""
+    global _EXT
+    if _EXT is None:
+        import torch_ext
+        _EXT = torch_ext.load()
+    return _EXT
 
 
 def ffn_forward(x, wg, wu, wd, out=None, act_limit=0.0, save=False, accumulate=False):
@@ -493,145 +414,35 @@ def ffn_forward(x, wg, wu, wd, out=None, act_limit=0.0, save=False, accumulate=F
     x fp16 or bf16 [..., H] (rows may have a stride), wg and wu [I, H], wd [H, I] as nn.Linear keeps them. out: of x's type
     (the default) or fp32; accumulate (fp32 out): out += the block. save=True returns (out, g, u) with the fp32 g and u [M, I]
     that ffn_backward takes."""
-    T = _torch()
-    H, I = _ffn_sizes("ffn_forward", x, wg, wu, wd)
-    M, ldx = _rows("ffn_forward: x", x, H)
-    dev = _device_of("ffn_forward", x, wg, wu, wd, out)
-    code = _CODES[x.dtype]
-    if out is None:
-        if accumulate:
-            raise ValueError("ffn_forward: accumulate needs out")
-        out, ldo, ocode = T.empty(x.shape, dtype=x.dtype, device=x.device), H, code
-    else:
-        if out.shape != x.shape or out.dtype not in (x.dtype, T.float32):
-            raise ValueError("ffn_forward: out must have x's shape and be of its type or fp32")
-        (_, ldo), ocode = _rows("ffn_forward: out", out, H), _CODES[out.dtype]
-    g = u = None
-    if save:
-        g, u = (T.empty((M, I), dtype=T.float32, device=x.device) for _ in range(2))
-    L = _LIB
-    ws = _workspace(_need(L.gfl_ffn_workspace, code, M, H, I, _need, None), x)
-    _launch(dev, L.gfl_ffn_forward, x.data_ptr(), ldx, wg.data_ptr(), wu.data_ptr(), wd.data_ptr(), code, M, H, I, act_limit,
-            _addr(g), _addr(u), out.data_ptr(), ldo, ocode, bool(accumulate), _addr(ws), 0 if ws is None else ws.numel())
-    return (out, g, u) if save else out
+    r = (_EXT or _ext()).ffn_forward(x, wg, wu, wd, out, act_limit, save, accumulate)
+    return r if save else r[0]
 
 
 def ffn_backward(dy, x, g, u, wg, wu, wd, act_limit=0.0, need=(True, True, True, True)):
     """Gradients of the block (gfl_ffn_backward) for dy of out's shape in x's type, g and u as ffn_forward(save=True)
     returned them: (dx, dwg, dwu, dwd) in x's type, None where `need` says so."""
-    T = _torch()
-    H, I = _ffn_sizes("ffn_backward", x, wg, wu, wd)
-    if dy.shape != x.shape or dy.dtype != x.dtype:
-        raise ValueError("ffn_backward: dy must have x's shape and type")
-    M, ldx = _rows("ffn_backward: x", x, H)
-    _, ldy = _rows("ffn_backward: dy", dy, H)
-    for n, t in (("g", g), ("u", u)):
-        if tuple(t.shape) != (M, I) or t.dtype != T.float32 or not t.is_contiguous():
-            raise ValueError(f"ffn_backward: {n} must be contiguous fp32 [{M}, {I}]")
-    dev = _device_of("ffn_backward", x, dy, g, u, wg, wu, wd)
-    dx = T.empty(x.shape, dtype=x.dtype, device=x.device) if need[0] else None
-    dw = [T.empty_like(t) if n else None for t, n in zip((wg, wu, wd), need[1:])]
-    L, code = _LIB, _CODES[x.dtype]
-    ws = _workspace(_need(L.gfl_ffn_workspace, code, M, H, I, None, _need), x)
-    _launch(dev, L.gfl_ffn_backward, dy.data_ptr(), ldy, x.data_ptr(), ldx, g.data_ptr(), u.data_ptr(), wg.data_ptr(),
-            wu.data_ptr(), wd.data_ptr(), code, M, H, I, act_limit, _addr(dx), H, _addr(dw[0]), _addr(dw[1]), _addr(dw[2]),
-            _addr(ws), 0 if ws is None else ws.numel())
-    return (dx, *dw)
+    return (_EXT or _ext()).ffn_backward(dy, x, g, u, wg, wu, wd, act_limit, tuple(need))
 
 
 def quant_i8(x):
     """Rows of x (fp16 or bf16 [..., K]) to 8 bits (gfl_quant_i8): (q int8 of x's shape, scale fp32 [...])."""
-    T = _torch()
-    if _CODES.get(x.dtype, 2) > 1 or x.dim() < 1 or x.shape[-1] < 1:
-        raise ValueError("quant_i8: x must be fp16 or bf16 [..., K]")
-    K = x.shape[-1]
-    M, ldx = _rows("quant_i8: x", x, K)
-    dev = _device_of("quant_i8", x)
-    q = T.empty(x.shape, dtype=T.int8, device=x.device)
-    scale = T.empty(x.shape[:-1], dtype=T.float32, device=x.device)
-    _launch(dev, _LIB.gfl_quant_i8, x.data_ptr(), ldx, _CODES[x.dtype], M, K, q.data_ptr(), scale.data_ptr())
-    return q, scale
-
-
-def _i8_weight(name, K, b, sb):
-    if b.dtype != _T.int8 or b.dim() != 2 or b.shape[1] != K:
-        raise ValueError(f"{name}: b must be int8 [N, {K}]")
-    N, ldb = _rows(f"{name}: b", b, K)
-    if sb.dtype != _T.float32 or sb.shape != (N,) or not sb.is_contiguous():
-        raise ValueError(f"{name}: sb must be contiguous fp32 [{N}]")
-    return N, ldb
-
-
-def _i8_out(name, a, N, out, dtype):
-    shape = (*a.shape[:-1], N)
-    if out is None:
-        if dtype not in _CODES:
-            raise ValueError(f"{name}: dtype must be fp16, bf16 or fp32")
-        return _T.empty(shape, dtype=dtype, device=a.device), N
-    if dtype is not None and out.dtype != dtype:
-        raise ValueError(f"{name}: out is {out.dtype}, dtype says {dtype}")
-    if tuple(out.shape) != shape or out.dtype not in _CODES:
-        raise ValueError(f"{name}: out must be fp16, bf16 or fp32 {list(shape)}")
-    return out, _rows(f"{name}: out", out, N)[1]
+    return (_EXT or _ext()).quant_i8(x)
 
 
 def gemm_i8(a, sa, b, sb, out=None, dtype=None):
     """out[..., n] = (sum_k a[..., k] b[n, k]) * sa[...] * sb[n] (gfl_gemm_i8): a int8 [..., K] with a scale fp32 per token, b
     int8 [N, K] with one per channel. out in `dtype` (fp16 by default, bf16 or fp32)."""
-    T = _torch()
-    if a.dtype != T.int8 or a.dim() < 1 or a.shape[-1] < 1:
-        raise ValueError("gemm_i8: a must be int8 [..., K]")
-    K = a.shape[-1]
-    M, lda = _rows("gemm_i8: a", a, K)
-    if sa.dtype != T.float32 or sa.shape != a.shape[:-1] or not sa.is_contiguous():
-        raise ValueError(f"gemm_i8: sa must be contiguous fp32 {list(a.shape[:-1])}")
-    N, ldb = _i8_weight("gemm_i8", K, b, sb)
-    dev = _device_of("gemm_i8", a, sa, b, sb, out)
-    out, ldo = _i8_out("gemm_i8", a, N, out, T.float16 if dtype is None and out is None else dtype)
-    L = _LIB
-    ws = _workspace(_need(L.gfl_i8_workspace, M, N, K, _need, None), a)
-    _launch(dev, L.gfl_gemm_i8, a.data_ptr(), lda, sa.data_ptr(), b.data_ptr(), ldb, sb.data_ptr(), M, N, K, out.data_ptr(),
-            ldo, _CODES[out.dtype], _addr(ws), 0 if ws is None else ws.numel())
-    return out
+    return (_EXT or _ext()).gemm_i8(a, sa, b, sb, out, dtype)
 
 
 def linear_i8(x, b, sb, out=None, dtype=None):
     """gemm_i8 of x (fp16 or bf16 [..., K]) quantised per token as quant_i8 does (gfl_linear_i8): a linear layer with an 8-bit
     weight b [N, K] and its channels' scales sb. out in `dtype` (x's type by default)."""
-    _torch()
-    if _CODES.get(x.dtype, 2) > 1 or x.dim() < 1 or x.shape[-1] < 1:
-        raise ValueError("linear_i8: x must be fp16 or bf16 [..., K]")
-    K = x.shape[-1]
-    M, ldx = _rows("linear_i8: x", x, K)
-    N, ldb = _i8_weight("linear_i8", K, b, sb)
-    dev = _device_of("linear_i8", x, b, sb, out)
-    out, ldo = _i8_out("linear_i8", x, N, out, x.dtype if dtype is None and out is None else dtype)
-    L = _LIB
-    ws = _workspace(_need(L.gfl_i8_workspace, M, N, K, None, _need), x)
-    _launch(dev, L.gfl_linear_i8, x.data_ptr(), ldx, _CODES[x.dtype], b.data_ptr(), ldb, sb.data_ptr(), M, N, K,
-            out.data_ptr(), ldo, _CODES[out.dtype], _addr(ws), 0 if ws is None else ws.numel())
-    return out
+    return (_EXT or _ext()).linear_i8(x, b, sb, out, dtype)
 
 
 def sample(logits, u, temperature=None, top_k=None, top_p=None, min_p=None):
     """A token for each row of logits (fp32, fp16 or bf16 [B, V]) from uniform numbers u fp32 [B] (gfl_sample):
     (token int64 [B], prob fp32 [B]). temperature, top_p, min_p fp32 [B] and top_k int32 [B] on the device, None = off; a
     temperature not above 0 makes its row greedy."""
-    T = _torch()
-    if logits.dim() != 2 or logits.dtype not in _CODES or logits.shape[1] < 1:
-        raise ValueError("sample: logits must be fp32, fp16 or bf16 [B, V]")
-    B, V = logits.shape
-    _, ld = _rows("sample: logits", logits, V)
-    for n, t, dt in (("u", u, T.float32), ("temperature", temperature, T.float32), ("top_k", top_k, T.int32),
-                     ("top_p", top_p, T.float32), ("min_p", min_p, T.float32)):
-        if t is not None and (t.dtype != dt or t.shape != (B,) or not t.is_contiguous()):
-            raise ValueError(f"sample: {n} must be contiguous {dt} [{B}]")
-    dev = _device_of("sample", logits, u, temperature, top_k, top_p, min_p)
-    token = T.empty((B,), dtype=T.int64, device=logits.device)
-    prob = T.empty((B,), dtype=T.float32, device=logits.device)
-    L = _LIB
-    ws = _workspace(_need(L.gfl_sample_workspace, B, V, _need), logits)
-    _launch(dev, L.gfl_sample, logits.data_ptr(), ld, _CODES[logits.dtype], B, V, _addr(temperature), _addr(top_k),
-            _addr(top_p), _addr(min_p), u.data_ptr(), token.data_ptr(), prob.data_ptr(), _addr(ws),
-            0 if ws is None else ws.numel())
-    return token, prob
+    return (_EXT or _ext()).sample(logits, u, temperature, top_k, top_p, min_p)

@@ -78,7 +78,7 @@ def build_torch_ext(verbose=False):
     torch_lib = os.path.join(os.path.dirname(ce.__file__), "..", "lib")
     # a host-only C++ translation unit: HIP runtime and c10_hip headers/libraries named directly (no device code, no
     # source translation step)
-    ce.load(name=EXT_NAME, sources=[os.path.join(CSRC, "torch_ext.cpp")], build_directory=EXT_DIR,
+    ce.load(name=EXT_NAME, sources=[os.path.join(CSRC, f) for f in ("torch_ext.cpp", "torch_dense.cpp")], build_directory=EXT_DIR,
             extra_include_paths=[os.path.join(ROOT, "include"), os.path.join(rocm, "include")],
             extra_cflags=["-O2", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1"],
             extra_ldflags=["-L" + HERE, "-lgfl_moe", "-L" + os.path.abspath(torch_lib), "-lc10_hip",

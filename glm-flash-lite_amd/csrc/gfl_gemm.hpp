@@ -288,9 +288,8 @@ __device__ __forceinline__ void gm_put4(void* out, int odt, int64_t at, const fl
 // the block's forward epilogue for 4 neighbouring columns: h, and g and u of a training pass in fp32 (16-bit ones doubled the
 // gradients' error: 2.0 against 1.4 roundings in the root mean square; their traffic is 2% of a training step)
 template <typename E>
-__device__ __forceinline__ void gm_gate4(const GmArgs& a, int m, int n, const float (&g)[4], const float (&u)[4])
+__device__ __forceinline__ void gm_gate4(const GmArgs& a, int m, int n, const float (&g)[4], const float (&u)[4], int left)
 {
-    const int left = a.N - n;
     float h[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -518,7 +517,7 @@ __global__ __launch_bounds__(WM* WN * 64, (WM * WN + 3) / 4) void gm_kernel(GmAr
                     float w[4];
 #pragma unroll
                     for (int r = 0; r < 4; ++r) w[r] = static_cast<float>(acc[i + 1 < NI ? i + 1 : i][j][r]);
-                    gm_gate4<typename T::elem>(a, m, n, v, w);
+                    gm_gate4<typename T::elem>(a, m, n, v, w, a.N - n);
                 }
                 else if constexpr (EP == EP_DACT) gm_dact4<typename T::elem>(a, m, n, v);
                 else
@@ -558,7 +557,7 @@ __global__ __launch_bounds__(256) void gm_join_kernel(GmArgs a, const void* part
     float v[4], w[4];
 #pragma unroll
     for (int r = 0; r < 4; ++r) v[r] = static_cast<float>(s0[r]), w[r] = static_cast<float>(s1[r]);
-    if constexpr (EP == EP_GATE) gm_gate4<typename T::elem>(a, m, n, v, w);
+    if constexpr (EP == EP_GATE) gm_gate4<typename T::elem>(a, m, n, v, w, a.N - n);
     else
     {
         if constexpr (EP == EP_I8)
@@ -573,42 +572,224 @@ __global__ __launch_bounds__(256) void gm_join_kernel(GmArgs a, const void* part
     }
 }
 
-// Few tokens (M <= 16): D of 16 rows of B by a workgroup of NW waves, which take the K steps of 64 bytes a row in turn. An MFMA
-// fragment's 16 bytes a lane come straight from memory (16 rows x 64 bytes a load, U loads in flight per wave), so there is no
-// LDS staging and no barrier until the waves' partial sums meet in LDS. DUAL: 8 rows of each matrix. Bound by the weights'
-// bytes: 5120 x 1536 x 2 fp16 in one launch, against a split over workgroups whose parts a second launch joined.
-template <typename T, bool DUAL, int EP, int NW>
-__global__ __launch_bounds__(NW * 64) void gm_skinny_kernel(GmArgs a)
+// ---- few tokens (M <= 16): bound by the weights' bytes, one launch per product, no parts to join ----
+
+// Results of 4 neighbouring columns (n..n+3, the first `left` of them wanted) of token m.
+template <typename T, bool DUAL, int EP>
+__device__ __forceinline__ void gm_finish4(const GmArgs& a, int m, int n, float (&v)[4], const float (&up)[4], int left)
 {
-    constexpr int ES = sizeof(typename T::elem), U = 8;
-    typedef typename T::acc acc_t;
-    __shared__ acc_t red[NW][16][4];   // [wave][token][4 rows]
-    const int wave = threadIdx.x / 64, lane = threadIdx.x % 64, i = lane & 15, q = lane >> 4;
-    constexpr int NR = DUAL ? 8 : 16;
-    const int n0 = blockIdx.x * NR;
-    const char* w = DUAL && i >= 8 ? a.B[1] : a.B[0];
-    w += (int64_t)min(n0 + (DUAL ? i & 7 : i), a.N - 1) * a.ldb + q * 16;
-    const char* x = a.A[0] + (int64_t)min(i, a.M - 1) * a.lda + q * 16;
-    const bool live = i < a.M;
-    const int kb = a.K * ES, whole = kb / 64;   // whole steps
-    acc_t acc = { 0, 0, 0, 0 };
+    if constexpr (EP == EP_GATE) gm_gate4<typename T::elem>(a, m, n, v, up, left);
+    else
+    {
+        if constexpr (EP == EP_I8)
+        {
+            float sn[4];
+            gm_load4(a.sb + n, sn, left);
+            const float sm = a.sa[m];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[k] = v[k] * sm * sn[k];
+        }
+        gm_put4(a.out[0], a.odt, (int64_t)m * a.ldo + n, v, left, a.accumulate);
+    }
+}
+
+// sum over a fragment's 16 bytes of products
+__device__ __forceinline__ float gm_dot(GmF16, gm_i4 a, gm_i4 b, float c)
+{
+    const gm_h8 x = __builtin_bit_cast(gm_h8, a), y = __builtin_bit_cast(gm_h8, b);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) c = fmaf((float)x[i], (float)y[i], c);
+    return c;
+}
+__device__ __forceinline__ float gm_dot(GmBF16, gm_i4 a, gm_i4 b, float c)
+{
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+    {
+        c = fmaf(__int_as_float(a[i] << 16), __int_as_float(b[i] << 16), c);
+        c = fmaf(__int_as_float(a[i] & 0xFFFF0000), __int_as_float(b[i] & 0xFFFF0000), c);
+    }
+    return c;
+}
+__device__ __forceinline__ int gm_dot(GmI8, gm_i4 a, gm_i4 b, int c)
+{
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_sdot4(a[i], b[i], c, false);
+    return c;
+}
+
+// One or two tokens: a wave forms two dot products (a gate and an up row, or two neighbouring rows), 1 KB of a row a load, U
+// loads of each in flight. With the MFMA fragments of the kernels below 16 rows share a load, 64 or 128 bytes of each: 5120 x
+// 1536 fp16 gate|up, weights from HBM, 9.4 and 8.4 us against 7.9 here (4.0 TB/s with the launch; a large copy reaches 4.8).
+template <typename T, bool DUAL, int EP, int MM, int U>
+__global__ __launch_bounds__(256) void gm_row_kernel(GmArgs a)
+{
+    constexpr int ES = sizeof(typename T::elem);
+    const int lane = threadIdx.x % 64, row = (blockIdx.x * 4 + threadIdx.x / 64) * (DUAL ? 1 : 2);
+    if (row >= a.N) return;
+    const int kb = a.K * ES, whole = kb / 1024;
+    const char* w0 = a.B[0] + (int64_t)row * a.ldb + lane * 16;
+    const char* w1 = DUAL ? a.B[1] + (int64_t)row * a.ldb + lane * 16 : row + 1 < a.N ? w0 + a.ldb : w0;
+    const char* x = a.A[0] + lane * 16;
+    typename T::scalar acc[2][MM] = {};
     auto ld = [](const char* p) {
         gm_i4 v;
         __builtin_memcpy(&v, p, 16);
         return v;
     };
-    int t = wave;
-    for (; t + (U - 1) * NW < whole; t += U * NW)
+    int c = 0;
+    for (; c + U <= whole; c += U)
     {
-        gm_i4 fw[U], fx[U];
+        gm_i4 f0[U], f1[U];
 #pragma unroll
-        for (int j = 0; j < U; ++j) fw[j] = ld(w + (int64_t)(t + j * NW) * 64);
+        for (int j = 0; j < U; ++j) f0[j] = ld(w0 + (c + j) * 1024), f1[j] = ld(w1 + (c + j) * 1024);
 #pragma unroll
-        for (int j = 0; j < U; ++j) fx[j] = live ? ld(x + (int64_t)(t + j * NW) * 64) : gm_i4{ 0, 0, 0, 0 };
+        for (int j = 0; j < U; ++j)
 #pragma unroll
-        for (int j = 0; j < U; ++j) acc = T::mfma(fw[j], fx[j], acc);
+            for (int m = 0; m < MM; ++m)
+            {
+                const gm_i4 v = ld(x + m * a.lda + (c + j) * 1024);
+                acc[0][m] = gm_dot(T{}, f0[j], v, acc[0][m]);
+                acc[1][m] = gm_dot(T{}, f1[j], v, acc[1][m]);
+            }
     }
-    if (t < whole)
+    for (; c * 1024 < kb; ++c)
+    {
+        const int nb = kb - c * 1024 - lane * 16;
+        const gm_i4 f0 = gm_masked<ES>(w0 + c * 1024, nb), f1 = gm_masked<ES>(w1 + c * 1024, nb);
+#pragma unroll
+        for (int m = 0; m < MM; ++m)
+        {
+            const gm_i4 v = gm_masked<ES>(x + m * a.lda + c * 1024, nb);
+            acc[0][m] = gm_dot(T{}, f0, v, acc[0][m]);
+            acc[1][m] = gm_dot(T{}, f1, v, acc[1][m]);
+        }
+    }
+#pragma unroll
+    for (int m = 0; m < MM; ++m)
+    {
+        typename T::scalar s0 = acc[0][m], s1 = acc[1][m];
+#pragma unroll
+        for (int o = 32; o; o >>= 1) s0 += __shfl_xor(s0, o), s1 += __shfl_xor(s1, o);
+        if (lane != m) continue;
+        float v[4] = { (float)s0, DUAL ? 0.f : (float)s1, 0.f, 0.f }, up[4] = { (float)s1, 0.f, 0.f, 0.f };
+        gm_finish4<T, DUAL, EP>(a, m, row, v, up, DUAL ? 1 : min(2, a.N - row));
+    }
+}
+
+// the waves' partial 16 x 16 tiles (rows of B x tokens) joined in LDS by wave 0
+template <typename T, bool DUAL, int EP, int NW>
+__device__ __forceinline__ void gm_join_waves(const GmArgs& a, typename T::acc acc, typename T::acc (*red)[16][4], int n0)
+{
+    const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
+    red[wave][lane & 15][lane >> 4] = acc;
+    __syncthreads();
+    if (wave) return;
+    const int m = lane / 4, r = lane % 4;
+    typename T::acc sum = red[0][m][r];
+#pragma unroll
+    for (int k = 1; k < NW; ++k) sum += red[k][m][r];
+    float v[4], up[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+    {
+        v[k] = static_cast<float>(sum[k]);
+        up[k] = DUAL ? __shfl_down(v[k], 2) : 0.f;
+    }
+    const int n = n0 + r * 4;
+    if (m >= a.M || (DUAL && r >= 2) || n >= a.N) return;
+    gm_finish4<T, DUAL, EP>(a, m, n, v, up, a.N - n);
+}
+
+// 3 to 16 tokens, B's rows from 4-byte aligned addresses: 16 rows of B (DUAL: 8 of each matrix) by a workgroup of NW waves that
+// take the K steps of 128 bytes a row in turn. Each wave keeps S steps in flight, its rows in an LDS ring of its own
+// (loads of 8 rows x 128 bytes, no barrier before the join) and the tokens' fragments in registers.
+template <typename T, bool DUAL, int EP, int NW, int S>
+__global__ __launch_bounds__(NW * 64) void gm_ring_kernel(GmArgs a)
+{
+    constexpr int ES = sizeof(typename T::elem), NR = DUAL ? 8 : 16;
+    extern __shared__ __align__(16) char gm_lds[];
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / 64), lane = threadIdx.x % 64;
+    const int i = lane & 15, q = lane >> 4, n0 = blockIdx.x * NR;
+    char* ring = gm_lds + wave * S * 2048;
+    const int last = a.N - 1 - n0;   // >= 0
+    const char* base0 = gm_uniform(a.B[0] + (int64_t)n0 * a.ldb);
+    const char* base1 = DUAL ? gm_uniform(a.B[1] + (int64_t)n0 * a.ldb) : base0;
+    const int lr = lane / 8;
+    const uint32_t v0 = (uint32_t)(min(lr, last) * (int)a.ldb + (((lane & 7) ^ ((lr >> 1) & 7)) << 4));
+    const uint32_t v1 = (uint32_t)(min(DUAL ? lr : lr + 8, last) * (int)a.ldb + (((lane & 7) ^ (((lr + 8) >> 1) & 7)) << 4));
+    const char* x = a.A[0] + (int64_t)min(i, a.M - 1) * a.lda + q * 16;
+    const bool live = i < a.M;
+    const int kb = a.K * ES, steps = kb / 128;   // whole steps
+    typename T::acc acc = { 0, 0, 0, 0 };
+    gm_i4 fx[S][2];
+    auto issue = [&](int t, int s) {
+        const __amdgpu_buffer_rsrc_t r0 = gm_rsrc(base0 + (int64_t)t * 128), r1 = gm_rsrc(base1 + (int64_t)t * 128);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(r0, (gm_lds_void*)(ring + s * 2048), 16, v0, 0, 0, 0);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(r1, (gm_lds_void*)(ring + s * 2048 + 1024), 16, v1, 0, 0, 0);
+        fx[s][0] = fx[s][1] = gm_i4{ 0, 0, 0, 0 };
+        if (live)
+        {
+            __builtin_memcpy(&fx[s][0], x + (int64_t)t * 128, 16);
+            __builtin_memcpy(&fx[s][1], x + (int64_t)t * 128 + 64, 16);
+        }
+    };
+#pragma unroll
+    for (int s = 0; s < S; ++s)
+        if (wave + s * NW < steps) issue(wave + s * NW, s);
+    for (int t = wave; t < steps; t += S * NW)
+    {
+#pragma unroll
+        for (int s = 0; s < S; ++s)
+        {
+            if (t + s * NW >= steps) break;
+            // this step's loads have landed: those of the S - 1 steps after it are younger
+            if (t + (s + S - 1) * NW < steps) gm_wait_vmcnt<4 * (S - 1)>();
+            else gm_wait_vmcnt<0>();
+            gm_i4 fw[2];
+#pragma unroll
+            for (int kk = 0; kk < 2; ++kk)
+                fw[kk] = *reinterpret_cast<const gm_i4*>(ring + s * 2048 + i * 128 + (((kk * 4 + q) ^ ((i >> 1) & 7)) << 4));
+            acc = T::mfma(fw[0], fx[s][0], acc);
+            acc = T::mfma(fw[1], fx[s][1], acc);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the slot is read
+            if (t + (s + S) * NW < steps) issue(t + (s + S) * NW, s);
+        }
+    }
+    if (kb % 128 && wave == steps % NW)
+    {
+        const char* w = (DUAL && i >= 8 ? a.B[1] : a.B[0]) + (int64_t)min(n0 + (DUAL ? i & 7 : i), a.N - 1) * a.ldb + q * 16;
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk)
+        {
+            const int at = steps * 128 + kk * 64, nb = kb - at - q * 16;
+            acc = T::mfma(gm_masked<ES>(w + at, nb), gm_masked<ES>(x + at, live ? nb : 0), acc);
+        }
+    }
+    __syncthreads();   // the rings are done with
+    gm_join_waves<T, DUAL, EP, NW>(a, acc, reinterpret_cast<typename T::acc(*)[16][4]>(gm_lds), n0);
+}
+
+// The same from rows of any alignment: an MFMA fragment's 16 bytes a lane come straight from memory, U loads in flight.
+template <typename T, bool DUAL, int EP, int NW>
+__global__ __launch_bounds__(NW * 64) void gm_skinny_kernel(GmArgs a)
+{
+    constexpr int ES = sizeof(typename T::elem), U = 8;
+    __shared__ typename T::acc red[NW][16][4];   // [wave][token][4 rows]
+    const int wave = threadIdx.x / 64, lane = threadIdx.x % 64, i = lane & 15, q = lane >> 4;
+    const int n0 = blockIdx.x * (DUAL ? 8 : 16);
+    const char* w = DUAL && i >= 8 ? a.B[1] : a.B[0];
+    w += (int64_t)min(n0 + (DUAL ? i & 7 : i), a.N - 1) * a.ldb + q * 16;
+    const char* x = a.A[0] + (int64_t)min(i, a.M - 1) * a.lda + q * 16;
+    const bool live = i < a.M;
+    const int kb = a.K * ES, whole = kb / 64;   // whole steps
+    typename T::acc acc = { 0, 0, 0, 0 };
+    auto ld = [](const char* p) {
+        gm_i4 v;
+        __builtin_memcpy(&v, p, 16);
+        return v;
+    };
+    for (int t = wave; t < whole; t += U * NW)
     {
         gm_i4 fw[U], fx[U];
 #pragma unroll
@@ -626,35 +807,7 @@ __global__ __launch_bounds__(NW * 64) void gm_skinny_kernel(GmArgs a)
         const int nb = kb - whole * 64 - q * 16;
         acc = T::mfma(gm_masked<ES>(w + (int64_t)whole * 64, nb), gm_masked<ES>(x + (int64_t)whole * 64, live ? nb : 0), acc);
     }
-    red[wave][i][q] = acc;
-    __syncthreads();
-    if (wave) return;
-    const int m = lane / 4, r = lane % 4;
-    acc_t sum = red[0][m][r];
-#pragma unroll
-    for (int k = 1; k < NW; ++k) sum += red[k][m][r];
-    float v[4], up[4];
-#pragma unroll
-    for (int k = 0; k < 4; ++k)
-    {
-        v[k] = static_cast<float>(sum[k]);
-        if (DUAL) up[k] = __shfl_down(v[k], 2);
-    }
-    const int n = n0 + r * 4;
-    if (m >= a.M || (DUAL && r >= 2) || n >= a.N) return;
-    if constexpr (EP == EP_GATE) gm_gate4<typename T::elem>(a, m, n, v, up);
-    else
-    {
-        if constexpr (EP == EP_I8)
-        {
-            float sn[4];
-            gm_load4(a.sb + n, sn, a.N - n);
-            const float sm = a.sa[m];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) v[k] = v[k] * sm * sn[k];
-        }
-        gm_put4(a.out[0], a.odt, (int64_t)m * a.ldo + n, v, a.N - n, a.accumulate);
-    }
+    gm_join_waves<T, DUAL, EP, NW>(a, acc, red, n0);
 }
 
 }  // namespace gfl

@@ -37,19 +37,43 @@ static int gm_tiles(GmArgs& a, const GmPlan& p, int aligned, int nz, hipStream_t
     return gm_go<T, 256, 256, 2, 4, AKS, BKS, DUAL, 2, true, EP>(a, nz, st);
 }
 
+template <typename T, bool DUAL, int EP, int NW>
+static void gm_ring(const GmArgs& a, int wg, hipStream_t st)
+{
+    constexpr int S = 4, lds = NW * S * 2048;
+    auto* kern = gm_ring_kernel<T, DUAL, EP, NW, S>;
+    static const bool opened = hipFuncSetAttribute(reinterpret_cast<const void*>(kern),
+                                                   hipFuncAttributeMaxDynamicSharedMemorySize, lds) == hipSuccess;
+    (void)opened;
+    hipLaunchKernelGGL(kern, dim3(wg), dim3(NW * 64), lds, st, a);
+}
+
+// up to 16 tokens, B [N][K]
+template <typename T, bool DUAL, int EP>
+static int gm_few(const GmArgs& a, int aligned, hipStream_t st)
+{
+    if (a.M <= 2)
+    {
+        const int wg = (a.N + (DUAL ? 3 : 7)) / (DUAL ? 4 : 8);
+        if (a.M == 1) hipLaunchKernelGGL((gm_row_kernel<T, DUAL, EP, 1, 5>), dim3(wg), dim3(256), 0, st, a);
+        else hipLaunchKernelGGL((gm_row_kernel<T, DUAL, EP, 2, 5>), dim3(wg), dim3(256), 0, st, a);
+        return 0;
+    }
+    const int wg = (a.N + (DUAL ? 7 : 15)) / (DUAL ? 8 : 16);
+    // 16 waves where the workgroups do not fill the CUs twice and each wave still has 3 steps (192 workgroups of 5120 fp16:
+    // 8.4 us against 9.8 with 8 waves); else 8 (4096 workgroups of 4096 int8: 55 us against 63 with 4)
+    const int steps = a.K * (int)sizeof(typename T::elem) / 128;
+    if (!aligned) hipLaunchKernelGGL((gm_skinny_kernel<T, DUAL, EP, 8>), dim3(wg), dim3(512), 0, st, a);
+    else if (wg <= 256 && steps >= 48) gm_ring<T, DUAL, EP, 16>(a, wg, st);
+    else gm_ring<T, DUAL, EP, 8>(a, wg, st);
+    return 0;
+}
+
 template <typename T, bool AKS, bool BKS, bool DUAL, int EP>
 static int gm_run(int form, int ep, int aligned, GmArgs& a, void* ws, size_t ws_bytes, int nz, hipStream_t st)
 {
-    if constexpr (!AKS && !BKS && EP != EP_PART)
-        if (a.M <= 16)
-        {
-            const int per = DUAL ? 8 : 16, wg = (a.N + per - 1) / per;
-            // waves of a workgroup: enough loads in flight over the card's CUs, few workgroups taking more waves each
-            if (wg <= 768) hipLaunchKernelGGL((gm_skinny_kernel<T, DUAL, EP, 16>), dim3(wg), dim3(1024), 0, st, a);
-            else if (wg <= 2048) hipLaunchKernelGGL((gm_skinny_kernel<T, DUAL, EP, 8>), dim3(wg), dim3(512), 0, st, a);
-            else hipLaunchKernelGGL((gm_skinny_kernel<T, DUAL, EP, 4>), dim3(wg), dim3(256), 0, st, a);
-            return 0;
-        }
+    if constexpr (!AKS && !BKS)
+        if (a.M <= 16) return gm_few<T, DUAL, EP>(a, aligned, st);
     GmPlan p = gm_plan(form, ep, DUAL, aligned, a.M, a.N, a.K, a.segs);
     if (p.parts > 1 && (!ws || ws_bytes < p.part_bytes)) return -2;
     if (p.parts == 1) return gm_tiles<T, AKS, BKS, DUAL, EP>(a, p, aligned, nz, st);

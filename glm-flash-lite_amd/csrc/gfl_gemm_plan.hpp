@@ -21,7 +21,7 @@ inline GmPlan gm_plan(int form, int ep, int dual, int aligned, int M, int N, int
     const int64_t cu = 256;
     auto tiles = [&](int64_t tm, int64_t tn) { return ((M + tm - 1) / tm) * ((N + tn - 1) / tn); };
     const int d = dual ? 2 : 1;
-    if (M <= 16 && form == GM_NT)   // gm_skinny_kernel
+    if (M <= 16 && form == GM_NT)   // the kernels for few tokens
     {
         p.tm = 16, p.tn = 16 / d, p.parts = 1, p.ldp = 0, p.part_bytes = 0;
         return p;

@@ -332,21 +332,40 @@ static size_t sm_carve(void* base, int B, int V, SmWs& w)
     return (size_t)(p - static_cast<char*>(base));
 }
 
-// use(index, key) for this thread's logits of [lo, hi): 4 neighbours at a time
-template <typename E, int NT, typename F>
-__device__ __forceinline__ void sm_each(const E* row, int lo, int hi, F&& use)
+// use(index, key) for this thread's logits of [lo, hi): 4 neighbours at a time, 4 loads in flight (`first`: the first 4, loaded
+// ahead of what the launch waits for otherwise)
+template <typename E, int NT>
+struct SmBatch
 {
     typedef E vec __attribute__((ext_vector_type(4)));
-    int i = lo + (int)threadIdx.x * 4;
-#pragma unroll 4
-    for (; i + 4 <= hi; i += NT * 4)
+    vec v[4];
+    __device__ __forceinline__ void load(const E* row, int i, int hi)
     {
-        vec v;
-        __builtin_memcpy(&v, row + i, sizeof(v));
 #pragma unroll
-        for (int j = 0; j < 4; ++j) use(i + j, sm_key(static_cast<float>(v[j])));
+        for (int j = 0; j < 4; ++j)
+            if (i + j * NT * 4 + 4 <= hi) __builtin_memcpy(&v[j], row + i + j * NT * 4, sizeof(vec));
     }
-    for (; i < hi; ++i) use(i, sm_key(static_cast<float>(row[i])));   // the slice's last, not whole, chunk: one thread's
+};
+template <typename E, int NT, typename F>
+__device__ __forceinline__ void sm_each(const E* row, int lo, int hi, SmBatch<E, NT> b, F&& use)
+{
+    for (int i = lo + (int)threadIdx.x * 4; i < hi;)
+    {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+        {
+            const int at = i + j * NT * 4;
+            if (at + 4 <= hi)
+            {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) use(at + k, sm_key(static_cast<float>(b.v[j][k])));
+            }
+            else
+                for (int k = at; k < hi; ++k) use(k, sm_key(static_cast<float>(row[k])));   // the slice's last, not whole, chunk
+        }
+        i += 4 * NT * 4;
+        b.load(row, i, hi);
+    }
 }
 
 // what every launch after the first knows of a row
@@ -410,9 +429,11 @@ __global__ __launch_bounds__(SM_PT) void sm_top_kernel(SampleArgs a, SmWs w)
         w.mass[(size_t)b * SM_BINS + i] = 0;
     }
     if (s == 0 && threadIdx.x == 0) w.state[b].count = 0;
+    SmBatch<E, SM_PT> first;
+    first.load(row, lo + threadIdx.x * 4, hi);
     uint32_t top = 0, low = ~0u;
     int arg = 0x7FFFFFFF;
-    sm_each<E, SM_PT>(row, lo, hi, [&](int i, uint32_t k) {
+    sm_each<E, SM_PT>(row, lo, hi, first, [&](int i, uint32_t k) {
         if (k > top) top = k, arg = i;
         if (k > SM_MASKED) low = min(low, k);
     });
@@ -460,23 +481,25 @@ __global__ __launch_bounds__(SM_PT) void sm_bins_kernel(SampleArgs a, SmWs w)
     __shared__ uint32_t cnt[SM_BINS];
     __shared__ unsigned long long mass[SM_BINS];
     const int b = blockIdx.y, s = blockIdx.x, lo = s * w.len, hi = min(a.V, lo + w.len);
+    const E* row = static_cast<const E*>(a.logits) + (int64_t)b * a.ld;
+    SmBatch<E, SM_PT> first;
+    first.load(row, lo + threadIdx.x * 4, hi);
     const SmHead h = sm_head(a, w, b);
     const int k = sm_topk(a, b);
     const bool p = sm_topp(a, b) < 1.0f;
     if (h.done || h.wide || (!k && !p)) return;
     const bool weigh = p && (!k || k > SM_LISTK);   // a small top-k's list gives its weights itself
-    const E* row = static_cast<const E*>(a.logits) + (int64_t)b * a.ld;
     for (int i = threadIdx.x; i < SM_BINS; i += SM_PT) cnt[i] = 0, mass[i] = 0;
     __syncthreads();
     if (weigh)
-        sm_each<E, SM_PT>(row, lo, hi, [&](int, uint32_t key) {
+        sm_each<E, SM_PT>(row, lo, hi, first, [&](int, uint32_t key) {
             if (key <= SM_MASKED) return;
             const int bin = h.bin(key);
             atomicAdd(&cnt[bin], 1u);
             if (bin < SM_BINS - 1) atomicAdd(&mass[bin], (unsigned long long)sm_weight(key, h.top, h.scale));
         });
     else
-        sm_each<E, SM_PT>(row, lo, hi, [&](int, uint32_t key) {
+        sm_each<E, SM_PT>(row, lo, hi, first, [&](int, uint32_t key) {
             if (key > SM_MASKED) atomicAdd(&cnt[h.bin(key)], 1u);
         });
     __syncthreads();
@@ -590,6 +613,9 @@ __global__ __launch_bounds__(SM_PT) void sm_cut_kernel(SampleArgs a, SmWs w)
     __shared__ unsigned long long scratch[SM_PT / 64 + 1];
     __shared__ int found[2];
     const int b = blockIdx.y, s = blockIdx.x, lo = s * w.len, hi = min(a.V, lo + w.len);
+    const E* row = static_cast<const E*>(a.logits) + (int64_t)b * a.ld;
+    SmBatch<E, SM_PT> first;
+    first.load(row, lo + threadIdx.x * 4, hi);
     const SmHead h = sm_head(a, w, b);
     if (h.done) return;
     const SmCut c = sm_cut(a, w, b, h, scratch, found);
@@ -600,7 +626,6 @@ __global__ __launch_bounds__(SM_PT) void sm_cut_kernel(SampleArgs a, SmWs w)
         w.state[b].above = c.above;
     }
     if (c.mode == SM_SLOW) return;
-    const E* row = static_cast<const E*>(a.logits) + (int64_t)b * a.ld;
     unsigned long long* list = w.list + (size_t)b * SM_LIST;
     auto put = [&](int i, uint32_t key) {
         const int at = atomicAdd(&w.state[b].count, 1);
@@ -608,7 +633,7 @@ __global__ __launch_bounds__(SM_PT) void sm_cut_kernel(SampleArgs a, SmWs w)
     };
     if (c.mode == SM_TOPK)
     {
-        sm_each<E, SM_PT>(row, lo, hi, [&](int i, uint32_t key) {
+        sm_each<E, SM_PT>(row, lo, hi, first, [&](int i, uint32_t key) {
             if (key > SM_MASKED && h.bin(key) <= c.bin) put(i, key);
         });
         return;
@@ -616,7 +641,7 @@ __global__ __launch_bounds__(SM_PT) void sm_cut_kernel(SampleArgs a, SmWs w)
     const float mp = a.min_p ? a.min_p[b] : 0.0f;
     const double m = mp > 0.0f ? (double)mp : 0.0;
     unsigned long long mine = 0, total;
-    sm_each<E, SM_PT>(row, lo, hi, [&](int i, uint32_t key) {
+    sm_each<E, SM_PT>(row, lo, hi, first, [&](int i, uint32_t key) {
         if (key <= SM_MASKED) return;
         const int bin = c.mode == SM_ALL ? 0 : h.bin(key);
         if (bin > c.bin) return;
@@ -631,19 +656,22 @@ __global__ __launch_bounds__(SM_PT) void sm_cut_kernel(SampleArgs a, SmWs w)
     if (threadIdx.x == 0) w.slice[(size_t)b * w.S + s].mass = total;
 }
 
-// descending bitonic sort of n (a power of two) entries in LDS
+// descending bitonic sort of n (a power of two) entries in LDS. A wave's 64 exchanges over distances up to 64 stay within
+// its own 128 entries, so only the longer ones need a barrier.
 __device__ __forceinline__ void sm_sort(unsigned long long* v, int n)
 {
+    __syncthreads();
     for (int k = 2; k <= n; k <<= 1)
         for (int j = k >> 1; j; j >>= 1)
         {
-            __syncthreads();
             for (int t = threadIdx.x; t < n / 2; t += SM_T)
             {
                 const int i = 2 * t - (t & (j - 1)), l = i + j;
                 const unsigned long long x = v[i], y = v[l];
                 if ((x < y) == ((i & k) == 0)) v[i] = y, v[l] = x;
             }
+            if (j > 64 || (j == 1 && k >= 128)) __syncthreads();
+            else asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         }
     __syncthreads();
 }
@@ -664,6 +692,13 @@ __global__ __launch_bounds__(SM_T) void sm_pick_kernel(SampleArgs a, SmWs w)
         } f;
     } sh;
     const int b = blockIdx.x, V = a.V;
+    // loaded ahead of the head: the list's entries of this thread (those past its end are not used) and a slice's weight
+    const unsigned long long* list = w.list + (size_t)b * SM_LIST;
+    unsigned long long entry[SM_LIST / SM_T], slice_mass = 0;
+#pragma unroll
+    for (int j = 0; j < SM_LIST / SM_T; ++j) entry[j] = list[threadIdx.x + j * SM_T];
+    if ((int)threadIdx.x < w.S) slice_mass = w.slice[(size_t)b * w.S + threadIdx.x].mass;
+    const SmState st = w.state[b];
     const SmHead h = sm_head(a, w, b);
     if (h.done)
     {
@@ -675,7 +710,6 @@ __global__ __launch_bounds__(SM_T) void sm_pick_kernel(SampleArgs a, SmWs w)
         }
         return;
     }
-    const SmState st = w.state[b];
     const E* rowp = static_cast<const E*>(a.logits) + (int64_t)b * a.ld;
     if (st.mode == SM_SLOW)
     {
@@ -697,8 +731,12 @@ __global__ __launch_bounds__(SM_T) void sm_pick_kernel(SampleArgs a, SmWs w)
     if (threadIdx.x == 0) f.n = n, f.pick = -1;
     if (n)
     {
-        const unsigned long long* list = w.list + (size_t)b * SM_LIST;
-        for (int i = threadIdx.x; i < pow2; i += SM_T) f.list[i] = i < n ? list[i] : 0;
+#pragma unroll
+        for (int j = 0; j < SM_LIST / SM_T; ++j)
+        {
+            const int i = threadIdx.x + j * SM_T;
+            if (i < pow2) f.list[i] = i < n ? entry[j] : 0;
+        }
         sm_sort(f.list, pow2);
     }
     else __syncthreads();
@@ -789,7 +827,7 @@ __global__ __launch_bounds__(SM_T) void sm_pick_kernel(SampleArgs a, SmWs w)
         return;
     }
     // from the slices: their weight above the bin and that of the list's kept entries
-    for (int s = threadIdx.x; s < w.S; s += SM_T) f.part[s] = w.slice[(size_t)b * w.S + s].mass;
+    if ((int)threadIdx.x < w.S) f.part[threadIdx.x] = slice_mass;
     __syncthreads();
     for (int i = threadIdx.x; i < kept; i += SM_T)
     {

@@ -338,8 +338,11 @@ std::tuple<bool, bool, double, int64_t> tier_state()
     return { true, T->running, double(g_act_limit), n };
 }
 
+void bind_dense(pybind11::module& m);   // torch_dense.cpp
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
 {
+    bind_dense(m);
     m.def("tier_init", &tier_init);
     m.def("tier_add_layer", &tier_add_layer, pybind11::arg("li"), pybind11::arg("ptrs"), pybind11::arg("suh_g"),
           pybind11::arg("svh_g"), pybind11::arg("suh_u"), pybind11::arg("svh_u"), pybind11::arg("suh_d"),
