@@ -50,7 +50,12 @@ FfnSizes ffn_sizes(int M, int H, int I, bool backward)
     // aligned and other operands may be split differently: room for both
     for (int al = 0; al < 2; ++al)
     {
-        if (!backward)
+        if (backward)
+        {
+            z.part = std::max(z.part, gfl::gm_plan(gfl::GM_NN, gfl::EP_DACT, 0, al, M, I, H, 1).part_bytes);
+            z.part = std::max(z.part, gfl::gm_plan(gfl::GM_NN, gfl::EP_OUT, 0, al, M, H, I, 2).part_bytes);
+        }
+        else
         {
             z.part = std::max(z.part, gfl::gm_plan(gfl::GM_NT, gfl::EP_GATE, 1, al, M, I, H, 1).part_bytes);
             z.part = std::max(z.part, gfl::gm_plan(gfl::GM_NT, gfl::EP_OUT, 0, al, M, H, I, 1).part_bytes);
@@ -143,7 +148,7 @@ int gfl_ffn_backward(const void* dy, int64_t lddy, const void* x, int64_t ldx, c
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     if (!dx && !dwg && !dwu && !dwd) return GFL_OK;
     const FfnSizes z = ffn_sizes(std::max(M, 1), H, I, true);
-    char *dg = static_cast<char*>(ws), *du = dg + z.h, *h = du + z.h;
+    char *dg = static_cast<char*>(ws), *du = dg + z.h, *h = du + z.h, *part = h + z.h;
     if (M > 0)
     {
         if (!dy || !x || !g || !u || !wg || !wu || !wd) return api_fail(GFL_EINVAL, "gfl_ffn_backward: NULL argument");
@@ -164,7 +169,7 @@ int gfl_ffn_backward(const void* dy, int64_t lddy, const void* x, int64_t ldx, c
         a.g = const_cast<float*>(g); a.u = const_cast<float*>(u); a.ldg = I;
         const int al = words(dy, a.lda) && words(wd, a.ldb);
         a.ragged = H % 8 != 0 || I % 8 != 0;
-        if (int rc = gemm16("gfl_ffn_backward: dh", dtype, gfl::GM_NN, gfl::EP_DACT, 0, al, a, nullptr, 0, 1, st)) return rc;
+        if (int rc = gemm16("gfl_ffn_backward: dh", dtype, gfl::GM_NN, gfl::EP_DACT, 0, al, a, part, z.part, 1, st)) return rc;
         if (dx)
         {
             gfl::GmArgs b;   // dx = dg Wg + du Wu
@@ -179,7 +184,7 @@ int gfl_ffn_backward(const void* dy, int64_t lddy, const void* x, int64_t ldx, c
             b.odt = dtype;
             const int bl = words(wg, b.ldb) && words(wu, b.ldb);
             b.ragged = H % 8 != 0 || I % 8 != 0;
-            if (int rc = gemm16("gfl_ffn_backward: dx", dtype, gfl::GM_NN, gfl::EP_OUT, 0, bl, b, nullptr, 0, 1, st)) return rc;
+            if (int rc = gemm16("gfl_ffn_backward: dx", dtype, gfl::GM_NN, gfl::EP_OUT, 0, bl, b, part, z.part, 1, st)) return rc;
         }
     }
     // the weights' gradients: [dg | du]^T x and dy^T h (zeros at M = 0: no K step)

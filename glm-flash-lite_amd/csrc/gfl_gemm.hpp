@@ -310,14 +310,12 @@ __device__ __forceinline__ void gm_gate4(const GmArgs& a, int m, int n, const fl
     }
 }
 
-// dh -> dg = dh * clamp(u) * [silu(g) <= L] * silu'(g), du = dh * min(silu(g), L) * [|u| <= L], h
+// dh -> dg = dh * clamp(u) * [silu(g) <= L] * silu'(g), du = dh * min(silu(g), L) * [|u| <= L], h, for 4 neighbouring columns
 template <typename E>
-__device__ __forceinline__ void gm_dact4(const GmArgs& a, int m, int n, const float (&dh)[4])
+__device__ __forceinline__ void gm_dact4(const GmArgs& a, int m, int n, const float (&dh)[4], const float (&g)[4],
+                                         const float (&u)[4], int left)
 {
-    const int left = a.N - n;
-    float g[4], u[4], dg[4], du[4], h[4];
-    gm_load4(a.g + (int64_t)m * a.ldg + n, g, left);
-    gm_load4(a.u + (int64_t)m * a.ldg + n, u, left);
+    float dg[4], du[4], h[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i)
     {
@@ -340,14 +338,17 @@ __device__ __forceinline__ void gm_dact4(const GmArgs& a, int m, int n, const fl
     gm_store4(static_cast<E*>(a.out[0]) + at, h, left);
 }
 
-// Tile of a workgroup: consecutive workgroups go to the 8 XCDs in turn, each XCD takes a run of neighbouring tiles, in
-// groups of GM_GROUP tile rows, so that the tiles an XCD's CUs work on at once share their operands in its L2.
+// Work of a workgroup: consecutive workgroups go to the 8 XCDs in turn, and each XCD takes a run of neighbouring work, K parts
+// first (a part's slice of the operands then stays in one XCD's L2), then tiles in groups of GM_GROUP tile rows, so that the
+// tiles that an XCD's CUs work on at once share their operands.
 constexpr int GM_GROUP = 4;
-__device__ __forceinline__ void gm_tile(int b, int tm, int tn, int& im, int& in)
+__device__ __forceinline__ void gm_tile(int b, int tm, int tn, int parts, int& part, int& im, int& in)
 {
-    const int total = tm * tn, per = total / 8, extra = total % 8;
+    const int tiles = tm * tn, total = tiles * parts, per = total / 8, extra = total % 8;
     const int x = b % 8, s = b / 8;
-    const int p = x * per + min(x, extra) + s;
+    int p = x * per + min(x, extra) + s;
+    part = p / tiles;
+    p -= part * tiles;
     const int wide = GM_GROUP * tn, grp = p / wide, first = grp * GM_GROUP;
     const int rows = min(GM_GROUP, tm - first), r = p - grp * wide;
     im = first + r % rows;
@@ -368,8 +369,8 @@ __global__ __launch_bounds__(WM* WN * 64, (WM * WN + 3) / 4) void gm_kernel(GmAr
 
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / 64), lane = threadIdx.x % 64;
     const int wm = wave / WN, wn = wave % WN;
-    int im, in;
-    gm_tile(blockIdx.x, a.tm, a.tn, im, in);
+    int part, im, in;
+    gm_tile(blockIdx.x, a.tm, a.tn, a.parts, part, im, in);
     constexpr int TNC = DUAL ? TN / 2 : TN;   // columns of a tile
     const int m0 = im * TM, n0 = in * TNC;
     const int z = blockIdx.z;
@@ -379,15 +380,16 @@ __global__ __launch_bounds__(WM* WN * 64, (WM * WN + 3) / 4) void gm_kernel(GmAr
     int t0 = 0, t1 = steps1 * a.segs;
     if (a.parts > 1)
     {
-        t0 = (int)((int64_t)steps1 * blockIdx.y / a.parts);
-        t1 = (int)((int64_t)steps1 * (blockIdx.y + 1) / a.parts);
+        t0 = (int)((int64_t)t1 * part / a.parts);
+        t1 = (int)((int64_t)t1 * (part + 1) / a.parts);
     }
     SA sa;
     SB sb;
-    sa.init(wave, lane, a.A[z], a.A[z], a.lda, m0, a.M);
-    sb.init(wave, lane, DUAL ? a.B[0] : a.B[z], a.B[1], a.ldb, n0, a.N);
-    sa.advance(t0);
-    sb.advance(t0);
+    const int seg0 = t0 >= steps1 && a.segs > 1 ? 1 : 0;   // the segment that the part starts in (z: one segment)
+    sa.init(wave, lane, a.A[z + seg0], nullptr, a.lda, m0, a.M);
+    sb.init(wave, lane, DUAL ? a.B[0] : a.B[z + seg0], a.B[1], a.ldb, n0, a.N);
+    sa.advance(t0 - seg0 * steps1);
+    sb.advance(t0 - seg0 * steps1);
     // the step whose loads are issued next
     int ti = t0;
     auto rem_of = [&](int t) { return a.K - (t < steps1 ? t : t - steps1) * BK; };
@@ -489,6 +491,48 @@ __global__ __launch_bounds__(WM* WN * 64, (WM * WN + 3) / 4) void gm_kernel(GmAr
     }
 
     const int i16 = lane & 15, q = lane >> 4;
+    if constexpr (EP == EP_DACT)
+    {
+        // g and u of a tile row's fragments are loaded together, and the next row's under this one's arithmetic (clamped into
+        // the matrix): one by one they cost 15 us of a 50 us launch (333 x 5504)
+        const bool quads = a.N % 4 == 0;   // then 4 neighbouring columns are all inside or all outside
+        const int nw = n0 + wn * (TNC / WN) + q * 4;
+        gm_f4 g[2][NI], u[2][NI];
+        auto fetch = [&](int j, int s) {
+            const int64_t row = (int64_t)min(m0 + wm * (TM / WM) + j * 16 + i16, a.M - 1) * a.ldg;
+#pragma unroll
+            for (int i = 0; i < NI; ++i)
+            {
+                const int64_t at = row + min(nw + i * 16, a.N - 4);
+                g[s][i] = *reinterpret_cast<const gm_f4*>(a.g + at);
+                u[s][i] = *reinterpret_cast<const gm_f4*>(a.u + at);
+            }
+        };
+        if (quads) fetch(0, 0);
+#pragma unroll
+        for (int j = 0; j < MI; ++j)
+        {
+            if (quads && j + 1 < MI) fetch(j + 1, (j + 1) & 1);
+            const int m = m0 + wm * (TM / WM) + j * 16 + i16;
+            if (m >= a.M) continue;
+#pragma unroll
+            for (int i = 0; i < NI; ++i)
+            {
+                const int n = nw + i * 16;
+                if (n >= a.N) continue;
+                float v[4], gv[4], uv[4];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) v[r] = static_cast<float>(acc[i][j][r]), gv[r] = g[j & 1][i][r], uv[r] = u[j & 1][i][r];
+                if (!quads)
+                {
+                    gm_load4(a.g + (int64_t)m * a.ldg + n, gv, a.N - n);
+                    gm_load4(a.u + (int64_t)m * a.ldg + n, uv, a.N - n);
+                }
+                gm_dact4<typename T::elem>(a, m, n, v, gv, uv, a.N - n);
+            }
+        }
+        return;
+    }
 #pragma unroll
     for (int j = 0; j < MI; ++j)
     {
@@ -502,7 +546,7 @@ __global__ __launch_bounds__(WM* WN * 64, (WM * WN + 3) / 4) void gm_kernel(GmAr
             if constexpr (EP == EP_PART)
             {
                 typename T::scalar* p = static_cast<typename T::scalar*>(a.out[0]) +
-                                        ((int64_t)blockIdx.y * (DUAL ? 2 : 1) * a.M + m) * a.ldo + n;
+                                        ((int64_t)part * (DUAL ? 2 : 1) * a.M + m) * a.ldo + n;
                 // ldo is a multiple of 4 and rows are padded to it: whole vectors
                 *reinterpret_cast<typename T::acc*>(p) = acc[i][j];
                 if (DUAL) *reinterpret_cast<typename T::acc*>(p + (int64_t)a.M * a.ldo) = acc[i + 1 < NI ? i + 1 : i][j];
@@ -519,7 +563,6 @@ __global__ __launch_bounds__(WM* WN * 64, (WM * WN + 3) / 4) void gm_kernel(GmAr
                     for (int r = 0; r < 4; ++r) w[r] = static_cast<float>(acc[i + 1 < NI ? i + 1 : i][j][r]);
                     gm_gate4<typename T::elem>(a, m, n, v, w, a.N - n);
                 }
-                else if constexpr (EP == EP_DACT) gm_dact4<typename T::elem>(a, m, n, v);
                 else
                 {
                     if constexpr (EP == EP_I8)
@@ -558,6 +601,13 @@ __global__ __launch_bounds__(256) void gm_join_kernel(GmArgs a, const void* part
 #pragma unroll
     for (int r = 0; r < 4; ++r) v[r] = static_cast<float>(s0[r]), w[r] = static_cast<float>(s1[r]);
     if constexpr (EP == EP_GATE) gm_gate4<typename T::elem>(a, m, n, v, w, a.N - n);
+    else if constexpr (EP == EP_DACT)
+    {
+        float g[4], u[4];
+        gm_load4(a.g + (int64_t)m * a.ldg + n, g, a.N - n);
+        gm_load4(a.u + (int64_t)m * a.ldg + n, u, a.N - n);
+        gm_dact4<typename T::elem>(a, m, n, v, g, u, a.N - n);
+    }
     else
     {
         if constexpr (EP == EP_I8)

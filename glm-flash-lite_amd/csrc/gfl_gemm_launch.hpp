@@ -14,7 +14,7 @@ static int gm_go(const GmArgs& a, int nz, hipStream_t st)
     static const bool opened = hipFuncSetAttribute(reinterpret_cast<const void*>(kern),
                                                    hipFuncAttributeMaxDynamicSharedMemorySize, lds) == hipSuccess;
     (void)opened;
-    hipLaunchKernelGGL(kern, dim3((unsigned)(a.tm * a.tn), a.parts, nz), dim3(WM * WN * 64), lds, st, a);
+    hipLaunchKernelGGL(kern, dim3((unsigned)(a.tm * a.tn * a.parts), 1, nz), dim3(WM * WN * 64), lds, st, a);
     return 0;
 }
 
@@ -32,7 +32,11 @@ static int gm_tiles(GmArgs& a, const GmPlan& p, int aligned, int nz, hipStream_t
     }
     if constexpr (BKS && !AKS)
         if (p.tm == 16) return gm_go<T, 16, 128, 1, 4, AKS, BKS, DUAL, 4, true, EP>(a, nz, st);
-    if (p.tm == 64) return gm_go<T, 64, 128, 1, 4, AKS, BKS, DUAL, 3, true, EP>(a, nz, st);
+    if constexpr (!AKS)
+    {
+        if (p.tm == 64) return gm_go<T, 64, 128, 1, 4, AKS, BKS, DUAL, 3, true, EP>(a, nz, st);
+        if (p.deep) return gm_go<T, 128, 128, 2, 4, AKS, BKS, DUAL, 4, true, EP>(a, nz, st);
+    }
     if (p.tm == 128) return gm_go<T, 128, 128, 2, 2, AKS, BKS, DUAL, 2, true, EP>(a, nz, st);
     return gm_go<T, 256, 256, 2, 4, AKS, BKS, DUAL, 2, true, EP>(a, nz, st);
 }
@@ -77,7 +81,7 @@ static int gm_run(int form, int ep, int aligned, GmArgs& a, void* ws, size_t ws_
     GmPlan p = gm_plan(form, ep, DUAL, aligned, a.M, a.N, a.K, a.segs);
     if (p.parts > 1 && (!ws || ws_bytes < p.part_bytes)) return -2;
     if (p.parts == 1) return gm_tiles<T, AKS, BKS, DUAL, EP>(a, p, aligned, nz, st);
-    if constexpr (EP == EP_DACT || AKS) return -1;   // never split (gm_plan)
+    if constexpr (AKS) return -1;   // never split (gm_plan)
     else
     {
         GmArgs b = a;
