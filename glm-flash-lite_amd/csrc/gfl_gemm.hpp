@@ -1,12 +1,12 @@
 // The tile GEMM of the dense operators (gated feed-forward block and its gradients, 8-bit integer product):
 //   D[m][n] = sum_k A(m, k) * B(n, k), in fp32 (f16, bf16 inputs) or int32 (i8).
 //
-// A workgroup of WM x WN waves forms a TM x TN tile over K steps of 128 bytes a row (64 16-bit elements, 128 bytes of
-// i8). Each operand is stored either with K contiguous ("KC": [rows][K], as activations and nn.Linear weights are) or
+// A workgroup of WM x WN waves forms a TM x TN tile over K steps of SB = 128 or 64 bytes a row (128: 64 16-bit elements, 128
+// of i8). Each operand is stored either with K contiguous ("KC": [rows][K], as activations and nn.Linear weights are) or
 // with K as the rows ("KS": [K][cols], the transposed products of the gradients):
-//   KC tiles lie in LDS as [rows][8 chunks of 16 bytes], chunk c of row r at place c ^ ((r >> 1) & 7); a fragment is one
-//   ds_read_b128 per lane;
-//   KS tiles (16-bit types) lie as [64 k][cols], chunk c of row k at place c ^ ks_swz(k); a fragment is two
+//   KC tiles lie in LDS as [rows][SB / 16 chunks of 16 bytes], chunk c of row r at place c ^ kc_swz(r), which spreads 16
+//   neighbouring rows over all banks; a fragment is one ds_read_b128 per lane;
+//   KS tiles (16-bit types) lie as [k][cols], chunk c of row k at place c ^ ks_swz(k); a fragment is two
 //   ds_read_b64_tr_b16, which hand lane i of each 16 the 4 k values of column i.
 // MFMA operands are (B rows, A rows), so that a lane's 4 accumulators are 4 neighbouring n of one m: vector stores.
 //
@@ -17,6 +17,9 @@
 // columns that are not stored. AL = 0 takes any strides and alignment: every chunk goes through registers.
 #pragma once
 #include "gfl_internal.hpp"
+
+#include <type_traits>
+#include <utility>
 
 namespace gfl {
 
@@ -37,6 +40,10 @@ struct GmF16
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(gm_h8, a), __builtin_bit_cast(gm_h8, b), c, 0, 0,
                                                       0);
     }
+    static __device__ __forceinline__ void mfma_agpr(gm_i4 a, gm_i4 b, acc& c)
+    {
+        asm volatile("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+    }
 };
 struct GmBF16
 {
@@ -48,6 +55,10 @@ struct GmBF16
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(gm_b8, a), __builtin_bit_cast(gm_b8, b), c, 0,
                                                        0, 0);
     }
+    static __device__ __forceinline__ void mfma_agpr(gm_i4 a, gm_i4 b, acc& c)
+    {
+        asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+    }
 };
 struct GmI8
 {
@@ -57,6 +68,10 @@ struct GmI8
     static __device__ __forceinline__ acc mfma(gm_i4 a, gm_i4 b, acc c)
     {
         return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ void mfma_agpr(gm_i4 a, gm_i4 b, acc& c)
+    {
+        asm volatile("v_mfma_i32_16x16x64_i8 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
     }
 };
 
@@ -76,10 +91,24 @@ __device__ __forceinline__ const char* gm_uniform(const char* p)
     return reinterpret_cast<const char*>(((uint64_t)hi << 32) | lo);
 }
 
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t gm_rsrc(const char* p)
+// buffer descriptor of 2 GiB from p on (uniform)
+__device__ __forceinline__ gm_i4 gm_rsrc(const char* p, int bytes = 0x7FFFFFFF)
 {
-    return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(p), (short)0, 0x7FFFFFFF, 0x00020000);
+    const uint64_t v = reinterpret_cast<uint64_t>(p);
+    return gm_i4{ __builtin_amdgcn_readfirstlane((int)(uint32_t)v), __builtin_amdgcn_readfirstlane((int)(uint32_t)(v >> 32) & 0xFFFF),
+                  __builtin_amdgcn_readfirstlane(bytes), 0x00020000 };
 }
+// LDS-direct load: lane l's 16 bytes at byte offset v of the buffer go to LDS address lds + 16 l (lds the same for the wave). In asm, because
+// after the builtin the compiler waits for all outstanding loads before each ds_read_b64_tr (it takes that builtin for a possible
+// write to the loads' LDS), which leaves nothing in flight; it holds no result register, and the waits for it are explicit
+// everywhere. An s_nop between the write of M0 and its use.
+__device__ __forceinline__ int gm_lds_at(char* lds) { return (int)(uint32_t)reinterpret_cast<uintptr_t>((gm_lds_void*)lds); }
+__device__ __forceinline__ void gm_load_lds(gm_i4 r, int lds, uint32_t v)
+{
+    const int at = __builtin_amdgcn_readfirstlane(lds);
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(at), "v"(v), "s"(r) : "memory");
+}
+
 constexpr uint32_t GM_OUT = 0x80000000u;   // a lane offset past every buffer: reads as zero
 
 // the 16 bytes at p of which the first nb (a multiple of ES, at most 16; may be <= 0) exist; the rest is zero
@@ -106,24 +135,28 @@ __device__ __forceinline__ gm_i4 gm_masked(const char* p, int nb)
     return r;
 }
 
+template <int CH>
+__device__ __forceinline__ int gm_kc_swz(int r)
+{
+    return CH == 8 ? (r >> 1) & 7 : (r >> 2) & 3;
+}
 __device__ __forceinline__ int gm_ks_swz(int k, int chunks) { return (2 * ((k & 3) | ((k >> 1) & 4))) & (chunks - 1); }
 
 // One operand of a tile: R rows (KC) or columns (KS) from r0 on of a matrix with `rows` of them.
 // p points at the tile's first k; advance by step() bytes per K step.
-template <typename T, int R, bool KS, bool DUAL, int NW>
+template <typename T, int R, bool KS, bool DUAL, int NW, int SB = 128>
 struct GmSide
 {
     static constexpr int ES = sizeof(typename T::elem);
-    static constexpr int BK = 128 / ES;                  // elements per K step
-    static constexpr int CH = KS ? R * ES / 16 : 8;      // chunks of 16 bytes per LDS row
+    static constexpr int BK = SB / ES;                   // elements per K step
+    static constexpr int CH = KS ? R * ES / 16 : SB / 16;   // chunks of 16 bytes per LDS row
     static constexpr int LROWS = 64 / CH;                // LDS rows per load of a wave
-    static constexpr int NI = R * 128 / 1024;            // wave loads per K step
+    static constexpr int NI = R * SB / 1024;             // wave loads per K step
     static constexpr int NV = (NI + NW - 1) / NW;        // per wave (waves past NI repeat others' loads)
-    static constexpr int BYTES = R * 128;
+    static constexpr int BYTES = R * SB;
     static_assert(CH <= 64, "an LDS row is at most one wave load");
 
-    int lrow[NV], chunk[NV];                             // this lane's LDS row and source chunk
-    uint32_t voff[NV];                                   // AL: byte offset from the base
+    uint32_t voff[NV];                                   // AL: this lane's byte offset from the base in load j
     const char* p0;
     const char* p1;                                      // DUAL: the second matrix (rows 16..31 of every 32)
     int64_t ld;
@@ -138,65 +171,66 @@ struct GmSide
 #pragma unroll
         for (int j = 0; j < NV; ++j)
         {
-            const int ii = (wave + NW * j) % NI;
-            const int r = ii * LROWS + lane / CH;
-            lrow[j] = r;
-            chunk[j] = KS ? (lane % CH) ^ gm_ks_swz(r, CH) : (lane % CH) ^ ((r >> 1) & 7);
-            if constexpr (KS)
-                voff[j] = (uint32_t)(r * (int)ld + min(chunk[j] * 16, ((nrow + 7) / 8 - 1) * 16));
-            else
-                voff[j] = (uint32_t)(min(src_row(r), nrow - 1) * (int)ld + chunk[j] * 16);
+            const int r = lrow(wave, lane, j), c = chunk(lane, r);
+            if constexpr (KS) voff[j] = (uint32_t)(r * (int)ld + min(c * 16, ((nrow + 7) / 8 - 1) * 16));
+            else voff[j] = (uint32_t)(min(src_row(r), nrow - 1) * (int)ld + c * 16);
         }
+    }
+    // LDS row of this lane in load j, and the source chunk that belongs to its place in row r
+    static __device__ __forceinline__ int lrow(int wave, int lane, int j) { return (wave + NW * j) % NI * LROWS + lane / CH; }
+    static __device__ __forceinline__ int chunk(int lane, int r)
+    {
+        return (lane % CH) ^ (KS ? gm_ks_swz(r, CH) : gm_kc_swz<CH>(r));
     }
     // row of the matrix that LDS row r holds (DUAL: rows 16..31 of every 32 come from the second matrix)
     static __device__ __forceinline__ int src_row(int r) { return DUAL ? (r >> 5) * 16 + (r & 15) : r; }
-    static __device__ __forceinline__ bool second(int wave, int j) { return DUAL && ((((wave + NW * j) % NI) >> 1) & 1); }
-    __device__ __forceinline__ int64_t step() const { return KS ? (int64_t)BK * ld : 128; }
+    static __device__ __forceinline__ bool second(int wave, int j) { return DUAL && ((((wave + NW * j) % NI) * LROWS >> 4) & 1); }
+    __device__ __forceinline__ int64_t step() const { return KS ? (int64_t)BK * ld : SB; }
     __device__ __forceinline__ void advance(int64_t n)
     {
         p0 += n * step();
         if (DUAL) p1 += n * step();
     }
 
-    // LDS-direct loads of one K step of which `rem` elements exist
-    __device__ __forceinline__ void issue(char* lds, int wave, int rem) const
+    // load j of a whole K step, LDS-direct, from the descriptors of p0 and p1
+    __device__ __forceinline__ void issue_whole(int j, int lds, int wave, gm_i4 r0, gm_i4 r1) const
     {
-        const __amdgpu_buffer_rsrc_t r0 = gm_rsrc(p0);
-        const __amdgpu_buffer_rsrc_t r1 = DUAL ? gm_rsrc(p1) : r0;
+        gm_load_lds(second(wave, j) ? r1 : r0, lds + (wave + NW * j) % NI * 1024, voff[j]);
+    }
+    // LDS-direct loads of one K step of which `rem` elements exist
+    __device__ __forceinline__ void issue(char* lds, int wave, int lane, int rem) const
+    {
+        const int at = gm_lds_at(lds);
+        const gm_i4 r0 = gm_rsrc(p0), r1 = DUAL ? gm_rsrc(p1) : r0;
 #pragma unroll
         for (int j = 0; j < NV; ++j)
         {
-            const int ii = (wave + NW * j) % NI;
             uint32_t v = voff[j];
-            if (rem < BK) v = (KS ? lrow[j] : chunk[j] * (16 / ES)) < rem ? v : GM_OUT;
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(second(wave, j) ? r1 : r0, (gm_lds_void*)(lds + ii * 1024), 16, v, 0, 0,
-                                                     0);
+            if (rem < BK)
+            {
+                const int r = lrow(wave, lane, j);
+                v = (KS ? r : chunk(lane, r) * (16 / ES)) < rem ? v : GM_OUT;
+            }
+            gm_load_lds(second(wave, j) ? r1 : r0, at + (wave + NW * j) % NI * 1024, v);
         }
     }
     // the same chunks through registers
-    __device__ __forceinline__ void fetch(gm_i4 (&b)[NV], int wave, int rem) const
+    __device__ __forceinline__ void fetch(gm_i4 (&b)[NV], int wave, int lane, int rem) const
     {
 #pragma unroll
         for (int j = 0; j < NV; ++j)
         {
             const char* base = second(wave, j) ? p1 : p0;
-            if constexpr (KS)
-            {
-                const int c = chunk[j] * (16 / ES);
-                b[j] = gm_masked<ES>(base + lrow[j] * ld + c * ES, lrow[j] < rem ? (nrow - c) * ES : 0);
-            }
-            else
-            {
-                const int c = chunk[j] * (16 / ES);
-                b[j] = gm_masked<ES>(base + (int64_t)min(src_row(lrow[j]), nrow - 1) * ld + c * ES, (rem - c) * ES);
-            }
+            const int r = lrow(wave, lane, j), c = chunk(lane, r) * (16 / ES);
+            if constexpr (KS) b[j] = gm_masked<ES>(base + r * ld + c * ES, r < rem ? (nrow - c) * ES : 0);
+            else b[j] = gm_masked<ES>(base + (int64_t)min(src_row(r), nrow - 1) * ld + c * ES, (rem - c) * ES);
         }
     }
     // one K step through registers at once
     __device__ __forceinline__ void carry(char* lds, int wave, int lane, int rem) const
     {
         gm_i4 b[NV];
-        fetch(b, wave, rem);
+        fetch(b, wave, lane, rem);
         commit(b, lds, wave, lane);
     }
     __device__ __forceinline__ void commit(const gm_i4 (&b)[NV], char* lds, int wave, int lane) const
@@ -206,12 +240,12 @@ struct GmSide
             *reinterpret_cast<gm_i4*>(lds + (wave + NW * j) % NI * 1024 + lane * 16) = b[j];
     }
 
-    // fragment f (rows 16f..16f+15), half kk (0, 1) of the K step
+    // fragment f (rows 16f..16f+15), 64 bytes kk of the K step's rows
     static __device__ __forceinline__ gm_i4 frag(const char* lds, int lane, int f, int kk)
     {
         const int i = lane & 15, q = lane >> 4;
         if constexpr (!KS)
-            return *reinterpret_cast<const gm_i4*>(lds + f * 2048 + i * 128 + (((kk * 4 + q) ^ ((i >> 1) & 7)) << 4));
+            return *reinterpret_cast<const gm_i4*>(lds + (f * 16 + i) * SB + (((kk * 4 + q) ^ gm_kc_swz<CH>(i)) << 4));
         else
         {
             union { gm_i4 v; gm_s4 h[2]; } r;
@@ -226,6 +260,13 @@ struct GmSide
         }
     }
 };
+
+// p[i] by a select: an index into the arguments would put them into memory
+template <typename P>
+__device__ __forceinline__ P gm_pick(P const (&p)[2], int i)
+{
+    return i ? p[1] : p[0];
+}
 
 template <typename E>
 __device__ __forceinline__ float gm_silu(float g, float& s)
@@ -288,20 +329,25 @@ __device__ __forceinline__ void gm_put4(void* out, int odt, int64_t at, const fl
 // the block's forward epilogue for 4 neighbouring columns: h, and g and u of a training pass in fp32 (16-bit ones doubled the
 // gradients' error: 2.0 against 1.4 roundings in the root mean square; their traffic is 2% of a training step)
 template <typename E>
-__device__ __forceinline__ void gm_gate4(const GmArgs& a, int m, int n, const float (&g)[4], const float (&u)[4], int left)
+__device__ __forceinline__ void gm_gate_of(float limit, const float (&g)[4], const float (&u)[4], float (&h)[4])
 {
-    float h[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i)
     {
         float s, t = gm_silu<E>(g[i], s), v = u[i];
-        if (a.limit != 0.f)
+        if (limit != 0.f)
         {
-            t = fminf(t, a.limit);
-            v = fminf(fmaxf(v, -a.limit), a.limit);
+            t = fminf(t, limit);
+            v = fminf(fmaxf(v, -limit), limit);
         }
         h[i] = t * v;
     }
+}
+template <typename E>
+__device__ __forceinline__ void gm_gate4(const GmArgs& a, int m, int n, const float (&g)[4], const float (&u)[4], int left)
+{
+    float h[4];
+    gm_gate_of<E>(a.limit, g, u, h);
     gm_store4(static_cast<E*>(a.out[0]) + (int64_t)m * a.ldo + n, h, left);
     if (a.g)
     {
@@ -312,26 +358,32 @@ __device__ __forceinline__ void gm_gate4(const GmArgs& a, int m, int n, const fl
 
 // dh -> dg = dh * clamp(u) * [silu(g) <= L] * silu'(g), du = dh * min(silu(g), L) * [|u| <= L], h, for 4 neighbouring columns
 template <typename E>
-__device__ __forceinline__ void gm_dact4(const GmArgs& a, int m, int n, const float (&dh)[4], const float (&g)[4],
-                                         const float (&u)[4], int left)
+__device__ __forceinline__ void gm_dact_of(float limit, const float (&dh)[4], const float (&g)[4], const float (&u)[4],
+                                           float (&dg)[4], float (&du)[4], float (&h)[4])
 {
-    float dg[4], du[4], h[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i)
     {
         float s, t = gm_silu<E>(g[i], s), v = u[i];
         float kg = s + t * (1.0f - s), ku = 1.0f;
-        if (a.limit != 0.f)
+        if (limit != 0.f)
         {
-            if (t > a.limit) kg = 0.f;
-            if (fabsf(v) > a.limit) ku = 0.f;
-            t = fminf(t, a.limit);
-            v = fminf(fmaxf(v, -a.limit), a.limit);
+            if (t > limit) kg = 0.f;
+            if (fabsf(v) > limit) ku = 0.f;
+            t = fminf(t, limit);
+            v = fminf(fmaxf(v, -limit), limit);
         }
         dg[i] = dh[i] * v * kg;
         du[i] = dh[i] * t * ku;
         h[i] = t * v;
     }
+}
+template <typename E>
+__device__ __forceinline__ void gm_dact4(const GmArgs& a, int m, int n, const float (&dh)[4], const float (&g)[4],
+                                         const float (&u)[4], int left)
+{
+    float dg[4], du[4], h[4];
+    gm_dact_of<E>(a.limit, dh, g, u, dg, du, h);
     const int64_t at = (int64_t)m * a.ldo + n;
     gm_store4(static_cast<E*>(a.dg) + at, dg, left);
     gm_store4(static_cast<E*>(a.du) + at, du, left);
@@ -353,6 +405,114 @@ __device__ __forceinline__ void gm_tile(int b, int tm, int tn, int parts, int& p
     const int rows = min(GM_GROUP, tm - first), r = p - grp * wide;
     im = first + r % rows;
     in = r / rows;
+}
+
+// f(integral_constant 0), ..., f(integral_constant N - 1)
+template <typename F, int... I>
+__device__ __forceinline__ void gm_each(F&& f, std::integer_sequence<int, I...>)
+{
+    (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, typename F>
+__device__ __forceinline__ void gm_each(F&& f)
+{
+    gm_each(f, std::make_integer_sequence<int, N>{});
+}
+
+// A wave's tile of MI x NI fragments (tokens x columns, from m0 and n0 on) to where it goes.
+template <typename T, int EP, bool DUAL, int MI, int NI>
+__device__ __forceinline__ void gm_epilogue(const GmArgs& a, const typename T::acc (&acc)[NI][MI], int lane, int m0, int n0, int part,
+                                            int z)
+{
+    const int i16 = lane & 15, q = lane >> 4;
+    if constexpr (EP == EP_DACT)
+    {
+        // g and u of 4 fragments are loaded together, and the next 4's under these ones' arithmetic (clamped into
+        // the matrix): one by one they cost 15 us of a 50 us launch (333 x 5504)
+        const bool quads = a.N % 4 == 0;   // then 4 neighbouring columns are all inside or all outside
+        const int nw = n0 + q * 4;
+        constexpr int NB = NI < 4 ? NI : 4, HB = NI / NB;   // fragments of a load, loads of a tile row
+        gm_f4 g[2][NB], u[2][NB];
+        auto fetch = [&](auto kc) {
+            constexpr int k = decltype(kc)::value;
+            const int64_t row = (int64_t)min(m0 + k / HB * 16 + i16, a.M - 1) * a.ldg;
+#pragma unroll
+            for (int i = 0; i < NB; ++i)
+            {
+                const int64_t at = row + min(nw + (k % HB * NB + i) * 16, a.N - 4);
+                g[k & 1][i] = *reinterpret_cast<const gm_f4*>(a.g + at);
+                u[k & 1][i] = *reinterpret_cast<const gm_f4*>(a.u + at);
+            }
+        };
+        if (quads) fetch(std::integral_constant<int, 0>{});
+        gm_each<MI * HB>([&](auto kc) {
+            constexpr int k = decltype(kc)::value, j = k / HB;
+            if constexpr (k + 1 < MI * HB)
+                if (quads) fetch(std::integral_constant<int, k + 1>{});
+            const int m = m0 + j * 16 + i16;
+            if (m >= a.M) return;
+#pragma unroll
+            for (int i = 0; i < NB; ++i)
+            {
+                const int n = nw + (k % HB * NB + i) * 16;
+                if (n >= a.N) continue;
+                float v[4], gv[4], uv[4];
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    v[r] = static_cast<float>(acc[k % HB * NB + i][j][r]), gv[r] = g[k & 1][i][r], uv[r] = u[k & 1][i][r];
+                if (!quads)
+                {
+                    gm_load4(a.g + (int64_t)m * a.ldg + n, gv, a.N - n);
+                    gm_load4(a.u + (int64_t)m * a.ldg + n, uv, a.N - n);
+                }
+                gm_dact4<typename T::elem>(a, m, n, v, gv, uv, a.N - n);
+            }
+        });
+        return;
+    }
+    gm_each<MI>([&](auto jc) {
+        constexpr int j = decltype(jc)::value;
+        const int m = m0 + j * 16 + i16;
+        if (m >= a.M) return;
+        gm_each<NI / (DUAL ? 2 : 1)>([&](auto ic) {
+            constexpr int i = decltype(ic)::value * (DUAL ? 2 : 1);
+            const int n = n0 + decltype(ic)::value * 16 + q * 4;
+            if (n >= a.N) return;
+            if constexpr (EP == EP_PART)
+            {
+                typename T::scalar* p = static_cast<typename T::scalar*>(a.out[0]) +
+                                        ((int64_t)part * (DUAL ? 2 : 1) * a.M + m) * a.ldo + n;
+                // ldo is a multiple of 4 and rows are padded to it: whole vectors
+                *reinterpret_cast<typename T::acc*>(p) = acc[i][j];
+                if (DUAL) *reinterpret_cast<typename T::acc*>(p + (int64_t)a.M * a.ldo) = acc[i + DUAL][j];
+            }
+            else
+            {
+                float v[4];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) v[r] = static_cast<float>(acc[i][j][r]);
+                if constexpr (EP == EP_GATE)
+                {
+                    float w[4];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) w[r] = static_cast<float>(acc[i + DUAL][j][r]);
+                    gm_gate4<typename T::elem>(a, m, n, v, w, a.N - n);
+                }
+                else
+                {
+                    if constexpr (EP == EP_I8)
+                    {
+                        float sn[4];
+                        gm_load4(a.sb + n, sn, a.N - n);
+                        const float sm = a.sa[m];
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) v[r] = v[r] * sm * sn[r];
+                    }
+                    gm_put4(gm_pick(a.out, z), a.odt, (int64_t)m * a.ldo + n, v, a.N - n, a.accumulate);
+                }
+            }
+        });
+    });
 }
 
 template <typename T, int TM, int TN, int WM, int WN, bool AKS, bool BKS, bool DUAL, int NST, bool AL, int EP>
@@ -386,8 +546,8 @@ __global__ __launch_bounds__(WM* WN * 64, (WM * WN + 3) / 4) void gm_kernel(GmAr
     SA sa;
     SB sb;
     const int seg0 = t0 >= steps1 && a.segs > 1 ? 1 : 0;   // the segment that the part starts in (z: one segment)
-    sa.init(wave, lane, a.A[z + seg0], nullptr, a.lda, m0, a.M);
-    sb.init(wave, lane, DUAL ? a.B[0] : a.B[z + seg0], a.B[1], a.ldb, n0, a.N);
+    sa.init(wave, lane, gm_pick(a.A, z + seg0), nullptr, a.lda, m0, a.M);
+    sb.init(wave, lane, DUAL ? a.B[0] : gm_pick(a.B, z + seg0), a.B[1], a.ldb, n0, a.N);
     sa.advance(t0 - seg0 * steps1);
     sb.advance(t0 - seg0 * steps1);
     // the step whose loads are issued next
@@ -446,8 +606,8 @@ __global__ __launch_bounds__(WM* WN * 64, (WM * WN + 3) / 4) void gm_kernel(GmAr
             }
             else
             {
-                sa.issue(st, wave, rem);
-                sb.issue(st + SA::BYTES, wave, rem);
+                sa.issue(st, wave, lane, rem);
+                sb.issue(st + SA::BYTES, wave, lane, rem);
             }
             next();
         };
@@ -470,8 +630,8 @@ __global__ __launch_bounds__(WM* WN * 64, (WM * WN + 3) / 4) void gm_kernel(GmAr
         gm_i4 ba[SA::NV], bb[SB::NV];
         if (ti < t1)
         {
-            sa.fetch(ba, wave, rem_of(ti));
-            sb.fetch(bb, wave, rem_of(ti));
+            sa.fetch(ba, wave, lane, rem_of(ti));
+            sb.fetch(bb, wave, lane, rem_of(ti));
             next();
         }
         for (int t = t0; t < t1; ++t)
@@ -482,102 +642,298 @@ __global__ __launch_bounds__(WM* WN * 64, (WM * WN + 3) / 4) void gm_kernel(GmAr
             __syncthreads();
             if (ti < t1)
             {
-                sa.fetch(ba, wave, rem_of(ti));
-                sb.fetch(bb, wave, rem_of(ti));
+                sa.fetch(ba, wave, lane, rem_of(ti));
+                sb.fetch(bb, wave, lane, rem_of(ti));
                 next();
             }
             compute(gm_lds);
         }
     }
 
-    const int i16 = lane & 15, q = lane >> 4;
-    if constexpr (EP == EP_DACT)
-    {
-        // g and u of a tile row's fragments are loaded together, and the next row's under this one's arithmetic (clamped into
-        // the matrix): one by one they cost 15 us of a 50 us launch (333 x 5504)
-        const bool quads = a.N % 4 == 0;   // then 4 neighbouring columns are all inside or all outside
-        const int nw = n0 + wn * (TNC / WN) + q * 4;
-        gm_f4 g[2][NI], u[2][NI];
-        auto fetch = [&](int j, int s) {
-            const int64_t row = (int64_t)min(m0 + wm * (TM / WM) + j * 16 + i16, a.M - 1) * a.ldg;
+    gm_epilogue<T, EP, DUAL, MI, NI>(a, acc, lane, m0 + wm * (TM / WM), n0 + wn * (TNC / WN), part, z);
+}
+
+// A wave's 16-bit results by way of LDS: lanes put 4 neighbouring columns each, then whole runs of a row go out (a fragment's own
+// stores are 16 rows x 32 bytes; with them a 4096 x 12288 output of 256 x 256 tiles took 80 us at K = 128). Rows are padded by 16
+// bytes, so that 16 neighbouring rows' puts spread over the banks.
+template <typename E, int C>
+__device__ __forceinline__ void gm_put_row(char* lds, int row, int col, const float (&v)[4])
+{
+    typedef E vec __attribute__((ext_vector_type(4)));
+    vec o;
 #pragma unroll
-            for (int i = 0; i < NI; ++i)
+    for (int i = 0; i < 4; ++i) o[i] = static_cast<E>(v[i]);
+    *reinterpret_cast<vec*>(lds + row * (C * 2 + 16) + col * 2) = o;
+}
+template <int ROWS, int C>
+__device__ __forceinline__ void gm_flush_rows(const char* lds, int lane, void* out, int64_t ldo, int m0, int n0, int M, int N)
+{
+    constexpr int LPR = C / 8, RPI = 64 / LPR;   // lanes of a row, rows of a store
+    const int r0 = lane / LPR, c = lane % LPR * 8;
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // this wave's puts
+    if (n0 + c < N)
+#pragma unroll
+        for (int i = 0; i < ROWS / RPI; ++i)
+        {
+            const int r = i * RPI + r0;
+            if (m0 + r < M)
+                *reinterpret_cast<gm_i4*>(static_cast<uint16_t*>(out) + (int64_t)(m0 + r) * ldo + n0 + c) =
+                    *reinterpret_cast<const gm_i4*>(lds + r * (C * 2 + 16) + c * 2);
+        }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // read, before the next puts
+}
+
+constexpr int GM_BIG_LDS = 4 * 128 * 272;   // 4 waves' rows on the way out; the K steps' ring takes 128 KB of it
+
+// gm_epilogue of a wave's 128 x 128 results (DUAL: 128 x 64 of each matrix) where whole chunks of 16 bytes can be stored
+template <typename T, int EP, bool DUAL>
+__device__ __forceinline__ void gm_big_epilogue(const GmArgs& a, const typename T::acc (&acc)[8][8], char* lds, int lane, int m0, int n0,
+                                                int z)
+{
+    typedef typename T::elem E;
+    const int i16 = lane & 15, q = lane >> 4;
+    if constexpr (EP == EP_GATE)
+    {
+        gm_each<8>([&](auto jc) {
+            constexpr int j = decltype(jc)::value;
+            const int m = m0 + j * 16 + i16;
+            gm_each<4>([&](auto ic) {
+                constexpr int i = decltype(ic)::value;
+                float g[4], u[4], h[4];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) g[r] = acc[2 * i][j][r], u[r] = acc[2 * i + 1][j][r];
+                gm_gate_of<E>(a.limit, g, u, h);
+                gm_put_row<E, 64>(lds, j * 16 + i16, i * 16 + q * 4, h);
+                const int n = n0 + i * 16 + q * 4;
+                if (a.g && m < a.M && n < a.N)
+                {
+                    gm_store4(a.g + (int64_t)m * a.ldg + n, g, 4);
+                    gm_store4(a.u + (int64_t)m * a.ldg + n, u, 4);
+                }
+            });
+        });
+        gm_flush_rows<128, 64>(lds, lane, a.out[0], a.ldo, m0, n0, a.M, a.N);
+    }
+    else if constexpr (EP == EP_DACT)
+    {
+        constexpr int R = 32, REG = R * 272;   // rows at a time, of three outputs
+        gm_f4 g[2][4], u[2][4];
+        auto fetch = [&](auto kc) {            // 4 fragments' g and u, clamped into the matrix
+            constexpr int k = decltype(kc)::value;
+            const int64_t row = (int64_t)min(m0 + k / 2 * 16 + i16, a.M - 1) * a.ldg;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
             {
-                const int64_t at = row + min(nw + i * 16, a.N - 4);
-                g[s][i] = *reinterpret_cast<const gm_f4*>(a.g + at);
-                u[s][i] = *reinterpret_cast<const gm_f4*>(a.u + at);
+                const int64_t at = row + min(n0 + q * 4 + (k % 2 * 4 + i) * 16, a.N - 4);
+                g[k & 1][i] = *reinterpret_cast<const gm_f4*>(a.g + at);
+                u[k & 1][i] = *reinterpret_cast<const gm_f4*>(a.u + at);
             }
         };
-        if (quads) fetch(0, 0);
+        fetch(std::integral_constant<int, 0>{});
+        gm_each<16>([&](auto kc) {
+            constexpr int k = decltype(kc)::value, j = k / 2, b = k % 2 * 4;
+            if constexpr (k + 1 < 16) fetch(std::integral_constant<int, k + 1>{});
+            gm_each<4>([&](auto ic) {
+                constexpr int i = decltype(ic)::value;
+                float v[4], gv[4], uv[4], dg[4], du[4], h[4];
 #pragma unroll
-        for (int j = 0; j < MI; ++j)
-        {
-            if (quads && j + 1 < MI) fetch(j + 1, (j + 1) & 1);
-            const int m = m0 + wm * (TM / WM) + j * 16 + i16;
-            if (m >= a.M) continue;
-#pragma unroll
-            for (int i = 0; i < NI; ++i)
+                for (int r = 0; r < 4; ++r) v[r] = acc[b + i][j][r], gv[r] = g[k & 1][i][r], uv[r] = u[k & 1][i][r];
+                gm_dact_of<E>(a.limit, v, gv, uv, dg, du, h);
+                const int row = j % 2 * 16 + i16, col = (b + i) * 16 + q * 4;
+                gm_put_row<E, 128>(lds, row, col, dg);
+                gm_put_row<E, 128>(lds + REG, row, col, du);
+                gm_put_row<E, 128>(lds + 2 * REG, row, col, h);
+            });
+            if constexpr (k % 4 == 3)
             {
-                const int n = nw + i * 16;
-                if (n >= a.N) continue;
-                float v[4], gv[4], uv[4];
-#pragma unroll
-                for (int r = 0; r < 4; ++r) v[r] = static_cast<float>(acc[i][j][r]), gv[r] = g[j & 1][i][r], uv[r] = u[j & 1][i][r];
-                if (!quads)
-                {
-                    gm_load4(a.g + (int64_t)m * a.ldg + n, gv, a.N - n);
-                    gm_load4(a.u + (int64_t)m * a.ldg + n, uv, a.N - n);
-                }
-                gm_dact4<typename T::elem>(a, m, n, v, gv, uv, a.N - n);
+                const int at = m0 + j / 2 * R;
+                gm_flush_rows<R, 128>(lds, lane, a.dg, a.ldo, at, n0, a.M, a.N);
+                gm_flush_rows<R, 128>(lds + REG, lane, a.du, a.ldo, at, n0, a.M, a.N);
+                gm_flush_rows<R, 128>(lds + 2 * REG, lane, a.out[0], a.ldo, at, n0, a.M, a.N);
             }
-        }
-        return;
+        });
     }
-#pragma unroll
-    for (int j = 0; j < MI; ++j)
+    else
     {
-        const int m = m0 + wm * (TM / WM) + j * 16 + i16;
-        if (m >= a.M) continue;
+        float sn[8][4];
+        if constexpr (EP == EP_I8)
 #pragma unroll
-        for (int i = 0; i < NI; i += DUAL ? 2 : 1)
-        {
-            const int n = n0 + wn * (TNC / WN) + (DUAL ? i / 2 : i) * 16 + q * 4;
-            if (n >= a.N) continue;
-            if constexpr (EP == EP_PART)
-            {
-                typename T::scalar* p = static_cast<typename T::scalar*>(a.out[0]) +
-                                        ((int64_t)part * (DUAL ? 2 : 1) * a.M + m) * a.ldo + n;
-                // ldo is a multiple of 4 and rows are padded to it: whole vectors
-                *reinterpret_cast<typename T::acc*>(p) = acc[i][j];
-                if (DUAL) *reinterpret_cast<typename T::acc*>(p + (int64_t)a.M * a.ldo) = acc[i + 1 < NI ? i + 1 : i][j];
-            }
-            else
-            {
+            for (int i = 0; i < 8; ++i) gm_load4(a.sb + min(n0 + i * 16 + q * 4, a.N - 4), sn[i], 4);
+        gm_each<8>([&](auto jc) {
+            constexpr int j = decltype(jc)::value;
+            float sm = 0.f;
+            if constexpr (EP == EP_I8) sm = a.sa[min(m0 + j * 16 + i16, a.M - 1)];
+            gm_each<8>([&](auto ic) {
+                constexpr int i = decltype(ic)::value;
                 float v[4];
 #pragma unroll
-                for (int r = 0; r < 4; ++r) v[r] = static_cast<float>(acc[i][j][r]);
-                if constexpr (EP == EP_GATE)
+                for (int r = 0; r < 4; ++r)
                 {
-                    float w[4];
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) w[r] = static_cast<float>(acc[i + 1 < NI ? i + 1 : i][j][r]);
-                    gm_gate4<typename T::elem>(a, m, n, v, w, a.N - n);
+                    v[r] = static_cast<float>(acc[i][j][r]);
+                    if constexpr (EP == EP_I8) v[r] = v[r] * sm * sn[i][r];
                 }
-                else
-                {
-                    if constexpr (EP == EP_I8)
-                    {
-                        float sn[4];
-                        gm_load4(a.sb + n, sn, a.N - n);
-                        const float sm = a.sa[m];
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) v[r] = v[r] * sm * sn[r];
-                    }
-                    gm_put4(a.out[z], a.odt, (int64_t)m * a.ldo + n, v, a.N - n, a.accumulate);
-                }
-            }
-        }
+                if (a.odt == 1) gm_put_row<__bf16, 128>(lds, j * 16 + i16, i * 16 + q * 4, v);
+                else gm_put_row<_Float16, 128>(lds, j * 16 + i16, i * 16 + q * 4, v);
+            });
+        });
+        gm_flush_rows<128, 128>(lds, lane, gm_pick(a.out, z), a.ldo, m0, n0, a.M, a.N);
     }
+}
+
+// The largest products: 256 x 256 by 4 waves of 128 x 128, one to a SIMD. Bound by LDS reads: 8 waves of 128 x 64 read 192 KB for
+// a tile's 64 k (1536 cycles of 128 bytes, beside 512 of writes and 2048 of MFMA), these 128 KB. A wave's accumulators
+// are all 256 AGPRs (by asm constraint; left to itself the compiler copied or spilled them), its fragments of this step and of the
+// next 128 VGPRs. K steps of 64 bytes a row, NST slots of 32 KB: a step's MFMAs run under the reads of the next step's
+// fragments and the loads of the step NST - 1 ahead, spread evenly, one barrier a step. bf16 4096 x 12288 x 5120: 370 us (1.39
+// PFLOP/s) against 408 by 8 waves; 8192 x 8192 x 8192: 759 (1.45) against 905.
+template <typename T, bool AKS, bool BKS, bool DUAL, int EP>
+__global__ __launch_bounds__(256, 1) void gm_big_kernel(GmArgs a)
+{
+    constexpr int NST = 4;
+    typedef GmSide<T, 256, AKS, false, 4, 64> SA;
+    typedef GmSide<T, 256, BKS, DUAL, 4, 64> SB;
+    constexpr int STAGE = SA::BYTES + SB::BYTES, BK = SA::BK, NV = SA::NV + SB::NV;
+    static_assert(SA::NV == 4 && SB::NV == 4, "a load for every second group of MFMAs");
+    extern __shared__ __align__(16) char gm_lds[];
+
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / 64), lane = threadIdx.x % 64;
+    const int wm = wave / 2, wn = wave % 2, z = blockIdx.z;
+    int part, im, in;
+    gm_tile(blockIdx.x, a.tm, a.tn, 1, part, im, in);
+    constexpr int TNC = DUAL ? 128 : 256;
+    const int m0 = im * 256, n0 = in * TNC;
+    // whole steps by the pipeline; a segment's last step that is not whole comes after it, through registers
+    const int steps1 = a.K / BK, steps = steps1 * a.segs, tail = a.K % BK;
+    SA sa;
+    SB sb;
+    sa.init(wave, lane, gm_pick(a.A, z), nullptr, a.lda, m0, a.M);
+    sb.init(wave, lane, DUAL ? a.B[0] : gm_pick(a.B, z), a.B[1], a.ldb, n0, a.N);
+    auto segment = [&](int s) {
+        sa.p0 = gm_uniform(AKS ? gm_pick(a.A, s) + (int64_t)m0 * SA::ES : gm_pick(a.A, s) + (int64_t)m0 * a.lda);
+        sb.p0 = gm_uniform(BKS ? gm_pick(a.B, s) + (int64_t)n0 * SB::ES : gm_pick(a.B, s) + (int64_t)n0 * a.ldb);
+    };
+    int ti = 0;   // the step whose loads are issued next
+    auto next = [&]() {
+        ++ti;
+        if (a.segs > 1 && ti == steps1) segment(1);
+        else if (ti < steps)
+        {
+            sa.advance(1);
+            sb.advance(1);
+        }
+    };
+
+    typename T::acc acc[8][8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) acc[i][j] = typename T::acc{ 0, 0, 0, 0 };
+    gm_i4 fa[2][8], fb[2][8];
+    auto slot_a = [&](int s) { return gm_lds + s * STAGE + (AKS ? 0 : wm * 128 * 64); };
+    auto slot_b = [&](int s) { return gm_lds + s * STAGE + SA::BYTES + (BKS ? 0 : wn * 128 * 64); };
+    const int f0a = AKS ? wm * 8 : 0, f0b = BKS ? wn * 8 : 0, lds0 = gm_lds_at(gm_lds);
+
+    for (int s = 0; s < NST - 1; ++s)
+    {
+        const int live = ti < steps ? 0x7FFFFFFF : 0;   // past the end nothing is read (zeros are written)
+        const gm_i4 ra = gm_rsrc(sa.p0, live), rb = gm_rsrc(sb.p0, live), rb1 = DUAL ? gm_rsrc(sb.p1, live) : rb;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+        {
+            sa.issue_whole(j, lds0 + s * STAGE, wave, ra, ra);
+            sb.issue_whole(j, lds0 + s * STAGE + SA::BYTES, wave, rb, rb1);
+        }
+        next();
+    }
+    gm_wait_vmcnt<(NST - 2) * NV>();
+    gm_barrier();
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+    {
+        fb[0][i] = SB::frag(slot_b(0), lane, f0b + i, 0);
+        fa[0][i] = SA::frag(slot_a(0), lane, f0a + i, 0);
+    }
+    int cur = 0;
+    // one step on fragment set c; cur is its slot
+    auto step = [&](auto set) {
+        constexpr int c = decltype(set)::value;
+        gm_wait_vmcnt<(NST - 3) * NV>();   // this wave's loads of the next step have landed
+        gm_barrier();                      // every wave's have; every wave has read this step's slot and the one before
+        const int live = ti < steps ? 0x7FFFFFFF : 0;
+        const gm_i4 ra = gm_rsrc(sa.p0, live), rb = gm_rsrc(sb.p0, live), rb1 = DUAL ? gm_rsrc(sb.p1, live) : rb;
+        const int nxt = cur + 1 == NST ? 0 : cur + 1, fill = cur == 0 ? NST - 1 : cur - 1;
+        const int to = lds0 + fill * STAGE;
+        const char *la = slot_a(nxt), *lb = slot_b(nxt);
+        // the next step's fragment r, the columns' first
+        auto read = [&](auto rc) {
+            constexpr int r = decltype(rc)::value;
+            if constexpr (r < 8) fb[c ^ 1][r] = SB::frag(lb, lane, f0b + r, 0);
+            else fa[c ^ 1][r - 8] = SA::frag(la, lane, f0a + r - 8, 0);
+        };
+        // 4 MFMAs, then what goes out under them: the reads end some 250 cycles before the barrier that waits for them
+        gm_each<16>([&](auto gc) {
+            constexpr int g = decltype(gc)::value;
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+            {
+                const int e = g * 4 + k;
+                T::mfma_agpr(fb[c][e % 8], fa[c][e / 8], acc[e % 8][e / 8]);
+            }
+            if constexpr (g < 4)
+            {
+                read(std::integral_constant<int, 2 * g>{});
+                read(std::integral_constant<int, 2 * g + 1>{});
+            }
+            else if constexpr (g < 12) read(std::integral_constant<int, g + 4>{});
+            if constexpr (g % 2 == 0)
+            {
+                if constexpr (g < 8) sa.issue_whole(g / 2, to, wave, ra, ra);
+                else sb.issue_whole(g / 2 - 4, to + SA::BYTES, wave, rb, rb1);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        });
+        next();
+        cur = nxt;
+    };
+    for (int p = 0; p < steps / 2; ++p)
+    {
+        step(std::integral_constant<int, 0>{});
+        step(std::integral_constant<int, 1>{});
+    }
+    if (steps & 1) step(std::integral_constant<int, 0>{});
+    gm_wait_vmcnt<0>();
+    if (tail)
+        for (int s = 0; s < a.segs; ++s)
+        {
+            if (a.segs > 1) segment(s);
+            else
+            {
+                sa.p0 = gm_uniform(AKS ? gm_pick(a.A, z) + (int64_t)m0 * SA::ES : gm_pick(a.A, z) + (int64_t)m0 * a.lda);
+                sb.p0 = gm_uniform(DUAL ? a.B[0] + (int64_t)n0 * a.ldb : BKS ? gm_pick(a.B, z) + (int64_t)n0 * SB::ES : gm_pick(a.B, z) + (int64_t)n0 * a.ldb);
+                if (DUAL) sb.p1 = gm_uniform(a.B[1] + (int64_t)n0 * a.ldb);
+            }
+            sa.advance(steps1);
+            sb.advance(steps1);
+            gm_barrier();   // the slot is read
+            sa.carry(gm_lds, wave, lane, tail);
+            sb.carry(gm_lds + SA::BYTES, wave, lane, tail);
+            gm_barrier();
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+            {
+                fb[0][i] = SB::frag(slot_b(0), lane, f0b + i, 0);
+                fa[0][i] = SA::frag(slot_a(0), lane, f0a + i, 0);
+            }
+#pragma unroll
+            for (int e = 0; e < 64; ++e) T::mfma_agpr(fb[0][e % 8], fa[0][e / 8], acc[e % 8][e / 8]);
+        }
+    asm volatile("s_nop 15\n\ts_nop 15");   // the last MFMAs' results, which the compiler does not track
+    if (a.wide)
+    {
+        gm_barrier();   // the ring is done with
+        gm_big_epilogue<T, EP, DUAL>(a, acc, gm_lds + wave * (GM_BIG_LDS / 4), lane, m0 + wm * 128, n0 + wn * (TNC / 2), z);
+    }
+    else gm_epilogue<T, EP, DUAL, 8, 8>(a, acc, lane, m0 + wm * 128, n0 + wn * (TNC / 2), 0, z);
 }
 
 // Joins the K parts of a split product and runs its epilogue: a thread per 4 neighbouring columns.
@@ -774,9 +1130,9 @@ __global__ __launch_bounds__(NW * 64) void gm_ring_kernel(GmArgs a)
     typename T::acc acc = { 0, 0, 0, 0 };
     gm_i4 fx[S][2];
     auto issue = [&](int t, int s) {
-        const __amdgpu_buffer_rsrc_t r0 = gm_rsrc(base0 + (int64_t)t * 128), r1 = gm_rsrc(base1 + (int64_t)t * 128);
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(r0, (gm_lds_void*)(ring + s * 2048), 16, v0, 0, 0, 0);
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(r1, (gm_lds_void*)(ring + s * 2048 + 1024), 16, v1, 0, 0, 0);
+        const gm_i4 r0 = gm_rsrc(base0 + (int64_t)t * 128), r1 = gm_rsrc(base1 + (int64_t)t * 128);
+        gm_load_lds(r0, gm_lds_at(ring) + s * 2048, v0);
+        gm_load_lds(r1, gm_lds_at(ring) + s * 2048 + 1024, v1);
         fx[s][0] = fx[s][1] = gm_i4{ 0, 0, 0, 0 };
         if (live)
         {

@@ -18,6 +18,14 @@ static int gm_go(const GmArgs& a, int nz, hipStream_t st)
     return 0;
 }
 
+static int gm_wide(const GmArgs& a, int ep, int nz)
+{
+    auto ok = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
+    if (a.N % 8 || a.ldo % 8 || !ok(a.out[0]) || (nz > 1 && !ok(a.out[1]))) return 0;
+    if (ep == EP_DACT) return ok(a.dg) && ok(a.du);
+    return ep == EP_GATE || a.odt != 2;
+}
+
 template <typename T, bool AKS, bool BKS, bool DUAL, int EP>
 static int gm_tiles(GmArgs& a, const GmPlan& p, int aligned, int nz, hipStream_t st)
 {
@@ -38,7 +46,18 @@ static int gm_tiles(GmArgs& a, const GmPlan& p, int aligned, int nz, hipStream_t
         if (p.deep) return gm_go<T, 128, 128, 2, 4, AKS, BKS, DUAL, 4, true, EP>(a, nz, st);
     }
     if (p.tm == 128) return gm_go<T, 128, 128, 2, 2, AKS, BKS, DUAL, 2, true, EP>(a, nz, st);
-    return gm_go<T, 256, 256, 2, 4, AKS, BKS, DUAL, 2, true, EP>(a, nz, st);
+    if constexpr (EP == EP_PART) return -1;   // not split (gm_plan)
+    else
+    {
+        a.wide = gm_wide(a, EP, nz);
+        constexpr int lds = GM_BIG_LDS;
+        auto* kern = &gm_big_kernel<T, AKS, BKS, DUAL, EP>;
+        static const bool opened = hipFuncSetAttribute(reinterpret_cast<const void*>(kern),
+                                                       hipFuncAttributeMaxDynamicSharedMemorySize, lds) == hipSuccess;
+        (void)opened;
+        hipLaunchKernelGGL(kern, dim3((unsigned)(a.tm * a.tn), 1, nz), dim3(256), lds, st, a);
+        return 0;
+    }
 }
 
 template <typename T, bool DUAL, int EP, int NW>

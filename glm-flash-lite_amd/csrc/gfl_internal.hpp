@@ -200,6 +200,7 @@ struct GmArgs
     int64_t ldo = 0;                           // elements
     int odt = 0;                               // GFL_F16 / GFL_BF16 / GFL_F32
     int accumulate = 0;                        // EP_OUT, fp32: out += D
+    int wide = 0;                              // 16-bit outputs in whole aligned chunks of 16 bytes (gm_wide)
     float limit = 0.f;                         // SwiGLU clamp, 0 = off
     float* g = nullptr;                        // [M][N]: EP_GATE written (may be NULL), EP_DACT read
     float* u = nullptr;
