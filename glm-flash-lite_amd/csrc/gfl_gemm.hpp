@@ -138,7 +138,7 @@ __device__ __forceinline__ gm_i4 gm_masked(const char* p, int nb)
 template <int CH>
 __device__ __forceinline__ int gm_kc_swz(int r)
 {
-    return CH == 8 ? (r >> 1) & 7 : (r >> 2) & 3;
+    return CH == 8 ? (r >> 1) & 7 : (r >> 1) & 3;
 }
 __device__ __forceinline__ int gm_ks_swz(int k, int chunks) { return (2 * ((k & 3) | ((k >> 1) & 4))) & (chunks - 1); }
 
@@ -784,8 +784,9 @@ __device__ __forceinline__ void gm_big_epilogue(const GmArgs& a, const typename 
 // a tile's 64 k (1536 cycles of 128 bytes, beside 512 of writes and 2048 of MFMA), these 128 KB. A wave's accumulators
 // are all 256 AGPRs (by asm constraint; left to itself the compiler copied or spilled them), its fragments of this step and of the
 // next 128 VGPRs. K steps of 64 bytes a row, NST slots of 32 KB: a step's MFMAs run under the reads of the next step's
-// fragments and the loads of the step NST - 1 ahead, spread evenly, one barrier a step. bf16 4096 x 12288 x 5120: 370 us (1.39
-// PFLOP/s) against 408 by 8 waves; 8192 x 8192 x 8192: 759 (1.45) against 905.
+// fragments and the loads of the step NST - 1 ahead, one barrier a step. bf16 4096 x 12288 x 5120: 384 us (1.34
+// PFLOP/s) against 466 by 8 waves on one card; 8192 x 8192 x 8192: 785 (1.40) against 914. Clocks fall to 2.0 GHz under it; MFMAs
+// fill 63% of the CUs' cycles. A fifth slot and other orders of the reads made no difference.
 template <typename T, bool AKS, bool BKS, bool DUAL, int EP>
 __global__ __launch_bounds__(256, 1) void gm_big_kernel(GmArgs a)
 {
@@ -853,15 +854,22 @@ __global__ __launch_bounds__(256, 1) void gm_big_kernel(GmArgs a)
         fb[0][i] = SB::frag(slot_b(0), lane, f0b + i, 0);
         fa[0][i] = SA::frag(slot_a(0), lane, f0a + i, 0);
     }
-    int cur = 0;
-    // one step on fragment set c; cur is its slot
+    // what a step's reads and loads need, worked out during the step before: its descriptors, the slot its loads go to, the slot its
+    // reads come from (the next step's)
+    int nxt = 1, fill = NST - 1;
+    gm_i4 ra, rb, rb1;
+    auto prepare = [&]() {
+        const int live = ti < steps ? 0x7FFFFFFF : 0;
+        ra = gm_rsrc(sa.p0, live);
+        rb = gm_rsrc(sb.p0, live);
+        rb1 = DUAL ? gm_rsrc(sb.p1, live) : rb;
+    };
+    prepare();
+    // one step on fragment set c
     auto step = [&](auto set) {
         constexpr int c = decltype(set)::value;
         gm_wait_vmcnt<(NST - 3) * NV>();   // this wave's loads of the next step have landed
         gm_barrier();                      // every wave's have; every wave has read this step's slot and the one before
-        const int live = ti < steps ? 0x7FFFFFFF : 0;
-        const gm_i4 ra = gm_rsrc(sa.p0, live), rb = gm_rsrc(sb.p0, live), rb1 = DUAL ? gm_rsrc(sb.p1, live) : rb;
-        const int nxt = cur + 1 == NST ? 0 : cur + 1, fill = cur == 0 ? NST - 1 : cur - 1;
         const int to = lds0 + fill * STAGE;
         const char *la = slot_a(nxt), *lb = slot_b(nxt);
         // the next step's fragment r, the columns' first
@@ -890,10 +898,15 @@ __global__ __launch_bounds__(256, 1) void gm_big_kernel(GmArgs a)
                 if constexpr (g < 8) sa.issue_whole(g / 2, to, wave, ra, ra);
                 else sb.issue_whole(g / 2 - 4, to + SA::BYTES, wave, rb, rb1);
             }
+            if constexpr (g == 14) next();
+            if constexpr (g == 15)
+            {
+                prepare();
+                nxt = nxt + 1 == NST ? 0 : nxt + 1;
+                fill = fill + 1 == NST ? 0 : fill + 1;
+            }
             __builtin_amdgcn_sched_barrier(0);
         });
-        next();
-        cur = nxt;
     };
     for (int p = 0; p < steps / 2; ++p)
     {
