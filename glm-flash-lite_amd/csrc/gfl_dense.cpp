@@ -328,8 +328,7 @@ int gfl_linear_i8(const void* x, int64_t ldx, int dtype, const int8_t* b, int64_
 
 int gfl_sample_workspace(int B, int V, size_t* bytes)
 {
-    if (B < 0 || B > 65535 || V < 1 || V > gfl::MAX_VOCAB)
-        return api_fail(GFL_EINVAL, "gfl_sample: need 0 <= B <= 65535 (grid) and 1 <= V <= 2^20");
+    if (B < 0 || V < 1 || V > gfl::MAX_VOCAB) return api_fail(GFL_EINVAL, "gfl_sample: need B >= 0 and 1 <= V <= 2^20");
     if (bytes) *bytes = gfl::sample_ws_bytes(B, V);
     return GFL_OK;
 }

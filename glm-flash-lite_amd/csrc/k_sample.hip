@@ -70,13 +70,49 @@ __device__ __forceinline__ uint64_t sm_weight(uint32_t key, uint32_t top, double
     return key > SM_MASKED ? sm_units(sm_exp(key, top, scale)) : 0;
 }
 
+// Wave scans by DPP: shifts by 1, 2, 4, 8 within rows of 16 lanes, then the rows' last lanes to the rows after them. `id` is
+// what a lane without a source takes.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t sm_dpp(uint32_t id, uint32_t v)
+{
+    return (uint32_t)__builtin_amdgcn_update_dpp((int)id, (int)v, CTRL, ROWS, 0xF, false);
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ unsigned long long sm_dpp64(unsigned long long v)
+{
+    return (unsigned long long)sm_dpp<CTRL, ROWS>(0, (uint32_t)(v >> 32)) << 32 | sm_dpp<CTRL, ROWS>(0, (uint32_t)v);
+}
+__device__ __forceinline__ unsigned long long sm_wave_scan(unsigned long long v)   // inclusive
+{
+    v += sm_dpp64<0x111, 0xF>(v);
+    v += sm_dpp64<0x112, 0xF>(v);
+    v += sm_dpp64<0x114, 0xF>(v);
+    v += sm_dpp64<0x118, 0xF>(v);
+    v += sm_dpp64<0x142, 0xA>(v);
+    v += sm_dpp64<0x143, 0xC>(v);
+    return v;
+}
+__device__ __forceinline__ unsigned long long sm_lane64(unsigned long long v, int lane)
+{
+    return (unsigned long long)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(v >> 32), lane) << 32 |
+           (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, lane);
+}
 template <typename V>
 __device__ __forceinline__ V sm_wave_sum(V v)
 {
-#pragma unroll
-    for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
-    return v;
+    return (V)sm_lane64(sm_wave_scan(v), 63);
 }
+__device__ __forceinline__ uint32_t sm_wave_max(uint32_t v)
+{
+    v = max(v, sm_dpp<0x111, 0xF>(0, v));
+    v = max(v, sm_dpp<0x112, 0xF>(0, v));
+    v = max(v, sm_dpp<0x114, 0xF>(0, v));
+    v = max(v, sm_dpp<0x118, 0xF>(0, v));
+    v = max(v, sm_dpp<0x142, 0xA>(0, v));
+    v = max(v, sm_dpp<0x143, 0xC>(0, v));
+    return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+}
+__device__ __forceinline__ uint32_t sm_wave_min(uint32_t v) { return ~sm_wave_max(~v); }
 
 struct SmShared
 {
@@ -261,44 +297,48 @@ __device__ void sm_row_slow(SmShared& s, const SampleArgs& a, int b, const SmRow
 // ---- the launches ----
 //
 // A row is cut into S slices, a workgroup each, so that a few rows fill the card (B = 1, V = 131,072: 64 workgroups; the same
-// work in one workgroup took 547 us). Four launches:
+// work in one workgroup took 547 us). Four launches, for up to SM_ROWS rows at a time:
 //   top     each slice's largest and smallest logit and the largest's index; clears the row's histogram
 //   bins    2,047 bins of equal width from the largest logit down to where weights round to zero (or to the smallest), and
-//           one for what lies below: logits per bin, and where the nucleus needs it their weight
-//   cut     every workgroup finds the bin in which the kept prefix ends from the row's histogram. With a top-k (and few
-//           logits down to its bin) all logits down to that bin go into the row's list; else the list takes the bin alone
-//           and each slice sums the weight of its logits above it
-//   pick    a workgroup per row sorts the list, finds the threshold in it, and draws: from the list itself (top-k), or
+//           one for what lies below: logits per bin for a top-k, else the weight per bin (of the row and of each slice)
+//   cut     every workgroup finds the bins in which the kept prefix ends from the row's histogram. With a top-k (and few
+//           logits down to its bin) all logits down to that bin go into the row's list; else the list takes the bins
+//           where the nucleus and min-p end, and each slice sums the weight of its bins above them
+//   pick    a workgroup per row finds the last kept logit in the list, and draws: from the list itself (top-k), or
 //           from the slice in which the target lies
-constexpr int SM_LIST = 4096;         // logits a row's list holds (32 KB of LDS)
+constexpr int SM_LIST = 4096;         // logits a row's list holds
 constexpr int SM_LISTK = 1024;        // top-k up to which the list is expected to hold the whole kept set
 constexpr int SM_PT = 256;            // threads of the slice launches
 constexpr int SM_MAXS = 256;          // slices of a row
+constexpr int SM_ROWS = 1024;         // rows of one round of launches, which bounds the workspace
+constexpr int SM_PER = SM_LIST / SM_T;   // list entries of a thread of the last launch
 
 struct SmSlice
 {
     uint32_t top, low;                // largest key, smallest key above -inf (0, ~0 without any)
     int32_t arg;                      // lowest index of the largest
     int32_t pad;
-    unsigned long long mass;          // weight above the cut bin (of the kept by min-p)
+    unsigned long long mass;          // weight above the list's bins (every kept weight: SM_ALL)
 };
 enum
 {
     SM_ALL = 0,                       // every logit kept (but for min-p): draw from the slices
-    SM_BIN = 1,                       // the list holds the bin where the nucleus ends
+    SM_BIN = 1,                       // the list holds the bins where the nucleus and min-p end
     SM_TOPK = 2,                      // the list holds everything that may be kept
     SM_SLOW = 3,
 };
 struct SmState                        // of a row
 {
-    int32_t count;                    // list entries
+    int32_t count;                    // list entries (more than SM_LIST: it overflowed)
     int32_t mode;
-    unsigned long long want, above;   // SM_BIN: weight at which the nucleus ends, weight above the bin
+    int32_t lo, hi;                   // the list's bins
+    unsigned long long want, above;   // SM_BIN: weight at which the nucleus ends, weight above the list's bins
 };
 struct SmWs
 {
     uint32_t* cnt;                    // [B][SM_BINS]
     unsigned long long* mass;         // [B][SM_BINS]
+    unsigned long long* part;         // [B][S][SM_BINS] the slices' weights
     unsigned long long* list;         // [B][SM_LIST] key << 32 | ~index
     SmSlice* slice;                   // [B][S]
     SmState* state;                   // [B]
@@ -318,21 +358,22 @@ static void sm_split(int B, int V, int& S, int& len)
 static size_t sm_carve(void* base, int B, int V, SmWs& w)
 {
     sm_split(B, V, w.S, w.len);
-    char* p = static_cast<char*>(base);
+    size_t at = 0;
     auto take = [&](size_t n) {
-        char* r = p;
-        p += (n + 255) / 256 * 256;
+        char* r = static_cast<char*>(base) + at;
+        at += (n + 255) / 256 * 256;
         return r;
     };
     w.mass = reinterpret_cast<unsigned long long*>(take((size_t)B * SM_BINS * 8));
+    w.part = reinterpret_cast<unsigned long long*>(take((size_t)B * w.S * SM_BINS * 8));
     w.list = reinterpret_cast<unsigned long long*>(take((size_t)B * SM_LIST * 8));
     w.slice = reinterpret_cast<SmSlice*>(take((size_t)B * w.S * sizeof(SmSlice)));
     w.state = reinterpret_cast<SmState*>(take((size_t)B * sizeof(SmState)));
     w.cnt = reinterpret_cast<uint32_t*>(take((size_t)B * SM_BINS * 4));
-    return (size_t)(p - static_cast<char*>(base));
+    return at;
 }
 
-// use(index, key) for this thread's logits of [lo, hi): 4 neighbours at a time, 4 loads in flight (`first`: the first 4, loaded
+// use(index, key) for this thread's logits of [lo, hi): 4 neighbours at a time, 4 loads in flight (`b`: the first 4, loaded
 // ahead of what the launch waits for otherwise)
 template <typename E, int NT>
 struct SmBatch
@@ -351,6 +392,9 @@ __device__ __forceinline__ void sm_each(const E* row, int lo, int hi, SmBatch<E,
 {
     for (int i = lo + (int)threadIdx.x * 4; i < hi;)
     {
+        const int next = i + 4 * NT * 4;
+        SmBatch<E, NT> n;
+        n.load(row, next, hi);   // under this batch's work
 #pragma unroll
         for (int j = 0; j < 4; ++j)
         {
@@ -363,8 +407,8 @@ __device__ __forceinline__ void sm_each(const E* row, int lo, int hi, SmBatch<E,
             else
                 for (int k = at; k < hi; ++k) use(k, sm_key(static_cast<float>(row[k])));   // the slice's last, not whole, chunk
         }
-        i += 4 * NT * 4;
-        b.load(row, i, hi);
+        i = next;
+        b = n;
     }
 }
 
@@ -377,10 +421,8 @@ struct SmHead
     bool wide;            // a range past fp32: no bins
     float T, top_x, bins; // bins per unit of logit
     double scale;
-    __device__ __forceinline__ int bin(uint32_t key) const
-    {
-        return key == top ? 0 : (int)fminf((top_x - sm_value(key)) * bins, (float)(SM_BINS - 1));
-    }
+    __device__ __forceinline__ float place(uint32_t key) const { return key == top ? 0.0f : (top_x - sm_value(key)) * bins; }
+    __device__ __forceinline__ int bin(uint32_t key) const { return (int)fminf(place(key), (float)(SM_BINS - 1)); }
 };
 
 __device__ __forceinline__ SmHead sm_head(const SampleArgs& a, const SmWs& w, int b)
@@ -395,24 +437,16 @@ __device__ __forceinline__ SmHead sm_head(const SampleArgs& a, const SmWs& w, in
         if (c.top > top) top = c.top, arg = c.arg;   // slices in order: the first of equals has the lowest index
         low = min(low, c.low);
     }
-#pragma unroll
-    for (int o = 32; o; o >>= 1)
-    {
-        const uint32_t t = (uint32_t)__shfl_xor((int)top, o);
-        const int f = __shfl_xor(arg, o);
-        if (t > top || (t == top && f < arg)) top = t, arg = f;
-        low = min(low, (uint32_t)__shfl_xor((int)low, o));
-    }
-    h.top = top;
-    h.low = low;
-    h.arg = arg;
+    h.top = sm_wave_max(top);
+    h.low = sm_wave_min(low);
+    h.arg = (int)sm_wave_min(top == h.top ? (uint32_t)arg : 0x7FFFFFFFu);
     h.T = a.temperature ? a.temperature[b] : 1.0f;
-    h.done = top <= SM_MASKED || !(h.T > 0.0f);
-    h.top_x = sm_value(top);
+    h.done = h.top <= SM_MASKED || !(h.T > 0.0f);
+    h.top_x = sm_value(h.top);
     h.scale = 1.4426950408889634074 / (double)h.T;
     // down to the smallest logit (a little past it, so that it lies in a bin of its own right) or to where weights round to
     // zero units: what falls into the last bin, below the range, weighs nothing
-    const float range = fmaxf(fminf((h.top_x - sm_value(low)) * 1.001f, 31.0f * h.T), 1e-30f);
+    const float range = fmaxf(fminf((h.top_x - sm_value(h.low)) * 1.001f, 31.0f * h.T), 1e-30f);
     h.bins = (float)(SM_BINS - 1) / range;
     h.wide = !(range < __builtin_inff());
     return h;
@@ -423,14 +457,14 @@ __global__ __launch_bounds__(SM_PT) void sm_top_kernel(SampleArgs a, SmWs w)
 {
     const int b = blockIdx.y, s = blockIdx.x, lo = s * w.len, hi = min(a.V, lo + w.len);
     const E* row = static_cast<const E*>(a.logits) + (int64_t)b * a.ld;
+    SmBatch<E, SM_PT> first;
+    first.load(row, lo + threadIdx.x * 4, hi);
     for (int i = s * SM_PT + threadIdx.x; i < SM_BINS; i += w.S * SM_PT)
     {
         w.cnt[(size_t)b * SM_BINS + i] = 0;
         w.mass[(size_t)b * SM_BINS + i] = 0;
     }
     if (s == 0 && threadIdx.x == 0) w.state[b].count = 0;
-    SmBatch<E, SM_PT> first;
-    first.load(row, lo + threadIdx.x * 4, hi);
     uint32_t top = 0, low = ~0u;
     int arg = 0x7FFFFFFF;
     sm_each<E, SM_PT>(row, lo, hi, first, [&](int i, uint32_t k) {
@@ -439,28 +473,22 @@ __global__ __launch_bounds__(SM_PT) void sm_top_kernel(SampleArgs a, SmWs w)
     });
     __shared__ uint32_t st[SM_PT / 64], sl[SM_PT / 64];
     __shared__ int sa[SM_PT / 64];
-#pragma unroll
-    for (int o = 32; o; o >>= 1)
-    {
-        const uint32_t t = (uint32_t)__shfl_xor((int)top, o);
-        const int f = __shfl_xor(arg, o);
-        if (t > top || (t == top && f < arg)) top = t, arg = f;
-        low = min(low, (uint32_t)__shfl_xor((int)low, o));
-    }
-    if (threadIdx.x % 64 == 0) st[threadIdx.x / 64] = top, sl[threadIdx.x / 64] = low, sa[threadIdx.x / 64] = arg;
+    const uint32_t wt = sm_wave_max(top), wl = sm_wave_min(low);
+    const int wa = (int)sm_wave_min(top == wt ? (uint32_t)arg : 0x7FFFFFFFu);
+    if (threadIdx.x % 64 == 0) st[threadIdx.x / 64] = wt, sl[threadIdx.x / 64] = wl, sa[threadIdx.x / 64] = wa;
     __syncthreads();
     if (threadIdx.x == 0)
     {
+        SmSlice& c = w.slice[(size_t)b * w.S + s];
+        c.top = st[0];
+        c.low = sl[0];
+        c.arg = sa[0];
+        c.mass = 0;
         for (int i = 1; i < SM_PT / 64; ++i)
         {
-            if (st[i] > top || (st[i] == top && sa[i] < arg)) top = st[i], arg = sa[i];
-            low = min(low, sl[i]);
+            if (st[i] > c.top || (st[i] == c.top && sa[i] < c.arg)) c.top = st[i], c.arg = sa[i];
+            c.low = min(c.low, sl[i]);
         }
-        SmSlice& c = w.slice[(size_t)b * w.S + s];
-        c.top = top;
-        c.low = low;
-        c.arg = arg;
-        c.mass = 0;
     }
 }
 
@@ -474,6 +502,14 @@ __device__ __forceinline__ float sm_topp(const SampleArgs& a, int b)
     const float p = a.top_p ? a.top_p[b] : 1.0f;
     return p < 1.0f ? p : 1.0f;
 }
+__device__ __forceinline__ double sm_minp(const SampleArgs& a, int b)
+{
+    const float m = a.min_p ? a.min_p[b] : 0.0f;
+    return m > 0.0f ? (double)m : 0.0;
+}
+
+// rows whose list a top-k fills take logits per bin; the others with a nucleus their weight
+__device__ __forceinline__ bool sm_weighs(int k, float p) { return p < 1.0f && (!k || k > SM_LISTK); }
 
 template <typename E>
 __global__ __launch_bounds__(SM_PT) void sm_bins_kernel(SampleArgs a, SmWs w)
@@ -486,16 +522,16 @@ __global__ __launch_bounds__(SM_PT) void sm_bins_kernel(SampleArgs a, SmWs w)
     first.load(row, lo + threadIdx.x * 4, hi);
     const SmHead h = sm_head(a, w, b);
     const int k = sm_topk(a, b);
-    const bool p = sm_topp(a, b) < 1.0f;
-    if (h.done || h.wide || (!k && !p)) return;
-    const bool weigh = p && (!k || k > SM_LISTK);   // a small top-k's list gives its weights itself
+    const float p = sm_topp(a, b);
+    if (h.done || h.wide || (!k && !(p < 1.0f))) return;
+    const bool weigh = sm_weighs(k, p);
     for (int i = threadIdx.x; i < SM_BINS; i += SM_PT) cnt[i] = 0, mass[i] = 0;
     __syncthreads();
     if (weigh)
         sm_each<E, SM_PT>(row, lo, hi, first, [&](int, uint32_t key) {
             if (key <= SM_MASKED) return;
             const int bin = h.bin(key);
-            atomicAdd(&cnt[bin], 1u);
+            if (k) atomicAdd(&cnt[bin], 1u);
             if (bin < SM_BINS - 1) atomicAdd(&mass[bin], (unsigned long long)sm_weight(key, h.top, h.scale));
         });
     else
@@ -503,10 +539,15 @@ __global__ __launch_bounds__(SM_PT) void sm_bins_kernel(SampleArgs a, SmWs w)
             if (key > SM_MASKED) atomicAdd(&cnt[h.bin(key)], 1u);
         });
     __syncthreads();
+    unsigned long long* part = w.part + ((size_t)b * w.S + s) * SM_BINS;
     for (int i = threadIdx.x; i < SM_BINS; i += SM_PT)
     {
         if (cnt[i]) atomicAdd(&w.cnt[(size_t)b * SM_BINS + i], cnt[i]);
-        if (mass[i]) atomicAdd(&w.mass[(size_t)b * SM_BINS + i], mass[i]);
+        if (weigh)
+        {
+            part[i] = mass[i];
+            if (mass[i]) atomicAdd(&w.mass[(size_t)b * SM_BINS + i], mass[i]);
+        }
     }
 }
 
@@ -516,31 +557,20 @@ __device__ __forceinline__ unsigned long long sm_scan(unsigned long long v, unsi
                                                       unsigned long long& total)
 {
     const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-    unsigned long long c = v;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1)
-    {
-        const unsigned long long t = __shfl_up(c, o);
-        if (lane >= o) c += t;
-    }
+    const unsigned long long c = sm_wave_scan(v);
     __syncthreads();
     if (lane == 63) scratch[wave] = c;
     __syncthreads();
-    unsigned long long before = 0;
-    total = 0;
-#pragma unroll
-    for (int i = 0; i < NT / 64; ++i)
-    {
-        if (i < wave) before += scratch[i];
-        total += scratch[i];
-    }
-    return before + c - v;
+    // every wave scans the waves' sums in its first lanes
+    const unsigned long long all = sm_wave_scan(lane < NT / 64 ? scratch[lane] : 0);
+    total = sm_lane64(all, NT / 64 - 1);
+    return (wave ? sm_lane64(all, __builtin_amdgcn_readfirstlane(wave) - 1) : 0) + c - v;
 }
 
-// the bin in which the kept prefix of a row ends, and the row's mode
+// the bins in which the kept prefix of a row ends, and the row's mode
 struct SmCut
 {
-    int mode, bin;
+    int mode, lo, hi;
     unsigned long long want, above;
 };
 __device__ SmCut sm_cut(const SampleArgs& a, const SmWs& w, int b, const SmHead& h, unsigned long long* scratch, int* found)
@@ -548,7 +578,7 @@ __device__ SmCut sm_cut(const SampleArgs& a, const SmWs& w, int b, const SmHead&
     constexpr int PER = SM_BINS / SM_PT;
     const int k = sm_topk(a, b);
     const float p = sm_topp(a, b);
-    SmCut c = { SM_ALL, SM_BINS, 0, 0 };
+    SmCut c = { SM_ALL, 0, SM_BINS - 1, 0, 0 };
     if (!k && !(p < 1.0f)) return c;
     if (h.wide)
     {
@@ -557,53 +587,71 @@ __device__ SmCut sm_cut(const SampleArgs& a, const SmWs& w, int b, const SmHead&
     }
     const uint32_t* cnt = w.cnt + (size_t)b * SM_BINS + threadIdx.x * PER;
     const unsigned long long* mass = w.mass + (size_t)b * SM_BINS + threadIdx.x * PER;
+    unsigned long long total = 0;
     if (threadIdx.x == 0) found[0] = -1, found[1] = 0;
-    unsigned long long n = 0, total;
-    uint32_t each[PER];
-#pragma unroll
-    for (int i = 0; i < PER; ++i) n += each[i] = cnt[i];
-    unsigned long long at = sm_scan<SM_PT>(n, scratch, total);
-    bool topk = false;
-    if (k && (k <= SM_LISTK || total > (unsigned long long)k))
+    if (k)
     {
-        // the bin of the k-th logit; all of them where the row has no more
-        const unsigned long long want = total < (unsigned long long)k ? total : (unsigned long long)k;
+        uint32_t each[PER];
+        unsigned long long n = 0;
 #pragma unroll
-        for (int i = 0; i < PER; ++i)
+        for (int i = 0; i < PER; ++i) n += each[i] = cnt[i];
+        unsigned long long at = sm_scan<SM_PT>(n, scratch, total);
+        if (k <= SM_LISTK || total > (unsigned long long)k)
         {
-            const int bin = threadIdx.x * PER + i;
-            // a prefix that ends in the last bin is the one before it: what lies there weighs nothing
-            if (at < want && at + each[i] >= want)
-                found[0] = min(bin, SM_BINS - 2), found[1] = (int)(bin == SM_BINS - 1 ? at : at + each[i]);
-            at += each[i];
-        }
-        topk = true;
-    }
-    else if (p < 1.0f)
-    {
-        unsigned long long m = 0, eachm[PER];
+            // the bin of the k-th logit; all of them where the row has no more
+            const unsigned long long want = total < (unsigned long long)k ? total : (unsigned long long)k;
 #pragma unroll
-        for (int i = 0; i < PER; ++i) m += eachm[i] = mass[i];
-        at = sm_scan<SM_PT>(m, scratch, total);
-        const double goal = (double)p * (double)total;
-        c.want = goal > 1.0 ? (unsigned long long)ceil(goal) : 1ull;
-#pragma unroll
-        for (int i = 0; i < PER; ++i)
-        {
-            if (at < c.want && at + eachm[i] >= c.want)
+            for (int i = 0; i < PER; ++i)
             {
-                found[0] = threadIdx.x * PER + i;
-                found[1] = (int)each[i];
-                scratch[SM_PT / 64] = at;
+                const int bin = threadIdx.x * PER + i;
+                // a prefix that ends in the last bin is the one before it: what lies there weighs nothing
+                if (at < want && at + each[i] >= want)
+                    found[0] = min(bin, SM_BINS - 2), found[1] = (int)(bin == SM_BINS - 1 ? at : at + each[i]);
+                at += each[i];
             }
-            at += eachm[i];
+            __syncthreads();
+            c.hi = found[0];
+            c.mode = found[1] > SM_LIST ? SM_SLOW : SM_TOPK;
+            return c;
         }
+        if (!(p < 1.0f)) return c;   // a top-k that keeps every logit
+        __syncthreads();
     }
-    else return c;   // a top-k that keeps every logit
+    unsigned long long each[PER], m = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) m += each[i] = mass[i];
+    const unsigned long long before = sm_scan<SM_PT>(m, scratch, total);
+    unsigned long long at = before;
+    const double goal = (double)p * (double)total;
+    c.want = goal > 1.0 ? (unsigned long long)ceil(goal) : 1ull;
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+    {
+        if (at < c.want && at + each[i] >= c.want) found[0] = threadIdx.x * PER + i;
+        at += each[i];
+    }
     __syncthreads();
-    c.bin = found[0];
-    c.mode = found[1] > SM_LIST ? SM_SLOW : topk ? SM_TOPK : SM_BIN;
-    if (!topk) c.above = scratch[SM_PT / 64];
+    c.mode = SM_BIN;
+    c.lo = c.hi = found[0];
+    const double mp = sm_minp(a, b);
+    if (mp > 0.0)
+    {
+        // min-p ends where exp(-d / T) = m: the bins beside that place, too, where they are not past the nucleus
+        const float place = (float)(-log(mp) * (double)h.T) * h.bins;
+        const int bm = (int)fminf(fmaxf(place, 0.0f), (float)(SM_BINS - 1));
+        c.lo = min(c.lo, max(bm - 1, 0));
+        c.hi = min(c.hi, bm + 1);
+    }
+    // weight above the list's bins
+    at = before;
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+    {
+        if (threadIdx.x * PER + i == c.lo) scratch[SM_PT / 64] = at;
+        at += each[i];
+    }
+    __syncthreads();
+    c.above = scratch[SM_PT / 64];
     return c;
 }
 
@@ -621,59 +669,98 @@ __global__ __launch_bounds__(SM_PT) void sm_cut_kernel(SampleArgs a, SmWs w)
     const SmCut c = sm_cut(a, w, b, h, scratch, found);
     if (s == 0 && threadIdx.x == 0)
     {
-        w.state[b].mode = c.mode;
-        w.state[b].want = c.want;
-        w.state[b].above = c.above;
+        SmState& st = w.state[b];
+        st.mode = c.mode;
+        st.lo = c.lo;
+        st.hi = c.hi;
+        st.want = c.want;
+        st.above = c.above;
     }
     if (c.mode == SM_SLOW) return;
-    unsigned long long* list = w.list + (size_t)b * SM_LIST;
-    auto put = [&](int i, uint32_t key) {
-        const int at = atomicAdd(&w.state[b].count, 1);
-        if (at < SM_LIST) list[at] = (unsigned long long)key << 32 | (uint32_t)~i;
-    };
-    if (c.mode == SM_TOPK)
-    {
-        sm_each<E, SM_PT>(row, lo, hi, first, [&](int i, uint32_t key) {
-            if (key > SM_MASKED && h.bin(key) <= c.bin) put(i, key);
-        });
-        return;
-    }
-    const float mp = a.min_p ? a.min_p[b] : 0.0f;
-    const double m = mp > 0.0f ? (double)mp : 0.0;
     unsigned long long mine = 0, total;
-    sm_each<E, SM_PT>(row, lo, hi, first, [&](int i, uint32_t key) {
-        if (key <= SM_MASKED) return;
-        const int bin = c.mode == SM_ALL ? 0 : h.bin(key);
-        if (bin > c.bin) return;
-        if (bin == c.bin) put(i, key);
-        else
-        {
+    if (c.mode == SM_ALL)
+    {
+        const double m = sm_minp(a, b);
+        sm_each<E, SM_PT>(row, lo, hi, first, [&](int, uint32_t key) {
+            if (key <= SM_MASKED) return;
             const double e = sm_exp(key, h.top, h.scale);
             if (key == h.top || e >= m) mine += sm_units(e);
-        }
-    });
+        });
+    }
+    else
+    {
+        unsigned long long* list = w.list + (size_t)b * SM_LIST;
+        sm_each<E, SM_PT>(row, lo, hi, first, [&](int i, uint32_t key) {
+            const int bin = h.bin(key);
+            if (key <= SM_MASKED || bin < c.lo || bin > c.hi) return;
+            const int at = atomicAdd(&w.state[b].count, 1);
+            if (at < SM_LIST) list[at] = (unsigned long long)key << 32 | (uint32_t)~i;
+        });
+        if (c.mode == SM_TOPK) return;
+        const unsigned long long* part = w.part + ((size_t)b * w.S + s) * SM_BINS;
+        for (int i = threadIdx.x; i < c.lo; i += SM_PT) mine += part[i];
+    }
     sm_scan<SM_PT>(mine, scratch, total);
     if (threadIdx.x == 0) w.slice[(size_t)b * w.S + s].mass = total;
 }
 
-// descending bitonic sort of n (a power of two) entries in LDS. A wave's 64 exchanges over distances up to 64 stay within
-// its own 128 entries, so only the longer ones need a barrier.
-__device__ __forceinline__ void sm_sort(unsigned long long* v, int n)
+struct SmPick
+{
+    unsigned long long hist[SM_T], comp[SM_T], wt[SM_T];
+    unsigned long long scratch[SM_W];
+    unsigned long long part[SM_MAXS];
+    unsigned long long at, cut, cut_wt;
+    int bin, m, pick;
+};
+
+// Of the list's entries (SM_PER a thread; wt 0: not one) the one at which the weights summed in order reach `want`, the sum
+// starting at `before`: order is by place (0 .. SM_T - 1) and within a place by comp, largest first. s.cut = its comp and
+// s.cut_wt = its weight. Returns 0 = found, 1 = the sum stays below, 2 = too many entries share the place.
+__device__ int sm_cross(SmPick& s, const int (&place)[SM_PER], const unsigned long long (&comp)[SM_PER],
+                        const unsigned long long (&wt)[SM_PER], unsigned long long before, unsigned long long want)
 {
     __syncthreads();
-    for (int k = 2; k <= n; k <<= 1)
-        for (int j = k >> 1; j; j >>= 1)
+    s.hist[threadIdx.x] = 0;
+    if (threadIdx.x == 0) s.bin = -1, s.m = 0;
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < SM_PER; ++j)
+        if (wt[j]) atomicAdd(&s.hist[place[j]], wt[j]);
+    __syncthreads();
+    const unsigned long long mine = s.hist[threadIdx.x];
+    unsigned long long total;
+    const unsigned long long at = before + sm_scan<SM_T>(mine, s.scratch, total);
+    if (at < want && at + mine >= want) s.bin = (int)threadIdx.x, s.at = at;
+    __syncthreads();
+    const int bin = s.bin;
+    if (bin < 0) return 1;
+#pragma unroll
+    for (int j = 0; j < SM_PER; ++j)
+        if (wt[j] && place[j] == bin)
         {
-            for (int t = threadIdx.x; t < n / 2; t += SM_T)
-            {
-                const int i = 2 * t - (t & (j - 1)), l = i + j;
-                const unsigned long long x = v[i], y = v[l];
-                if ((x < y) == ((i & k) == 0)) v[i] = y, v[l] = x;
-            }
-            if (j > 64 || (j == 1 && k >= 128)) __syncthreads();
-            else asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            const int i = atomicAdd(&s.m, 1);
+            if (i < SM_T) s.comp[i] = comp[j], s.wt[i] = wt[j];
         }
     __syncthreads();
+    const int m = s.m;
+    if (m > SM_T) return 2;
+    if ((int)threadIdx.x < m)
+    {
+        const unsigned long long c = s.comp[threadIdx.x], x = s.wt[threadIdx.x];
+        unsigned long long sum = s.at;
+        for (int i = 0; i < m; ++i)
+            if (s.comp[i] > c) sum += s.wt[i];
+        if (sum < want && sum + x >= want) s.cut = c, s.cut_wt = x;
+    }
+    __syncthreads();
+    return 0;
+}
+
+// the sum at which the draw stops: the smallest whole number past u * total
+__device__ __forceinline__ unsigned long long sm_target(float u, unsigned long long total)
+{
+    const double t = fmax((double)u * (double)total, 0.0);   // a NaN too becomes 0
+    return t < (double)total ? min((unsigned long long)t + 1, total) : total;
 }
 
 template <typename E>
@@ -682,204 +769,150 @@ __global__ __launch_bounds__(SM_T) void sm_pick_kernel(SampleArgs a, SmWs w)
     __shared__ union
     {
         SmShared slow;
-        struct
-        {
-            unsigned long long list[SM_LIST];
-            unsigned long long scratch[SM_W];
-            unsigned long long part[SM_MAXS];
-            unsigned long long cut, at;
-            int n, pick;
-        } f;
+        SmPick f;
     } sh;
     const int b = blockIdx.x, V = a.V;
-    // loaded ahead of the head: the list's entries of this thread (those past its end are not used) and a slice's weight
+    SmPick& f = sh.f;
+    // loaded ahead of the head: this thread's list entries (those past its end are not used) and a slice's weight
     const unsigned long long* list = w.list + (size_t)b * SM_LIST;
-    unsigned long long entry[SM_LIST / SM_T], slice_mass = 0;
+    unsigned long long comp[SM_PER], slice_mass = 0;
 #pragma unroll
-    for (int j = 0; j < SM_LIST / SM_T; ++j) entry[j] = list[threadIdx.x + j * SM_T];
+    for (int j = 0; j < SM_PER; ++j) comp[j] = list[threadIdx.x + j * SM_T];
     if ((int)threadIdx.x < w.S) slice_mass = w.slice[(size_t)b * w.S + threadIdx.x].mass;
     const SmState st = w.state[b];
     const SmHead h = sm_head(a, w, b);
+    auto answer = [&](int token, unsigned long long x, unsigned long long total) {
+        a.token[b] = token;
+        if (a.prob) a.prob[b] = (float)((double)x / (double)total);
+    };
     if (h.done)
     {
         if (threadIdx.x == 0)
         {
             const bool none = h.top <= SM_MASKED;
-            a.token[b] = none ? -1 : h.arg;
-            if (a.prob) a.prob[b] = none ? 0.0f : 1.0f;
+            answer(none ? -1 : h.arg, none ? 0 : 1, 1);
         }
         return;
     }
-    const E* rowp = static_cast<const E*>(a.logits) + (int64_t)b * a.ld;
-    if (st.mode == SM_SLOW)
-    {
-        SmRow row;
-        row.dtype = a.dtype;
-        row.p = rowp;
-        sm_row_slow(sh.slow, a, b, row, h.top, h.scale);
-        return;
-    }
-    const float mpf = a.min_p ? a.min_p[b] : 0.0f;
-    const double mp = mpf > 0.0f ? (double)mpf : 0.0;
-    const double u = (double)a.u[b];
-    auto& f = sh.f;
-    const int n = st.mode == SM_ALL ? 0 : min(st.count, SM_LIST);
-    int pow2 = 2;
-    while (pow2 < n) pow2 <<= 1;
-    constexpr int PER = SM_LIST / SM_T;   // entries of a thread: 4 neighbours
-    unsigned long long total = 0;
-    if (threadIdx.x == 0) f.n = n, f.pick = -1;
-    if (n)
-    {
-#pragma unroll
-        for (int j = 0; j < SM_LIST / SM_T; ++j)
-        {
-            const int i = threadIdx.x + j * SM_T;
-            if (i < pow2) f.list[i] = i < n ? entry[j] : 0;
-        }
-        sm_sort(f.list, pow2);
-    }
-    else __syncthreads();
-    // weight of a list entry; the masked never enter the list
-    auto exp_of = [&](unsigned long long e) { return sm_exp((uint32_t)(e >> 32), h.top, h.scale); };
-    const int k = sm_topk(a, b);
-    if (n)
-    {
-        // how many entries of the sorted list are kept
-        const int lim = st.mode == SM_TOPK ? min(n, k) : n;
-        unsigned long long wt[PER], mine = 0, sum;
-        bool drop[PER];
-#pragma unroll
-        for (int j = 0; j < PER; ++j)
-        {
-            const int i = threadIdx.x * PER + j;
-            const double e = i < lim ? exp_of(f.list[i]) : 0.0;
-            drop[j] = i < lim && e < mp && (uint32_t)(f.list[i] >> 32) != h.top;
-            wt[j] = sm_units(e);
-            mine += wt[j];
-        }
-        unsigned long long at = sm_scan<SM_T>(mine, f.scratch, sum);
-        unsigned long long want = st.want;
-        if (st.mode == SM_TOPK)
-        {
-            const float p = sm_topp(a, b);
-            const double goal = p < 1.0f ? (double)p * (double)sum : (double)sum;
-            want = p < 1.0f ? (goal > 1.0 ? (unsigned long long)ceil(goal) : 1ull) : ~0ull;
-        }
-        else at += st.above;
-        int keep = lim;
-#pragma unroll
-        for (int j = 0; j < PER; ++j)
-        {
-            const int i = threadIdx.x * PER + j;
-            if (i < lim && at < want && at + wt[j] >= want) keep = min(keep, i + 1);
-            if (drop[j]) keep = min(keep, i);
-            at += wt[j];
-        }
-        if (keep < lim) atomicMin(&f.n, keep);
-        else if (threadIdx.x == 0) atomicMin(&f.n, lim);
+    const E* row = static_cast<const E*>(a.logits) + (int64_t)b * a.ld;
+    auto slow = [&]() {
+        SmRow r;
+        r.dtype = a.dtype;
+        r.p = row;
         __syncthreads();
+        sm_row_slow(sh.slow, a, b, r, h.top, h.scale);
+    };
+    if (st.mode == SM_SLOW || (st.mode != SM_ALL && st.count > SM_LIST)) return slow();
+    const double mp = sm_minp(a, b);
+    const int n = st.mode == SM_ALL ? 0 : st.count;
+    unsigned long long wt[SM_PER], total = 0, cut = 0;
+    int place[SM_PER];
+    const float per_bin = (float)SM_T / (float)(st.hi - st.lo + 1);
+#pragma unroll
+    for (int j = 0; j < SM_PER; ++j)
+    {
+        const bool in = (int)threadIdx.x + j * SM_T < n;
+        const uint32_t key = (uint32_t)(comp[j] >> 32);
+        wt[j] = 0;
+        place[j] = 0;
+        if (in)
+        {
+            const double e = sm_exp(key, h.top, h.scale);
+            wt[j] = sm_units(e);
+            place[j] = (int)fminf(fmaxf((fminf(h.place(key), (float)SM_BINS) - (float)st.lo) * per_bin, 0.0f), (float)(SM_T - 1));
+        }
     }
-    const int kept = f.n;
+    auto kept_by_min = [&](uint32_t key) { return mp == 0.0 || key == h.top || sm_exp(key, h.top, h.scale) >= mp; };
+
     if (st.mode == SM_TOPK)
     {
-        // the kept entries in index order
-        __syncthreads();
-        int p2 = 2;
-        while (p2 < kept) p2 <<= 1;
-        unsigned long long mv[PER];
-#pragma unroll
-        for (int j = 0; j < PER; ++j)
+        const int k = sm_topk(a, b);
+        const float p = sm_topp(a, b);
+        if (n > k)
         {
-            const int i = threadIdx.x + j * SM_T;
-            if (i < p2) mv[j] = i < kept ? f.list[i] << 32 | f.list[i] >> 32 : 0;   // ~index first: descending is by index
+            unsigned long long one[SM_PER];
+#pragma unroll
+            for (int j = 0; j < SM_PER; ++j) one[j] = (int)threadIdx.x + j * SM_T < n;
+            if (sm_cross(f, place, comp, one, 0, (unsigned long long)k)) return slow();
+            cut = f.cut;
+#pragma unroll
+            for (int j = 0; j < SM_PER; ++j)
+                if (comp[j] < cut) wt[j] = 0;
         }
-        __syncthreads();
-#pragma unroll
-        for (int j = 0; j < PER; ++j)
+        unsigned long long mine = 0;
+        if (p < 1.0f)
         {
-            const int i = threadIdx.x + j * SM_T;
-            if (i < p2) f.list[i] = mv[j];
+#pragma unroll
+            for (int j = 0; j < SM_PER; ++j) mine += wt[j];
+            sm_scan<SM_T>(mine, f.scratch, total);
+            const double goal = (double)p * (double)total;
+            if (sm_cross(f, place, comp, wt, 0, goal > 1.0 ? (unsigned long long)ceil(goal) : 1ull)) return slow();
+            cut = f.cut;
+#pragma unroll
+            for (int j = 0; j < SM_PER; ++j)
+                if (comp[j] < cut) wt[j] = 0;
         }
-        sm_sort(f.list, p2);
-        unsigned long long wt[PER], mine = 0;
+        mine = 0;
+        unsigned long long by_index[SM_PER];
+        const float per_index = (float)SM_T / (float)V;
 #pragma unroll
-        for (int j = 0; j < PER; ++j)
+        for (int j = 0; j < SM_PER; ++j)
         {
-            const int i = threadIdx.x * PER + j;
-            wt[j] = i < kept ? sm_units(exp_of(f.list[i] << 32)) : 0;
+            if (wt[j] && !kept_by_min((uint32_t)(comp[j] >> 32))) wt[j] = 0;
             mine += wt[j];
+            by_index[j] = (uint32_t)comp[j];   // ~index: the lowest index is the largest
+            place[j] = min((int)((float)~(uint32_t)comp[j] * per_index), SM_T - 1);
         }
-        unsigned long long at = sm_scan<SM_T>(mine, f.scratch, total);
-        const double target = fmax(u * (double)total, 0.0);   // a NaN too becomes 0
-#pragma unroll
-        for (int j = 0; j < PER; ++j)
-        {
-            const int i = threadIdx.x * PER + j;
-            // the first entry past the target, or the last with weight where none is
-            if (wt[j] && !((double)at > target) && ((double)(at + wt[j]) > target || at + wt[j] == total))
-            {
-                a.token[b] = (int32_t)~(uint32_t)(f.list[i] >> 32);
-                if (a.prob) a.prob[b] = (float)((double)wt[j] / (double)total);
-            }
-            at += wt[j];
-        }
+        sm_scan<SM_T>(mine, f.scratch, total);
+        if (sm_cross(f, place, by_index, wt, 0, sm_target(a.u[b], total))) return slow();
+        if (threadIdx.x == 0) answer((int)~(uint32_t)f.cut, f.cut_wt, total);
         return;
     }
-    // from the slices: their weight above the bin and that of the list's kept entries
+    // from the slices: their weight above the list's bins and that of the list's kept entries
+    if (st.mode == SM_BIN)
+    {
+        const int r = sm_cross(f, place, comp, wt, st.above, st.want);
+        if (r == 2) return slow();
+        cut = r ? 0 : f.cut;   // not reached: min-p ends first
+    }
+    __syncthreads();
     if ((int)threadIdx.x < w.S) f.part[threadIdx.x] = slice_mass;
     __syncthreads();
-    for (int i = threadIdx.x; i < kept; i += SM_T)
-    {
-        const uint32_t idx = ~(uint32_t)f.list[i];
-        atomicAdd(&f.part[idx / (uint32_t)w.len], (unsigned long long)sm_units(exp_of(f.list[i])));
-    }
-    if (threadIdx.x == 0) f.cut = st.mode == SM_ALL ? 0 : kept ? f.list[kept - 1] : ~0ull;
+#pragma unroll
+    for (int j = 0; j < SM_PER; ++j)
+        if (wt[j] && comp[j] >= cut && kept_by_min((uint32_t)(comp[j] >> 32)))
+            atomicAdd(&f.part[~(uint32_t)comp[j] / (uint32_t)w.len], wt[j]);
     __syncthreads();
-    // the last kept entry as key and index; an empty list keeps what lies above the bin, which starts at the list's first
-    const unsigned long long none_above = n ? f.list[0] : 0;
-    const unsigned long long cut = f.cut;
-    unsigned long long at = 0;
     const unsigned long long mine = (int)threadIdx.x < w.S ? f.part[threadIdx.x] : 0;
-    at = sm_scan<SM_T>(mine, f.scratch, total);
-    const double target = fmax(u * (double)total, 0.0);
-    if (mine && !((double)at > target) && ((double)(at + mine) > target || at + mine == total))
-        f.pick = (int)threadIdx.x, f.at = at;
+    unsigned long long at = sm_scan<SM_T>(mine, f.scratch, total);
+    const unsigned long long target = sm_target(a.u[b], total);
+    if (at < target && at + mine >= target) f.pick = (int)threadIdx.x, f.at = at;
     __syncthreads();
     const int s = f.pick, lo = s * w.len, hi = min(V, lo + w.len), per = (hi - lo + SM_T - 1) / SM_T;
     const int i0 = lo + (int)threadIdx.x * per, i1 = min(hi, i0 + per);
     const unsigned long long base = f.at;
     auto weight = [&](int i) -> unsigned long long {
-        const uint32_t key = sm_key(static_cast<float>(rowp[i]));
-        if (key <= SM_MASKED) return 0;
-        const unsigned long long e = (unsigned long long)key << 32 | (uint32_t)~i;
-        if (cut == ~0ull ? e <= none_above : e < cut) return 0;
+        const uint32_t key = sm_key(static_cast<float>(row[i]));
+        if (key <= SM_MASKED || ((unsigned long long)key << 32 | (uint32_t)~i) < cut) return 0;
         const double x = sm_exp(key, h.top, h.scale);
         return key == h.top || x >= mp ? sm_units(x) : 0;
     };
     unsigned long long sum = 0, all;
     for (int i = i0; i < i1; ++i) sum += weight(i);
     unsigned long long c = base + sm_scan<SM_T>(sum, f.scratch, all);
-    const unsigned long long end = base + all;
-    if (sum && !((double)c > target) && ((double)(c + sum) > target || c + sum == end))
+    if (c < target && c + sum >= target)
         for (int i = i0; i < i1; ++i)
         {
             const unsigned long long x = weight(i);
-            if (!x) continue;
+            if (c < target && c + x >= target) answer(i, x, total);
             c += x;
-            if ((double)c > target || c == end)
-            {
-                a.token[b] = i;
-                if (a.prob) a.prob[b] = (float)((double)x / (double)total);
-                break;
-            }
         }
 }
 
 size_t sample_ws_bytes(int B, int V)
 {
     SmWs w;
-    return B ? sm_carve(nullptr, B, V, w) : 0;
+    return B ? sm_carve(nullptr, B < SM_ROWS ? B : SM_ROWS, V, w) : 0;
 }
 
 template <typename E>
@@ -892,13 +925,26 @@ static void sm_go(const SampleArgs& a, const SmWs& w, hipStream_t st)
     hipLaunchKernelGGL(sm_pick_kernel<E>, dim3(a.B), dim3(SM_T), 0, st, a, w);
 }
 
-void launch_sample(const SampleArgs& a, hipStream_t st)
+void launch_sample(const SampleArgs& all, hipStream_t st)
 {
     SmWs w;
-    sm_carve(a.ws, a.B, a.V, w);
-    if (a.dtype == 2) sm_go<float>(a, w, st);
-    else if (a.dtype == 1) sm_go<__bf16>(a, w, st);
-    else sm_go<_Float16>(a, w, st);
+    sm_carve(all.ws, all.B < SM_ROWS ? all.B : SM_ROWS, all.V, w);
+    for (int b = 0; b < all.B; b += SM_ROWS)
+    {
+        SampleArgs a = all;
+        a.B = all.B - b < SM_ROWS ? all.B - b : SM_ROWS;
+        a.logits = static_cast<const char*>(all.logits) + (int64_t)b * all.ld * (all.dtype == 2 ? 4 : 2);
+        if (a.temperature) a.temperature += b;
+        if (a.top_k) a.top_k += b;
+        if (a.top_p) a.top_p += b;
+        if (a.min_p) a.min_p += b;
+        a.u += b;
+        a.token += b;
+        if (a.prob) a.prob += b;
+        if (a.dtype == 2) sm_go<float>(a, w, st);
+        else if (a.dtype == 1) sm_go<__bf16>(a, w, st);
+        else sm_go<_Float16>(a, w, st);
+    }
 }
 
 }  // namespace gfl

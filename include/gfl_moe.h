@@ -316,7 +316,7 @@ int gfl_i8_workspace(int M, int N, int K, size_t* gemm, size_t* linear);
  * kept weights summed up to i exceed u * their sum; prob (fp32 [B], may be NULL) = its weight / that sum. -inf and NaN logits
  * are never drawn; a row with nothing else gives token -1 and prob 0. With +inf logits only they are drawn. Weights are
  * computed in fp64 and summed as integers in units of 2^-43 of the largest, so results do not depend on the order of
- * sums. B <= 65535, V <= 2^20. */
+ * sums. V <= 2^20. */
 int gfl_sample(const void* logits, int64_t ld, int dtype, int B, int V, const float* temperature, const int32_t* top_k,
                const float* top_p, const float* min_p, const float* u, int64_t* token, float* prob, void* ws,
                size_t ws_bytes, gfl_stream stream);

@@ -77,7 +77,7 @@ def test_sample_refusals(lib):
     def call(logits=P, ld=100, dtype=2, B=2, V=100, u=P, token=P, ws=P, nb=1 << 24):
         return lib.gfl_sample(logits, ld, dtype, B, V, None, None, None, None, u, token, None, ws, nb, None)
 
-    for kw, word in ((dict(dtype=3), "dtype"), (dict(B=-1), "B"), (dict(B=65536), "B"), (dict(V=0), "V"), (dict(V=(1 << 20) + 1, ld=1 << 21), "V"),
+    for kw, word in ((dict(dtype=3), "dtype"), (dict(B=-1), "B"), (dict(V=0), "V"), (dict(V=(1 << 20) + 1, ld=1 << 21), "V"),
                      (dict(ld=99), "stride"), (dict(logits=None), "NULL"), (dict(u=None), "NULL"), (dict(token=None), "NULL")):
         _refused(lib, call(**kw), word)
     assert call(B=0, logits=None, u=None, token=None) == 0

@@ -403,6 +403,21 @@ def test_sample_large_k_and_low_temperature(gpu, dt):
         _check_draw(x, u, temperature=[t] * 6, min_p=[0.02] * 6, skip=1)
 
 
+def test_sample_many_rows(gpu):
+    """More rows than one round of launches takes: each row's token as the same rows give a round of their own."""
+    import _native
+    g = _rng(23)
+    B, V = 2500, 700
+    x = (torch.randn((B, V), generator=g) * 3).cuda()
+    u, p = torch.rand(B, generator=g).cuda(), (0.5 + torch.rand(B, generator=g)).cuda()
+    k = torch.randint(0, 60, (B,), generator=g, dtype=torch.int32).cuda()
+    tok, prob = _native.sample(x, u, top_k=k, top_p=p)
+    for lo, hi in ((0, 700), (700, 1500), (1500, 2500)):
+        t, q = _native.sample(x[lo:hi], u[lo:hi], top_k=k[lo:hi], top_p=p[lo:hi])
+        assert torch.equal(t, tok[lo:hi]) and torch.equal(q, prob[lo:hi])
+    _check_draw(x[-40:].cpu(), u[-40:].cpu(), top_k=k[-40:].cpu(), top_p=p[-40:].cpu())
+
+
 def test_sample_strided_rows(gpu):
     x = torch.randn((5, 1003), generator=_rng(2))
     buf = torch.full((5, 1100), 1e30, device="cuda")
