@@ -40,9 +40,10 @@ struct SmRow
 // |x| <= ln 2 / 2, whose remainder after degree 12 is below 2^-51. scale = log2(e) / T.
 __device__ __forceinline__ double sm_exp(uint32_t key, uint32_t top, double scale)
 {
-    if (key == top) return 1.0;
-    double y = ((double)sm_value(key) - (double)sm_value(top)) * scale;
-    if (!(y > -1000.0)) return 0.0;   // also a NaN: finite - inf over an infinite T
+    // without branches, so that a thread's values run side by side
+    const double y0 = ((double)sm_value(key) - (double)sm_value(top)) * scale;
+    const bool any = y0 > -1000.0;      // not so for a NaN: finite - inf over an infinite T, inf - inf
+    const double y = any ? y0 : 0.0;
     const double n = rint(y), x = (y - n) * 0.693147180559945309417;
     double p = 1.0 / 479001600;
     p = fma(p, x, 1.0 / 39916800);
@@ -57,7 +58,8 @@ __device__ __forceinline__ double sm_exp(uint32_t key, uint32_t top, double scal
     p = fma(p, x, 0.5);
     p = fma(p, x, 1.0);
     p = fma(p, x, 1.0);
-    return __longlong_as_double(__double_as_longlong(p) + ((long long)(int)n << 52));
+    const double e = __longlong_as_double(__double_as_longlong(p) + ((long long)(int)n << 52));
+    return key == top ? 1.0 : any ? e : 0.0;
 }
 
 // a weight in units of 2^-43 of the largest logit's: added to 2^52, the last bit of the sum is a unit
@@ -216,7 +218,7 @@ __device__ void sm_row_slow(SmShared& s, const SampleArgs& a, int b, const SmRow
         __syncthreads();
     }
     const float mp = a.min_p ? a.min_p[b] : 0.0f;
-    auto kept_by_min = [&](uint32_t key) { return !(mp > 0.0f) || key == top || sm_exp(key, top, scale) >= (double)mp; };
+    auto kept_by_min = [&](uint32_t key) { return !(mp > 0.0f) || sm_exp(key, top, scale) >= (double)mp; };
 
     // each wave takes a run of the row: weight and ties of its run, then the wave that holds the drawn token walks it
     const int per = (V + SM_W * 64 - 1) / (SM_W * 64) * 64, lo = wave * per, hi = min(V, lo + per);
@@ -298,8 +300,10 @@ __device__ void sm_row_slow(SmShared& s, const SampleArgs& a, int b, const SmRow
 //
 // A row is cut into S slices, a workgroup each, so that a few rows fill the card (B = 1, V = 131,072: 64 workgroups; the same
 // work in one workgroup took 547 us). Four launches, for up to SM_ROWS rows at a time:
-//   top     each slice's largest and smallest logit and the largest's index; clears the row's histogram
-//   bins    2,047 bins of equal width from the largest logit down to where weights round to zero (or to the smallest), and
+//   top     each slice's largest and smallest logit and the largest's index, and the largest of each of up to 1,024 groups
+//           of the row; clears the row's histogram
+//   bins    (not for a top-k of up to half the groups: the k-th largest group maximum, rounded down, has at least k logits at
+//           or above it and few more, and is the list's floor) 2,047 bins of equal width from the largest logit down to where weights round to zero (or to the smallest), and
 //           one for what lies below: logits per bin for a top-k, else the weight per bin (of the row and of each slice)
 //   cut     every workgroup finds the bins in which the kept prefix ends from the row's histogram. With a top-k (and few
 //           logits down to its bin) all logits down to that bin go into the row's list; else the list takes the bins
@@ -310,6 +314,7 @@ constexpr int SM_LIST = 4096;         // logits a row's list holds
 constexpr int SM_LISTK = 1024;        // top-k up to which the list is expected to hold the whole kept set
 constexpr int SM_PT = 256;            // threads of the slice launches
 constexpr int SM_MAXS = 256;          // slices of a row
+constexpr int SM_GROUPS = 1024;       // group maxima of a row, at most
 constexpr int SM_ROWS = 1024;         // rows of one round of launches, which bounds the workspace
 constexpr int SM_PER = SM_LIST / SM_T;   // list entries of a thread of the last launch
 
@@ -342,12 +347,14 @@ struct SmWs
     unsigned long long* list;         // [B][SM_LIST] key << 32 | ~index
     SmSlice* slice;                   // [B][S]
     SmState* state;                   // [B]
+    uint32_t* group;                  // [B][SM_GROUPS] keys
     int S, len;                       // slices of a row, logits of a slice
+    int G;                            // groups of a slice: 256 / G neighbouring threads' logits each
 };
 
 static void sm_split(int B, int V, int& S, int& len)
 {
-    const int want = (1024 + B - 1) / B;                     // four workgroups a CU
+    const int want = (2048 + B - 1) / B;                     // eight workgroups a CU
     S = V / 2048 < 1 ? 1 : V / 2048;
     if (S > want) S = want;
     if (S > SM_MAXS) S = SM_MAXS;
@@ -370,10 +377,13 @@ static size_t sm_carve(void* base, int B, int V, SmWs& w)
     w.slice = reinterpret_cast<SmSlice*>(take((size_t)B * w.S * sizeof(SmSlice)));
     w.state = reinterpret_cast<SmState*>(take((size_t)B * sizeof(SmState)));
     w.cnt = reinterpret_cast<uint32_t*>(take((size_t)B * SM_BINS * 4));
+    w.group = reinterpret_cast<uint32_t*>(take((size_t)B * SM_GROUPS * 4));
+    w.G = SM_PT;
+    while (w.G * w.S > SM_GROUPS) w.G /= 2;
     return at;
 }
 
-// use(index, key) for this thread's logits of [lo, hi): 4 neighbours at a time, 4 loads in flight (`b`: the first 4, loaded
+// use(index, 4 keys) for this thread's logits of [lo, hi): 4 neighbours at a time (key 0: none), 4 loads in flight (`b`: the first 4, loaded
 // ahead of what the launch waits for otherwise)
 template <typename E, int NT>
 struct SmBatch
@@ -399,13 +409,13 @@ __device__ __forceinline__ void sm_each(const E* row, int lo, int hi, SmBatch<E,
         for (int j = 0; j < 4; ++j)
         {
             const int at = i + j * NT * 4;
-            if (at + 4 <= hi)
-            {
+            // what lies past the slice counts as masked
+            uint32_t key[4];
 #pragma unroll
-                for (int k = 0; k < 4; ++k) use(at + k, sm_key(static_cast<float>(b.v[j][k])));
-            }
-            else
-                for (int k = at; k < hi; ++k) use(k, sm_key(static_cast<float>(row[k])));   // the slice's last, not whole, chunk
+            for (int k = 0; k < 4; ++k)
+                key[k] = at + 4 <= hi ? sm_key(static_cast<float>(b.v[j][k]))
+                         : at + k < hi ? sm_key(static_cast<float>(row[at + k])) : 0;
+            use(at, key);
         }
         i = next;
         b = n;
@@ -417,7 +427,7 @@ struct SmHead
 {
     uint32_t top, low;
     int arg;
-    bool done;            // greedy, or nothing to draw from
+    bool done;            // the largest logit, or nothing to draw from
     bool wide;            // a range past fp32: no bins
     float T, top_x, bins; // bins per unit of logit
     double scale;
@@ -441,7 +451,8 @@ __device__ __forceinline__ SmHead sm_head(const SampleArgs& a, const SmWs& w, in
     h.low = sm_wave_min(low);
     h.arg = (int)sm_wave_min(top == h.top ? (uint32_t)arg : 0x7FFFFFFFu);
     h.T = a.temperature ? a.temperature[b] : 1.0f;
-    h.done = h.top <= SM_MASKED || !(h.T > 0.0f);
+    // a min-p past 1 keeps the largest logit alone
+    h.done = h.top <= SM_MASKED || !(h.T > 0.0f) || (a.min_p && a.min_p[b] > 1.0f);
     h.top_x = sm_value(h.top);
     h.scale = 1.4426950408889634074 / (double)h.T;
     // down to the smallest logit (a little past it, so that it lies in a bin of its own right) or to where weights round to
@@ -467,10 +478,18 @@ __global__ __launch_bounds__(SM_PT) void sm_top_kernel(SampleArgs a, SmWs w)
     if (s == 0 && threadIdx.x == 0) w.state[b].count = 0;
     uint32_t top = 0, low = ~0u;
     int arg = 0x7FFFFFFF;
-    sm_each<E, SM_PT>(row, lo, hi, first, [&](int i, uint32_t k) {
-        if (k > top) top = k, arg = i;
-        if (k > SM_MASKED) low = min(low, k);
+    sm_each<E, SM_PT>(row, lo, hi, first, [&](int i, const uint32_t (&key)[4]) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+        {
+            if (key[j] > top) top = key[j], arg = i + j;
+            if (key[j] > SM_MASKED) low = min(low, key[j]);
+        }
     });
+    uint32_t group = top;
+    const int lanes = SM_PT / w.G;   // 1 to 64
+    for (int o = 1; o < lanes; o <<= 1) group = max(group, (uint32_t)__shfl_xor((int)group, o));
+    if (threadIdx.x % lanes == 0) w.group[(size_t)b * SM_GROUPS + s * w.G + threadIdx.x / lanes] = group;
     __shared__ uint32_t st[SM_PT / 64], sl[SM_PT / 64];
     __shared__ int sa[SM_PT / 64];
     const uint32_t wt = sm_wave_max(top), wl = sm_wave_min(low);
@@ -508,6 +527,57 @@ __device__ __forceinline__ double sm_minp(const SampleArgs& a, int b)
     return m > 0.0f ? (double)m : 0.0;
 }
 
+// The list's floor for a top-k from the group maxima: a key that at least k logits reach, the k-th largest maximum with all but
+// its leading 14 bits past those common to all cleared. False where the groups do not tell. One wave's work (sm_floor asks the
+// first one).
+__device__ __forceinline__ bool sm_floor_wave(const SmWs& w, int b, int k, uint32_t top, uint32_t& floor)
+{
+    const int ng = w.S * w.G, lane = threadIdx.x % 64;
+    if (!k || 2 * k > ng) return false;
+    uint32_t v[SM_GROUPS / 64], low = ~0u;
+    int valid = 0;
+#pragma unroll
+    for (int i = 0; i < SM_GROUPS / 64; ++i)
+        v[i] = i * 64 + lane < ng ? w.group[(size_t)b * SM_GROUPS + i * 64 + lane] : 0;
+#pragma unroll
+    for (int i = 0; i < SM_GROUPS / 64; ++i)
+    {
+        const bool in = v[i] > SM_MASKED;
+        valid += __popcll(__ballot(in));
+        if (in) low = min(low, v[i]);
+    }
+    if (valid < k) return false;
+    low = sm_wave_min(low);
+    floor = top;
+    if (low == top) return true;
+    const int first = 31 - __clz((int)(top ^ low));
+    floor = top >> first >> 1 << first << 1;
+    for (int bit = first; bit >= 0 && bit > first - 14; --bit)
+    {
+        const uint32_t c = floor | 1u << bit;
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < SM_GROUPS / 64; ++i) n += __popcll(__ballot(v[i] >= c));
+        if (n >= k) floor = c;
+    }
+    return true;
+}
+__device__ __forceinline__ bool sm_floor(const SmWs& w, int b, int k, uint32_t top, uint32_t& floor, int* shared)
+{
+    if (!k || 2 * k > w.S * w.G) return false;
+    if (threadIdx.x < 64)
+    {
+        uint32_t f = 0;
+        const bool ok = sm_floor_wave(w, b, k, top, f);
+        if (threadIdx.x == 0) shared[0] = ok, shared[1] = (int)f;
+    }
+    __syncthreads();
+    const bool ok = shared[0];
+    floor = (uint32_t)shared[1];
+    __syncthreads();
+    return ok;
+}
+
 // rows whose list a top-k fills take logits per bin; the others with a nucleus their weight
 __device__ __forceinline__ bool sm_weighs(int k, float p) { return p < 1.0f && (!k || k > SM_LISTK); }
 
@@ -524,19 +594,31 @@ __global__ __launch_bounds__(SM_PT) void sm_bins_kernel(SampleArgs a, SmWs w)
     const int k = sm_topk(a, b);
     const float p = sm_topp(a, b);
     if (h.done || h.wide || (!k && !(p < 1.0f))) return;
+    uint32_t floor;
+    __shared__ int shared[2];
+    if (sm_floor(w, b, k, h.top, floor, shared)) return;
     const bool weigh = sm_weighs(k, p);
     for (int i = threadIdx.x; i < SM_BINS; i += SM_PT) cnt[i] = 0, mass[i] = 0;
     __syncthreads();
     if (weigh)
-        sm_each<E, SM_PT>(row, lo, hi, first, [&](int, uint32_t key) {
-            if (key <= SM_MASKED) return;
-            const int bin = h.bin(key);
-            if (k) atomicAdd(&cnt[bin], 1u);
-            if (bin < SM_BINS - 1) atomicAdd(&mass[bin], (unsigned long long)sm_weight(key, h.top, h.scale));
+        sm_each<E, SM_PT>(row, lo, hi, first, [&](int, const uint32_t (&key)[4]) {
+            unsigned long long x[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[j] = sm_weight(key[j], h.top, h.scale);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (key[j] > SM_MASKED)
+                {
+                    const int bin = h.bin(key[j]);
+                    if (k) atomicAdd(&cnt[bin], 1u);
+                    if (bin < SM_BINS - 1) atomicAdd(&mass[bin], x[j]);
+                }
         });
     else
-        sm_each<E, SM_PT>(row, lo, hi, first, [&](int, uint32_t key) {
-            if (key > SM_MASKED) atomicAdd(&cnt[h.bin(key)], 1u);
+        sm_each<E, SM_PT>(row, lo, hi, first, [&](int, const uint32_t (&key)[4]) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (key[j] > SM_MASKED) atomicAdd(&cnt[h.bin(key[j])], 1u);
         });
     __syncthreads();
     unsigned long long* part = w.part + ((size_t)b * w.S + s) * SM_BINS;
@@ -572,14 +654,22 @@ struct SmCut
 {
     int mode, lo, hi;
     unsigned long long want, above;
+    uint32_t floor;      // smallest key of the list (where it is not given by the bins: 0)
 };
 __device__ SmCut sm_cut(const SampleArgs& a, const SmWs& w, int b, const SmHead& h, unsigned long long* scratch, int* found)
 {
     constexpr int PER = SM_BINS / SM_PT;
     const int k = sm_topk(a, b);
     const float p = sm_topp(a, b);
-    SmCut c = { SM_ALL, 0, SM_BINS - 1, 0, 0 };
+    SmCut c = { SM_ALL, 0, SM_BINS - 1, 0, 0, 0 };
     if (!k && !(p < 1.0f)) return c;
+    if (sm_floor(w, b, k, h.top, c.floor, found))
+    {
+        c.mode = SM_TOPK;
+        c.hi = h.bin(c.floor);
+        return c;
+    }
+    c.floor = 0;
     if (h.wide)
     {
         c.mode = SM_SLOW;
@@ -662,8 +752,10 @@ __global__ __launch_bounds__(SM_PT) void sm_cut_kernel(SampleArgs a, SmWs w)
     __shared__ int found[2];
     const int b = blockIdx.y, s = blockIdx.x, lo = s * w.len, hi = min(a.V, lo + w.len);
     const E* row = static_cast<const E*>(a.logits) + (int64_t)b * a.ld;
+    // short slices are loaded ahead; of long ones many rows read only some groups
+    const bool ahead = w.len <= SM_PT * 16;
     SmBatch<E, SM_PT> first;
-    first.load(row, lo + threadIdx.x * 4, hi);
+    if (ahead) first.load(row, lo + threadIdx.x * 4, hi);
     const SmHead h = sm_head(a, w, b);
     if (h.done) return;
     const SmCut c = sm_cut(a, w, b, h, scratch, found);
@@ -677,25 +769,47 @@ __global__ __launch_bounds__(SM_PT) void sm_cut_kernel(SampleArgs a, SmWs w)
         st.above = c.above;
     }
     if (c.mode == SM_SLOW) return;
+    if (!ahead && !(c.floor && w.group[(size_t)b * SM_GROUPS + s * w.G + threadIdx.x / (SM_PT / w.G)] < c.floor))
+        first.load(row, lo + threadIdx.x * 4, hi);
     unsigned long long mine = 0, total;
     if (c.mode == SM_ALL)
     {
         const double m = sm_minp(a, b);
-        sm_each<E, SM_PT>(row, lo, hi, first, [&](int, uint32_t key) {
-            if (key <= SM_MASKED) return;
-            const double e = sm_exp(key, h.top, h.scale);
-            if (key == h.top || e >= m) mine += sm_units(e);
+        sm_each<E, SM_PT>(row, lo, hi, first, [&](int, const uint32_t (&key)[4]) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+            {
+                const double e = sm_exp(key[j], h.top, h.scale);
+                mine += key[j] > SM_MASKED && e >= m ? sm_units(e) : 0;
+            }
         });
     }
     else
     {
         unsigned long long* list = w.list + (size_t)b * SM_LIST;
-        sm_each<E, SM_PT>(row, lo, hi, first, [&](int i, uint32_t key) {
-            const int bin = h.bin(key);
-            if (key <= SM_MASKED || bin < c.lo || bin > c.hi) return;
+        auto put = [&](int i, uint32_t key) {
             const int at = atomicAdd(&w.state[b].count, 1);
             if (at < SM_LIST) list[at] = (unsigned long long)key << 32 | (uint32_t)~i;
-        });
+        };
+        if (c.floor)
+        {
+            // only the groups that reach the floor are read
+            if (w.group[(size_t)b * SM_GROUPS + s * w.G + threadIdx.x / (SM_PT / w.G)] >= c.floor)
+                sm_each<E, SM_PT>(row, lo, hi, first, [&](int i, const uint32_t (&key)[4]) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        if (key[j] >= c.floor && key[j] > SM_MASKED) put(i + j, key[j]);
+                });
+        }
+        else
+            sm_each<E, SM_PT>(row, lo, hi, first, [&](int i, const uint32_t (&key)[4]) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                {
+                    const int bin = h.bin(key[j]);
+                    if (key[j] > SM_MASKED && bin >= c.lo && bin <= c.hi) put(i + j, key[j]);
+                }
+            });
         if (c.mode == SM_TOPK) return;
         const unsigned long long* part = w.part + ((size_t)b * w.S + s) * SM_BINS;
         for (int i = threadIdx.x; i < c.lo; i += SM_PT) mine += part[i];
@@ -822,7 +936,7 @@ __global__ __launch_bounds__(SM_T) void sm_pick_kernel(SampleArgs a, SmWs w)
             place[j] = (int)fminf(fmaxf((fminf(h.place(key), (float)SM_BINS) - (float)st.lo) * per_bin, 0.0f), (float)(SM_T - 1));
         }
     }
-    auto kept_by_min = [&](uint32_t key) { return mp == 0.0 || key == h.top || sm_exp(key, h.top, h.scale) >= mp; };
+    auto kept_by_min = [&](uint32_t key) { return mp == 0.0 || sm_exp(key, h.top, h.scale) >= mp; };
 
     if (st.mode == SM_TOPK)
     {
@@ -895,7 +1009,7 @@ __global__ __launch_bounds__(SM_T) void sm_pick_kernel(SampleArgs a, SmWs w)
         const uint32_t key = sm_key(static_cast<float>(row[i]));
         if (key <= SM_MASKED || ((unsigned long long)key << 32 | (uint32_t)~i) < cut) return 0;
         const double x = sm_exp(key, h.top, h.scale);
-        return key == h.top || x >= mp ? sm_units(x) : 0;
+        return x >= mp ? sm_units(x) : 0;
     };
     unsigned long long sum = 0, all;
     for (int i = i0; i < i1; ++i) sum += weight(i);

@@ -363,6 +363,8 @@ def test_sample_ties(gpu, V):
         _check_draw(x, [u] * 6, top_p=[0.3001] * 6, skip=6)
         _check_draw(x, [u] * 6, top_k=[40] * 6, top_p=[0.5013] * 6)
         _check_draw(x, [u] * 6, min_p=[0.9] * 6)
+        _check_draw(x, [u] * 6, min_p=[1.0] * 6)
+        _check_draw(x, [u] * 6, min_p=[2.0] * 6, top_p=[0.6] * 6, skip=6)
     tok, _ = _draw(x, [0.0] * 6, temperature=[0.0] * 6)
     assert tok.tolist() == [0, 5, 0, 17, 200, 0]
 
