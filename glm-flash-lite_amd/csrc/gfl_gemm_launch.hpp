@@ -43,7 +43,7 @@ static int gm_tiles(GmArgs& a, const GmPlan& p, int aligned, int nz, hipStream_t
     if constexpr (!AKS)
     {
         if (p.tm == 64) return gm_go<T, 64, 128, 1, 4, AKS, BKS, DUAL, 3, true, EP>(a, nz, st);
-        if (p.deep) return gm_go<T, 128, 128, 2, 4, AKS, BKS, DUAL, 4, true, EP>(a, nz, st);
+        if (p.deep) return gm_go<T, 128, 128, 2, 4, AKS, BKS, DUAL, 5, true, EP>(a, nz, st);
     }
     if (p.tm == 128) return gm_go<T, 128, 128, 2, 2, AKS, BKS, DUAL, 2, true, EP>(a, nz, st);
     if constexpr (EP == EP_PART) return -1;   // not split (gm_plan)
@@ -97,7 +97,7 @@ static int gm_run(int form, int ep, int aligned, GmArgs& a, void* ws, size_t ws_
 {
     if constexpr (!AKS && !BKS)
         if (a.M <= 16) return gm_few<T, DUAL, EP>(a, aligned, st);
-    GmPlan p = gm_plan(form, ep, DUAL, aligned, a.M, a.N, a.K, a.segs);
+    GmPlan p = gm_plan(form, ep, DUAL, aligned, a.M, a.N, a.K, a.segs, nz);
     if (p.parts > 1 && (!ws || ws_bytes < p.part_bytes)) return -2;
     if (p.parts == 1) return gm_tiles<T, AKS, BKS, DUAL, EP>(a, p, aligned, nz, st);
     if constexpr (AKS) return -1;   // never split (gm_plan)

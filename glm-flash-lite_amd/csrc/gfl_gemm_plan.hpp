@@ -10,7 +10,7 @@ namespace gfl {
 struct GmPlan
 {
     int tm, tn;          // output rows and columns of a tile (tn: of each of the two matrices of a gate|up product)
-    int deep;            // 128-row tiles: 8 waves and 4 steps of loads, one workgroup a CU (else 4 waves, 2 steps, two a CU)
+    int deep;            // 128-row tiles: 8 waves and 5 steps of loads, one workgroup a CU (else 4 waves, 2 steps, two a CU)
     int parts;           // K parts
     int64_t ldp;         // elements between the rows of a part
     size_t part_bytes;
@@ -18,12 +18,14 @@ struct GmPlan
 
 // Estimated time of each tile and number of K parts, the least of which is taken. A workgroup's K step of 128 bytes a row
 // costs nearly the same whether its CU's other places are filled or not (it waits for its loads), so what counts is how many
-// rounds of workgroups there are and how full they are; and the bytes of B, read at 4.8 TB/s, are a floor. Measured, bf16, us a
-// step, in a round that fills half the places and in a fuller one: 128 x 128 0.83 and 1.03, deep 0.62 (1.0 with B [K][N]), 64 x
-// 128 0.5, 256 x 256 1.05 and 1.5; 3 for the launch with its first loads and last stores; a join 2.5 and the parts' bytes written and read at 4 TB/s.
-// Against measured launches it is within 15%: 333 x 2048 x 11008 in 10 parts 37 (33 measured), in 1 part 146 (167); 101 x 2 x
-// 12288 x 5120 deep 56 (53), 128 x 128 69 (72); 4096 x 12288 x 5120 of 256 x 256 393 (370), 4096 x 5120 x 12288 493 (486).
-inline GmPlan gm_plan(int form, int ep, int dual, int aligned, int M, int N, int K, int segs)
+// rounds of workgroups there are and how full they are, with the first loads and last stores of each; and the bytes of B, read
+// at 4.8 TB/s, are a floor. Measured, 16-bit types, us a step, in a round that fills half the places and in a fuller one: 128 x
+// 128 0.83 and 1.03, deep 0.62, 64 x 128 0.5, 256 x 256 1.05 and 1.5; a round's ends 14 for 256 x 256, 4 for 128 x 128, 2 for the others; 3 for
+// the launch; a join 2.5 and the parts' bytes written and read at 4 TB/s. nz: products of one launch (the gradients of gate and
+// up), which fill rounds together.
+// Against the other choice, us of a backward call for the gradients of gate's and up's weights: 2048 tokens of 5504 x 2048 128 x
+// 128 176, 256 x 256 191; 333 tokens 58 and 65; 1024 tokens of 11008 x 4096 256 x 256 335, 128 x 128 364.
+inline GmPlan gm_plan(int form, int ep, int dual, int aligned, int M, int N, int K, int segs, int nz = 1)
 {
     GmPlan best = {};
     const int d = dual ? 2 : 1;
@@ -34,11 +36,11 @@ inline GmPlan gm_plan(int form, int ep, int dual, int aligned, int M, int N, int
     }
     const int steps = (int)((((int64_t)K * (ep == EP_I8 ? 1 : 2) + 127) / 128) * segs);
     const int64_t ldp = ((int64_t)N + 3) / 4 * 4;
-    struct Tile { int tm, tn, deep, places; double alone, beside; };
-    const double deep = form == GM_NN ? 1.0 : 0.62;
-    const Tile tiles[] = { { 16, 128, 0, 512, 0.45, 0.45 },  { 64, 128, 0, 512, 0.5, 0.5 },   { 128, 128, 1, 256, deep, deep },
-                           { 128, 128, 0, 512, 0.83, 1.03 }, { 256, 256, 0, 256, 1.05, 1.5 } };
-    const double floor = (double)d * N * K * (ep == EP_I8 ? 1 : 2) * segs / 4.8e6;
+    struct Tile { int tm, tn, deep, places; double alone, beside, ends; };
+    const Tile tiles[] = { { 16, 128, 0, 512, 0.45, 0.45, 2 },  { 64, 128, 0, 512, 0.5, 0.5, 2 },
+                           { 128, 128, 1, 256, 0.62, 0.62, 2 }, { 128, 128, 0, 512, 0.83, 1.03, 4 },
+                           { 256, 256, 0, 256, 1.05, 1.5, 14 } };
+    const double floor = (double)d * nz * N * K * (ep == EP_I8 ? 1 : 2) * segs / 4.8e6;
     double least = 0;
     for (const Tile& t : tiles)
     {
@@ -51,10 +53,14 @@ inline GmPlan gm_plan(int form, int ep, int dual, int aligned, int M, int N, int
         for (int p = 1; p <= most; ++p)
         {
             if (p > 1 && wg * (p - 1) >= t.places) break;
-            const int64_t whole = wg * p / t.places, left = wg * p % t.places;
-            double r = whole * t.beside + (left > t.places / 2 ? t.beside : left ? t.alone : 0);
-            if (whole >= 3) r = ((double)(wg * p) / t.places + 0.25) * t.beside;   // many rounds overlap at their ends
-            const double time = std::max(r * ((steps + p - 1) / p), floor) + 3 +
+            const int64_t whole = nz * wg * p / t.places, left = nz * wg * p % t.places;
+            double r = whole * t.beside + (left > t.places / 2 ? t.beside : left ? t.alone : 0), ends = whole + (left > 0);
+            if (whole >= 3)   // many rounds overlap at their ends
+            {
+                ends = (double)(nz * wg * p) / t.places + 0.25;
+                r = ends * t.beside;
+            }
+            const double time = std::max(r * ((steps + p - 1) / p) + ends * t.ends, floor) + 3 +
                                 (p > 1 ? 2.5 + (double)p * d * M * ldp * 8 / 4e6 : 0);
             if (best.parts == 0 || time < least)
             {
