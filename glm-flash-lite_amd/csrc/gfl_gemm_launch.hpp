@@ -92,13 +92,41 @@ static int gm_few(const GmArgs& a, int aligned, hipStream_t st)
     return 0;
 }
 
+// The columns from n on, as a product of their own.
+template <typename T, bool BKS>
+static GmArgs gm_from(const GmArgs& a, int n)
+{
+    constexpr int ES = sizeof(typename T::elem);
+    GmArgs b = a;
+    b.N -= n;
+    const int size = a.odt == 2 ? 4 : 2;   // GFL_F32
+    for (int i = 0; i < 2; ++i)
+    {
+        if (b.B[i]) b.B[i] += (int64_t)n * (BKS ? ES : a.ldb);
+        if (b.out[i]) b.out[i] = static_cast<char*>(b.out[i]) + (int64_t)n * size;
+    }
+    if (b.g) b.g += n;
+    if (b.u) b.u += n;
+    if (b.dg) b.dg = static_cast<char*>(b.dg) + (int64_t)n * 2;
+    if (b.du) b.du = static_cast<char*>(b.du) + (int64_t)n * 2;
+    if (b.sb) b.sb += n;
+    return b;
+}
+
 template <typename T, bool AKS, bool BKS, bool DUAL, int EP>
 static int gm_run(int form, int ep, int aligned, GmArgs& a, void* ws, size_t ws_bytes, int nz, hipStream_t st)
 {
     if constexpr (!AKS && !BKS)
         if (a.M <= 16) return gm_few<T, DUAL, EP>(a, aligned, st);
     GmPlan p = gm_plan(form, ep, DUAL, aligned, a.M, a.N, a.K, a.segs, nz);
-    if (p.parts > 1 && (!ws || ws_bytes < p.part_bytes)) return -2;
+    if (p.part_bytes && (!ws || ws_bytes < p.part_bytes)) return -2;
+    if (p.first)
+    {
+        GmArgs b = gm_from<T, BKS>(a, p.first);
+        a.N = p.first;
+        if (gm_tiles<T, AKS, BKS, DUAL, EP>(a, p, aligned, nz, st)) return -1;
+        return gm_run<T, AKS, BKS, DUAL, EP>(form, ep, aligned, b, ws, ws_bytes, nz, st);
+    }
     if (p.parts == 1) return gm_tiles<T, AKS, BKS, DUAL, EP>(a, p, aligned, nz, st);
     if constexpr (AKS) return -1;   // never split (gm_plan)
     else

@@ -12,6 +12,8 @@ struct GmPlan
     int tm, tn;          // output rows and columns of a tile (tn: of each of the two matrices of a gate|up product)
     int deep;            // 128-row tiles: 8 waves and 5 steps of loads, one workgroup a CU (else 4 waves, 2 steps, two a CU)
     int parts;           // K parts
+    int first;           // columns of a first launch of whole rounds (the rest is planned by itself), 0: all in one
+    double time;         // estimated, us
     int64_t ldp;         // elements between the rows of a part
     size_t part_bytes;
 };
@@ -25,7 +27,7 @@ struct GmPlan
 // up), which fill rounds together.
 // Against the other choice, us of a backward call for the gradients of gate's and up's weights: 2048 tokens of 5504 x 2048 128 x
 // 128 176, 256 x 256 191; 333 tokens 58 and 65; 1024 tokens of 11008 x 4096 256 x 256 335, 128 x 128 364.
-inline GmPlan gm_plan(int form, int ep, int dual, int aligned, int M, int N, int K, int segs, int nz = 1)
+inline GmPlan gm_plan_one(int form, int ep, int dual, int aligned, int M, int N, int K, int segs, int nz = 1)
 {
     GmPlan best = {};
     const int d = dual ? 2 : 1;
@@ -41,7 +43,6 @@ inline GmPlan gm_plan(int form, int ep, int dual, int aligned, int M, int N, int
                            { 128, 128, 1, 256, 0.62, 0.62, 2 }, { 128, 128, 0, 512, 0.83, 1.03, 4 },
                            { 256, 256, 0, 256, 1.05, 1.5, 14 } };
     const double floor = (double)d * nz * N * K * (ep == EP_I8 ? 1 : 2) * segs / 4.8e6;
-    double least = 0;
     for (const Tile& t : tiles)
     {
         if ((t.tm == 16) != (M <= 16 && form == GM_NN)) continue;
@@ -62,9 +63,9 @@ inline GmPlan gm_plan(int form, int ep, int dual, int aligned, int M, int N, int
             }
             const double time = std::max(r * ((steps + p - 1) / p) + ends * t.ends, floor) + 3 +
                                 (p > 1 ? 2.5 + (double)p * d * M * ldp * 8 / 4e6 : 0);
-            if (best.parts == 0 || time < least)
+            if (best.parts == 0 || time < best.time)
             {
-                least = time;
+                best.time = time;
                 best.tm = t.tm, best.tn = t.tn / d, best.deep = t.deep, best.parts = p;
             }
         }
@@ -72,6 +73,24 @@ inline GmPlan gm_plan(int form, int ep, int dual, int aligned, int M, int N, int
     best.ldp = ldp;
     best.part_bytes = best.parts > 1 ? (size_t)best.parts * d * M * ldp * 4 : 0;
     return best;
+}
+
+// The 256 x 256 tiles of a product in whole rounds, and the columns left in a launch of their own where a smaller tile spreads
+// them better than a last round that leaves most CUs idle: 4096 x 5120 x 12288 (320 tiles) 463 us, 572 in
+// one launch.
+inline GmPlan gm_plan(int form, int ep, int dual, int aligned, int M, int N, int K, int segs, int nz = 1)
+{
+    GmPlan p = gm_plan_one(form, ep, dual, aligned, M, N, K, segs, nz);
+    if (p.tm != 256) return p;
+    const int rows = (M + 255) / 256 * nz, cols = (N + p.tn - 1) / p.tn, first = (int)((int64_t)rows * cols / 256 * 256 / rows);
+    if (first == 0 || first == cols) return p;
+    const GmPlan a = gm_plan_one(form, ep, dual, aligned, M, first * p.tn, K, segs, nz);
+    const GmPlan b = gm_plan(form, ep, dual, aligned, M, N - first * p.tn, K, segs, nz);
+    if (a.tm != 256 || a.time + b.time >= p.time) return p;
+    p.first = first * p.tn;
+    p.time = a.time + b.time;
+    p.part_bytes = b.part_bytes;
+    return p;
 }
 
 }  // namespace gfl

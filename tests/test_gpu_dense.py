@@ -80,6 +80,27 @@ def test_ffn_large_tiles(gpu):
             R.within(a, v, e, n)
 
 
+@pytest.mark.parametrize("M,H,I,dt", [(1934, 1280, 6144, F16), (4014, 6144, 1280, BF16), (4014, 1280, 6144, F16),
+                                      (1154, 6144, 2048, BF16), (1154, 4096, 6144, F16)])
+def test_ffn_products_in_two_launches(gpu, M, H, I, dt):
+    """Sizes at which one of the products (gate|up; down and dx; dh; the gradients of gate and up; of down) takes a launch of
+    large tiles and another for its last columns. Some tokens' outputs, and the gradients of some of the I channels, against
+    the definition over those tokens and those channels."""
+    import _native
+    x, wg, wu, wd, dy = _ffn_inputs(M, H, I, dt, M + I)
+    print("ffn_two_launches", M, H, I, dt, flush=True)
+    y, g, u = _native.ffn_forward(x, wg, wu, wd, save=True)
+    dx, dwg, dwu, dwd = _native.ffn_backward(dy, x, g, u, wg, wu, wd)
+    rows = torch.tensor(list(range(0, M, 97)) + [M - 1], device="cuda")
+    ref = R.FFN(x[rows], wg, wu, wd)
+    R.within(y[rows], ref.y, ref.ey, "y")
+    R.within(dx[rows], *ref.backward(dy[rows])[0], "dx")
+    ch = torch.tensor(list(range(0, I, 61)) + [I - 1], device="cuda")
+    ref = R.FFN(x, wg[ch], wu[ch], wd[:, ch])
+    for n, a, (v, e) in zip(("dwg", "dwu", "dwd"), (dwg[ch], dwu[ch], dwd[:, ch]), ref.backward(dy)[1:]):
+        R.within(a, v, e, n)
+
+
 @pytest.mark.parametrize("pad", [8, 32, 3])
 def test_ffn_strided_rows_and_outputs(gpu, pad):
     """Rows of a wider buffer (NaN around them), an out of wider rows whose surroundings stay as they were, fp32 out, and
@@ -249,6 +270,15 @@ def test_gemm_i8_sums_past_2_31(gpu):
     want, bound, _ = _i8_ref(a, sa, b, sb, F32)
     assert float((a.double().cpu() @ b.double().cpu().t()).max()) == 131071 * 16384
     R.within(_native.gemm_i8(a, sa, b, sb, dtype=F32), want, bound)
+
+
+@pytest.mark.parametrize("dt", [BF16, F32])
+def test_gemm_i8_in_two_launches(gpu, dt):
+    import _native
+    a, sa, b, sb = _i8(4014, 6144, 2432, 10)
+    rows = torch.tensor(list(range(0, 4014, 97)) + [4013], device="cuda")
+    want, bound, _ = _i8_ref(a[rows], sa[rows], b, sb, dt)
+    R.within(_native.gemm_i8(a, sa, b, sb, dtype=dt)[rows], want, bound)
 
 
 def test_gemm_i8_large_tiles_and_strides(gpu):
