@@ -10,7 +10,8 @@ registered with a context.
 Checkpoint keys (exllamav3 EXL3 linears): `<prefix>.layers.<L>.mlp.experts.<e>.<gate|up|down>_proj.<trellis|suh|svh>`
 and, for the shared expert, `<prefix>.layers.<L>.mlp.shared_experts.<gate|up|down>_proj.<...>`. A linear [k -> n]
 holds suh fp16 [k], svh fp16 [n] and its trellis as (k/16) * (n/16) tiles of 32*K bytes, row-major [k/16][n/16] (any
-dtype/shape with that byte count); K follows from the byte count.
+dtype/shape with that byte count); K follows from the byte count. A shared expert that the checkpoint keeps unquantised is
+`...shared_experts.<gate|up|down>_proj.weight` in fp16 or bf16, [n][k] each; its I may differ from the routed experts'.
 
 `self_test` repeats the reference's tier self-test (glm53/cpu_tier.py:738-770): fp64 truth from the effective weights
 (this build's dequant, then the 128-wide Hadamards and suh/svh) against the device forward, as a relative RMS error.
@@ -25,6 +26,8 @@ _ROUTED = re.compile(r"^(?P<pre>.*?)\.layers\.(?P<layer>\d+)\.mlp\.experts\.(?P<
                      r"(?P<proj>gate|up|down)_proj\.(?P<kind>trellis|suh|svh)$")
 _SHARED = re.compile(r"^(?P<pre>.*?)\.layers\.(?P<layer>\d+)\.mlp\.shared_experts\."
                      r"(?P<proj>gate|up|down)_proj\.(?P<kind>trellis|suh|svh)$")
+_DENSE = re.compile(r"^(?P<pre>.*?)\.layers\.(?P<layer>\d+)\.mlp\.shared_experts\."
+                    r"(?P<proj>gate|up|down)_proj\.weight$")
 PROJ = ("gate", "up", "down")
 HAD = 1.0 / math.sqrt(128.0)
 
@@ -44,6 +47,7 @@ class LayerSpec:
     Ks: tuple = ()
     entries: dict = field(default_factory=dict)
     has_shared: bool = False
+    dense: dict = field(default_factory=dict)     # the unquantised shared expert: {proj: (file, key)}
 
     @property
     def tile_bytes(self):
@@ -81,10 +85,16 @@ def scan(paths):
     from safetensors import safe_open
     if isinstance(paths, str):
         paths = [paths]
-    raw = {}
+    raw, dense = {}, {}
     for path in paths:
         with safe_open(path, framework="pt", device="cpu") as f:
             for key in f.keys():
+                m = _DENSE.match(key)
+                if m:
+                    sl = f.get_slice(key)
+                    if sl.get_dtype() in ("F16", "BF16"):   # other types (and their scales) are not this build's
+                        dense.setdefault(int(m.group("layer")), {})[m.group("proj")] = (path, key, tuple(sl.get_shape()))
+                    continue
                 m = _ROUTED.match(key) or _SHARED.match(key)
                 if not m:
                     continue
@@ -131,6 +141,12 @@ def scan(paths):
                     raise ValueError(f"layer {L}: expert {who} {proj}_proj vectors disagree with [{k} -> {n}]")
                 if ent[(who, proj, "trellis")][2] != sp.tile_bytes[p]:
                     raise ValueError(f"layer {L}: expert {who} {proj}_proj.trellis size differs from expert 0's")
+        ds = dense.get(L, {})
+        if len(ds) == len(PROJ) and not sp.has_shared:
+            n = ds["gate"][2][0]
+            if [ds[p][2] for p in PROJ] != [(n, sp.H), (n, sp.H), (sp.H, n)]:
+                raise ValueError(f"layer {L}: shared expert weights {[ds[p][2] for p in PROJ]} do not fit hidden {sp.H}")
+            sp.dense = {p: ds[p][:2] for p in PROJ}
         specs[L] = sp
     return specs
 
@@ -142,7 +158,8 @@ _DT_BYTES = {"F16": 2, "BF16": 2, "F32": 4, "I16": 2, "U16": 2, "I32": 4, "U32":
 class ResidentLayer:
     """One layer's experts in HBM: `arena` uint8 [E * record] (gate | up | down trellis per expert, 256-byte aligned)
     and `scales` fp16 [E * scale record]; `ptr_table` is gfl_register_layer's [E][9] address table. The shared
-    expert, when the checkpoint has one, sits in a one-expert arena of its own (`shared`)."""
+    expert, when the checkpoint has one, sits in a one-expert arena of its own (`shared`); an unquantised one as its fp16
+    gate, up and down weights (`dense`)."""
 
     def __init__(self, spec, device, experts):
         import torch
@@ -154,6 +171,7 @@ class ResidentLayer:
         self.scales = torch.zeros(self.E * self.srec, dtype=torch.float16, device=device)
         self.experts = experts
         self.shared = None
+        self.dense = None
 
     def trellis_ptr(self, i, p):
         return self.arena.data_ptr() + i * self.rec + (0, self.off_u, self.off_d)[p]
@@ -180,10 +198,24 @@ def _copy_expert(res, i, who, spec, handles):
             res.scales[o: o + v.numel()].copy_(v)
 
 
+def _dense_weight(L, proj, spec, handles, dev):
+    """A weight of the unquantised shared expert in fp16, the type of the experts' input. bf16 values of 2^-14 up to fp16's
+    largest are exact in it; smaller ones are rounded to its step of 2^-24, larger ones refused."""
+    import torch
+    path, key = spec.dense[proj]
+    t = handles[path].get_tensor(key)
+    if t.dtype == torch.bfloat16:
+        big = float(t.float().abs().nan_to_num(0.0, posinf=0.0).max()) if t.numel() else 0.0
+        if big > torch.finfo(torch.float16).max:
+            raise ValueError(f"layer {L}: shared_experts.{proj}_proj.weight reaches {big}, past fp16")
+    return t.to(device=dev, dtype=torch.float16).contiguous()
+
+
 def load(paths, ctx, layers=None, device=0, shared=None):
     """Copy the routed experts of `layers` (default: all layers found) into HBM and register each as context layer
     index L. With `shared` (a k_overlap.SharedOverlap), shared experts are registered there under the same index,
-    and with the routed layer in ctx too (gfl_register_shared), so that both can run in one call's launches.
+    and with the routed layer in ctx too (gfl_register_shared), so that both can run in one call's launches; unquantised ones
+    are registered there by register_dense (and left in the checkpoint without `shared`).
     Returns {L: ResidentLayer}."""
     import torch
     from safetensors import safe_open
@@ -211,6 +243,9 @@ def load(paths, ctx, layers=None, device=0, shared=None):
                 res.shared = sh
                 if shared is not None:
                     shared.register(L, sp.H, sp.I, sp.Ks, sh.ptr_table, keep=sh, routed=ctx)
+            if sp.dense and shared is not None:
+                res.dense = tuple(_dense_weight(L, p, sp, handles, dev) for p in PROJ)
+                shared.register_dense(L, *res.dense)
             out[L] = res
     finally:
         for h in handles.values():

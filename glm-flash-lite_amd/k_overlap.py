@@ -23,6 +23,9 @@ config-0-shaped shared expert, us per token; gate|up tile columns = tokens x top
   expert on narrow launches);
 - above that the routed call fills every SIMD for longer, and the shared expert's context is told so
   (gfl_ctx_set_shared), so that its launches leave SIMDs free: 40.0 against 40.5 sequential at M = 4.
+
+A checkpoint may keep the shared expert unquantised (16-bit gate, up and down weights). Such a layer (register_dense) runs
+after the routed call on the caller's stream and adds into its fp32 output itself (_native.ffn_forward, accumulate).
 """
 import torch
 
@@ -45,6 +48,8 @@ class SharedOverlap:
         self.overlapped = 0
         self.sequential = 0
         self.fused = 0
+        self.dense = 0
+        self._dense = {}         # layer: (wg, wu, wd, act_limit)
         self._attached = set()   # (routed context, layer) pairs that hold the shared expert
 
     def register(self, li, H, I, ks, ptr_row, keep=None, routed=None):
@@ -53,9 +58,23 @@ class SharedOverlap:
         layer li, registered already; it then also holds the shared expert, so that forward can run both in one
         call's launches (gfl_register_shared)."""
         self.ctx.register_layer(li, 1, H, I, ks, list(ptr_row), keep=keep)
+        self._dense.pop(li, None)
         if routed is not None:
             routed.register_shared(li, ks, list(ptr_row), keep=keep)
             self._attached.add((id(routed), li))
+
+    def register_dense(self, li, wg, wu, wd, act_limit=0.0):
+        """Register layer li's shared expert with 16-bit weights instead: wg and wu [I, H], wd [H, I], contiguous fp16 (the
+        type of forward's x) on this device. Its I need not be the routed experts'. act_limit: its SwiGLU clamp, 0 = off."""
+        if wg.dim() != 2 or wu.shape != wg.shape or wd.shape != wg.shape[::-1]:
+            raise ValueError(f"register_dense: wg and wu must be [I, H] and wd [H, I], not {list(wg.shape)}, {list(wu.shape)}, "
+                             f"{list(wd.shape)}")
+        for t in (wg, wu, wd):
+            if t.dtype != torch.float16 or not t.is_contiguous() or t.device != self.device:
+                raise ValueError(f"register_dense: weights must be contiguous fp16 on {self.device}")
+        if not act_limit >= 0.0:
+            raise ValueError(f"register_dense: act_limit must be >= 0, not {act_limit}")
+        self._dense[li] = (wg, wu, wd, float(act_limit))
 
     def _bufs(self, M, H):
         if M not in self._sel:
@@ -70,7 +89,13 @@ class SharedOverlap:
         allows it (gfl_moe_forward_shared), else on two streams, or in the stock order for a routed call of at most
         1,536 gate|up tile columns, where the overlap measured slower. overlap=False runs the shared expert after the
         routed call on the caller's stream (the reference's stock order), for comparison. Every order gives the same
-        bits."""
+        bits. A layer of register_dense always runs in the stock order."""
+        if li in self._dense:
+            wg, wu, wd, limit = self._dense[li]
+            routed.moe_forward(li, x, sel, w, out)
+            _native.ffn_forward(x, wg, wu, wd, out=out, act_limit=limit, accumulate=True)
+            self.dense += 1
+            return out
         M, H = x.shape
         s1, w1, y = self._bufs(M, H)
         main = torch.cuda.current_stream(self.device)
@@ -115,4 +140,4 @@ class SharedOverlap:
         return self._I[li]
 
     def summary(self):
-        return {"overlapped": self.overlapped, "sequential": self.sequential, "fused": self.fused}
+        return {"overlapped": self.overlapped, "sequential": self.sequential, "fused": self.fused, "dense": self.dense}

@@ -53,3 +53,15 @@ def host_experts(paths, L, E, H, I, Ks, shared=False):
                             t[base + ".svh"].view(np.uint16), k, n, Ks[p]))
         out.append(tuple(mats))
     return out
+
+
+def write_dense(tmpdir, L, H, Is, dtype, name=None, seed=9):
+    """Layer L's unquantised shared expert in a shard of its own (dense-0000L.safetensors); returns (gate, up, down)."""
+    import torch
+    from safetensors.torch import save_file
+    g = torch.Generator()
+    g.manual_seed(seed + L)
+    w = [(torch.randn(s, generator=g) / s[1] ** 0.5).to(dtype) for s in ((Is, H), (Is, H), (H, Is))]
+    save_file({f"{PREFIX}.layers.{L}.mlp.shared_experts.{p}_proj.weight": t for p, t in zip(("gate", "up", "down"), w)},
+              str(tmpdir / (name or f"dense-{L:05d}.safetensors")))
+    return w

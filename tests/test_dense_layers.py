@@ -1,0 +1,80 @@
+"""The dense layers without a GPU: which unquantised shared experts exl3_loader.scan finds, and what it,
+SharedOverlap.register_dense and k_dense refuse."""
+import pytest
+import torch
+
+import ckpt_synth
+
+KS = {1: (3, 3, 3)}
+
+
+def _scan(tmp_path, H, Is, dtype, shared=False):
+    import exl3_loader
+    paths = ckpt_synth.write(tmp_path, [1], E=2, H=512, I=256, Ks_by_layer=KS, shared=shared)
+    ckpt_synth.write_dense(tmp_path, 1, H, Is, dtype)
+    return exl3_loader.scan(paths + [str(tmp_path / "dense-00001.safetensors")])[1]
+
+
+@pytest.mark.parametrize("dtype,found", [(torch.float16, True), (torch.bfloat16, True), (torch.float32, False)])
+def test_scan_finds_the_unquantised_shared_expert(tmp_path, dtype, found):
+    sp = _scan(tmp_path, 512, 384, dtype)
+    assert not sp.has_shared and sorted(sp.dense) == (["down", "gate", "up"] if found else [])
+
+
+def test_scan_prefers_the_quantised_one(tmp_path):
+    sp = _scan(tmp_path, 512, 384, torch.float16, shared=True)
+    assert sp.has_shared and not sp.dense
+
+
+def test_scan_refuses_weights_of_another_hidden_size(tmp_path):
+    with pytest.raises(ValueError, match="do not fit hidden 512"):
+        _scan(tmp_path, 520, 384, torch.float16)
+
+
+def test_bf16_weights_past_fp16(tmp_path):
+    import exl3_loader
+    from safetensors import safe_open
+    from safetensors.torch import save_file
+    key, path = "a", str(tmp_path / "w.safetensors")
+    for vals, ok in (([1.0, 65280.0, 2.0 ** -20], True), ([-65536.0, 0.0], False), ([3e38], False)):
+        t = torch.tensor([vals], dtype=torch.bfloat16)
+        save_file({key: t}, path)
+        sp = exl3_loader.LayerSpec(layer=1, dense={"gate": (path, key)})
+        with safe_open(path, framework="pt", device="cpu") as f:
+            if ok:
+                assert torch.equal(exl3_loader._dense_weight(1, "gate", sp, {path: f}, "cpu").float(), t.float())
+            else:
+                with pytest.raises(ValueError, match="past fp16"):
+                    exl3_loader._dense_weight(1, "gate", sp, {path: f}, "cpu")
+
+
+def test_register_dense_refusals():
+    import k_overlap
+    so = object.__new__(k_overlap.SharedOverlap)     # no context: nothing here reaches the device
+    so.device, so._dense = torch.device("cpu"), {}
+    w = lambda *s, dt=torch.float16: torch.zeros(s, dtype=dt)
+    ok = (w(8, 16), w(8, 16), w(16, 8))
+    so.register_dense(0, *ok, act_limit=7.0)
+    assert so._dense[0][3] == 7.0
+    for bad, word in (((w(8, 16), w(9, 16), w(16, 8)), "must be"), ((w(8, 16), w(8, 16), w(8, 16)), "must be"),
+                      ((w(128), w(128), w(128)), "must be"), ((w(8, 16, dt=torch.bfloat16),) + ok[1:], "fp16"),
+                      ((w(16, 8).t(),) + ok[1:], "contiguous"), ((w(8, 16).to("meta"),) + ok[1:], "on cpu")):
+        with pytest.raises(ValueError, match=word):
+            so.register_dense(1, *bad)
+    for limit in (-1.0, float("nan")):
+        with pytest.raises(ValueError, match="act_limit"):
+            so.register_dense(1, *ok, act_limit=limit)
+    assert list(so._dense) == [0]
+
+
+def test_layers_refuse_host_tensors_and_shapes():
+    import k_dense
+    w = lambda *s: torch.zeros(s, dtype=torch.float16)
+    for grad in (False, True):
+        with pytest.raises(ValueError, match="device"):
+            k_dense.gated_ffn(w(2, 16), w(8, 16).requires_grad_(grad), w(8, 16), w(16, 8))
+    for bad in (w(8), w(8, 0), torch.zeros((1, 131072), dtype=torch.float16, device="meta"), w(2, 3, 4)):
+        with pytest.raises(ValueError, match="Linear8"):
+            k_dense.Linear8(bad)
+    with pytest.raises(ValueError, match="device"):
+        k_dense.Linear8(w(4, 8))
