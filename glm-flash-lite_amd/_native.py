@@ -413,7 +413,7 @@ def ffn_forward(x, wg, wu, wd, out=None, act_limit=0.0, save=False, accumulate=F
     """Gated feed-forward block (gfl_ffn_forward): (min(silu(x wg^T), L) * clamp(x wu^T, -L, L)) wd^T, L = act_limit, 0 = off.
     x fp16 or bf16 [..., H] (rows may have a stride), wg and wu [I, H], wd [H, I] as nn.Linear keeps them. out: of x's type
     (the default) or fp32; accumulate (fp32 out): out += the block. save=True returns (out, g, u) with the fp32 g and u [M, I]
-    that ffn_backward takes."""
+    that ffn_backward takes. Not seen by autograd: k_dense.gated_ffn is the differentiable form."""
     r = (_EXT or _ext()).ffn_forward(x, wg, wu, wd, out, act_limit, save, accumulate)
     return r if save else r[0]
 

@@ -68,8 +68,8 @@ FfnSizes ffn_sizes(int M, int H, int I, bool backward)
 int ffn_check(const char* what, int dtype, int M, int H, int I)
 {
     if (dtype != GFL_F16 && dtype != GFL_BF16) return api_fail(GFL_EINVAL, "gfl_ffn: dtype must be GFL_F16 or GFL_BF16");
-    if (M < 0 || H < 1 || I < 1 || H >= GFL_MAX_LD || I >= GFL_MAX_LD)
-        return api_fail(GFL_EINVAL, "gfl_ffn: need M >= 0 and 1 <= H, I < GFL_MAX_LD");
+    if (M < 0 || M >= GFL_MAX_ROWS || H < 1 || I < 1 || H >= GFL_MAX_LD || I >= GFL_MAX_LD)
+        return api_fail(GFL_EINVAL, "gfl_ffn: need M >= 0, M < GFL_MAX_ROWS and 1 <= H, I < GFL_MAX_LD");
     (void)what;
     return GFL_OK;
 }
@@ -226,8 +226,10 @@ int gfl_ffn_backward(const void* dy, int64_t lddy, const void* x, int64_t ldx, c
 
 static int i8_check(int M, int N, int K)
 {
-    if (M < 0 || N < 1 || K < 1 || K > 131071 || N >= (1 << 30))
-        return api_fail(GFL_EINVAL, "gfl_i8: need M >= 0, 1 <= N < 2^30 and 1 <= K <= 131071 (the int32 sum is then exact)");
+    // N: a launch of 64 threads a channel has fewer than 2^32; M likewise, 256 a row
+    if (M < 0 || M >= GFL_MAX_ROWS || N < 1 || K < 1 || K > 131071 || N >= GFL_MAX_N)
+        return api_fail(GFL_EINVAL, "gfl_i8: need 0 <= M < GFL_MAX_ROWS (M >= 0), 1 <= N < GFL_MAX_N and 1 <= K <= 131071 (the "
+                                    "int32 sum is then exact)");
     return GFL_OK;
 }
 
@@ -250,7 +252,8 @@ int gfl_i8_workspace(int M, int N, int K, size_t* gemm, size_t* linear)
 int gfl_quant_i8(const void* x, int64_t ldx, int dtype, int M, int K, int8_t* q, float* scale, gfl_stream stream)
 {
     if (dtype != GFL_F16 && dtype != GFL_BF16) return api_fail(GFL_EINVAL, "gfl_quant_i8: dtype must be GFL_F16 or GFL_BF16");
-    if (M < 0 || K < 1 || K >= GFL_MAX_LD) return api_fail(GFL_EINVAL, "gfl_quant_i8: need M >= 0 and 1 <= K < GFL_MAX_LD");
+    if (M < 0 || M >= GFL_MAX_ROWS || K < 1 || K >= GFL_MAX_LD)
+        return api_fail(GFL_EINVAL, "gfl_quant_i8: need 0 <= M < GFL_MAX_ROWS and 1 <= K < GFL_MAX_LD");
     if (M == 0) return GFL_OK;
     if (!x || !q || !scale) return api_fail(GFL_EINVAL, "gfl_quant_i8: NULL argument");
     if (ldx < K || ldx >= GFL_MAX_LD) return api_fail(GFL_EINVAL, "gfl_quant_i8: the row stride must be in [K, GFL_MAX_LD)");

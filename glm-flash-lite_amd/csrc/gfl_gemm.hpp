@@ -804,7 +804,8 @@ __global__ __launch_bounds__(256, 1) void gm_big_kernel(GmArgs a)
     constexpr int TNC = DUAL ? 128 : 256;
     const int m0 = im * 256, n0 = in * TNC;
     // whole steps by the pipeline; a segment's last step that is not whole comes after it, through registers
-    const int steps1 = a.K / BK, steps = steps1 * a.segs, tail = a.K % BK;
+    // (where rows end inside a chunk of 16 bytes the last step of whole rows does too: its last row's chunk would reach past the matrix)
+    const int steps1 = (a.K - (a.ragged && (AKS || BKS) ? 1 : 0)) / BK, steps = steps1 * a.segs, tail = a.K - steps1 * BK;
     SA sa;
     SB sb;
     sa.init(wave, lane, gm_pick(a.A, z), nullptr, a.lda, m0, a.M);

@@ -3,7 +3,19 @@
 #include "gfl_gemm.hpp"
 #include "gfl_gemm_plan.hpp"
 
+#include <atomic>
+
 namespace gfl {
+
+// Allows a kernel its LDS, once on each device (the attribute belongs to the device's copy of the kernel; `opened`: a bit for each).
+static inline void gm_open(const void* kern, int lds, std::atomic<uint64_t>& opened)
+{
+    int dev = 0;
+    if (hipGetDevice(&dev) != hipSuccess) return;   // the launch reports it
+    const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+    if (bit && (opened.load(std::memory_order_relaxed) & bit)) return;
+    if (hipFuncSetAttribute(kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds) == hipSuccess) opened.fetch_or(bit);
+}
 
 template <typename T, int TM, int TN, int WM, int WN, bool AKS, bool BKS, bool DUAL, int NST, bool AL, int EP>
 static int gm_go(const GmArgs& a, int nz, hipStream_t st)
@@ -11,9 +23,8 @@ static int gm_go(const GmArgs& a, int nz, hipStream_t st)
     constexpr int lds = (AL ? NST : 1) * (TM + TN) * 128;
     static_assert(lds <= LDS_LIMIT, "tiles fit the LDS");
     auto* kern = gm_kernel<T, TM, TN, WM, WN, AKS, BKS, DUAL, NST, AL, EP>;
-    static const bool opened = hipFuncSetAttribute(reinterpret_cast<const void*>(kern),
-                                                   hipFuncAttributeMaxDynamicSharedMemorySize, lds) == hipSuccess;
-    (void)opened;
+    static std::atomic<uint64_t> opened{ 0 };
+    gm_open(reinterpret_cast<const void*>(kern), lds, opened);
     hipLaunchKernelGGL(kern, dim3((unsigned)(a.tm * a.tn * a.parts), 1, nz), dim3(WM * WN * 64), lds, st, a);
     return 0;
 }
@@ -52,9 +63,8 @@ static int gm_tiles(GmArgs& a, const GmPlan& p, int aligned, int nz, hipStream_t
         a.wide = gm_wide(a, EP, nz);
         constexpr int lds = GM_BIG_LDS;
         auto* kern = &gm_big_kernel<T, AKS, BKS, DUAL, EP>;
-        static const bool opened = hipFuncSetAttribute(reinterpret_cast<const void*>(kern),
-                                                       hipFuncAttributeMaxDynamicSharedMemorySize, lds) == hipSuccess;
-        (void)opened;
+        static std::atomic<uint64_t> opened{ 0 };
+        gm_open(reinterpret_cast<const void*>(kern), lds, opened);
         hipLaunchKernelGGL(kern, dim3((unsigned)(a.tm * a.tn), 1, nz), dim3(256), lds, st, a);
         return 0;
     }
@@ -65,9 +75,8 @@ static void gm_ring(const GmArgs& a, int wg, hipStream_t st)
 {
     constexpr int S = 4, lds = NW * S * 2048;
     auto* kern = gm_ring_kernel<T, DUAL, EP, NW, S>;
-    static const bool opened = hipFuncSetAttribute(reinterpret_cast<const void*>(kern),
-                                                   hipFuncAttributeMaxDynamicSharedMemorySize, lds) == hipSuccess;
-    (void)opened;
+    static std::atomic<uint64_t> opened{ 0 };
+    gm_open(reinterpret_cast<const void*>(kern), lds, opened);
     hipLaunchKernelGGL(kern, dim3(wg), dim3(NW * 64), lds, st, a);
 }
 

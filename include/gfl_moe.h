@@ -258,14 +258,17 @@ int gfl_route(const float* logits, int M, int E, int topk, int64_t* sel, uint16_
  * caller gives the workspace (16-byte aligned device memory; its size from the *_workspace calls, which depend on the
  * arguments alone). Calls that may overlap need workspaces of their own, two captured graphs among them. Outputs must
  * not overlap inputs. Any sizes and strides are taken; above 16 tokens matrices whose addresses and row strides are
- * multiples of 4 bytes run faster than others. Row strides stay below 2^22 elements. Empty calls (M = 0) launch nothing, but gfl_ffn_backward then writes zeros to the weights' gradients. */
+ * multiples of 4 bytes run faster than others. Empty calls (M = 0) launch nothing, but gfl_ffn_backward then writes zeros to
+ * the weights' gradients. */
 enum
 {
     GFL_F16 = 0,
     GFL_BF16 = 1,
     GFL_F32 = 2, /* outputs only */
 };
-#define GFL_MAX_LD 4194304
+#define GFL_MAX_LD 4194304     /* row strides, H, I, K */
+#define GFL_MAX_ROWS 16777216  /* tokens of a call (not gfl_sample) */
+#define GFL_MAX_N 67108864     /* channels of an 8-bit product */
 
 /* Gated feed-forward block, unquantised: g = x Wg^T, u = x Wu^T, h = min(silu(g), L) * clamp(u, -L, L),
  * y = h Wd^T, with the experts' clamp L = act_limit (0 = off). x [M, H], Wg and Wu [I, H], Wd [H, I] contiguous (as

@@ -115,3 +115,14 @@ def test_python_calls_refuse_what_does_not_fit():
                      ((f(2, 9), f(2)), {})):
         with pytest.raises(ValueError):
             _native.sample(*args, **kw)
+
+
+def test_sizes_past_a_launch(lib):
+    """What a grid could not hold is refused by size."""
+    _refused(lib, _ffn(lib, M=1 << 24), "GFL_MAX_ROWS")
+    _refused(lib, _bwd(lib, M=1 << 24), "GFL_MAX_ROWS")
+    _refused(lib, lib.gfl_quant_i8(P, 64, 0, 1 << 24, 64, P, P, None), "GFL_MAX_ROWS")
+    for M, N in ((1 << 24, 8), (1, 1 << 26)):
+        _refused(lib, lib.gfl_gemm_i8(P, 64, P, P, 64, P, M, N, 64, P, N, 0, P, 1 << 24, None), "GFL_MAX")
+        _refused(lib, lib.gfl_linear_i8(P, 64, 0, P, 64, P, M, N, 64, P, N, 0, P, 1 << 24, None), "GFL_MAX")
+        _refused(lib, lib.gfl_i8_workspace(M, N, 64, None, None), "GFL_MAX")

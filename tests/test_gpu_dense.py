@@ -80,15 +80,10 @@ def test_ffn_large_tiles(gpu):
             R.within(a, v, e, n)
 
 
-@pytest.mark.parametrize("M,H,I,dt", [(1934, 1280, 6144, F16), (4014, 6144, 1280, BF16), (4014, 1280, 6144, F16),
-                                      (1154, 6144, 2048, BF16), (1154, 4096, 6144, F16)])
-def test_ffn_products_in_two_launches(gpu, M, H, I, dt):
-    """Sizes at which one of the products (gate|up; down and dx; dh; the gradients of gate and up; of down) takes a launch of
-    large tiles and another for its last columns. Some tokens' outputs, and the gradients of some of the I channels, against
-    the definition over those tokens and those channels."""
+def _part_of_a_pass(M, H, I, dt):
     import _native
     x, wg, wu, wd, dy = _ffn_inputs(M, H, I, dt, M + I)
-    print("ffn_two_launches", M, H, I, dt, flush=True)
+    print("ffn_part", M, H, I, dt, flush=True)
     y, g, u = _native.ffn_forward(x, wg, wu, wd, save=True)
     dx, dwg, dwu, dwd = _native.ffn_backward(dy, x, g, u, wg, wu, wd)
     rows = torch.tensor(list(range(0, M, 97)) + [M - 1], device="cuda")
@@ -99,6 +94,20 @@ def test_ffn_products_in_two_launches(gpu, M, H, I, dt):
     ref = R.FFN(x, wg[ch], wu[ch], wd[:, ch])
     for n, a, (v, e) in zip(("dwg", "dwu", "dwd"), (dwg[ch], dwu[ch], dwd[:, ch]), ref.backward(dy)[1:]):
         R.within(a, v, e, n)
+
+
+@pytest.mark.parametrize("M,H,I,dt", [(1934, 1280, 6144, F16), (4014, 6144, 1280, BF16), (4014, 1280, 6144, F16),
+                                      (1154, 6144, 2048, BF16), (1154, 4096, 6144, F16)])
+def test_ffn_products_in_two_launches(gpu, M, H, I, dt):
+    """Sizes at which one of the products (gate|up; down and dx; dh; the gradients of gate and up; of down) takes a launch of
+    large tiles and another for its last columns. Some tokens' outputs, and the gradients of some of the I channels, against
+    the definition over those tokens and those channels."""
+    _part_of_a_pass(M, H, I, dt)
+
+
+def test_ffn_large_tiles_with_rows_that_end_inside_a_chunk(gpu):
+    """Whole K steps (2048 tokens) of rows of 2050 and 2308: the last row's last chunk reaches past the matrix."""
+    _part_of_a_pass(2048, 2050, 2308, BF16)
 
 
 @pytest.mark.parametrize("pad", [8, 32, 3])
@@ -128,6 +137,41 @@ def test_ffn_strided_rows_and_outputs(gpu, pad):
     a = _native.ffn_backward(wide_dy[:, :H], x, g, u, wg, wu, wd)
     for n, t, (v, e) in zip(("dx", "dwg", "dwu", "dwd"), a, ref.backward(dy)):
         R.within(t, v, e, n)
+
+
+@pytest.mark.parametrize("ld", [(1 << 22) - 8, (1 << 22) - 1])
+def test_ffn_widest_strides(gpu, ld):
+    """Rows as far apart as allowed: offsets within a tile near 2^31 bytes, within the tensors past it."""
+    import _native
+    M, H, I = 300, 136, 72
+    x, wg, wu, wd, dy = _ffn_inputs(M, H, I, F16, 12)
+
+    def spread(t):
+        out = torch.zeros((M, ld), dtype=F16, device="cuda")[:, :H]
+        return out if t is None else out.copy_(t)
+
+    print("ffn_widest", ld, flush=True)
+    y, g, u = _native.ffn_forward(x, wg, wu, wd, save=True)
+    xs, dys = spread(x), spread(dy)
+    ys, gs, us = _native.ffn_forward(xs, wg, wu, wd, out=spread(None), save=True)
+    ref = R.FFN(x, wg, wu, wd)
+    R.within(ys, ref.y, ref.ey, "y")
+    for n, a, (v, e) in zip(("dx", "dwg", "dwu", "dwd"), _native.ffn_backward(dys, xs, gs, us, wg, wu, wd), ref.backward(dy)):
+        R.within(a, v, e, n)
+    R.within(_native.ffn_forward(xs[:5], wg, wu, wd), ref.y[:5], ref.ey[:5], "y of 5")
+    R.within(_native.ffn_forward(xs[298:], wg, wu, wd), ref.y[298:], ref.ey[298:], "y of 2")
+
+
+@pytest.mark.parametrize("ld", [(1 << 22) - 16, (1 << 22) - 1])
+def test_gemm_i8_widest_strides(gpu, ld):
+    import _native
+    a, sa, b, sb = _i8(600, 520, 144, 4)
+    want, bound, _ = _i8_ref(a, sa, b, sb, F32)
+    far = [torch.zeros((len(t), ld), dtype=torch.int8, device="cuda")[:, :144].copy_(t) for t in (a, b)]
+    print("gemm_i8_widest", ld, flush=True)
+    R.within(_native.gemm_i8(far[0], sa, far[1], sb, dtype=F32), want, bound)
+    for m in (1, 9):
+        R.within(_native.gemm_i8(far[0][-m:], sa[-m:], far[1], sb, dtype=F32), want[-m:], bound[-m:])
 
 
 def test_ffn_partial_gradients_and_empty(gpu):
