@@ -320,6 +320,21 @@ int gfl_linear_i8(const void* x, int64_t ldx, int dtype, const int8_t* b, int64_
     if (!ws || ws_bytes < need || reinterpret_cast<uintptr_t>(ws) % 16)
         return api_fail(GFL_EINVAL, "gfl_linear_i8: workspace missing, too small or not 16-byte aligned");
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+    if (M <= 2 && K % 8 == 0 && K >= 1024 && K <= gfl::LQ_K && reinterpret_cast<uintptr_t>(x) % 16 == 0 && (M == 1 || ldx % 8 == 0))
+    {
+        gfl::GmArgs g;
+        g.A[0] = static_cast<const char*>(x);
+        g.B[0] = reinterpret_cast<const char*>(b);
+        g.lda = ldx * 2;
+        g.ldb = ldb;
+        g.M = M; g.N = N; g.K = K;
+        g.out[0] = out;
+        g.ldo = ldo;
+        g.odt = out_dtype;
+        g.sb = sb;
+        gfl::launch_linear_row_i8(g, dtype == GFL_BF16, st);
+        return check_launch("gfl_linear_i8");
+    }
     const size_t part = i8_part(M, N, K);
     const int64_t ldq = i8_ldq(K);
     int8_t* q = static_cast<int8_t*>(ws) + part;

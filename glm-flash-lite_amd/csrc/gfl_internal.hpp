@@ -228,6 +228,11 @@ int launch_gemm_i8(int form, int ep, int dual, int aligned, GmArgs& a, void* ws,
 // int8 rows of x [M][K] (16-bit, ldx elements between rows): q [M][ldq], scale [M] (k_quant.hip)
 void launch_quant_i8(const void* x, int64_t ldx, int bf16, int M, int K, int8_t* q, int64_t ldq, float* scale, hipStream_t st);
 
+// gfl_linear_i8 of 1 or 2 tokens in one launch (k_dense_i8.hip): a.A[0], a.lda the 16-bit tokens, K a multiple of 8 up to LQ_K
+constexpr int LQ_K = 8192;
+constexpr int LQ_WG = 2048;   // workgroups; past 8 columns each they take more
+void launch_linear_row_i8(const GmArgs& a, int bf16, hipStream_t st);
+
 // token selection (k_sample.hip)
 constexpr int MAX_VOCAB = 1 << 20;
 struct SampleArgs

@@ -1,20 +1,11 @@
 // Rows of 16-bit activations to 8 bits with a scale each.
-#include "gfl_internal.hpp"
+#include "gfl_quant.hpp"
 
 namespace gfl {
 
-// A workgroup per row. max |x| is the integer maximum of the magnitudes' bits, which puts NaN above infinity above every
-// number, so a row that is not finite is seen as such. q = x * 127 / max: the product is exact in fp32 (at most 18
-// significant bits), so the correctly rounded quotient lies on the true side of every half and q is the exact rounding.
-// Values past 2^100 are scaled down first so that the product stays finite. Bound by memory: K is read once (16 values a
-// thread stay in registers; longer rows are read again, from cache).
+// A workgroup per row. Bound by memory: K is read once (16 values a thread stay in registers; longer rows are read again, from
+// cache).
 constexpr int QT = 256;
-
-template <bool BF>
-__device__ __forceinline__ float q_val(uint16_t b)
-{
-    return BF ? __uint_as_float((uint32_t)b << 16) : static_cast<float>(__builtin_bit_cast(_Float16, b));
-}
 
 template <bool BF>
 __global__ __launch_bounds__(QT) void quant_i8_kernel(const uint16_t* x, int64_t ldx, int K, int8_t* q, int64_t ldq,
@@ -43,24 +34,20 @@ __global__ __launch_bounds__(QT) void quant_i8_kernel(const uint16_t* x, int64_t
     if (threadIdx.x % 64 == 0) red[threadIdx.x / 64] = top;
     __syncthreads();
     top = max(max(red[0], red[1]), max(red[2], red[3]));
-    float amax = q_val<BF>((uint16_t)top);
-    if (threadIdx.x == 0) scale[m] = amax / 127.0f;
-    const bool ok = top != 0 && top < (BF ? 0x7F80u : 0x7C00u);
-    const float pre = amax > 0x1p100f ? 0x1p-64f : 1.0f;
-    amax *= pre;
-    auto one = [&](uint16_t b) { return ok ? (int8_t)(int)rintf(q_val<BF>(b) * pre * 127.0f / amax) : (int8_t)0; };
+    const QRow<BF> r(top);
+    if (threadIdx.x == 0) scale[m] = r.scale;
     for (int c = threadIdx.x, s = 0; c < nv; c += QT, ++s)
     {
         u16x8 v;
         if (s == 0) v = keep[0];
         else if (s == 1) v = keep[1];
         else v = *reinterpret_cast<const u16x8*>(row + 8 * c);
-        uint64_t o = 0;
+        uint16_t e[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) o |= (uint64_t)(uint8_t)one(v[i]) << (8 * i);
-        *reinterpret_cast<uint64_t*>(out + 8 * c) = o;
+        for (int i = 0; i < 8; ++i) e[i] = v[i];
+        *reinterpret_cast<uint64_t*>(out + 8 * c) = r.eight(e);
     }
-    for (int k = 8 * nv + threadIdx.x; k < K; k += QT) out[k] = one(row[k]);
+    for (int k = 8 * nv + threadIdx.x; k < K; k += QT) out[k] = r.one(row[k]);
 }
 
 void launch_quant_i8(const void* x, int64_t ldx, int bf16, int M, int K, int8_t* q, int64_t ldq, float* scale, hipStream_t st)

@@ -355,6 +355,29 @@ def test_linear_i8(gpu, M, N, K, dt):
     R.within(got, want, want.abs() * (R.half_step(dt) + 5 * 2.0 ** -24) + R.tiny(dt))
 
 
+@pytest.mark.parametrize("dt", [F16, BF16])
+@pytest.mark.parametrize("M,N,K,pad", [(1, 1, 8, 0), (2, 7, 1000, 8), (1, 513, 5120, 0), (2, 20011, 264, 0), (1, 40, 8192, 0),
+                                       (2, 33, 8192, 24), (1, 24, 8200, 0), (2, 24, 520, 4), (1, 17, 4096, 0), (2, 9, 1032, 1)])
+def test_linear_i8_few_tokens(gpu, M, N, K, pad, dt):
+    """One and two tokens, whichever launches they take: the same bits as the rows quantised by a call of their own; rows
+    of zeros and rows that are not finite too."""
+    import _native
+    _, _, b, sb = _i8(1, N, K, 5)
+    x = torch.randn((M, K + pad), generator=_rng(K + N)).to(dt).cuda()[:, :K]
+    for k in range(4):
+        if k == 1:
+            x[M - 1] = 0
+        elif k == 2:
+            x[0, K // 2] = math.inf
+        elif k == 3:
+            x[0, K // 2] = math.nan
+        q, s = _native.quant_i8(x)
+        for out in (dt, F32):
+            got, want = _native.linear_i8(x, b, sb, dtype=out), _native.gemm_i8(q, s, b, sb, dtype=out)
+            assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.nan_to_num(), want.nan_to_num())
+            assert bool(got[0].isnan().all()) == (k >= 2)
+
+
 # ---------------------------------------------------------------------------------------------------------------
 
 def _draw(logits, u, **kw):
