@@ -36,29 +36,39 @@ struct SmRow
     }
 };
 
-// exp((x - max) / T) as 2^n p, n the nearest whole number to the exponent in base 2 and p by the Taylor series of e^x on
-// |x| <= ln 2 / 2, whose remainder after degree 12 is below 2^-51. scale = log2(e) / T.
+// exp((x - max) / T) = 2^(n / 64) e^x, n the nearest whole number to 64 times the exponent in base 2: 2^(n / 64) from a table of
+// 2^0 .. 2^(63 / 64) and e^x by its Taylor series on |x| <= ln 2 / 128, whose remainder after degree 5 is below 2^-54. (By degree
+// 12 on ln 2 / 2 without a table, 256 rows of 131,072 without top-k or top-p took 108 us, 100 with it.) scale = log2(e) / T.
+__device__ __forceinline__ double* sm_powers()
+{
+    __shared__ double t[64];
+    return t;
+}
+// fills the table; a barrier before its first use is the caller's
+__device__ __forceinline__ void sm_powers_init()
+{
+    if (threadIdx.x >= 64) return;
+    const double n = threadIdx.x > 32 ? 1.0 : 0.0, x = ((int)threadIdx.x / 64.0 - n) * 0.693147180559945309417;
+    double p = 1.0;   // e^x by Horner's rule: remainder below 2^-51 for |x| <= ln 2 / 2
+#pragma unroll
+    for (int k = 13; k; --k) p = fma(p, x * (1.0 / k), 1.0);
+    sm_powers()[threadIdx.x] = n > 0 ? 2.0 * p : p;
+}
 __device__ __forceinline__ double sm_exp(uint32_t key, uint32_t top, double scale)
 {
     // without branches, so that a thread's values run side by side
-    const double y0 = ((double)sm_value(key) - (double)sm_value(top)) * scale;
-    const bool any = y0 > -1000.0;      // not so for a NaN: finite - inf over an infinite T, inf - inf
+    const double y0 = ((double)sm_value(key) - (double)sm_value(top)) * (64.0 * scale);
+    const bool any = y0 > -64000.0;     // not so for a NaN: finite - inf over an infinite T, inf - inf
     const double y = any ? y0 : 0.0;
-    const double n = rint(y), x = (y - n) * 0.693147180559945309417;
-    double p = 1.0 / 479001600;
-    p = fma(p, x, 1.0 / 39916800);
-    p = fma(p, x, 1.0 / 3628800);
-    p = fma(p, x, 1.0 / 362880);
-    p = fma(p, x, 1.0 / 40320);
-    p = fma(p, x, 1.0 / 5040);
-    p = fma(p, x, 1.0 / 720);
-    p = fma(p, x, 1.0 / 120);
+    const double n = rint(y), x = (y - n) * (0.693147180559945309417 / 64);
+    const int i = (int)n;
+    double p = 1.0 / 120;
     p = fma(p, x, 1.0 / 24);
     p = fma(p, x, 1.0 / 6);
     p = fma(p, x, 0.5);
     p = fma(p, x, 1.0);
-    p = fma(p, x, 1.0);
-    const double e = __longlong_as_double(__double_as_longlong(p) + ((long long)(int)n << 52));
+    p = fma(p, x, 1.0) * sm_powers()[i & 63];
+    const double e = __longlong_as_double(__double_as_longlong(p) + ((long long)(i >> 6) << 52));
     return key == top ? 1.0 : any ? e : 0.0;
 }
 
@@ -70,6 +80,20 @@ __device__ __forceinline__ uint64_t sm_units(double e)
 __device__ __forceinline__ uint64_t sm_weight(uint32_t key, uint32_t top, double scale)
 {
     return key > SM_MASKED ? sm_units(sm_exp(key, top, scale)) : 0;
+}
+
+// The weights of 4 keys, those whose exponential lies below `least` or that are masked 0. Every key's exponential is worked out,
+// held by the empty asm, so that the four run side by side: behind a branch each (which the compiler makes of the selects) 256
+// rows of 131,072 without top-k or top-p took 100 us, 95 now, 1024 rows 740 and 630.
+__device__ __forceinline__ void sm_weights(const uint32_t (&key)[4], uint32_t top, double scale, double least,
+                                           unsigned long long (&x)[4])
+{
+    double e[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) e[j] = sm_exp(key[j], top, scale);
+    asm volatile("" : "+v"(e[0]), "+v"(e[1]), "+v"(e[2]), "+v"(e[3]));
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] = (key[j] > SM_MASKED) & (e[j] >= least) ? sm_units(e[j]) : 0;
 }
 
 // Wave scans by DPP: shifts by 1, 2, 4, 8 within rows of 16 lanes, then the rows' last lanes to the rows after them. `id` is
@@ -303,8 +327,9 @@ __device__ void sm_row_slow(SmShared& s, const SampleArgs& a, int b, const SmRow
 //   top     each slice's largest and smallest logit and the largest's index, and the largest of each of up to 1,024 groups
 //           of the row; clears the row's histogram
 //   bins    (not for a top-k of up to half the groups: the k-th largest group maximum, rounded down, has at least k logits at
-//           or above it and few more, and is the list's floor) 2,047 bins of equal width from the largest logit down to where weights round to zero (or to the smallest), and
-//           one for what lies below: logits per bin for a top-k, else the weight per bin (of the row and of each slice)
+//           or above it and few more, and is the list's floor) 2,047 bins of equal width from the largest logit down to where
+//           weights round to zero (or to the smallest), and one for what lies below: logits per bin for a top-k, else the
+//           weight per bin (of the row and of each slice)
 //   cut     every workgroup finds the bins in which the kept prefix ends from the row's histogram. With a top-k (and few
 //           logits down to its bin) all logits down to that bin go into the row's list; else the list takes the bins
 //           where the nucleus and min-p end, and each slice sums the weight of its bins above them
@@ -590,6 +615,7 @@ __global__ __launch_bounds__(SM_PT) void sm_bins_kernel(SampleArgs a, SmWs w)
     const E* row = static_cast<const E*>(a.logits) + (int64_t)b * a.ld;
     SmBatch<E, SM_PT> first;
     first.load(row, lo + threadIdx.x * 4, hi);
+    sm_powers_init();   // under the loads
     const SmHead h = sm_head(a, w, b);
     const int k = sm_topk(a, b);
     const float p = sm_topp(a, b);
@@ -603,8 +629,7 @@ __global__ __launch_bounds__(SM_PT) void sm_bins_kernel(SampleArgs a, SmWs w)
     if (weigh)
         sm_each<E, SM_PT>(row, lo, hi, first, [&](int, const uint32_t (&key)[4]) {
             unsigned long long x[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) x[j] = sm_weight(key[j], h.top, h.scale);
+            sm_weights(key, h.top, h.scale, 0.0, x);
 #pragma unroll
             for (int j = 0; j < 4; ++j)
                 if (key[j] > SM_MASKED)
@@ -756,6 +781,7 @@ __global__ __launch_bounds__(SM_PT) void sm_cut_kernel(SampleArgs a, SmWs w)
     const bool ahead = w.len <= SM_PT * 16;
     SmBatch<E, SM_PT> first;
     if (ahead) first.load(row, lo + threadIdx.x * 4, hi);
+    sm_powers_init();   // under the loads
     const SmHead h = sm_head(a, w, b);
     if (h.done) return;
     const SmCut c = sm_cut(a, w, b, h, scratch, found);
@@ -775,13 +801,11 @@ __global__ __launch_bounds__(SM_PT) void sm_cut_kernel(SampleArgs a, SmWs w)
     if (c.mode == SM_ALL)
     {
         const double m = sm_minp(a, b);
+        __syncthreads();   // the table of powers
         sm_each<E, SM_PT>(row, lo, hi, first, [&](int, const uint32_t (&key)[4]) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-            {
-                const double e = sm_exp(key[j], h.top, h.scale);
-                mine += key[j] > SM_MASKED && e >= m ? sm_units(e) : 0;
-            }
+            unsigned long long x[4];
+            sm_weights(key, h.top, h.scale, m, x);
+            mine += x[0] + x[1] + (x[2] + x[3]);
         });
     }
     else
@@ -893,6 +917,7 @@ __global__ __launch_bounds__(SM_T) void sm_pick_kernel(SampleArgs a, SmWs w)
 #pragma unroll
     for (int j = 0; j < SM_PER; ++j) comp[j] = list[threadIdx.x + j * SM_T];
     if ((int)threadIdx.x < w.S) slice_mass = w.slice[(size_t)b * w.S + threadIdx.x].mass;
+    sm_powers_init();   // under the loads
     const SmState st = w.state[b];
     const SmHead h = sm_head(a, w, b);
     auto answer = [&](int token, unsigned long long x, unsigned long long total) {
@@ -916,6 +941,7 @@ __global__ __launch_bounds__(SM_T) void sm_pick_kernel(SampleArgs a, SmWs w)
         __syncthreads();
         sm_row_slow(sh.slow, a, b, r, h.top, h.scale);
     };
+    __syncthreads();   // the table of powers
     if (st.mode == SM_SLOW || (st.mode != SM_ALL && st.count > SM_LIST)) return slow();
     const double mp = sm_minp(a, b);
     const int n = st.mode == SM_ALL ? 0 : st.count;
@@ -1012,7 +1038,16 @@ __global__ __launch_bounds__(SM_T) void sm_pick_kernel(SampleArgs a, SmWs w)
         return x >= mp ? sm_units(x) : 0;
     };
     unsigned long long sum = 0, all;
-    for (int i = i0; i < i1; ++i) sum += weight(i);
+    for (int i = i0; i < i1; i += 4)   // 4 at a time, their exponentials side by side
+    {
+        uint32_t key[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) key[j] = i + j < i1 ? sm_key(static_cast<float>(row[i + j])) : 0;
+        unsigned long long x[4];
+        sm_weights(key, h.top, h.scale, mp, x);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sum += ((unsigned long long)key[j] << 32 | (uint32_t)~(i + j)) < cut ? 0 : x[j];
+    }
     unsigned long long c = base + sm_scan<SM_T>(sum, f.scratch, all);
     if (c < target && c + sum >= target)
         for (int i = i0; i < i1; ++i)
