@@ -61,7 +61,7 @@ __global__ __launch_bounds__(256) void linear_row_kernel(GmArgs a)
         for (int o = 32; o; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o));
         if (lane == 0) red[m][wave] = top;
     }
-    gm_barrier();   // (not __syncthreads, which waits for the weights too)
+    gm_barrier();   // (waits for LDS alone: the weights stay under way)
     float scale[MM];
 #pragma unroll
     for (int m = 0; m < MM; ++m)

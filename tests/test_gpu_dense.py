@@ -445,6 +445,23 @@ def test_sample_masks(gpu, V):
     assert tok.tolist()[1:3] == [-1, -1] and prob.tolist()[1:3] == [0.0, 0.0]
 
 
+@pytest.mark.parametrize("V", [700, 2930])
+def test_sample_rows_with_few_or_no_logits_left(gpu, V):
+    """A mask that leaves a row 0 to 5 logits or so, each row's own settings."""
+    g = _rng(V + 1)
+    B = 90
+    r = lambda: torch.rand(B, generator=g)
+    x = torch.randn((B, V), generator=g) * 3
+    x[torch.rand((B, V), generator=g) < 1 - 2.0 / V] = -math.inf
+    k = (torch.exp(r() * math.log(300.0))).int()
+    k[r() < 0.3] = 0
+    left = (x > -math.inf).sum(1)
+    assert int(left.min()) == 0 and int(left.max()) > 2
+    _check_draw(x, r(), temperature=0.5 + r(), top_k=k, top_p=0.6 + 0.4 * r(), min_p=0.1 * r())
+    _check_draw(x, r(), temperature=0.5 + r(), top_p=0.6 + 0.4 * r())
+    _check_draw(x, r())
+
+
 @pytest.mark.parametrize("V", [300, 66000])
 def test_sample_ties(gpu, V):
     """Equal logits: the lowest indices are kept, -0 equals +0, u walks the kept ones in order."""
