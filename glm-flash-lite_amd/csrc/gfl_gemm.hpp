@@ -941,7 +941,14 @@ __global__ __launch_bounds__(256, 1) void gm_big_kernel(GmArgs a)
 #pragma unroll
             for (int e = 0; e < 64; ++e) T::mfma_agpr(fb[0][e % 8], fa[0][e / 8], acc[e % 8][e / 8]);
         }
-    asm volatile("s_nop 15\n\ts_nop 15");   // the last MFMAs' results, which the compiler does not track
+    // The last MFMAs' results: the compiler puts no wait between an MFMA in asm and a read of what it writes, so these 32 wait
+    // states, more than any MFMA needs, come before every read: each accumulator passes an asm after them. (By themselves they
+    // hold nothing back: the reads were moved up to 5 instructions behind the MFMA.)
+    asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) asm volatile("" : "+a"(acc[i][j]));
     if (a.wide)
     {
         gm_barrier();   // the ring is done with
