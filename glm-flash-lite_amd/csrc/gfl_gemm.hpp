@@ -106,7 +106,7 @@ __device__ __forceinline__ int gm_lds_at(char* lds) { return (int)(uint32_t)rein
 __device__ __forceinline__ void gm_load_lds(gm_i4 r, int lds, uint32_t v)
 {
     const int at = __builtin_amdgcn_readfirstlane(lds);
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(at), "v"(v), "s"(r) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(at), "v"(v), "s"(r) : "memory", "m0");
 }
 
 constexpr uint32_t GM_OUT = 0x80000000u;   // a lane offset past every buffer: reads as zero

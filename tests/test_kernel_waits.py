@@ -83,3 +83,17 @@ def test_accumulators_are_read_after_the_wait(big):
                     work.append((to, waited))
                 if op != "s_branch":
                     work.append((j + 1, waited))
+
+
+def test_asm_names_m0_where_it_writes_it():
+    """An asm that sets M0 (the LDS address of direct loads) says so, or the compiler may keep a value of its own there."""
+    src = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "glm-flash-lite_amd", "csrc")
+    found = 0
+    for name in sorted(os.listdir(src)):
+        if name.endswith((".hip", ".hpp")):
+            with open(os.path.join(src, name)) as f:
+                for stmt in re.findall(r"asm volatile\((.*?)\);", f.read(), re.S):
+                    if re.search(r"\bm0, %", stmt):
+                        found += 1
+                        assert '"m0"' in stmt.rsplit(":", 1)[1], (name, stmt)
+    assert found
