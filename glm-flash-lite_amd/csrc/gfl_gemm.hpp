@@ -326,6 +326,10 @@ __device__ __forceinline__ void gm_put4(void* out, int odt, int64_t at, const fl
     else gm_store4(static_cast<_Float16*>(out) + at, v, n);
 }
 
+// The clamps of silu(g) and u, by comparison: a NaN stays one (fminf and fmaxf would give the limit for it).
+__device__ __forceinline__ float gm_clamp_gate(float t, float limit) { return t > limit ? limit : t; }
+__device__ __forceinline__ float gm_clamp_up(float v, float limit) { return v > limit ? limit : v < -limit ? -limit : v; }
+
 // the block's forward epilogue for 4 neighbouring columns: h, and g and u of a training pass in fp32 (16-bit ones doubled the
 // gradients' error: 2.0 against 1.4 roundings in the root mean square; their traffic is 2% of a training step)
 template <typename E>
@@ -337,8 +341,8 @@ __device__ __forceinline__ void gm_gate_of(float limit, const float (&g)[4], con
         float s, t = gm_silu<E>(g[i], s), v = u[i];
         if (limit != 0.f)
         {
-            t = fminf(t, limit);
-            v = fminf(fmaxf(v, -limit), limit);
+            t = gm_clamp_gate(t, limit);
+            v = gm_clamp_up(v, limit);
         }
         h[i] = t * v;
     }
@@ -370,8 +374,8 @@ __device__ __forceinline__ void gm_dact_of(float limit, const float (&dh)[4], co
         {
             if (t > limit) kg = 0.f;
             if (fabsf(v) > limit) ku = 0.f;
-            t = fminf(t, limit);
-            v = fminf(fmaxf(v, -limit), limit);
+            t = gm_clamp_gate(t, limit);
+            v = gm_clamp_up(v, limit);
         }
         dg[i] = dh[i] * v * kg;
         du[i] = dh[i] * t * ku;

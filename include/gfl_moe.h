@@ -274,7 +274,7 @@ enum
  * y = h Wd^T, with the experts' clamp L = act_limit (0 = off). x [M, H], Wg and Wu [I, H], Wd [H, I] contiguous (as
  * nn.Linear keeps them), all of one type dtype (GFL_F16 or GFL_BF16); out [M, H] of out_dtype: dtype or GFL_F32. accumulate
  * (GFL_F32 only): out += y, the shared expert's join. Sums are fp32; h is rounded to dtype before the down product (for
- * GFL_F16 its range is fp16's), everything else once at the end.
+ * GFL_F16 its range is fp16's), everything else once at the end. The clamps pass NaN on; silu(-inf) is NaN.
  * g, u fp32 [M, I] contiguous (both or neither): what the backward pass needs. */
 int gfl_ffn_forward(const void* x, int64_t ldx, const void* wg, const void* wu, const void* wd, int dtype, int M, int H,
                     int I, float act_limit, float* g, float* u, void* out, int64_t ldo, int out_dtype, int accumulate,
