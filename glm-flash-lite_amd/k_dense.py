@@ -5,6 +5,7 @@ Both hold plain torch tensors and run on torch's current stream of their device;
 torch's allocator, so calls on several streams and captured graphs share nothing but the weights.
 """
 import torch
+from torch.autograd import forward_ad
 
 import _native
 
@@ -35,10 +36,17 @@ def _no_capture(x, what):
                            "and ffn_backward, with gradients in tensors of your own")
 
 
+def _no_tangents(*inputs):
+    # a dual tensor need not have requires_grad, and the library's calls do not see its tangent
+    if any(forward_ad.unpack_dual(t).tangent is not None for t in inputs):
+        raise RuntimeError("gated_ffn: no forward-mode differentiation: an input has a tangent, which would be dropped")
+
+
 def gated_ffn(x, wg, wu, wd, act_limit=0.0):
     """_native.ffn_forward's block, differentiable: x fp16 or bf16 [..., H], wg and wu [I, H], wd [H, I] of its type. Keeps
-    8 bytes a token and I channel (g and u in fp32) for the backward where a gradient is wanted. Once differentiable; refuses
-    stream capture with gradients (RuntimeError)."""
+    8 bytes a token and I channel (g and u in fp32) for the backward where a gradient is wanted. Once differentiable, in reverse
+    mode: refuses inputs with tangents, and stream capture with gradients (RuntimeError)."""
+    _no_tangents(x, wg, wu, wd)
     if torch.is_grad_enabled() and any(t.requires_grad for t in (x, wg, wu, wd)):
         _no_capture(x, "forward")
         return _GatedFFN.apply(x, wg, wu, wd, float(act_limit))

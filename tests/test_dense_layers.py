@@ -78,3 +78,39 @@ def test_layers_refuse_host_tensors_and_shapes():
             k_dense.Linear8(bad)
     with pytest.raises(ValueError, match="device"):
         k_dense.Linear8(w(4, 8))
+
+
+def _plain_calls(monkeypatch):
+    """The layers over plain torch operations instead of the device's calls."""
+    import _native
+
+    def ffn_forward(x, wg, wu, wd, act_limit=0.0, save=False, **kw):
+        with torch.no_grad():
+            g, u = x.float() @ wg.float().t(), x.float() @ wu.float().t()
+            y = ((torch.sigmoid(g) * g * u) @ wd.float().t()).to(x.dtype)
+        return (y, g, u) if save else y
+
+    monkeypatch.setattr(_native, "ffn_forward", ffn_forward)
+    monkeypatch.setattr(_native, "quant_i8", lambda w: (torch.zeros(w.shape, dtype=torch.int8), torch.ones(w.shape[0])))
+    monkeypatch.setattr(_native, "linear_i8", lambda x, w, s, out=None, dtype=None: x.new_zeros(x.shape[:-1] + w.shape[:1]))
+
+
+@pytest.mark.parametrize("which", range(4))
+@pytest.mark.parametrize("grad", [False, True])
+def test_gated_ffn_refuses_forward_mode(monkeypatch, which, grad):
+    """A tangent that the block would drop without a word is refused, whichever input holds it."""
+    import k_dense
+    import torch.autograd.forward_ad as fwd
+    _plain_calls(monkeypatch)
+    w = lambda *s: torch.randn(s).half()
+    args = [w(2, 16), w(8, 16), w(8, 16), w(16, 8)]
+    if grad:
+        args[3 - which].requires_grad_()
+    k_dense.gated_ffn(*args)
+    with fwd.dual_level():
+        k_dense.gated_ffn(*args)     # no tangent: as outside
+        args[which] = fwd.make_dual(args[which], torch.ones_like(args[which]))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            k_dense.gated_ffn(*args)
+        with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+            k_dense.gated_ffn(*args)
