@@ -395,6 +395,7 @@ def grouped_rows(sel, w, take, E):
 
 # ---------------------------------------------------------------------------------------------------------------
 # dense operators: the gated feed-forward block, the 8-bit integer product, sampling
+# (the library's calls as they are: autograd does not see them; k_dense.py has the layers)
 # ---------------------------------------------------------------------------------------------------------------
 
 _EXT = None

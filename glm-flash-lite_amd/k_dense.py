@@ -36,17 +36,17 @@ def _no_capture(x, what):
                            "and ffn_backward, with gradients in tensors of your own")
 
 
-def _no_tangents(*inputs):
+def _no_tangents(who, *inputs):
     # a dual tensor need not have requires_grad, and the library's calls do not see its tangent
     if any(forward_ad.unpack_dual(t).tangent is not None for t in inputs):
-        raise RuntimeError("gated_ffn: no forward-mode differentiation: an input has a tangent, which would be dropped")
+        raise RuntimeError(f"{who}: no forward-mode differentiation: an input has a tangent, which would be dropped")
 
 
 def gated_ffn(x, wg, wu, wd, act_limit=0.0):
     """_native.ffn_forward's block, differentiable: x fp16 or bf16 [..., H], wg and wu [I, H], wd [H, I] of its type. Keeps
     8 bytes a token and I channel (g and u in fp32) for the backward where a gradient is wanted. Once differentiable, in reverse
     mode: refuses inputs with tangents, and stream capture with gradients (RuntimeError)."""
-    _no_tangents(x, wg, wu, wd)
+    _no_tangents("gated_ffn", x, wg, wu, wd)
     if torch.is_grad_enabled() and any(t.requires_grad for t in (x, wg, wu, wd)):
         _no_capture(x, "forward")
         return _GatedFFN.apply(x, wg, wu, wd, float(act_limit))
@@ -64,5 +64,10 @@ class Linear8:
         self.weight, self.scale = _native.quant_i8(weight.detach())
 
     def __call__(self, x, out=None, dtype=None):
-        """x fp16 or bf16 [..., K] -> [..., N] in `dtype` (x's by default), or into `out`."""
+        """x fp16 or bf16 [..., K] -> [..., N] in `dtype` (x's by default), or into `out`. Has no gradient: an x or out that
+        requires one, or an x with a tangent, is refused (RuntimeError); call it under torch.no_grad() or on x.detach()."""
+        if torch.is_grad_enabled() and (x.requires_grad or (out is not None and out.requires_grad)):
+            raise RuntimeError("Linear8: rounding to 8 bits has no gradient, and this call would drop the one that is asked "
+                               "for: call it under torch.no_grad() or on x.detach()")
+        _no_tangents("Linear8", x)
         return _native.linear_i8(x, self.weight, self.scale, out=out, dtype=dtype)

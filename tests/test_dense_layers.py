@@ -114,3 +114,26 @@ def test_gated_ffn_refuses_forward_mode(monkeypatch, which, grad):
             k_dense.gated_ffn(*args)
         with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
             k_dense.gated_ffn(*args)
+
+
+def test_linear8_refuses_gradients(monkeypatch):
+    """The 8-bit layer has no gradient: an input that asks for one is refused instead of being cut off."""
+    import k_dense
+    import torch.autograd.forward_ad as fwd
+    _plain_calls(monkeypatch)
+    head = k_dense.Linear8(torch.randn(4, 8).half().requires_grad_())    # the weight is taken as it stands
+    x = torch.randn(2, 8).half()
+    assert not head(x).requires_grad
+    y = x.clone().requires_grad_()
+    for t in (y, y * 2):
+        with pytest.raises(RuntimeError, match="Linear8.*gradient"):
+            head(t)
+        with torch.no_grad():
+            assert not head(t).requires_grad
+        assert not head(t.detach()).requires_grad
+    with torch.inference_mode():
+        head(y)
+    with fwd.dual_level(), pytest.raises(RuntimeError, match="Linear8.*forward-mode"):
+        head(fwd.make_dual(x, torch.ones_like(x)))
+    with pytest.raises(RuntimeError, match="Linear8.*gradient"):
+        head(x, out=torch.zeros(2, 4).requires_grad_())
