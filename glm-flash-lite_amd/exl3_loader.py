@@ -211,14 +211,17 @@ def _dense_weight(L, proj, spec, handles, dev):
     return t.to(device=dev, dtype=torch.float16).contiguous()
 
 
-def load(paths, ctx, layers=None, device=0, shared=None):
+def load(paths, ctx, layers=None, device=0, shared=None, act_limit=0.0):
     """Copy the routed experts of `layers` (default: all layers found) into HBM and register each as context layer
     index L. With `shared` (a k_overlap.SharedOverlap), shared experts are registered there under the same index,
     and with the routed layer in ctx too (gfl_register_shared), so that both can run in one call's launches; unquantised ones
-    are registered there by register_dense (and left in the checkpoint without `shared`).
+    are registered there by register_dense (and left in the checkpoint without `shared`) with the SwiGLU clamp act_limit, 0 =
+    off: the checkpoint's weights do not say it. (The quantised experts take theirs from each call.)
     Returns {L: ResidentLayer}."""
     import torch
     from safetensors import safe_open
+    if not act_limit >= 0.0:
+        raise ValueError(f"load: act_limit must be >= 0, not {act_limit}")
     if isinstance(paths, str):
         paths = [paths]
     specs = scan(paths)
@@ -245,7 +248,7 @@ def load(paths, ctx, layers=None, device=0, shared=None):
                     shared.register(L, sp.H, sp.I, sp.Ks, sh.ptr_table, keep=sh, routed=ctx)
             if sp.dense and shared is not None:
                 res.dense = tuple(_dense_weight(L, p, sp, handles, dev) for p in PROJ)
-                shared.register_dense(L, *res.dense)
+                shared.register_dense(L, *res.dense, act_limit=act_limit)
             out[L] = res
     finally:
         for h in handles.values():

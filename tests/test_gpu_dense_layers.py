@@ -229,3 +229,27 @@ def test_linear8(gpu, dt):
     assert lin(x, out=out) is not None
     want, bound = _head_ref(x.reshape(6, 200), weight, F32)
     R.within(out.reshape(6, 301), want, bound)
+
+
+@pytest.mark.parametrize("limit", [0.0, 0.05])
+def test_the_checkpoints_clamp(gpu, loaded, tmp_path, limit):
+    """load(act_limit=...) clamps the unquantised shared experts it registers."""
+    import exl3_loader
+    import k_overlap
+    L, M = 7, 9
+    paths = ckpt_synth.write(tmp_path, [L], E=E, H=H, I=I, Ks_by_layer={L: KS}, shared=False)
+    weights = [t.cuda() for t in ckpt_synth.write_dense(tmp_path, L, H, 384, F16)]
+    paths.append(str(tmp_path / f"dense-{L:05d}.safetensors"))
+    so = k_overlap.SharedOverlap(0)
+    for bad in (-1.0, math.nan):
+        with pytest.raises(ValueError, match="act_limit"):
+            exl3_loader.load(paths, gpu, shared=so, act_limit=bad)
+    exl3_loader.load(paths, gpu, shared=so, act_limit=limit)
+    x, sel, w = _picks(np.random.default_rng(70), M)
+    routed, both = (torch.empty((M, H), dtype=F32, device="cuda") for _ in range(2))
+    gpu.moe_forward(L, x, sel, w, routed)
+    so.forward(gpu, L, x, sel, w, both)
+    ref, off = R.FFN(x, *weights, limit, out_dt=F32), R.FFN(x, *weights, out_dt=F32)
+    assert limit == 0 or bool(((ref.y - off.y).abs() > ref.ey + off.ey).any())
+    want = routed.double().cpu() + ref.y
+    R.within(both, want, ref.ey + 2.0 ** -24 * (want.abs() + ref.ey), "routed + shared")
