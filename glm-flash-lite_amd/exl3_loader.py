@@ -48,6 +48,7 @@ class LayerSpec:
     entries: dict = field(default_factory=dict)
     has_shared: bool = False
     dense: dict = field(default_factory=dict)     # the unquantised shared expert: {proj: (file, key)}
+    dense_missing: tuple = ()                     # the weights that an unquantised shared expert lacks, where some are there
 
     @property
     def tile_bytes(self):
@@ -147,6 +148,8 @@ def scan(paths):
             if [ds[p][2] for p in PROJ] != [(n, sp.H), (n, sp.H), (sp.H, n)]:
                 raise ValueError(f"layer {L}: shared expert weights {[ds[p][2] for p in PROJ]} do not fit hidden {sp.H}")
             sp.dense = {p: ds[p][:2] for p in PROJ}
+        elif ds and not sp.has_shared:
+            sp.dense_missing = tuple(p for p in PROJ if p not in ds)
         specs[L] = sp
     return specs
 
@@ -211,12 +214,21 @@ def _dense_weight(L, proj, spec, handles, dev):
     return t.to(device=dev, dtype=torch.float16).contiguous()
 
 
+def _check_dense(specs, layers):
+    """Refuses layers whose unquantised shared expert lacks a weight (or has it in a type that scan leaves alone)."""
+    for L in layers:
+        if L in specs and specs[L].dense_missing:
+            raise ValueError(f"layer {L}: the unquantised shared expert has no fp16 or bf16 weight for "
+                             f"{', '.join(specs[L].dense_missing)}")
+
+
 def load(paths, ctx, layers=None, device=0, shared=None, act_limit=0.0):
     """Copy the routed experts of `layers` (default: all layers found) into HBM and register each as context layer
     index L. With `shared` (a k_overlap.SharedOverlap), shared experts are registered there under the same index,
     and with the routed layer in ctx too (gfl_register_shared), so that both can run in one call's launches; unquantised ones
     are registered there by register_dense (and left in the checkpoint without `shared`) with the SwiGLU clamp act_limit, 0 =
-    off: the checkpoint's weights do not say it. (The quantised experts take theirs from each call.)
+    off: the checkpoint's weights do not say it. (The quantised experts take theirs from each call.) One that lacks some of
+    its three weights is refused (ValueError).
     Returns {L: ResidentLayer}."""
     import torch
     from safetensors import safe_open
@@ -226,6 +238,8 @@ def load(paths, ctx, layers=None, device=0, shared=None, act_limit=0.0):
         paths = [paths]
     specs = scan(paths)
     want = sorted(specs) if layers is None else list(layers)
+    if shared is not None:
+        _check_dense(specs, want)
     dev = torch.device("cuda", device)
     out = {}
     handles = {}

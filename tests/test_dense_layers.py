@@ -137,3 +137,37 @@ def test_linear8_refuses_gradients(monkeypatch):
         head(fwd.make_dual(x, torch.ones_like(x)))
     with pytest.raises(RuntimeError, match="Linear8.*gradient"):
         head(x, out=torch.zeros(2, 4).requires_grad_())
+
+
+@pytest.mark.parametrize("have", [("gate",), ("gate", "down"), ("up", "down")])
+def test_load_refuses_part_of_a_shared_expert(tmp_path, have):
+    """One or two of the three unquantised weights: what is asked to load shared experts says what is missing, before anything
+    is copied. scan, and load without shared experts, leave it alone."""
+    import exl3_loader
+    from safetensors import safe_open
+    from safetensors.torch import save_file
+    paths = ckpt_synth.write(tmp_path, [1], E=2, H=512, I=256, Ks_by_layer=KS, shared=False)
+    ckpt_synth.write_dense(tmp_path, 1, 512, 384, torch.float16)
+    with safe_open(str(tmp_path / "dense-00001.safetensors"), framework="pt", device="cpu") as f:
+        part = {k: f.get_tensor(k) for k in f.keys() if any(f".{p}_proj." in k for p in have)}
+    save_file(part, str(tmp_path / "part.safetensors"))
+    paths.append(str(tmp_path / "part.safetensors"))
+    assert not exl3_loader.scan(paths)[1].dense
+    missing = [p for p in exl3_loader.PROJ if p not in have]
+    for layers in (None, [1]):
+        with pytest.raises(ValueError, match="layer 1.*" + ".*".join(missing)):
+            exl3_loader.load(paths, None, layers=layers, shared=object())
+
+
+def test_load_takes_other_layers_beside_part_of_a_shared_expert(tmp_path):
+    """A layer that is not asked for, or whose shared expert is there in quantised form, is no reason to refuse."""
+    import exl3_loader
+    paths = ckpt_synth.write(tmp_path, [1, 2], E=2, H=512, I=256, Ks_by_layer={1: (3, 3, 3), 2: (3, 3, 3)}, shared=True)
+    ckpt_synth.write_dense(tmp_path, 1, 512, 384, torch.float16)
+    from safetensors import safe_open
+    from safetensors.torch import save_file
+    with safe_open(str(tmp_path / "dense-00001.safetensors"), framework="pt", device="cpu") as f:
+        key = sorted(f.keys())[0]
+        save_file({key: f.get_tensor(key)}, str(tmp_path / "part.safetensors"))
+    specs = exl3_loader.scan(paths + [str(tmp_path / "part.safetensors")])
+    exl3_loader._check_dense(specs, [1, 2])
