@@ -92,6 +92,9 @@ class SharedOverlap:
         bits. A layer of register_dense always runs in the stock order."""
         if li in self._dense:
             wg, wu, wd, limit = self._dense[li]
+            if x.shape[-1] != wg.shape[1] or x.device != wg.device:   # before the routed call, not after it
+                raise ValueError(f"x is {list(x.shape)} on {x.device} but layer {li}'s shared expert has H = {wg.shape[1]} on "
+                                 f"{wg.device}")
             routed.moe_forward(li, x, sel, w, out)
             _native.ffn_forward(x, wg, wu, wd, out=out, act_limit=limit, accumulate=True)
             self.dense += 1

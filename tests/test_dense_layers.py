@@ -171,3 +171,19 @@ def test_load_takes_other_layers_beside_part_of_a_shared_expert(tmp_path):
         save_file({key: f.get_tensor(key)}, str(tmp_path / "part.safetensors"))
     specs = exl3_loader.scan(paths + [str(tmp_path / "part.safetensors")])
     exl3_loader._check_dense(specs, [1, 2])
+
+
+def test_a_shared_expert_of_another_width_is_refused_before_the_routed_call():
+    import k_overlap
+
+    class Routed:
+        def moe_forward(self, *a):
+            raise AssertionError("the routed call ran first, and left its output without the shared expert")
+
+    so = object.__new__(k_overlap.SharedOverlap)
+    so.device, so._dense = torch.device("cpu"), {}
+    w = lambda *s: torch.zeros(s, dtype=torch.float16)
+    so.register_dense(0, w(8, 16), w(8, 16), w(16, 8))
+    for x in (w(2, 24), w(2, 16).to("meta")):
+        with pytest.raises(ValueError, match="layer 0"):
+            so.forward(Routed(), 0, x, None, None, torch.zeros(x.shape))
