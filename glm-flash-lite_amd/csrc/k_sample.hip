@@ -751,11 +751,13 @@ __device__ SmCut sm_cut(const SampleArgs& a, const SmWs& w, int b, const SmHead&
     const double mp = sm_minp(a, b);
     if (mp > 0.0)
     {
-        // min-p ends where exp(-d / T) = m: the bins beside that place, too, where they are not past the nucleus
-        const float place = (float)(-log(mp) * (double)h.T) * h.bins;
-        const int bm = (int)fminf(fmaxf(place, 0.0f), (float)(SM_BINS - 1));
-        c.lo = min(c.lo, max(bm - 1, 0));
-        c.hi = min(c.hi, bm + 1);
+        // min-p ends where exp(-d / T) = m: the bins beside that place, too, where they are not past the nucleus. The place
+        // in d / T is known to fp64's roundings of 1 (2^-48 holds those of the exponential and of the logarithm): at an infinite T, or
+        // one of 2^48 bins, all weights reach m = 1, not the bin at d = 0 alone.
+        const double end = -log(mp), low = end - 0x1p-48, high = end + 0x1p-48;
+        auto bin = [&](double x) { return (int)fminf((float)(x * (double)h.T) * h.bins, (float)(SM_BINS - 1)); };
+        c.lo = min(c.lo, max((low > 0.0 ? bin(low) : 0) - 1, 0));
+        c.hi = min(c.hi, bin(high) + 1);
     }
     // weight above the list's bins
     at = before;
