@@ -49,8 +49,24 @@ def _products(plan, M, H, I):
 
 def test_training_pass_in_large_tiles(plan):
     import test_gpu_dense_tiles as T
-    M, H, I = T.ALL
-    p = _products(plan, M, H, I)
-    assert all(tm == 256 for tm, _ in p.values()), p
-    assert p["gate_up"][1] and p["dwd"][1]
-    assert M % 32 and H % 32 and I % 32 and H % 256 and I % 256
+    for M, H, I in [T.ALL] + T.RAGGED:
+        p = _products(plan, M, H, I)
+        assert all(tm == 256 for tm, _ in p.values()), p
+        assert p["gate_up"][1] and p["dwd"][1]
+        assert M % 32 and H % 32 and I % 32 and H % 256 and I % 256
+    assert [s[1] % 8 == s[2] % 8 == 0 for s in [T.ALL] + T.RAGGED] == [True, False, False]
+    assert [s[2] % 4 == 0 for s in T.RAGGED] == [True, False]
+
+
+def test_last_columns_in_a_launch_of_their_own(plan):
+    import test_gpu_dense_tiles as T
+    for name, (M, H, I) in T.REST.items():
+        p = _products(plan, M, H, I)[name]
+        assert p[0] == 256 and p[1] and M % 32 and H % 32 and I % 32, (name, p)
+
+
+def test_gemm_i8_in_large_tiles(plan):
+    import test_gpu_dense_tiles as T
+    p = [plan(NT, I8, *s) for s in T.I8]
+    assert all(tm == 256 for tm, _ in p) and [bool(f) for _, f in p] == [False, False, True, True], p
+    assert all(K % 64 and N % 256 for _, N, K in T.I8) and T.I8[1][2] % 4

@@ -378,6 +378,15 @@ def test_linear_i8_few_tokens(gpu, M, N, K, pad, dt):
             assert bool(got[0].isnan().all()) == (k >= 2)
 
 
+@pytest.mark.parametrize("dt", [F16, BF16])
+@pytest.mark.parametrize("M,N,K,pad", [(1, 33, 1032, 0), (2, 33, 5000, 8), (1, 16385, 1024, 0), (2, 20011, 1272, 0), (2, 16384, 2056, 0),
+                                       (1, 40000, 1024, 0)])
+def test_linear_i8_few_tokens_in_one_launch(gpu, M, N, K, pad, dt):
+    """Sizes that the launch of both takes (K from 1024 to 8192 in whole chunks): rows that end inside their last KB, and more
+    columns than its workgroups take at once (16,384)."""
+    test_linear_i8_few_tokens(gpu, M, N, K, pad, dt)
+
+
 # ---------------------------------------------------------------------------------------------------------------
 
 def _draw(logits, u, **kw):
