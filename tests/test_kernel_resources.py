@@ -61,3 +61,13 @@ def test_chain_gemm_fits_without_spills(kernels, K, slots, waves):
     """The chain GEMM's loops are bound by issue: a register spilled is a scratch reload in every tile row."""
     k = kernels["xg_gemm_kernel<%d, %d>" % (K, slots)]
     assert k[".vgpr_spill_count"] == 0 and k[".private_segment_fixed_size"] == 0 and _waves(k) >= waves
+
+
+def test_dense_kernels_spill_in_the_large_tiles_ends_alone(kernels):
+    """The tile GEMM's, the few-token and the sampling kernels keep their values in registers; the 256 x 256 kernel (all 512)
+    spills up to 28 around its epilogue (test_kernel_waits.py: not in its K loop)."""
+    dense = {n: k for n, k in kernels.items() if n.startswith(("gm_", "sm_", "quant_i8", "linear_row"))}
+    large = {n: k for n, k in dense.items() if n.startswith("gm_big_kernel")}
+    assert len(large) == 11 and len(dense) > 100
+    for n, k in dense.items():
+        assert k[".vgpr_spill_count"] <= (28 if n in large else 0), (n, k[".vgpr_spill_count"])

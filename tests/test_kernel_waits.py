@@ -97,3 +97,19 @@ def test_asm_names_m0_where_it_writes_it():
                         found += 1
                         assert '"m0"' in stmt.rsplit(":", 1)[1], (name, stmt)
     assert found
+
+
+def test_large_tiles_k_loop_has_no_scratch(big):
+    """The K loop, two steps of 64 MFMAs, touches no scratch memory; what the kernel spills it spills around its ends."""
+    for name, code in big.items():
+        at = {a: k for k, (a, _, _) in enumerate(code)}
+        start = code[0][0]
+        loops = []
+        for k, (_, ins, tail) in enumerate(code):
+            if ins.startswith(("s_cbranch", "s_branch")):
+                to = at[start + int(re.search(r"\+0x([0-9a-f]+)>", tail).group(1), 16)]
+                body = [i for _, i, _ in code[to:k + 1]]
+                if to < k and sum(i.startswith("v_mfma") for i in body) == 128:
+                    loops.append(body)
+        body = min(loops, key=len)
+        assert not [i for i in body if i.startswith("scratch_")], name
