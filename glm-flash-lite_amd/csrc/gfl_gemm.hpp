@@ -331,7 +331,10 @@ __device__ __forceinline__ float gm_clamp_gate(float t, float limit) { return t 
 __device__ __forceinline__ float gm_clamp_up(float v, float limit) { return v > limit ? limit : v < -limit ? -limit : v; }
 
 // the block's forward epilogue for 4 neighbouring columns: h, and g and u of a training pass in fp32 (16-bit ones doubled the
-// gradients' error: 2.0 against 1.4 roundings in the root mean square; their traffic is 2% of a training step)
+// gradients' error: 2.0 against 1.4 roundings in the root mean square; their traffic is 2% of a training step). h (like dg and du
+// of the backward pass) is rounded to the inputs' type, as the next product's MFMAs take it: y is off by 1.4 of the one rounding that it
+// has with an fp32 h (root mean square, relative: bf16 2.3e-3 and 1.7e-3, fp16 2.9e-4 and 2.1e-4). An h in two halves would give that
+// back for twice the MFMAs and bytes of down's product.
 template <typename E>
 __device__ __forceinline__ void gm_gate_of(float limit, const float (&g)[4], const float (&u)[4], float (&h)[4])
 {
@@ -787,10 +790,11 @@ __device__ __forceinline__ void gm_big_epilogue(const GmArgs& a, const typename 
 // The largest products: 256 x 256 by 4 waves of 128 x 128, one to a SIMD. Bound by LDS reads: 8 waves of 128 x 64 read 192 KB for
 // a tile's 64 k (1536 cycles of 128 bytes, beside 512 of writes and 2048 of MFMA), these 128 KB. A wave's accumulators
 // are all 256 AGPRs (by asm constraint; left to itself the compiler copied or spilled them), its fragments of this step and of the
-// next 128 VGPRs. K steps of 64 bytes a row, NST slots of 32 KB: a step's MFMAs run under the reads of the next step's
-// fragments and the loads of the step NST - 1 ahead, one barrier a step. bf16 4096 x 12288 x 5120: 384 us (1.34
-// PFLOP/s) against 466 by 8 waves on one card; 8192 x 8192 x 8192: 785 (1.40) against 914. Clocks fall to 2.0 GHz under it; MFMAs
-// fill 63% of the CUs' cycles. A fifth slot and other orders of the reads made no difference.
+// next 128 VGPRs. In the K loop nothing is spilled; around it 16 to 25 VGPRs are in the forms but dh's and i8's. K steps of 64 bytes a
+// row, NST slots of 32 KB: a step's MFMAs run under the reads of the next step's fragments and the loads of the step NST - 1 ahead,
+// one barrier a step. bf16 4096 x 12288 x 5120: 384 us (1.34 PFLOP/s) against 466 by 8 waves on one card; 8192 x 8192 x
+// 8192: 785 (1.40) against 914. Under it clocks are 1.9 to 2.1 GHz, and MFMAs fill 50 to 62% of the SIMDs' cycles (37 in the form
+// of dh, whose epilogue is the longest). A fifth slot and other orders of the reads made no difference.
 template <typename T, bool AKS, bool BKS, bool DUAL, int EP>
 __global__ __launch_bounds__(256, 1) void gm_big_kernel(GmArgs a)
 {
@@ -1202,6 +1206,7 @@ __global__ __launch_bounds__(NW * 64) void gm_ring_kernel(GmArgs a)
 }
 
 // The same from rows of any alignment: an MFMA fragment's 16 bytes a lane come straight from memory, U loads in flight.
+// 8 tokens, int8 12288 x 4096: 26 us, the ring 10.
 template <typename T, bool DUAL, int EP, int NW>
 __global__ __launch_bounds__(NW * 64) void gm_skinny_kernel(GmArgs a)
 {

@@ -25,8 +25,9 @@ struct GmPlan
 // 128 0.83 and 1.03, deep 0.62, 64 x 128 0.5, 256 x 256 1.05 and 1.5; a round's ends 14 for 256 x 256, 4 for 128 x 128, 2 for the others; 3 for
 // the launch; a join 2.5 and the parts' bytes written and read at 4 TB/s. nz: products of one launch (the gradients of gate and
 // up), which fill rounds together.
-// Against the other choice, us of a backward call for the gradients of gate's and up's weights: 2048 tokens of 5504 x 2048 128 x
-// 128 176, 256 x 256 191; 333 tokens 58 and 65; 1024 tokens of 11008 x 4096 256 x 256 335, 128 x 128 364.
+// Against the other choice, us of a backward call for the gradients of gate's and up's weights, dh's product with them: 333 tokens
+// of 5504 x 2048 128 x 128 69, 256 x 256 108; 1024 tokens of 11008 x 4096 256 x 256 343, 128 x 128 406; 2048 tokens of 5504 x 2048,
+// where the estimates are 2% apart, 190 by either.
 inline GmPlan gm_plan_one(int form, int ep, int dual, int aligned, int M, int N, int K, int segs, int nz = 1)
 {
     GmPlan best = {};

@@ -4,7 +4,8 @@
 namespace gfl {
 
 // A workgroup per row. Bound by memory: K is read once (16 values a thread stay in registers; longer rows are read again, from
-// cache).
+// cache). bf16 16384 x 8192 99 us (4.05 TB/s; a large copy reaches 4.8), 4096 x 5120 22 (2.9), 9 x 4096 4.0, the launch; rows that
+// start at no multiple of 16 bytes go value by value: 4096 x 5123 43.
 constexpr int QT = 256;
 
 template <bool BF>
