@@ -18,7 +18,9 @@ SYMBOLS = ("gfl_last_error", "gfl_version", "gfl_ctx_create", "gfl_ctx_destroy",
            "gfl_grouped_plan", "gfl_grouped_reserve", "gfl_layer_info", "gfl_route_split", "gfl_moe_forward_noalloc",
            "gfl_ctx_set_shared", "gfl_ctx_check", "gfl_ingress_serve", "gfl_register_shared",
            "gfl_moe_forward_shared", "gfl_ffn_forward", "gfl_ffn_backward", "gfl_ffn_workspace", "gfl_quant_i8",
-           "gfl_gemm_i8", "gfl_linear_i8", "gfl_i8_workspace", "gfl_sample", "gfl_sample_workspace")
+           "gfl_gemm_i8", "gfl_linear_i8", "gfl_i8_workspace", "gfl_quant_i4", "gfl_pack_i4", "gfl_linear_i4",
+           "gfl_linear_i4_dx", "gfl_i4_workspace", "gfl_route_experts", "gfl_route_experts_backward", "gfl_adjust_logits",
+           "gfl_sample", "gfl_sample_workspace")
 
 EUNSUPPORTED = 4   # GFL_EUNSUPPORTED: gfl_moe_forward_shared cannot fuse this call (nothing was launched)
 
@@ -91,6 +93,17 @@ def load(path=LIB_PATH):
     L.gfl_gemm_i8.argtypes = [_P, I64, _P, _P, I64, _P, C.c_int, C.c_int, C.c_int, _P, I64, C.c_int, _P, SZ, _P]
     L.gfl_linear_i8.argtypes = [_P, I64, C.c_int, _P, I64, _P, C.c_int, C.c_int, C.c_int, _P, I64, C.c_int, _P, SZ, _P]
     L.gfl_i8_workspace.argtypes = [C.c_int, C.c_int, C.c_int, PSZ, PSZ]
+    L.gfl_quant_i4.argtypes = [_P, I64, C.c_int, C.c_int, C.c_int, C.c_int, _P, _P, _P, _P]
+    L.gfl_pack_i4.argtypes = [_P, I64, C.c_int, C.c_int, _P, _P]
+    L.gfl_linear_i4.argtypes = [_P, I64, C.c_int, _P, _P, C.c_int, _P, C.c_int, C.c_int, C.c_int, C.c_int, _P, I64, C.c_int,
+                                _P, SZ, _P]
+    L.gfl_linear_i4_dx.argtypes = [_P, I64, C.c_int, _P, _P, C.c_int, _P, C.c_int, C.c_int, C.c_int, C.c_int, _P, I64, _P, SZ,
+                                   _P]
+    L.gfl_i4_workspace.argtypes = [C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, PSZ, PSZ]
+    L.gfl_route_experts.argtypes = [_P, I64, C.c_int, _P] + [C.c_int] * 8 + [C.c_float, _P, _P, C.c_int, _P]
+    L.gfl_route_experts_backward.argtypes = [_P, C.c_int, _P, I64, C.c_int, _P] + [C.c_int] * 5 + [C.c_float, _P, I64, _P]
+    L.gfl_adjust_logits.argtypes = [_P, I64, C.c_int, C.c_int, C.c_int, _P, I64, C.c_int, _P, _P, _P, _P, _P, _P, I64, _P, I64,
+                                    C.c_int, _P, I64, _P, I64, _P]
     L.gfl_sample.argtypes = [_P, I64, C.c_int, C.c_int, C.c_int, _P, _P, _P, _P, _P, _P, _P, _P, SZ, _P]
     L.gfl_sample_workspace.argtypes = [C.c_int, C.c_int, PSZ]
     for name in SYMBOLS:
@@ -394,7 +407,7 @@ def grouped_rows(sel, w, take, E):
 
 
 # ---------------------------------------------------------------------------------------------------------------
-# dense operators: the gated feed-forward block, the 8-bit integer product, sampling
+# dense operators: the gated feed-forward block, products with 8-bit and 4-bit weights, the choice of experts, logits, sampling
 # (the library's calls as they are: autograd does not see them; k_dense.py has the layers)
 # ---------------------------------------------------------------------------------------------------------------
 
@@ -440,6 +453,51 @@ def linear_i8(x, b, sb, out=None, dtype=None):
     """gemm_i8 of x (fp16 or bf16 [..., K]) quantised per token as quant_i8 does (gfl_linear_i8): a linear layer with an 8-bit
     weight b [N, K] and its channels' scales sb. out in `dtype` (x's type by default)."""
     return (_EXT or _ext()).linear_i8(x, b, sb, out, dtype)
+
+
+def quant_i4(weight, group=128, zeros=False):
+    """A weight fp16 or bf16 [N, K] to 4 bits with a scale for each `group` (32, 64 or 128) inputs of a channel (gfl_quant_i4):
+    (q uint8 [N, ceil(K / 128) * 64], scale [ceil(K / group), N] of its type, zero uint8 like scale or, without zeros, None)."""
+    return (_EXT or _ext()).quant_i4(weight, group, zeros)
+
+
+def pack_i4(values):
+    """Values 0..15 (uint8 [N, K]) that something else rounded, packed as linear_i4 reads them (gfl_pack_i4)."""
+    return (_EXT or _ext()).pack_i4(values)
+
+
+def linear_i4(x, q, scale, zero=None, group=128, out=None, dtype=None):
+    """out[..., n] = sum_k x[..., k] (v[n, k] - zero) scale (gfl_linear_i4): x fp16 or bf16 [..., K], the weight as quant_i4 gives
+    it; zero None: 8 throughout. out in `dtype` (x's type by default; fp16, bf16 or fp32)."""
+    return (_EXT or _ext()).linear_i4(x, q, scale, zero, group, out, dtype)
+
+
+def linear_i4_dx(dy, q, scale, K, zero=None, group=128):
+    """Gradient of linear_i4's input (gfl_linear_i4_dx) for dy fp16 or bf16 [..., N]: [..., K] of its type."""
+    return (_EXT or _ext()).linear_i4_dx(dy, q, scale, K, zero, group)
+
+
+def route_experts(logits, topk=8, bias=None, score="sigmoid", groups=1, top_groups=1, group_best=2, renorm=True, scale=1.0,
+                  dtype=None):
+    """The general router (gfl_route_experts): logits fp32, fp16 or bf16 [M, E] -> (sel int64 [M, topk], w [M, topk] in `dtype`,
+    fp16 by default). score "sigmoid" or "softmax"; bias fp32 [E] enters the choice alone; of `groups` equal parts the top_groups
+    with the largest sum of their group_best (1 or 2) best are chosen from; w = scale * score, with renorm over the picks' sum."""
+    return (_EXT or _ext()).route_experts(logits, topk, bias, score, groups, top_groups, group_best, renorm, scale, dtype)
+
+
+def route_experts_backward(dw, logits, sel, score="sigmoid", renorm=True, scale=1.0):
+    """Gradient of route_experts' logits (gfl_route_experts_backward) for dw [M, topk] (fp32, fp16 or bf16) of its weights."""
+    return (_EXT or _ext()).route_experts_backward(dw, logits, sel, score, renorm, scale)
+
+
+def adjust_logits(logits, history=None, lengths=None, prompt=None, repetition=None, frequency=None, presence=None, bias_ids=None,
+                  bias=None, allowed=None, out=None):
+    """Logits (fp32, fp16 or bf16 [B, V]) as each request's settings change them before sample (gfl_adjust_logits). history int32
+    [B, L], the first lengths[b] of a row valid and the first prompt[b] of those the prompt (int32 [B]); repetition, frequency,
+    presence fp32 [B]; bias fp32 [B, n] for the tokens bias_ids int32 [B, n]; allowed int32 [B, ceil(V / 32)], a bit a token.
+    None = off. out: of logits' shape and type, may be logits itself."""
+    return (_EXT or _ext()).adjust_logits(logits, history, lengths, prompt, repetition, frequency, presence, bias_ids, bias, allowed,
+                                          out)
 
 
 def sample(logits, u, temperature=None, top_k=None, top_p=None, min_p=None):

@@ -4,12 +4,16 @@
 #include "gfl_internal.hpp"
 
 #include <algorithm>
+#include <cmath>
 
 namespace {
 
 using gfl::api_fail;
 
 constexpr size_t up256(size_t x) { return (x + 255) & ~size_t(255); }
+
+// tokens up to which the weights of a 4-bit product are unpacked in the product's own launch (k_dense_i4.hip)
+constexpr int I4_FEW = 64;
 
 // rows of whole 4-byte words, which the direct tile loads need
 bool words(const void* p, int64_t ld_bytes)
@@ -370,6 +374,247 @@ int gfl_sample(const void* logits, int64_t ld, int dtype, int B, int V, const fl
     a.token = token; a.prob = prob; a.ws = ws;
     gfl::launch_sample(a, reinterpret_cast<hipStream_t>(stream));
     return check_launch("gfl_sample");
+}
+
+// ---- 4-bit weights ----
+
+static int i4_check(int64_t M, int N, int K, int group)
+{
+    if (M < 0 || M >= GFL_MAX_ROWS || N < 1 || N >= GFL_MAX_LD || K < 1 || K >= GFL_MAX_LD)
+        return api_fail(GFL_EINVAL, "gfl_i4: need 0 <= M < GFL_MAX_ROWS (M >= 0) and 1 <= N, K < GFL_MAX_LD");
+    if (((int64_t)K + 127) / 128 * 128 * N > (int64_t)1 << 32)   // a launch of 64 threads a block of 128 has fewer than 2^32
+        return api_fail(GFL_EINVAL, "gfl_i4: N * K (K up to a multiple of 128) must be at most 2^32");
+    if (group != 32 && group != 64 && group != 128) return api_fail(GFL_EINVAL, "gfl_i4: group must be 32, 64 or 128");
+    return GFL_OK;
+}
+
+static bool i4_exact(int M, int dtype, int out_dtype) { return M <= I4_FEW || out_dtype != dtype; }
+static int64_t i4_ldw(int K) { return ((int64_t)K + 7) / 8 * 8; }
+
+static size_t i4_part(int form, int M, int N, int K)
+{
+    return up256(std::max(gfl::gm_plan(form, gfl::EP_OUT, 0, 0, M, N, K, 1).part_bytes,
+                          gfl::gm_plan(form, gfl::EP_OUT, 0, 1, M, N, K, 1).part_bytes));
+}
+
+int gfl_i4_workspace(int dtype, int out_dtype, int M, int N, int K, size_t* forward, size_t* backward)
+{
+    if (dtype != GFL_F16 && dtype != GFL_BF16) return api_fail(GFL_EINVAL, "gfl_i4: dtype must be GFL_F16 or GFL_BF16");
+    if (int rc = i4_check(M, N, K, 32)) return rc;
+    const size_t w = up256((size_t)N * i4_ldw(K) * 2);
+    if (forward) *forward = i4_exact(M, dtype, out_dtype) ? 0 : w + i4_part(gfl::GM_NT, M, N, K);
+    if (backward) *backward = M ? w + i4_part(gfl::GM_NN, M, K, N) : 0;
+    return GFL_OK;
+}
+
+int gfl_quant_i4(const void* w, int64_t ldw, int dtype, int N, int K, int group, uint8_t* q, void* scale, uint8_t* zero,
+                 gfl_stream stream)
+{
+    if (dtype != GFL_F16 && dtype != GFL_BF16) return api_fail(GFL_EINVAL, "gfl_quant_i4: dtype must be GFL_F16 or GFL_BF16");
+    if (int rc = i4_check(0, N, K, group)) return rc;
+    if (!w || !q || !scale) return api_fail(GFL_EINVAL, "gfl_quant_i4: NULL argument");
+    if (ldw < K || ldw >= GFL_MAX_LD) return api_fail(GFL_EINVAL, "gfl_quant_i4: the row stride must be in [K, GFL_MAX_LD)");
+    if (reinterpret_cast<uintptr_t>(q) % 16) return api_fail(GFL_EINVAL, "gfl_quant_i4: q must be 16-byte aligned");
+    gfl::launch_quant_i4(w, ldw, dtype == GFL_BF16, N, K, group, q, scale, zero, reinterpret_cast<hipStream_t>(stream));
+    return check_launch("gfl_quant_i4");
+}
+
+int gfl_pack_i4(const uint8_t* v, int64_t ldv, int N, int K, uint8_t* q, gfl_stream stream)
+{
+    if (int rc = i4_check(0, N, K, 32)) return rc;
+    if (!v || !q) return api_fail(GFL_EINVAL, "gfl_pack_i4: NULL argument");
+    if (ldv < K || ldv >= GFL_MAX_LD) return api_fail(GFL_EINVAL, "gfl_pack_i4: the row stride must be in [K, GFL_MAX_LD)");
+    if (reinterpret_cast<uintptr_t>(q) % 16) return api_fail(GFL_EINVAL, "gfl_pack_i4: q must be 16-byte aligned");
+    gfl::launch_pack_i4(v, ldv, N, K, q, reinterpret_cast<hipStream_t>(stream));
+    return check_launch("gfl_pack_i4");
+}
+
+static int i4_args(gfl::Q4Args& a, const uint8_t* q, const void* scale, int scale_dtype, const uint8_t* zero, int N, int K, int group)
+{
+    if (scale_dtype != GFL_F16 && scale_dtype != GFL_BF16)
+        return api_fail(GFL_EINVAL, "gfl_i4: scale_dtype must be GFL_F16 or GFL_BF16");
+    if (!q || !scale) return api_fail(GFL_EINVAL, "gfl_i4: NULL argument");
+    if (reinterpret_cast<uintptr_t>(q) % 16) return api_fail(GFL_EINVAL, "gfl_i4: q must be 16-byte aligned");
+    a.q = q; a.scale = scale; a.zero = zero;
+    a.scale_bf = scale_dtype == GFL_BF16;
+    a.N = N; a.K = K; a.group = group;
+    a.blocks = (K + 127) / 128;
+    return GFL_OK;
+}
+
+int gfl_linear_i4(const void* x, int64_t ldx, int dtype, const uint8_t* q, const void* scale, int scale_dtype, const uint8_t* zero,
+                  int M, int N, int K, int group, void* out, int64_t ldo, int out_dtype, void* ws, size_t ws_bytes,
+                  gfl_stream stream)
+{
+    if (dtype != GFL_F16 && dtype != GFL_BF16) return api_fail(GFL_EINVAL, "gfl_linear_i4: dtype must be GFL_F16 or GFL_BF16");
+    if (out_dtype != GFL_F16 && out_dtype != GFL_BF16 && out_dtype != GFL_F32)
+        return api_fail(GFL_EINVAL, "gfl_linear_i4: out_dtype must be GFL_F16, GFL_BF16 or GFL_F32");
+    if (int rc = i4_check(M, N, K, group)) return rc;
+    if (M == 0) return GFL_OK;
+    gfl::Q4Args a;
+    if (int rc = i4_args(a, q, scale, scale_dtype, zero, N, K, group)) return rc;
+    if (!x || !out) return api_fail(GFL_EINVAL, "gfl_linear_i4: NULL argument");
+    if (ldx < K || ldx >= GFL_MAX_LD || ldo < N || ldo >= (1 << 30))
+        return api_fail(GFL_EINVAL, "gfl_linear_i4: row strides must be at least the width (x below GFL_MAX_LD, out below 2^30)");
+    size_t need = 0;
+    gfl_i4_workspace(dtype, out_dtype, M, N, K, &need, nullptr);
+    if (need && (!ws || ws_bytes < need || reinterpret_cast<uintptr_t>(ws) % 16))
+        return api_fail(GFL_EINVAL, "gfl_linear_i4: workspace missing, too small or not 16-byte aligned");
+    hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+    if (i4_exact(M, dtype, out_dtype))
+    {
+        a.x = static_cast<const char*>(x);
+        a.ldx = ldx * 2;
+        a.M = M;
+        a.out = out; a.ldo = ldo; a.odt = out_dtype;
+        gfl::launch_linear_i4(a, dtype == GFL_BF16, st);
+        return check_launch("gfl_linear_i4");
+    }
+    const int64_t ldw = i4_ldw(K);
+    const size_t wb = up256((size_t)N * ldw * 2);
+    gfl::launch_dequant_i4(a, dtype == GFL_BF16, ws, ldw, st);
+    if (int rc = check_launch("gfl_linear_i4: weights to 16 bits")) return rc;
+    gfl::GmArgs b;
+    b.A[0] = b.A[1] = static_cast<const char*>(x);
+    b.B[0] = b.B[1] = static_cast<const char*>(ws);
+    b.lda = ldx * 2;
+    b.ldb = ldw * 2;
+    b.M = M; b.N = N; b.K = K;
+    b.out[0] = out;
+    b.ldo = ldo;
+    b.odt = out_dtype;
+    b.ragged = K % 8 != 0;
+    return gemm16("gfl_linear_i4", dtype, gfl::GM_NT, gfl::EP_OUT, 0, words(x, b.lda), b, static_cast<char*>(ws) + wb,
+                  need - wb, 1, st);
+}
+
+int gfl_linear_i4_dx(const void* dy, int64_t lddy, int dtype, const uint8_t* q, const void* scale, int scale_dtype,
+                     const uint8_t* zero, int M, int N, int K, int group, void* dx, int64_t lddx, void* ws, size_t ws_bytes,
+                     gfl_stream stream)
+{
+    if (dtype != GFL_F16 && dtype != GFL_BF16) return api_fail(GFL_EINVAL, "gfl_linear_i4_dx: dtype must be GFL_F16 or GFL_BF16");
+    if (int rc = i4_check(M, N, K, group)) return rc;
+    if (M == 0) return GFL_OK;
+    gfl::Q4Args a;
+    if (int rc = i4_args(a, q, scale, scale_dtype, zero, N, K, group)) return rc;
+    if (!dy || !dx) return api_fail(GFL_EINVAL, "gfl_linear_i4_dx: NULL argument");
+    if (lddy < N || lddy >= GFL_MAX_LD || lddx < K || lddx >= GFL_MAX_LD)
+        return api_fail(GFL_EINVAL, "gfl_linear_i4_dx: row strides must be at least the width and below GFL_MAX_LD");
+    size_t need = 0;
+    gfl_i4_workspace(dtype, dtype, M, N, K, nullptr, &need);
+    if (!ws || ws_bytes < need || reinterpret_cast<uintptr_t>(ws) % 16)
+        return api_fail(GFL_EINVAL, "gfl_linear_i4_dx: workspace missing, too small or not 16-byte aligned");
+    hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+    const int64_t ldw = i4_ldw(K);
+    const size_t wb = up256((size_t)N * ldw * 2);
+    gfl::launch_dequant_i4(a, dtype == GFL_BF16, ws, ldw, st);
+    if (int rc = check_launch("gfl_linear_i4_dx: weights to 16 bits")) return rc;
+    gfl::GmArgs b;
+    b.A[0] = b.A[1] = static_cast<const char*>(dy);
+    b.B[0] = b.B[1] = static_cast<const char*>(ws);
+    b.lda = lddy * 2;
+    b.ldb = ldw * 2;
+    b.M = M; b.N = K; b.K = N;
+    b.out[0] = dx;
+    b.ldo = lddx;
+    b.odt = dtype;
+    b.ragged = N % 8 != 0 || K % 8 != 0;
+    return gemm16("gfl_linear_i4_dx", dtype, gfl::GM_NN, gfl::EP_OUT, 0, words(dy, b.lda), b, static_cast<char*>(ws) + wb,
+                  need - wb, 1, st);
+}
+
+// ---- choice of experts ----
+
+static bool known_dtype(int t) { return t == GFL_F16 || t == GFL_BF16 || t == GFL_F32; }
+
+static int route_check(int dtype, int w_dtype, int M, int E, int topk, int score, float scale)
+{
+    if (!known_dtype(dtype) || !known_dtype(w_dtype))
+        return api_fail(GFL_EINVAL, "gfl_route_experts: dtypes must be GFL_F16, GFL_BF16 or GFL_F32");
+    if (M < 0 || M >= GFL_MAX_ROWS) return api_fail(GFL_EINVAL, "gfl_route_experts: need M >= 0 and M < GFL_MAX_ROWS");
+    if (E < 1 || E > gfl::MAX_EXPERTS || topk < 1 || topk > E || topk > gfl::MAX_ROUTE_K)
+        return api_fail(GFL_EINVAL, "gfl_route_experts: need 1 <= E <= 1024 and 1 <= topk <= min(E, 64)");
+    if (score != GFL_SIGMOID && score != GFL_SOFTMAX)
+        return api_fail(GFL_EINVAL, "gfl_route_experts: score must be GFL_SIGMOID or GFL_SOFTMAX");
+    if (!std::isfinite(scale)) return api_fail(GFL_EINVAL, "gfl_route_experts: scale must be finite");
+    return GFL_OK;
+}
+
+int gfl_route_experts(const void* logits, int64_t ld, int dtype, const float* bias, int M, int E, int topk, int score, int groups,
+                      int top_groups, int group_best, int renorm, float scale, int64_t* sel, void* w, int w_dtype,
+                      gfl_stream stream)
+{
+    if (int rc = route_check(dtype, w_dtype, M, E, topk, score, scale)) return rc;
+    if (groups < 1 || groups > gfl::MAX_ROUTE_K || E % groups || top_groups < 1 || top_groups > groups)
+        return api_fail(GFL_EINVAL, "gfl_route_experts: groups must be 1..64 and divide E, top_groups 1..groups");
+    if (topk > E / groups * top_groups)
+        return api_fail(GFL_EINVAL, "gfl_route_experts: topk is more than top_groups groups hold");
+    if (group_best != 1 && group_best != 2) return api_fail(GFL_EINVAL, "gfl_route_experts: group_best must be 1 or 2");
+    if (M == 0) return GFL_OK;
+    if (!logits || !sel || !w) return api_fail(GFL_EINVAL, "gfl_route_experts: NULL argument");
+    if (ld < E) return api_fail(GFL_EINVAL, "gfl_route_experts: the row stride must be at least E");
+    gfl::RouteArgs a;
+    a.logits = logits; a.ld = ld; a.dtype = dtype; a.bias = bias;
+    a.M = M; a.E = E; a.topk = topk;
+    a.softmax = score == GFL_SOFTMAX;
+    a.groups = top_groups == groups ? 1 : groups;   // all of them: nothing to leave out
+    a.top_groups = top_groups; a.group_best = group_best;
+    a.renorm = renorm != 0;
+    a.scale = scale;
+    a.sel = sel; a.w = w; a.wdtype = w_dtype;
+    if (gfl::launch_route_experts(a, reinterpret_cast<hipStream_t>(stream)))
+        return api_fail(GFL_EINVAL, "gfl_route_experts: unsupported shape");
+    return check_launch("gfl_route_experts");
+}
+
+int gfl_route_experts_backward(const void* dw, int w_dtype, const void* logits, int64_t ld, int dtype, const int64_t* sel, int M,
+                               int E, int topk, int score, int renorm, float scale, void* dlogits, int64_t ldd,
+                               gfl_stream stream)
+{
+    if (int rc = route_check(dtype, w_dtype, M, E, topk, score, scale)) return rc;
+    if (M == 0) return GFL_OK;
+    if (!dw || !logits || !sel || !dlogits) return api_fail(GFL_EINVAL, "gfl_route_experts_backward: NULL argument");
+    if (ld < E || ldd < E) return api_fail(GFL_EINVAL, "gfl_route_experts_backward: row strides must be at least E");
+    gfl::RouteArgs a;
+    a.logits = logits; a.ld = ld; a.dtype = dtype;
+    a.M = M; a.E = E; a.topk = topk;
+    a.softmax = score == GFL_SOFTMAX;
+    a.renorm = renorm != 0;
+    a.scale = scale;
+    a.wdtype = w_dtype;
+    gfl::launch_route_backward(a, dw, sel, dlogits, ldd, reinterpret_cast<hipStream_t>(stream));
+    return check_launch("gfl_route_experts_backward");
+}
+
+// ---- logits before the draw ----
+
+int gfl_adjust_logits(const void* logits, int64_t ld, int dtype, int B, int V, const int32_t* history, int64_t ldh, int L,
+                      const int32_t* lengths, const int32_t* prompt, const float* repetition, const float* frequency,
+                      const float* presence, const int32_t* bias_ids, int64_t ldb, const float* bias, int64_t ldv, int n_bias,
+                      const int32_t* allowed, int64_t lda, void* out, int64_t ldo, gfl_stream stream)
+{
+    if (!known_dtype(dtype)) return api_fail(GFL_EINVAL, "gfl_adjust_logits: dtype must be GFL_F16, GFL_BF16 or GFL_F32");
+    if (B < 0 || B > 65535 || V < 1 || V > gfl::MAX_VOCAB)
+        return api_fail(GFL_EINVAL, "gfl_adjust_logits: need 0 <= B <= 65535 and 1 <= V <= 2^20");
+    if (L < 0 || L > GFL_MAX_HISTORY || n_bias < 0 || n_bias > GFL_MAX_BIASES)
+        return api_fail(GFL_EINVAL, "gfl_adjust_logits: need L in 0..GFL_MAX_HISTORY and n_bias in 0..GFL_MAX_BIASES");
+    if (!history && (L || lengths || prompt || repetition || frequency || presence))
+        return api_fail(GFL_EINVAL, "gfl_adjust_logits: lengths, prompt and penalties need a history");
+    if (B == 0) return GFL_OK;
+    if (!logits || !out || (n_bias && (!bias_ids || !bias))) return api_fail(GFL_EINVAL, "gfl_adjust_logits: NULL argument");
+    if (ld < V || ldo < V || (history && ldh < L) || (n_bias && (ldb < n_bias || ldv < n_bias)) || (allowed && lda < (V + 31) / 32))
+        return api_fail(GFL_EINVAL, "gfl_adjust_logits: row strides must be at least the width");
+    if (logits == out && ld != ldo && B > 1) return api_fail(GFL_EINVAL, "gfl_adjust_logits: in place, with one row stride");
+    gfl::LogitsArgs a;
+    a.logits = logits; a.ld = ld; a.out = out; a.ldo = ldo;
+    a.dtype = dtype; a.B = B; a.V = V;
+    a.history = history; a.ldh = ldh; a.L = history ? L : 0;
+    a.lengths = lengths; a.prompt = prompt;
+    a.repetition = repetition; a.frequency = frequency; a.presence = presence;
+    a.bias_ids = bias_ids; a.ldb = ldb; a.bias = bias; a.ldv = ldv; a.n_bias = n_bias;
+    a.allowed = allowed; a.lda = lda;
+    gfl::launch_logits(a, reinterpret_cast<hipStream_t>(stream));
+    return check_launch("gfl_adjust_logits");
 }
 
 }  // extern "C"

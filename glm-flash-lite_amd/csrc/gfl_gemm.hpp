@@ -326,6 +326,13 @@ __device__ __forceinline__ void gm_put4(void* out, int odt, int64_t at, const fl
     else gm_store4(static_cast<_Float16*>(out) + at, v, n);
 }
 
+__device__ __forceinline__ void gm_put1(void* out, int odt, int64_t at, float v)
+{
+    if (odt == 2) static_cast<float*>(out)[at] = v;
+    else if (odt == 1) static_cast<__bf16*>(out)[at] = static_cast<__bf16>(v);
+    else static_cast<_Float16*>(out)[at] = static_cast<_Float16>(v);
+}
+
 // The clamps of silu(g) and u, by comparison: a NaN stays one (fminf and fmaxf would give the limit for it).
 __device__ __forceinline__ float gm_clamp_gate(float t, float limit) { return t > limit ? limit : t; }
 __device__ __forceinline__ float gm_clamp_up(float v, float limit) { return v > limit ? limit : v < -limit ? -limit : v; }

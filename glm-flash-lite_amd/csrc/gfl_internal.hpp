@@ -233,6 +233,72 @@ constexpr int LQ_K = 8192;
 constexpr int LQ_WG = 2048;   // workgroups; past 8 columns each they take more
 void launch_linear_row_i8(const GmArgs& a, int bf16, hipStream_t st);
 
+// a product with a 4-bit weight (k_dense_i4.hip, k_quant4.hip)
+struct Q4Args
+{
+    const uint8_t* q = nullptr;      // [N][blocks][64], packed
+    const void* scale = nullptr;     // [groups][N], fp16 or bf16
+    const uint8_t* zero = nullptr;   // [groups][N], NULL: 8
+    int scale_bf = 0;
+    int N = 0, K = 0, group = 0, blocks = 0;   // group 32, 64 or 128; blocks of 128 inputs
+    const char* x = nullptr;
+    int64_t ldx = 0;                 // bytes
+    int M = 0;
+    void* out = nullptr;
+    int64_t ldo = 0;                 // elements
+    int odt = 0;
+};
+void launch_quant_i4(const void* w, int64_t ld, int bf16, int N, int K, int group, uint8_t* q, void* scale, uint8_t* zero,
+                     hipStream_t st);
+void launch_pack_i4(const uint8_t* v, int64_t ld, int N, int K, uint8_t* q, hipStream_t st);
+void launch_dequant_i4(const Q4Args& a, int bf16, void* w, int64_t ldw, hipStream_t st);   // w [N][ldw], ldw a multiple of 8
+void launch_linear_i4(const Q4Args& a, int bf16, hipStream_t st);
+
+// choice of experts (k_route.hip)
+constexpr int MAX_ROUTE_K = 64;   // picks, groups
+struct RouteArgs
+{
+    const void* logits = nullptr;
+    int64_t ld = 0;
+    int dtype = 0;
+    const float* bias = nullptr;
+    int M = 0, E = 0, topk = 0, softmax = 0, groups = 1, top_groups = 1, group_best = 1, renorm = 1;
+    float scale = 1.f;
+    int64_t* sel = nullptr;   // [M][topk]
+    void* w = nullptr;
+    int wdtype = 0;
+    int lpg = 0;              // lanes of a group
+};
+int launch_route_experts(RouteArgs& a, hipStream_t st);
+void launch_route_backward(const RouteArgs& a, const void* dw, const int64_t* sel, void* dx, int64_t ldx, hipStream_t st);
+
+// logits before the draw (k_logits.hip)
+constexpr int MAX_HISTORY = (1 << 20) - 1, MAX_BIASES = 2047;
+struct LogitsArgs
+{
+    const void* logits = nullptr;
+    int64_t ld = 0;
+    void* out = nullptr;
+    int64_t ldo = 0;
+    int dtype = 0, B = 0, V = 0;
+    const int32_t* history = nullptr;   // [B][L]
+    int64_t ldh = 0;
+    int L = 0;
+    const int32_t* lengths = nullptr;   // [B] each, NULL = L, 0, off
+    const int32_t* prompt = nullptr;
+    const float* repetition = nullptr;
+    const float* frequency = nullptr;
+    const float* presence = nullptr;
+    const int32_t* bias_ids = nullptr;  // [B][n_bias]
+    int64_t ldb = 0;
+    const float* bias = nullptr;
+    int64_t ldv = 0;
+    int n_bias = 0;
+    const int32_t* allowed = nullptr;   // [B][(V + 31) / 32] bits
+    int64_t lda = 0;
+};
+void launch_logits(const LogitsArgs& a, hipStream_t st);
+
 // token selection (k_sample.hip)
 constexpr int MAX_VOCAB = 1 << 20;
 struct SampleArgs

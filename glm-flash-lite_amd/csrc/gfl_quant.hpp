@@ -41,4 +41,11 @@ struct QRow
     }
 };
 
+// scale at place `at` ([groups][N]) of a 4-bit weight
+__device__ __forceinline__ float q4_scale(const Q4Args& a, int64_t at)
+{
+    const uint16_t b = static_cast<const uint16_t*>(a.scale)[at];
+    return a.scale_bf ? q_val<true>(b) : q_val<false>(b);
+}
+
 }  // namespace gfl

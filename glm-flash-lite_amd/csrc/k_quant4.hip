@@ -1,0 +1,132 @@
+// Weights of 4 bits: rounding, packing and unpacking.
+//
+// A row of K values lies in blocks of 128, 64 bytes each: the 32-bit word j of the 16-byte piece g holds the inputs 32 j + 8 g + 0, 2, 4,
+// 6, 1, 3, 5, 7, four bits each from the lowest on. A lane that loads a piece so has, in word j, the 8 values of lane group g of the
+// j-th MFMA of 32 inputs, and a shift and a mask put two neighbours into the halves of a register.
+#include "gfl_quant.hpp"
+
+namespace gfl {
+
+constexpr int Q4_T = 256;
+
+// The word of 8 values from the 4 lanes that hold two each (lane t: values 2 t and 2 t + 1): every lane gets it.
+__device__ __forceinline__ uint32_t q4_word(uint32_t even, uint32_t odd, int lane)
+{
+    const int t = lane & 3;
+    uint32_t w = even << (4 * t) | odd << (16 + 4 * t);
+    w |= (uint32_t)__shfl_xor((int)w, 1);
+    w |= (uint32_t)__shfl_xor((int)w, 2);
+    return w;
+}
+// byte offset in a block of the word with inputs 8 * (lane / 4) ..: j = lane / 16, g = lane / 4 % 4
+__device__ __forceinline__ int q4_at(int lane) { return lane / 4 % 4 * 16 + lane / 16 * 4; }
+
+// A wave per block of 128 inputs of a row, two inputs a lane. Symmetric: scale = max |w| / 7, value = w / scale rounded + 8. With
+// zero points: scale = (max - min) / 15 with 0 in the range, zero = -min / scale rounded, value = w / scale rounded + zero. The
+// scale is rounded to w's type first. A group that is all zeros, or whose scale rounds to zero, has scale 0; one that holds an infinity
+// or a NaN a scale of NaN: both have values of 8.
+template <typename E>
+__global__ __launch_bounds__(Q4_T) void quant_i4_kernel(const E* w, int64_t ld, int N, int K, int group, int blocks, uint8_t* q,
+                                                        E* scale, uint8_t* zero)
+{
+    const int lane = threadIdx.x % 64;
+    const int64_t at = (int64_t)blockIdx.x * (Q4_T / 64) + threadIdx.x / 64;
+    if (at >= (int64_t)N * blocks) return;
+    const int64_t n = at / blocks;
+    const int block = (int)(at % blocks), k = block * 128 + lane * 2;
+    const E* row = w + n * ld;
+    float v[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) v[i] = k + i < K ? static_cast<float>(row[k + i]) : 0.0f;
+    uint32_t bad = !(fabsf(v[0]) < INFINITY) || !(fabsf(v[1]) < INFINITY);
+    float lo = fminf(fminf(v[0], v[1]), 0.0f), hi = fmaxf(fmaxf(v[0], v[1]), 0.0f);
+    for (int o = 1; o < group / 2; o *= 2)
+    {
+        lo = fminf(lo, __shfl_xor(lo, o));
+        hi = fmaxf(hi, __shfl_xor(hi, o));
+        bad |= (uint32_t)__shfl_xor((int)bad, o);
+    }
+    const float wide = zero ? (hi - lo) / 15.0f : fmaxf(-lo, hi) / 7.0f;
+    const E se = bad ? static_cast<E>(NAN) : static_cast<E>(wide);
+    const float s = static_cast<float>(se);
+    const bool some = s > 0.0f && !bad;
+    const float z = zero && some ? fminf(rintf(-lo / s), 15.0f) : 8.0f;
+    uint32_t u[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) u[i] = k + i >= K ? 0 : some ? (uint32_t)fminf(fmaxf(rintf(v[i] / s) + z, 0.0f), 15.0f) : 8;
+    const uint32_t word = q4_word(u[0], u[1], lane);
+    if (lane % 4 == 0) *reinterpret_cast<uint32_t*>(q + n * blocks * 64 + block * 64 + q4_at(lane)) = word;
+    if (lane % (group / 2) == 0 && k < K)
+    {
+        const int64_t g = (int64_t)(k / group) * N + n;
+        scale[g] = se;
+        if (zero) zero[g] = (uint8_t)z;
+    }
+}
+
+__global__ __launch_bounds__(Q4_T) void pack_i4_kernel(const uint8_t* v, int64_t ld, int N, int K, int blocks, uint8_t* q)
+{
+    const int lane = threadIdx.x % 64;
+    const int64_t at = (int64_t)blockIdx.x * (Q4_T / 64) + threadIdx.x / 64;
+    if (at >= (int64_t)N * blocks) return;
+    const int64_t n = at / blocks;
+    const int block = (int)(at % blocks), k = block * 128 + lane * 2;
+    const uint8_t* row = v + n * ld;
+    const uint32_t word = q4_word(k < K ? row[k] & 15 : 0, k + 1 < K ? row[k + 1] & 15 : 0, lane);
+    if (lane % 4 == 0) *reinterpret_cast<uint32_t*>(q + n * blocks * 64 + block * 64 + q4_at(lane)) = word;
+}
+
+// (value - zero) * scale, rounded to E once, as rows of ldw elements (K up to a multiple of 8): what the
+// large products read as their weights. A thread per word.
+template <typename E>
+__global__ __launch_bounds__(Q4_T) void dequant_i4_kernel(Q4Args a, E* w, int64_t ldw)
+{
+    const int words = a.blocks * 16;
+    const int64_t at = (int64_t)blockIdx.x * Q4_T + threadIdx.x;
+    if (at >= (int64_t)a.N * words) return;
+    const int64_t n = at / words;
+    const int in = (int)(at % words), k = in / 16 * 128 + in % 4 * 32 + in / 4 % 4 * 8;
+    if (k >= a.K) return;
+    const uint32_t u = reinterpret_cast<const uint32_t*>(a.q)[at];
+    const int64_t g = (int64_t)(k / a.group) * a.N + n;
+    const float s = q4_scale(a, g), z = a.zero ? (float)a.zero[g] : 8.0f;
+    typedef E e8 __attribute__((ext_vector_type(8)));
+    e8 o;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+    {
+        const int v = u >> (i / 2 * 4 + i % 2 * 16) & 15;
+        o[i] = static_cast<E>(((float)v - z) * s);
+    }
+    *reinterpret_cast<e8*>(w + n * ldw + k) = o;
+}
+
+static unsigned q4_grid(int64_t n, int per) { return (unsigned)((n + per - 1) / per); }
+
+void launch_quant_i4(const void* w, int64_t ld, int bf16, int N, int K, int group, uint8_t* q, void* scale, uint8_t* zero,
+                     hipStream_t st)
+{
+    const int blocks = (K + 127) / 128;
+    const dim3 grid(q4_grid((int64_t)N * blocks, Q4_T / 64)), block(Q4_T);
+    if (bf16)
+        hipLaunchKernelGGL(quant_i4_kernel<__bf16>, grid, block, 0, st, static_cast<const __bf16*>(w), ld, N, K, group, blocks, q,
+                           static_cast<__bf16*>(scale), zero);
+    else
+        hipLaunchKernelGGL(quant_i4_kernel<_Float16>, grid, block, 0, st, static_cast<const _Float16*>(w), ld, N, K, group, blocks, q,
+                           static_cast<_Float16*>(scale), zero);
+}
+
+void launch_pack_i4(const uint8_t* v, int64_t ld, int N, int K, uint8_t* q, hipStream_t st)
+{
+    const int blocks = (K + 127) / 128;
+    hipLaunchKernelGGL(pack_i4_kernel, dim3(q4_grid((int64_t)N * blocks, Q4_T / 64)), dim3(Q4_T), 0, st, v, ld, N, K, blocks, q);
+}
+
+void launch_dequant_i4(const Q4Args& a, int bf16, void* w, int64_t ldw, hipStream_t st)
+{
+    const dim3 grid(q4_grid((int64_t)a.N * a.blocks * 16, Q4_T));
+    if (bf16) hipLaunchKernelGGL(dequant_i4_kernel<__bf16>, grid, dim3(Q4_T), 0, st, a, static_cast<__bf16*>(w), ldw);
+    else hipLaunchKernelGGL(dequant_i4_kernel<_Float16>, grid, dim3(Q4_T), 0, st, a, static_cast<_Float16*>(w), ldw);
+}
+
+}  // namespace gfl

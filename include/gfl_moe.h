@@ -308,6 +308,83 @@ int gfl_linear_i8(const void* x, int64_t ldx, int dtype, const int8_t* b, int64_
 /* Bytes of workspace: *gemm for gfl_gemm_i8, *linear for gfl_linear_i8 (either may be NULL). */
 int gfl_i8_workspace(int M, int N, int K, size_t* gemm, size_t* linear);
 
+/* Weights of 4 bits: w[n][k] = (v[n][k] - zero) * scale with whole v in 0..15, one scale and zero point for each channel n and
+ * group of `group` (32, 64 or 128) inputs k. v is packed: row n takes ceil(K / 128) blocks of 64 bytes, one for each 128 inputs, rows one
+ * after another; the 32-bit little-endian word j of a block's 16-byte piece g holds the inputs 32 j + 8 g + 0, 2, 4, 6, 1, 3, 5,
+ * 7 of the block, four bits each from the lowest on (what lies past K is not used). scale is [ceil(K / group)][N], fp16 or bf16;
+ * zero uint8 of the same shape, 0..15 (any value is taken), NULL: 8 throughout. N * K up to 2^32 values (K up to a
+ * multiple of 128), N and K below GFL_MAX_LD. */
+
+/* Rounds a weight w [N, K] (fp16 or bf16) to 4 bits: q, scale (of w's type) and, where zero is not NULL, zero points.
+ * Without: scale = max |w| / 7 of the group, v = w / scale rounded + 8. With: the range from min(w, 0) to max(w, 0) in 15 steps,
+ * zero = -min / scale rounded, v = w / scale rounded + zero. The scale is rounded to its type before it divides; the quotients
+ * are fp32 and rounded to nearest even. A group of zeros has scale 0, one that holds an infinity or a NaN a scale of NaN; v and zero
+ * are 8 in both. */
+int gfl_quant_i4(const void* w, int64_t ldw, int dtype, int N, int K, int group, uint8_t* q, void* scale, uint8_t* zero,
+                 gfl_stream stream);
+
+/* Packs values that something else rounded: v uint8 [N, K], of which the lower four bits count. */
+int gfl_pack_i4(const uint8_t* v, int64_t ldv, int N, int K, uint8_t* q, gfl_stream stream);
+
+/* out[m][n] = sum_k x[m][k] * w[n][k] for x [M, K] fp16 or bf16 (dtype); out fp16, bf16 or fp32. Sums are fp32. Up to 64 tokens, and
+ * where out is not of x's type, the weights enter exactly, as whole numbers; above they are rounded to x's type for the MFMAs.
+ * An infinity in a token's x makes its outputs NaN in the exact form. q 16-byte aligned. */
+int gfl_linear_i4(const void* x, int64_t ldx, int dtype, const uint8_t* q, const void* scale, int scale_dtype, const uint8_t* zero,
+                  int M, int N, int K, int group, void* out, int64_t ldo, int out_dtype, void* ws, size_t ws_bytes,
+                  gfl_stream stream);
+
+/* Its gradient with respect to x (the weight is frozen): dx[m][k] = sum_n dy[m][n] * w[n][k], both of dtype, the weights rounded to
+ * it. */
+int gfl_linear_i4_dx(const void* dy, int64_t lddy, int dtype, const uint8_t* q, const void* scale, int scale_dtype,
+                     const uint8_t* zero, int M, int N, int K, int group, void* dx, int64_t lddx, void* ws, size_t ws_bytes,
+                     gfl_stream stream);
+
+/* Bytes of workspace: *forward for gfl_linear_i4, *backward for gfl_linear_i4_dx (either may be NULL). */
+int gfl_i4_workspace(int dtype, int out_dtype, int M, int N, int K, size_t* forward, size_t* backward);
+
+/* The choice of experts in its general form, for routers that gfl_route does not cover: logits [M, E] (fp32, fp16 or bf16).
+ *   score s   GFL_SIGMOID: 1 / (1 + exp(-x)); GFL_SOFTMAX: exp(x) / sum of exp over the row
+ *   key       s + bias[e] (fp32 [E], NULL: none), which decides the choice but not the weight
+ *   groups    the E experts in `groups` equal parts, in order; a part is worth the sum of its group_best (1 or 2) largest keys,
+ *             and only the top_groups worthiest are chosen from (1 group: all)
+ *   sel       the topk largest keys, in descending order
+ *   w         scale * s, with renorm divided by the sum of the picks' s (0 where that is 0); fp16, bf16 or fp32
+ * Scores, keys and sums are fp64; equal keys go to the lower index (without a bias, among all experts, the logits are
+ * compared). Experts whose logit is -inf or NaN, or whose bias is, are never picked: where fewer than topk are left, the rest
+ * of sel is -1 with weight 0, which the expert calls skip. In a softmax with logits of +inf those share the row.
+ * E <= 1024, topk <= min(64, E / groups * top_groups), groups <= 64 dividing E. */
+enum
+{
+    GFL_SIGMOID = 0,
+    GFL_SOFTMAX = 1,
+};
+int gfl_route_experts(const void* logits, int64_t ld, int dtype, const float* bias, int M, int E, int topk, int score, int groups,
+                      int top_groups, int group_best, int renorm, float scale, int64_t* sel, void* w, int w_dtype,
+                      gfl_stream stream);
+
+/* Gradient of the logits (dlogits [M, E] of dtype) for a gradient dw [M, topk] of the weights (of w_dtype), sel as the forward call
+ * wrote it (ids outside [0, E) are skipped). The choice itself and the bias have none. */
+int gfl_route_experts_backward(const void* dw, int w_dtype, const void* logits, int64_t ld, int dtype, const int64_t* sel, int M,
+                               int E, int topk, int score, int renorm, float scale, void* dlogits, int64_t ldd,
+                               gfl_stream stream);
+
+/* Logits [B, V] (fp32, fp16 or bf16) as each request's settings change them before gfl_sample draws; out of the same type, which may
+ * be logits itself. Per row, each array [B] (NULL: off for every row):
+ *   history     int32 [B, L], of which the first lengths[b] (NULL: L) count, the first prompt[b] (NULL: 0) of those being the prompt
+ *   repetition  a logit of a token that occurs in the history, above 0 divided by it, else multiplied; not above 0: off
+ *   frequency   subtracted once for each time the token occurs after the prompt
+ *   presence    subtracted once where it occurs after the prompt
+ *   bias        fp32 [B, n_bias], added to the logits of the tokens bias_ids int32 [B, n_bias]; of entries with one id the last counts
+ *   allowed     bits [B, ceil(V / 32)], bit v % 32 of word v / 32: a token whose bit is 0 gets -inf, whatever its logit
+ * in this order, in fp32, rounded once to the type. Ids outside [0, V) are skipped. V <= 2^20, L <= GFL_MAX_HISTORY, n_bias <=
+ * GFL_MAX_BIASES. */
+#define GFL_MAX_HISTORY 1048575
+#define GFL_MAX_BIASES 2047
+int gfl_adjust_logits(const void* logits, int64_t ld, int dtype, int B, int V, const int32_t* history, int64_t ldh, int L,
+                      const int32_t* lengths, const int32_t* prompt, const float* repetition, const float* frequency,
+                      const float* presence, const int32_t* bias_ids, int64_t ldb, const float* bias, int64_t ldv, int n_bias,
+                      const int32_t* allowed, int64_t lda, void* out, int64_t ldo, gfl_stream stream);
+
 /* Draws a token for each row of logits [B, V] (fp32, fp16 or bf16) from given uniform numbers u [B] in [0, 1).
  * Per row, each array fp32 [B] (top_k int32), NULL = off for every row:
  *   temperature  weight of token i = exp((logit_i - max) / T); not above 0: the row is greedy (its largest logit)
