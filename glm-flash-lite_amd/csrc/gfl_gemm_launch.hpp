@@ -2,20 +2,9 @@
 #pragma once
 #include "gfl_gemm.hpp"
 #include "gfl_gemm_plan.hpp"
-
-#include <atomic>
+#include "gfl_open.hpp"
 
 namespace gfl {
-
-// Allows a kernel its LDS, once on each device (the attribute belongs to the device's copy of the kernel; `opened`: a bit for each).
-static inline void gm_open(const void* kern, int lds, std::atomic<uint64_t>& opened)
-{
-    int dev = 0;
-    if (hipGetDevice(&dev) != hipSuccess) return;   // the launch reports it
-    const uint64_t bit = dev < 64 ? 1ull << dev : 0;
-    if (bit && (opened.load(std::memory_order_relaxed) & bit)) return;
-    if (hipFuncSetAttribute(kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds) == hipSuccess) opened.fetch_or(bit);
-}
 
 template <typename T, int TM, int TN, int WM, int WN, bool AKS, bool BKS, bool DUAL, int NST, bool AL, int EP>
 static int gm_go(const GmArgs& a, int nz, hipStream_t st)

@@ -1,86 +1,302 @@
 // Logits as a request's settings change them before a token is drawn: penalties for tokens that were there before, biases, a mask.
 //
-// A workgroup takes a slice of a row. What the row's history and biases say of each of the slice's tokens is gathered in a word of
-// LDS a token by integer atomics (sums and maxima: the same in any order), then the slice is read, changed and written once.
+// A workgroup takes a slice of a row. What the row's history says of each of the slice's tokens is gathered in LDS by integer
+// atomics (the same in any order), then the slice is read, changed and written once.
 #include "gfl_internal.hpp"
+#include "gfl_open.hpp"
 
 #include <algorithm>
 
 namespace gfl {
 
-constexpr int LG_T = 512;
-constexpr uint32_t LG_SEEN = 1u << 20, LG_COUNT = LG_SEEN - 1;   // a token's word: bias entry + 1 | seen | count
-constexpr int LG_BIAS = 21;
+constexpr int LG_T = 512, LG_UNIT = 4 * LG_T;   // a slice is whole units: 4 neighbouring tokens a thread
+constexpr int LG_BIAS = (MAX_BIASES + LG_T - 1) / LG_T;   // biases a thread takes
 
+// v0 .. v0 + n - 1 of a row's elements as fp32, n <= 4; rows start anywhere
 template <typename E>
-__global__ __launch_bounds__(LG_T) void logits_kernel(LogitsArgs a, int slice)
+__device__ __forceinline__ void lg_load(const E* p, int n, float (&v)[4])
 {
-    extern __shared__ uint32_t word[];
-    const int64_t b = blockIdx.y;
-    const int v0 = blockIdx.x * slice, nv = min(slice, a.V - v0);
+    E e[4] = {};
+    if (n >= 4) __builtin_memcpy(e, p, sizeof e);
+    else
+#pragma unroll
+        for (int i = 0; i < 3; ++i)
+            if (i < n) e[i] = p[i];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = static_cast<float>(e[i]);
+}
+template <typename E>
+__device__ __forceinline__ void lg_store(E* p, int n, const float (&v)[4])
+{
+    E e[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) e[i] = static_cast<E>(v[i]);
+    if (n >= 4) __builtin_memcpy(p, e, sizeof e);
+    else
+#pragma unroll
+        for (int i = 0; i < 3; ++i)
+            if (i < n) p[i] = e[i];
+}
+
+// What the history says of a token: whether it is in the prompt, and how often it comes after. Histories of up to 32,767 tokens take
+// 16 bits a token, so that a slice of 32,768 fits twice into a CU's LDS: every slice reads the whole history.
+template <bool HALF>
+struct LgWord
+{
+    static constexpr uint32_t SEEN = HALF ? 0x8000u : 0x80000000u;
+    static constexpr int PER = HALF ? 2 : 1;   // tokens of a 32-bit word
+    static __device__ __forceinline__ void seen(uint32_t* w, uint32_t v)
+    {
+        if constexpr (HALF) atomicOr(&w[v / 2], SEEN << (v % 2 * 16));
+        else atomicOr(&w[v], SEEN);
+    }
+    static __device__ __forceinline__ void count(uint32_t* w, uint32_t v)
+    {
+        if constexpr (HALF) atomicAdd(&w[v / 2], 1u << (v % 2 * 16));
+        else atomicAdd(&w[v], 1u);
+    }
+    static __device__ __forceinline__ bool four(const uint32_t* w, int i, uint32_t (&out)[4])   // of 4 tokens from i on; any?
+    {
+        if constexpr (HALF)
+        {
+            const uint2 p = *reinterpret_cast<const uint2*>(w + i / 2);
+            out[0] = p.x & 0xFFFF, out[1] = p.x >> 16, out[2] = p.y & 0xFFFF, out[3] = p.y >> 16;
+            return (p.x | p.y) != 0;
+        }
+        else
+        {
+            const uint4 p = *reinterpret_cast<const uint4*>(w + i);
+            out[0] = p.x, out[1] = p.y, out[2] = p.z, out[3] = p.w;
+            return (p.x | p.y | p.z | p.w) != 0;
+        }
+    }
+};
+
+template <typename E, bool HALF>
+__global__ __launch_bounds__(LG_T, 4) void logits_kernel(LogitsArgs a)
+{
+    typedef LgWord<HALF> W;
+    extern __shared__ __align__(16) uint32_t word[];   // the slice's words; with biases, see below
+    const int tid = threadIdx.x, slice = a.slice;
+    uint32_t* marked = word + (a.L ? slice / W::PER : 0);
+    uint32_t* before = marked + slice / 32;
+    uint32_t* total = before + slice / 32;
+    uint32_t* last = total + LG_T / 64;
+    float* bval = reinterpret_cast<float*>(last + a.n_bias);
+
+    int64_t b = blockIdx.x / a.slices, s = blockIdx.x % a.slices;
+    if (a.by_xcd)
+    {
+        const int64_t k = blockIdx.x / 8;
+        b = k / a.slices * 8 + blockIdx.x % 8, s = k % a.slices;
+        if (b >= a.B) return;
+    }
+    s = (s + b) % a.slices;
+    const int v0 = (int)s * slice, nv = min(slice, a.V - v0);
     const E* x = static_cast<const E*>(a.logits) + b * a.ld + v0;
     E* out = static_cast<E*>(a.out) + b * a.ldo + v0;
+    const int32_t* allowed = a.allowed ? a.allowed + b * a.lda : nullptr;
+    const bool lazy = a.out == a.logits && !allowed;   // only what the lists name is read and written
+
+    constexpr int U = 4, NB = 2;   // loads of 4 ids, of 4 logits under way
+    const int32_t* h = a.L ? a.history + b * a.ldh : nullptr;
+    int32_t id[U][4];
+    auto ids_at = [&](int at) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) __builtin_memcpy(id[u], h + min(at + u * LG_UNIT, a.L - 4), 16);
+    };
+    const bool early = a.early && a.L >= 4;
+    if (early) ids_at(tid * 4);   // as many as the row has room for; which of them count is seen later
+    float y[NB][4];
+    uint32_t bits[NB];
+    auto read = [&](int at) {
+#pragma unroll
+        for (int j = 0; j < NB; ++j)
+        {
+            const int i = at + j * LG_UNIT;
+            bits[j] = ~0u;
+            if (i >= nv) continue;
+            lg_load(x + i, nv - i, y[j]);
+            if (allowed) bits[j] = (uint32_t)allowed[(v0 + i) / 32] >> ((v0 + i) % 32);   // (4 tokens from a multiple of 4 on: one word)
+        }
+    };
+    if (!lazy) read(tid * 4);
 
     float rep = a.repetition ? a.repetition[b] : 1.0f;
     if (!(rep > 0.0f)) rep = 1.0f;   // off
     const float freq = a.frequency ? a.frequency[b] : 0.0f, pres = a.presence ? a.presence[b] : 0.0f;
-    const bool penal = a.L > 0 && (rep != 1.0f || freq != 0.0f || pres != 0.0f);
-    const bool words = penal || a.n_bias > 0;
-    if (words)
+    const int len = a.lengths ? min(max(a.lengths[b], 0), a.L) : a.L, prompt = a.prompt ? min(max(a.prompt[b], 0), len) : 0;
+    const bool penal = len > 0 && (rep != 1.0f || freq != 0.0f || pres != 0.0f);
+    auto place = [&](int32_t t) { return (uint32_t)t - (uint32_t)v0; };   // (an id below v0 wraps to a large number)
+    if (penal)
+        for (int i = tid * 4; i < slice / W::PER; i += LG_UNIT) *reinterpret_cast<uint4*>(&word[i]) = uint4{ 0, 0, 0, 0 };
+    // Biases: a bit for each of the slice's tokens that has one (marked), how many have one before each 32 tokens (before), and by
+    // a token's number among them the last entry that names it: what a token's bias costs does not depend on how many there are.
+    int32_t mine[LG_BIAS] = {};
+    if (a.n_bias)
     {
-        for (int i = threadIdx.x; i < nv; i += LG_T) word[i] = 0;
-        __syncthreads();
-        const int32_t* ids = a.n_bias ? a.bias_ids + b * a.ldb : nullptr;
-        for (int i = threadIdx.x; i < a.n_bias; i += LG_T)
+        for (int i = tid; i < slice / 32; i += LG_T) marked[i] = 0;
+#pragma unroll
+        for (int k = 0; k < LG_BIAS; ++k)
         {
-            const uint32_t v = (uint32_t)(ids[i] - v0);
-            if (ids[i] >= v0 && v < (uint32_t)nv) atomicMax(&word[v], (uint32_t)(i + 1) << LG_BIAS);   // the last entry counts
+            const int i = tid + k * LG_T;
+            if (i >= a.n_bias) continue;
+            mine[k] = a.bias_ids[b * a.ldb + i];
+            bval[i] = a.bias[b * a.ldv + i];
+            last[i] = 0;
         }
+    }
+    if (penal || a.n_bias) __syncthreads();
+    if (a.n_bias)
+    {
+#pragma unroll
+        for (int k = 0; k < LG_BIAS; ++k)
+            if (tid + k * LG_T < a.n_bias && place(mine[k]) < (uint32_t)nv)
+                atomicOr(&marked[place(mine[k]) / 32], 1u << (place(mine[k]) % 32));
         __syncthreads();
-        if (penal)
+        // two words a thread (a slice has at most 1024)
+        const int w = tid * 2, n = slice / 32;
+        const uint32_t c0 = w < n ? __popc(marked[w]) : 0, c1 = w + 1 < n ? __popc(marked[w + 1]) : 0;
+        uint32_t sum = c0 + c1;
+#pragma unroll
+        for (int o = 1; o < 64; o *= 2)
         {
-            const int32_t* h = a.history + b * a.ldh;
-            const int len = a.lengths ? min(max(a.lengths[b], 0), a.L) : a.L;
-            const int prompt = a.prompt ? min(max(a.prompt[b], 0), len) : 0;
-            for (int i = threadIdx.x; i < len; i += LG_T)
-            {
-                const int id = h[i];
-                const uint32_t v = (uint32_t)(id - v0);
-                if (id < v0 || v >= (uint32_t)nv) continue;
-                if (i < prompt) atomicOr(&word[v], LG_SEEN);
-                else atomicAdd(&word[v], 1u);
-            }
+            const uint32_t up = __shfl_up(sum, o);
+            if (tid % 64 >= o) sum += up;
         }
+        if (tid % 64 == 63) total[tid / 64] = sum;
+        __syncthreads();
+        for (int k = 0; k < tid / 64; ++k) sum += total[k];
+        if (w < n) before[w] = sum - c0 - c1;
+        if (w + 1 < n) before[w + 1] = sum - c1;
         __syncthreads();
     }
-    const float* by = a.n_bias ? a.bias + b * a.ldv : nullptr;
-    const int32_t* allowed = a.allowed ? a.allowed + b * a.lda : nullptr;
-    for (int i = threadIdx.x; i < nv; i += LG_T)
+    auto number = [&](uint32_t v) { return before[v / 32] + __popc(marked[v / 32] & ((1u << (v % 32)) - 1)); };
+#pragma unroll
+    for (int k = 0; k < LG_BIAS; ++k)
+        if (tid + k * LG_T < a.n_bias && place(mine[k]) < (uint32_t)nv)
+            atomicMax(&last[number(place(mine[k]))], (uint32_t)(tid + k * LG_T + 1));
+    if (penal)
     {
-        float y = static_cast<float>(x[i]);
-        const uint32_t w = words ? word[i] : 0;
-        if (w)
+        auto edge = [&](int i) {
+            const uint32_t v = place(h[i]);
+            if (v >= (uint32_t)nv) return;
+            if (i < prompt) W::seen(word, v);
+            else W::count(word, v);
+        };
+        // four ids that all count, on one side of the prompt's end: an id costs a subtraction, a comparison and, where it is in the
+        // slice, an atomic
+        for (int at = tid * 4; at < len; at += U * LG_UNIT)
         {
-            if (w & (LG_SEEN | LG_COUNT)) y = y > 0.0f ? y / rep : y * rep;
-            if (w & LG_COUNT)
+            if (a.L >= 4 && !(early && at == tid * 4)) ids_at(at);
+#pragma unroll
+            for (int u = 0; u < U; ++u)
             {
-                y -= freq * (float)(w & LG_COUNT);
-                y -= pres;
+                const int from = at + u * LG_UNIT;
+                if (from + 4 <= prompt)
+                {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (place(id[u][i]) < (uint32_t)nv) W::seen(word, place(id[u][i]));
+                }
+                else if (from >= prompt && from + 4 <= len)
+                {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (place(id[u][i]) < (uint32_t)nv) W::count(word, place(id[u][i]));
+                }
+                else
+                    for (int i = from; i < min(from + 4, len); ++i) edge(i);
             }
-            if (w >> LG_BIAS) y += by[(w >> LG_BIAS) - 1];
         }
-        const int v = v0 + i;
-        if (allowed && !(allowed[v / 32] >> (v % 32) & 1)) y = -INFINITY;
-        out[i] = static_cast<E>(y);
     }
+    if (penal || a.n_bias) __syncthreads();
+
+    auto change = [&](int i, float (&v)[4], uint32_t ok) {   // tokens i .. i + 3 of the slice; true: something changed
+        uint32_t w[4] = {};
+        const bool any = penal && W::four(word, i, w);
+        if (any)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+            {
+                if (w[k]) v[k] = v[k] > 0.0f ? v[k] / rep : v[k] * rep;
+                const uint32_t n = w[k] & (W::SEEN - 1);
+                if (n)
+                {
+                    v[k] -= freq * (float)n;
+                    v[k] -= pres;
+                }
+            }
+        const uint32_t mark = a.n_bias ? marked[i / 32] >> (i % 32) & 15 : 0;
+        if (mark)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (mark >> k & 1) v[k] += bval[last[number(i + k)] - 1];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = ok >> k & 1 ? v[k] : -INFINITY;
+    };
+    if (lazy)
+    {
+        for (int i = tid * 4; i < nv; i += LG_UNIT)
+        {
+            uint32_t w[4];
+            if (!(penal && W::four(word, i, w)) && !(a.n_bias && (marked[i / 32] >> (i % 32) & 15))) continue;
+            lg_load(x + i, nv - i, y[0]);
+            change(i, y[0], ~0u);
+            lg_store(out + i, nv - i, y[0]);
+        }
+        return;
+    }
+    for (int at = tid * 4; at < nv; at += NB * LG_UNIT)
+    {
+        float v[NB][4];
+        uint32_t ok[NB];
+#pragma unroll
+        for (int j = 0; j < NB; ++j)
+        {
+            ok[j] = bits[j];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[j][k] = y[j][k];
+        }
+        read(at + NB * LG_UNIT);   // the next ones, before this step's stores
+#pragma unroll
+        for (int j = 0; j < NB; ++j)
+        {
+            const int i = at + j * LG_UNIT;
+            if (i >= nv) continue;
+            change(i, v[j], ok[j]);
+            lg_store(out + i, nv - i, v[j]);
+        }
+    }
+}
+
+template <typename E, bool HALF>
+static void logits_go(LogitsArgs a, hipStream_t st)
+{
+    constexpr int most = 65536;   // bytes of words: twice in a CU
+    auto* kern = &logits_kernel<E, HALF>;
+    static std::atomic<uint64_t> opened{ 0 };
+    gm_open(reinterpret_cast<const void*>(kern), LDS_LIMIT, opened);
+    const int64_t units = (int64_t)a.B * ((a.V + LG_UNIT - 1) / LG_UNIT);
+    const int largest = a.L ? most / 4 * LgWord<HALF>::PER : 4 * LG_UNIT;
+    a.slice = (int)std::min<int64_t>(std::max<int64_t>((units + 1023) / 1024, 1) * LG_UNIT, largest);
+    a.slices = (a.V + a.slice - 1) / a.slice;
+    a.by_xcd = a.B >= 64;
+    a.early = a.B < 64;
+    const unsigned grid = (unsigned)(a.by_xcd ? (a.B + 7) / 8 * 8 : a.B) * a.slices;
+    const size_t lds = (a.L ? a.slice / LgWord<HALF>::PER : 0) * 4 + (a.n_bias ? a.slice / 4 + LG_T / 16 + a.n_bias * 8 : 0);
+    hipLaunchKernelGGL(kern, dim3(grid), dim3(LG_T), lds, st, a);
+}
+
+template <typename E>
+static void logits_of(const LogitsArgs& a, hipStream_t st)
+{
+    (a.L <= 32767 ? &logits_go<E, true> : &logits_go<E, false>)(a, st);
 }
 
 void launch_logits(const LogitsArgs& a, hipStream_t st)
 {
-    const int slice = 8192;
-    const dim3 grid((a.V + slice - 1) / slice, a.B);
-    auto* kern = a.dtype == 2 ? &logits_kernel<float> : a.dtype == 1 ? &logits_kernel<__bf16> : &logits_kernel<_Float16>;
-    hipLaunchKernelGGL(kern, grid, dim3(LG_T), slice * sizeof(uint32_t), st, a, slice);
+    (a.dtype == 2 ? &logits_of<float> : a.dtype == 1 ? &logits_of<__bf16> : &logits_of<_Float16>)(a, st);
 }
 
 }  // namespace gfl
