@@ -402,7 +402,7 @@ int gfl_i4_workspace(int dtype, int out_dtype, int M, int N, int K, size_t* forw
     if (dtype != GFL_F16 && dtype != GFL_BF16) return api_fail(GFL_EINVAL, "gfl_i4: dtype must be GFL_F16 or GFL_BF16");
     if (int rc = i4_check(M, N, K, 32)) return rc;
     const size_t w = up256((size_t)N * i4_ldw(K) * 2);
-    if (forward) *forward = i4_exact(M, dtype, out_dtype) ? 0 : w + i4_part(gfl::GM_NT, M, N, K);
+    if (forward) *forward = i4_exact(M, dtype, out_dtype) ? up256(gfl::q4_plan(M, N, K).part_bytes) : w + i4_part(gfl::GM_NT, M, N, K);
     if (backward) *backward = M ? w + i4_part(gfl::GM_NN, M, K, N) : 0;
     return GFL_OK;
 }
@@ -467,7 +467,7 @@ int gfl_linear_i4(const void* x, int64_t ldx, int dtype, const uint8_t* q, const
         a.ldx = ldx * 2;
         a.M = M;
         a.out = out; a.ldo = ldo; a.odt = out_dtype;
-        gfl::launch_linear_i4(a, dtype == GFL_BF16, st);
+        gfl::launch_linear_i4(a, dtype == GFL_BF16, ws, st);
         return check_launch("gfl_linear_i4");
     }
     const int64_t ldw = i4_ldw(K);

@@ -94,4 +94,32 @@ inline GmPlan gm_plan(int form, int ep, int dual, int aligned, int M, int N, int
     return p;
 }
 
+// A product with a 4-bit weight whose weights are unpacked in its own launch: the kernel for few tokens, or tiles of 16 tt tokens and
+// 128 nt channels over `parts` of the inputs.
+struct Q4Plan
+{
+    int few, tt, nt, parts;
+    int64_t ldp;
+    size_t part_bytes;
+};
+
+constexpr int Q4_TOKENS = 144 << 10;   // bytes of LDS for the tokens of the kernel for few
+
+inline Q4Plan q4_plan(int M, int N, int K)
+{
+    Q4Plan p = {};
+    const int blocks = (K + 127) / 128;
+    p.few = M <= 16 && (int64_t)M * (blocks * 256 + 16) <= Q4_TOKENS;
+    p.parts = 1;
+    if (p.few) return p;
+    p.tt = M <= 16 ? 1 : M <= 32 ? 2 : 4;
+    const int64_t tall = (M + 16 * p.tt - 1) / (16 * p.tt);
+    p.nt = tall * ((N + 255) / 256) * (blocks / 4) < 256 ? 1 : 2;
+    const int64_t wg = tall * ((N + 128 * p.nt - 1) / (128 * p.nt));
+    p.parts = (int)std::max<int64_t>(1, std::min<int64_t>(std::min(blocks / 4, 16), 256 / wg));
+    p.ldp = ((int64_t)N + 3) / 4 * 4;
+    p.part_bytes = p.parts > 1 ? (size_t)p.parts * M * p.ldp * 4 : 0;
+    return p;
+}
+
 }  // namespace gfl

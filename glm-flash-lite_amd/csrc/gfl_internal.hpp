@@ -247,12 +247,16 @@ struct Q4Args
     void* out = nullptr;
     int64_t ldo = 0;                 // elements
     int odt = 0;
+    uint32_t magic = 0;              // 2^32 / (16-byte pieces of a token) rounded up
+    int parts = 1;                   // of the inputs, each with its sums in part [parts][M][ldp]
+    float* part = nullptr;
+    int64_t ldp = 0;
 };
 void launch_quant_i4(const void* w, int64_t ld, int bf16, int N, int K, int group, uint8_t* q, void* scale, uint8_t* zero,
                      hipStream_t st);
 void launch_pack_i4(const uint8_t* v, int64_t ld, int N, int K, uint8_t* q, hipStream_t st);
 void launch_dequant_i4(const Q4Args& a, int bf16, void* w, int64_t ldw, hipStream_t st);   // w [N][ldw], ldw a multiple of 8
-void launch_linear_i4(const Q4Args& a, int bf16, hipStream_t st);
+void launch_linear_i4(Q4Args& a, int bf16, void* ws, hipStream_t st);   // ws: q4_plan's part_bytes
 
 // choice of experts (k_route.hip)
 constexpr int MAX_ROUTE_K = 64;   // picks, groups
