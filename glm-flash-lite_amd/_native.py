@@ -99,7 +99,7 @@ def load(path=LIB_PATH):
                                 _P, SZ, _P]
     L.gfl_linear_i4_dx.argtypes = [_P, I64, C.c_int, _P, _P, C.c_int, _P, C.c_int, C.c_int, C.c_int, C.c_int, _P, I64, _P, SZ,
                                    _P]
-    L.gfl_i4_workspace.argtypes = [C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, PSZ, PSZ]
+    L.gfl_i4_workspace.argtypes = [C.c_int] * 6 + [PSZ, PSZ]
     L.gfl_route_experts.argtypes = [_P, I64, C.c_int, _P] + [C.c_int] * 8 + [C.c_float, _P, _P, C.c_int, _P]
     L.gfl_route_experts_backward.argtypes = [_P, C.c_int, _P, I64, C.c_int, _P] + [C.c_int] * 5 + [C.c_float, _P, I64, _P]
     L.gfl_adjust_logits.argtypes = [_P, I64, C.c_int, C.c_int, C.c_int, _P, I64, C.c_int, _P, _P, _P, _P, _P, _P, I64, _P, I64,

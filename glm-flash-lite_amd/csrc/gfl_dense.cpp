@@ -12,9 +12,6 @@ using gfl::api_fail;
 
 constexpr size_t up256(size_t x) { return (x + 255) & ~size_t(255); }
 
-// tokens up to which the weights of a 4-bit product are unpacked in the product's own launch (k_dense_i4.hip)
-constexpr int I4_FEW = 64;
-
 // rows of whole 4-byte words, which the direct tile loads need
 bool words(const void* p, int64_t ld_bytes)
 {
@@ -388,7 +385,11 @@ static int i4_check(int64_t M, int N, int K, int group)
     return GFL_OK;
 }
 
-static bool i4_exact(int M, int dtype, int out_dtype) { return M <= I4_FEW || out_dtype != dtype; }
+// (a result of more bits than the weights rounded to x's type have is formed from the exact ones)
+static bool i4_exact(int M, int N, int K, int group, int dtype, int out_dtype)
+{
+    return out_dtype != dtype || gfl::q4_exact(M, N, K, group);
+}
 static int64_t i4_ldw(int K) { return ((int64_t)K + 7) / 8 * 8; }
 
 static size_t i4_part(int form, int M, int N, int K)
@@ -397,12 +398,12 @@ static size_t i4_part(int form, int M, int N, int K)
                           gfl::gm_plan(form, gfl::EP_OUT, 0, 1, M, N, K, 1).part_bytes));
 }
 
-int gfl_i4_workspace(int dtype, int out_dtype, int M, int N, int K, size_t* forward, size_t* backward)
+int gfl_i4_workspace(int dtype, int out_dtype, int M, int N, int K, int group, size_t* forward, size_t* backward)
 {
     if (dtype != GFL_F16 && dtype != GFL_BF16) return api_fail(GFL_EINVAL, "gfl_i4: dtype must be GFL_F16 or GFL_BF16");
-    if (int rc = i4_check(M, N, K, 32)) return rc;
+    if (int rc = i4_check(M, N, K, group)) return rc;
     const size_t w = up256((size_t)N * i4_ldw(K) * 2);
-    if (forward) *forward = i4_exact(M, dtype, out_dtype) ? up256(gfl::q4_plan(M, N, K).part_bytes) : w + i4_part(gfl::GM_NT, M, N, K);
+    if (forward) *forward = i4_exact(M, N, K, group, dtype, out_dtype) ? up256(gfl::q4_plan(M, N, K).part_bytes) : w + i4_part(gfl::GM_NT, M, N, K);
     if (backward) *backward = M ? w + i4_part(gfl::GM_NN, M, K, N) : 0;
     return GFL_OK;
 }
@@ -457,11 +458,11 @@ int gfl_linear_i4(const void* x, int64_t ldx, int dtype, const uint8_t* q, const
     if (ldx < K || ldx >= GFL_MAX_LD || ldo < N || ldo >= (1 << 30))
         return api_fail(GFL_EINVAL, "gfl_linear_i4: row strides must be at least the width (x below GFL_MAX_LD, out below 2^30)");
     size_t need = 0;
-    gfl_i4_workspace(dtype, out_dtype, M, N, K, &need, nullptr);
+    gfl_i4_workspace(dtype, out_dtype, M, N, K, group, &need, nullptr);
     if (need && (!ws || ws_bytes < need || reinterpret_cast<uintptr_t>(ws) % 16))
         return api_fail(GFL_EINVAL, "gfl_linear_i4: workspace missing, too small or not 16-byte aligned");
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-    if (i4_exact(M, dtype, out_dtype))
+    if (i4_exact(M, N, K, group, dtype, out_dtype))
     {
         a.x = static_cast<const char*>(x);
         a.ldx = ldx * 2;
@@ -501,7 +502,7 @@ int gfl_linear_i4_dx(const void* dy, int64_t lddy, int dtype, const uint8_t* q, 
     if (lddy < N || lddy >= GFL_MAX_LD || lddx < K || lddx >= GFL_MAX_LD)
         return api_fail(GFL_EINVAL, "gfl_linear_i4_dx: row strides must be at least the width and below GFL_MAX_LD");
     size_t need = 0;
-    gfl_i4_workspace(dtype, dtype, M, N, K, nullptr, &need);
+    gfl_i4_workspace(dtype, dtype, M, N, K, group, nullptr, &need);
     if (!ws || ws_bytes < need || reinterpret_cast<uintptr_t>(ws) % 16)
         return api_fail(GFL_EINVAL, "gfl_linear_i4_dx: workspace missing, too small or not 16-byte aligned");
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);

@@ -109,7 +109,7 @@ inline Q4Plan q4_plan(int M, int N, int K)
 {
     Q4Plan p = {};
     const int blocks = (K + 127) / 128;
-    p.few = M <= 16 && (int64_t)M * (blocks * 256 + 16) <= Q4_TOKENS;
+    p.few = K < 8 || (M <= 16 && (int64_t)M * (blocks * 256 + 16) <= Q4_TOKENS);
     p.parts = 1;
     if (p.few) return p;
     p.tt = M <= 16 ? 1 : M <= 32 ? 2 : 4;
@@ -120,6 +120,20 @@ inline Q4Plan q4_plan(int M, int N, int K)
     p.ldp = ((int64_t)N + 3) / 4 * 4;
     p.part_bytes = p.parts > 1 ? (size_t)p.parts * M * p.ldp * 4 : 0;
     return p;
+}
+
+// Whether the weights are unpacked in the product's own launch, where they enter exactly, or to 16 bits first for the tile GEMM: by
+// estimated time. A round of 256 tiles of 64 x 256 takes 2.8 us a step of 256 inputs, 3.0 with groups of 64, 3.6 of 32, the launch and
+// the join 5 to 10; unpacking moves 2.5 bytes a weight at 4.2 TB/s. Measured, us, here and there: 5120 -> 12288 groups of 128 128
+// tokens 38 and 72, 256 58 and 84, 512 115 and 116, 1024 185 and 155, groups of 32 256 tokens 73 and 93, 512 147 and 125; 2048 -> 2048
+// 1024 tokens 25 and 32.
+inline bool q4_exact(int M, int N, int K, int group)
+{
+    if (M <= 64 || K < 8) return true;
+    const Q4Plan p = q4_plan(M, N, K);
+    const int64_t wg = (int64_t)((M + 63) / 64) * ((N + 128 * p.nt - 1) / (128 * p.nt)) * p.parts, steps = ((K + 127) / 128 / p.parts + 1) / 2;
+    const double own = 5 + (p.parts > 1 ? 5 : 0) + (double)((wg + 255) / 256) * steps * (group == 128 ? 2.8 : group == 64 ? 3.0 : 3.6);
+    return own <= 3 + 2.5 * N * K / 4.2e6 + gm_plan(GM_NT, EP_OUT, 0, 1, M, N, K, 1).time;
 }
 
 }  // namespace gfl

@@ -13,6 +13,17 @@
 
 namespace gfl {
 
+// a fragment of which the first n values (0..7; else as it is) are dropped and zeros follow
+__device__ __forceinline__ gm_i4 q4_shift(gm_i4 v, int n)
+{
+    n = n > 0 && n < 8 ? n : 0;
+    const bool four = n & 4, two = n & 2, one = n & 1;
+    v = gm_i4{ four ? v[2] : v[0], four ? v[3] : v[1], four ? 0 : v[2], four ? 0 : v[3] };
+    v = gm_i4{ two ? v[1] : v[0], two ? v[2] : v[1], two ? v[3] : v[2], two ? 0 : v[3] };
+    auto half = [](int hi, int lo) { return (int)(((uint32_t)hi << 16) | ((uint32_t)lo >> 16)); };
+    return one ? gm_i4{ half(v[1], v[0]), half(v[2], v[1]), half(v[3], v[2]), half(0, v[3]) } : v;
+}
+
 // 16 + v of a word's 8 values. The constants are asked into registers of their own (opaque, so that they stay there): a shift and
 // a v_and_or_b32 for two values, where literals take a shift, an and and an or.
 template <typename T>
@@ -45,7 +56,9 @@ __global__ __launch_bounds__(NW * 64) void q4_few_kernel(Q4Args a)
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / 64), lane = threadIdx.x % 64, r = lane % 16, g = lane / 16;
     const int groups = (a.K + G - 1) / G, tiles = (a.N + 15) / 16, last = a.blocks - 1;
     const int share = (a.blocks + KS - 1) / KS, c0 = wave % KS * share, batches = (share + U - 1) / U;
-    const int pieces = a.blocks * 16, total = pieces * a.M, ldr = a.blocks * 256 + 16;   // of 16 bytes
+    const int m0 = blockIdx.y * 16, M = min(a.M - m0, 16);
+    const int pieces = a.blocks * 16, total = pieces * M, ldr = a.blocks * 256 + 16;   // of 16 bytes
+    const char* xg = a.x + (int64_t)m0 * a.ldx;
     const Q4Frag<T> frag;
 
     gm_i4 w[U], wn[U], xp[NP];
@@ -59,13 +72,13 @@ __global__ __launch_bounds__(NW * 64) void q4_few_kernel(Q4Args a)
 #pragma unroll
         for (int l = 0; l < NS; ++l)
         {
-            const int64_t at = (int64_t)min(c * GB + 4 * l + g, groups - 1) * a.N + n;
+            const uint32_t at = (uint32_t)min(c * GB + 4 * l + g, groups - 1) * a.N + n;
             sc[l] = static_cast<const uint16_t*>(a.scale)[at];
             if constexpr (ZERO) zr[l] = a.zero[at];
         }
-        const char* p = reinterpret_cast<const char*>(a.q) + (int64_t)n * a.blocks * 64 + g * 16;
+        const uint32_t row = (uint32_t)n * a.blocks * 64 + g * 16;   // (a weight has up to 2^31 bytes)
 #pragma unroll
-        for (int i = 0; i < U; ++i) __builtin_memcpy(&v[i], p + min(c + i, last) * 64, 16);
+        for (int i = 0; i < U; ++i) __builtin_memcpy(&v[i], a.q + (row + min(c + i, last) * 64), 16);
     };
     // piece p of the tokens: 8 inputs of token p / pieces
     auto token_at = [&](int p, int& m, int& k) {
@@ -78,7 +91,7 @@ __global__ __launch_bounds__(NW * 64) void q4_few_kernel(Q4Args a)
         {
             int m, k;
             token_at(min(p0 + i * NW * 64, total - 1), m, k);
-            __builtin_memcpy(&xp[i], a.x + m * a.ldx + min(k, a.K - 8) * 2, 16);
+            __builtin_memcpy(&xp[i], xg + ((uint32_t)m * (uint32_t)a.ldx + min(k, a.K - 8) * 2), 16);
         }
     };
     auto keep = [&](int p0) {
@@ -111,11 +124,11 @@ __global__ __launch_bounds__(NW * 64) void q4_few_kernel(Q4Args a)
         {
             int m, k;
             token_at(p, m, k);
-            *reinterpret_cast<gm_i4*>(q4_lds + m * ldr + k * 2) = gm_masked<2>(a.x + m * a.ldx + k * 2, (a.K - k) * 2);
+            *reinterpret_cast<gm_i4*>(q4_lds + m * ldr + k * 2) = gm_masked<2>(xg + m * a.ldx + k * 2, (a.K - k) * 2);
         }
     }
     gm_barrier();   // (waits for LDS alone: the weights stay under way)
-    const char* x = q4_lds + min(r, a.M - 1) * ldr + g * 16;
+    const char* x = q4_lds + min(r, M - 1) * ldr + g * 16;
     // whole rounds of the workgroup, so that its waves meet as often as each other
     for (int it = 0, first = blockIdx.x * (NW / KS); first < tiles; ++it, first += step, tile += step)
     {
@@ -163,7 +176,7 @@ __global__ __launch_bounds__(NW * 64) void q4_few_kernel(Q4Args a)
             const int n = tile * 16 + r;
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-                if (g * 4 + e < a.M && n < a.N) gm_put1(a.out, a.odt, (int64_t)(g * 4 + e) * a.ldo + n, acc[e]);
+                if (g * 4 + e < M && n < a.N) gm_put1(a.out, a.odt, (int64_t)(m0 + g * 4 + e) * a.ldo + n, acc[e]);
         }
         else
         {
@@ -176,7 +189,7 @@ __global__ __launch_bounds__(NW * 64) void q4_few_kernel(Q4Args a)
                 float v = 0.0f;
 #pragma unroll
                 for (int k = 0; k < KS; ++k) v += red[it % 2][w0 + k][e][l];
-                if (m < a.M && n < a.N) gm_put1(a.out, a.odt, (int64_t)m * a.ldo + n, v);
+                if (m < M && n < a.N) gm_put1(a.out, a.odt, (int64_t)(m0 + m) * a.ldo + n, v);
             }
         }
     }
@@ -190,8 +203,9 @@ static void q4_few_go(Q4Args a, hipStream_t st)
     static std::atomic<uint64_t> opened{ 0 };
     gm_open(reinterpret_cast<const void*>(kern), Q4_TOKENS, opened);
     a.magic = (uint32_t)((1ull << 32) / (a.blocks * 16) + 1);
-    const int lds = a.M * (a.blocks * 256 + 16), tiles = (a.N + 15) / 16, wg = (tiles + NW / KS - 1) / (NW / KS);
-    hipLaunchKernelGGL(kern, dim3(std::min(wg, 256 * std::min(LDS_LIMIT / (lds + (KS > 1 ? NW * 2048 : 0)), 3))), dim3(NW * 64), lds, st, a);
+    const int lds = std::min(a.M, 16) * (a.blocks * 256 + 16), tiles = (a.N + 15) / 16, wg = (tiles + NW / KS - 1) / (NW / KS);
+    hipLaunchKernelGGL(kern, dim3(std::min(wg, 256 * std::min(LDS_LIMIT / (lds + (KS > 1 ? NW * 2048 : 0)), 3)), (a.M + 15) / 16),
+                       dim3(NW * 64), lds, st, a);
 }
 
 template <typename T, int GB, bool ZERO, int KS>
@@ -258,21 +272,21 @@ __global__ __launch_bounds__(512, TT * NT >= 8 ? 2 : 4) void q4_tile_kernel(Q4Ar
     const int share = ((a.blocks + a.parts - 1) / a.parts + 1) / 2 * 2, b0 = part * share, end = min(b0 + share, a.blocks);
     const Q4Frag<T> frag;
 
-    const char* wp[NT];
+    // all offsets from uniform addresses: a tile's rows of x lie within 2^29 bytes, a weight has up to 2^31, scales up to 2^28
+    const char* xg = a.x + (int64_t)m0 * a.ldx;
+    uint32_t wo[NT];
 #pragma unroll
-    for (int t = 0; t < NT; ++t) wp[t] = reinterpret_cast<const char*>(a.q) + (int64_t)min(nw + t * 16 + r, a.N - 1) * a.blocks * 64 + g * 16;
-    // lane group g has the scale of slot 4 l + g: of channel tile slot / SG and group slot % SG of the step
-    int sn_[NS];
-#pragma unroll
-    for (int l = 0; l < NS; ++l) sn_[l] = min(nw + min((4 * l + g) / SG, NT - 1) * 16 + r, a.N - 1);
+    for (int t = 0; t < NT; ++t) wo[t] = (uint32_t)min(nw + t * 16 + r, a.N - 1) * a.blocks * 64 + g * 16;
     uint16_t s[NS], s1[NS];
     uint8_t z[NS], z1[NS];
     gm_i4 w[NT][2], w1[NT][2], xv[TT];
+    // lane group g has the scale of slot 4 l + g: of channel tile slot / SG and group slot % SG of the step
     auto scales = [&](int b) {
 #pragma unroll
         for (int l = 0; l < NS; ++l)
         {
-            const int64_t at = (int64_t)min(b * GB + (4 * l + g) % SG, groups - 1) * a.N + sn_[l];
+            const int n = min(nw + min((4 * l + g) / SG, NT - 1) * 16 + r, a.N - 1);
+            const uint32_t at = (uint32_t)min(b * GB + (4 * l + g) % SG, groups - 1) * a.N + n;
             s1[l] = static_cast<const uint16_t*>(a.scale)[at];
             if constexpr (ZERO) z1[l] = a.zero[at];
         }
@@ -281,33 +295,25 @@ __global__ __launch_bounds__(512, TT * NT >= 8 ? 2 : 4) void q4_tile_kernel(Q4Ar
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
-            for (int i = 0; i < 2; ++i) __builtin_memcpy(&w1[t][i], wp[t] + min(b + i, last) * 64, 16);
+            for (int i = 0; i < 2; ++i) __builtin_memcpy(&w1[t][i], a.q + (wo[t] + min(b + i, last) * 64), 16);
     };
-    // a thread's pieces of the tokens: 8 inputs of one token each, 32 pieces a token
+    // a thread's pieces of the tokens: 8 inputs of one token each, 32 pieces a token. K >= 8: a piece that ends past the row is
+    // loaded from the row's last 8 inputs and shifted
     const int col = threadIdx.x % 32, row = threadIdx.x / 32;
+    uint32_t xo[TT];
+#pragma unroll
+    for (int t = 0; t < TT; ++t) xo[t] = (uint32_t)min(row + 16 * t, a.M - 1 - m0) * (uint32_t)a.ldx;
     auto fetch = [&](int b) {
-        const int k = b * 128 + col * 8;
-        if (a.K % 8 == 0)
-        {
+        const uint32_t k = (uint32_t)min(b * 128 + col * 8, a.K - 8) * 2;
 #pragma unroll
-            for (int t = 0; t < TT; ++t)
-            {
-                const int64_t m = min(m0 + row + 16 * t, a.M - 1);
-                __builtin_memcpy(&xv[t], a.x + m * a.ldx + min(k, a.K - 8) * 2, 16);
-            }
-        }
-        else
-        {
-#pragma unroll
-            for (int t = 0; t < TT; ++t)
-            {
-                const int64_t m = min(m0 + row + 16 * t, a.M - 1);
-                xv[t] = gm_masked<2>(a.x + m * a.ldx + (int64_t)k * 2, (a.K - k) * 2);
-            }
-        }
+        for (int t = 0; t < TT; ++t) __builtin_memcpy(&xv[t], xg + (xo[t] + k), 16);
     };
     auto keep = [&](int b, int buf) {
-        const bool there = b * 128 + col * 8 < a.K;
+        const int k = b * 128 + col * 8, over = k + 8 - a.K;
+        if (a.K % 8)
+#pragma unroll
+            for (int t = 0; t < TT; ++t) xv[t] = q4_shift(xv[t], over);
+        const bool there = k < a.K;
         char* xl = q4_lds + buf * (XB + SB);
         float* sl = reinterpret_cast<float*>(xl + XB);
 #pragma unroll
@@ -410,7 +416,11 @@ __global__ __launch_bounds__(512, TT * NT >= 8 ? 2 : 4) void q4_tile_kernel(Q4Ar
                     for (int t = 0; t < TT; ++t)
 #pragma unroll
                         for (int e = 0; e < 4; ++e) acc[n][t][e] = fmaf(sv[n], sum[n][t][e], acc[n][t][e]);
-                __builtin_amdgcn_sched_barrier(0);   // (the groups' sums side by side take more registers than there are)
+                // here and not later: all groups' MFMAs first, which is how the compiler would have it, take more registers than there are
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int t = 0; t < TT; ++t) asm volatile("" : "+v"(acc[n][t]));
             }
         if (more) keep(next, 1 - it % 2);
         gm_barrier();
@@ -466,10 +476,10 @@ template <typename T, int GB, bool ZERO>
 static void q4_run(Q4Args& a, void* ws, hipStream_t st)
 {
     const Q4Plan p = q4_plan(a.M, a.N, a.K);
-    if (p.few) return q4_few<T, GB, ZERO>(a, st);
-    // a launch has fewer than 2^32 threads: the rows in as many as it takes
-    const int64_t wide = (int64_t)((a.N + 128 * p.nt - 1) / (128 * p.nt)) * p.parts;
-    const int rows = (int)std::max<int64_t>(1, (1 << 22) / wide) * 16 * p.tt, M = a.M;
+    // a launch has fewer than 2^32 threads, and fewer than 2^16 workgroups in y: the rows in as many launches as it takes
+    const int64_t wide = p.few ? 768 : (int64_t)((a.N + 128 * p.nt - 1) / (128 * p.nt)) * p.parts;
+    const int tt = p.few ? 1 : p.tt, M = a.M;
+    const int rows = (int)std::max<int64_t>(1, std::min<int64_t>((1 << 22) / wide, 65535)) * 16 * tt;
     for (int m = 0; m < M; m += rows)
     {
         Q4Args b = a;
@@ -479,7 +489,8 @@ static void q4_run(Q4Args& a, void* ws, hipStream_t st)
         b.parts = p.parts;
         b.part = static_cast<float*>(ws);
         b.ldp = p.ldp;
-        q4_tiles<T, GB, ZERO>(b, p, st);
+        if (p.few) q4_few<T, GB, ZERO>(b, st);
+        else q4_tiles<T, GB, ZERO>(b, p, st);
     }
 }
 

@@ -307,7 +307,7 @@ Tensor linear_i4(const Tensor& x, const Tensor& q, const Tensor& scale, const Op
     const Rows o = rows_of("linear_i4: out", y, w.N);
     const int ycode = code_of(y.scalar_type());
     size_t need = 0;
-    check_rc(gfl_i4_workspace(code, ycode, r.n, w.N, w.K, &need, nullptr));
+    check_rc(gfl_i4_workspace(code, ycode, r.n, w.N, w.K, w.group, &need, nullptr));
     const Tensor ws = workspace(need, x);
     check_rc(gfl_linear_i4(x.data_ptr(), r.ld, code, q.data_ptr<uint8_t>(), scale.data_ptr(), w.scale_code, addr<uint8_t>(zero), r.n,
                            w.N, w.K, w.group, y.data_ptr(), o.ld, ycode, addr(ws), need, on.stream));
@@ -326,7 +326,7 @@ Tensor linear_i4_dx(const Tensor& dy, const Tensor& q, const Tensor& scale, int6
     shape.back() = w.K;
     Tensor dx = at::empty(shape, dy.options());
     size_t need = 0;
-    check_rc(gfl_i4_workspace(code, code, r.n, w.N, w.K, nullptr, &need));
+    check_rc(gfl_i4_workspace(code, code, r.n, w.N, w.K, w.group, nullptr, &need));
     const Tensor ws = workspace(need, dy);
     check_rc(gfl_linear_i4_dx(dy.data_ptr(), r.ld, code, q.data_ptr<uint8_t>(), scale.data_ptr(), w.scale_code, addr<uint8_t>(zero),
                               r.n, w.N, w.K, w.group, dx.data_ptr(), w.K, addr(ws), need, on.stream));

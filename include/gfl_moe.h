@@ -326,9 +326,10 @@ int gfl_quant_i4(const void* w, int64_t ldw, int dtype, int N, int K, int group,
 /* Packs values that something else rounded: v uint8 [N, K], of which the lower four bits count. */
 int gfl_pack_i4(const uint8_t* v, int64_t ldv, int N, int K, uint8_t* q, gfl_stream stream);
 
-/* out[m][n] = sum_k x[m][k] * w[n][k] for x [M, K] fp16 or bf16 (dtype); out fp16, bf16 or fp32. Sums are fp32. Up to 64 tokens, and
- * where out is not of x's type, the weights enter exactly, as whole numbers; above they are rounded to x's type for the MFMAs.
- * An infinity in a token's x makes its outputs NaN in the exact form. q 16-byte aligned. */
+/* out[m][n] = sum_k x[m][k] * w[n][k] for x [M, K] fp16 or bf16 (dtype); out fp16, bf16 or fp32. Sums are fp32. Up to 64 tokens,
+ * in larger calls as long as that is quicker (some hundred tokens), and wherever out is not of x's type, the weights enter
+ * exactly, as whole numbers; else they are rounded to x's type. An infinity in a token's x makes its outputs not finite (NaN in the
+ * exact form). q 16-byte aligned. */
 int gfl_linear_i4(const void* x, int64_t ldx, int dtype, const uint8_t* q, const void* scale, int scale_dtype, const uint8_t* zero,
                   int M, int N, int K, int group, void* out, int64_t ldo, int out_dtype, void* ws, size_t ws_bytes,
                   gfl_stream stream);
@@ -340,7 +341,7 @@ int gfl_linear_i4_dx(const void* dy, int64_t lddy, int dtype, const uint8_t* q, 
                      gfl_stream stream);
 
 /* Bytes of workspace: *forward for gfl_linear_i4, *backward for gfl_linear_i4_dx (either may be NULL). */
-int gfl_i4_workspace(int dtype, int out_dtype, int M, int N, int K, size_t* forward, size_t* backward);
+int gfl_i4_workspace(int dtype, int out_dtype, int M, int N, int K, int group, size_t* forward, size_t* backward);
 
 /* The choice of experts in its general form, for routers that gfl_route does not cover: logits [M, E] (fp32, fp16 or bf16).
  *   score s   GFL_SIGMOID: 1 / (1 + exp(-x)); GFL_SOFTMAX: exp(x) / sum of exp over the row

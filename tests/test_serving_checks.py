@@ -39,7 +39,9 @@ def test_linear_i4_refusals(lib):
     _refused(lib, linear(odt=3), "out_dtype")
     _refused(lib, linear(ldo=1 << 30), "stride")
     for kw in (dict(ws=None), dict(nb=16), dict(ws=P + 8)):
-        _refused(lib, linear(M=500, **kw), "workspace")
+        # 16-bit weights for 8192 tokens, parts of the sums for 40
+        _refused(lib, linear(M=8192, N=4096, K=4096, ldx=4096, ldo=4096, **kw), "workspace")
+        _refused(lib, linear(M=40, N=512, K=4096, ldx=4096, ldo=512, **kw), "workspace")
         _refused(lib, dx(**kw), "workspace")
 
 
@@ -63,12 +65,13 @@ def test_i4_workspace(lib):
     f, b = C.c_size_t(), C.c_size_t()
     for M in (0, 1, 64, 65, 5000):
         for N, K in ((1, 1), (77, 131), (12288, 5120)):
-            assert lib.gfl_i4_workspace(1, 1, M, N, K, C.byref(f), C.byref(b)) == 0
-            assert f.value == 0 if M <= 64 else f.value >= 2 * N * K
+            assert lib.gfl_i4_workspace(1, 1, M, N, K, 64, C.byref(f), C.byref(b)) == 0
+            assert f.value <= 64 * M * (N + 4) if M <= 64 else N < 12288 or M < 5000 or f.value >= 2 * N * K
             assert b.value >= 2 * N * K if M else b.value == 0
-            assert lib.gfl_i4_workspace(1, 2, M, N, K, C.byref(f), None) == 0
-    _refused(lib, lib.gfl_i4_workspace(2, 2, 1, 8, 8, C.byref(f), None), "dtype")
-    _refused(lib, lib.gfl_i4_workspace(0, 0, 1, 0, 8, C.byref(f), None), "N")
+            assert lib.gfl_i4_workspace(1, 2, M, N, K, 32, C.byref(f), None) == 0 and f.value <= 64 * M * (N + 4)
+    _refused(lib, lib.gfl_i4_workspace(2, 2, 1, 8, 8, 32, C.byref(f), None), "dtype")
+    _refused(lib, lib.gfl_i4_workspace(0, 0, 1, 8, 8, 16, C.byref(f), None), "group")
+    _refused(lib, lib.gfl_i4_workspace(0, 0, 1, 0, 8, 32, C.byref(f), None), "N")
 
 
 def test_route_experts_refusals(lib):
