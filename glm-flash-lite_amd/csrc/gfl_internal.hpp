@@ -271,10 +271,10 @@ struct RouteArgs
     int64_t* sel = nullptr;   // [M][topk]
     void* w = nullptr;
     int wdtype = 0;
-    int lpg = 0;              // lanes of a group
+    int lpg = 0, per = 0;     // lanes of a group, experts of a lane
 };
 int launch_route_experts(RouteArgs& a, hipStream_t st);
-void launch_route_backward(const RouteArgs& a, const void* dw, const int64_t* sel, void* dx, int64_t ldx, hipStream_t st);
+void launch_route_backward(RouteArgs& a, const void* dw, const int64_t* sel, void* dx, int64_t ldx, hipStream_t st);
 
 // logits before the draw (k_logits.hip)
 constexpr int MAX_HISTORY = (1 << 20) - 1, MAX_BIASES = 2047;

@@ -1,15 +1,19 @@
 // The choice of experts in its general form: scores (sigmoid or softmax), a bias for balance, groups, top-k, weights; and the
 // gradient of the logits.
 //
-// Scores are fp64: a choice is a comparison of scores + bias, and in fp32 some token in every few thousand has two experts beside
-// the border that fp32 cannot tell apart (or ties, which then go by index). Without a bias and groups the logits
-// themselves are compared, which order as the scores do.
+// The choice is that of fp64 scores: in fp32 some token in every few thousand has two experts beside the border that fp32 cannot tell
+// apart (or ties, which then go by index). It is made in fp32 first, whose keys are known to within a margin; where two picks, or the
+// last and what comes after it, lie closer, the candidates are ordered again by their fp64 keys, and where that does not settle it (a
+// border between groups, a softmax with a bias, a crowd at the border) the token is chosen for in fp64 by the whole wave. Without a bias and groups the logits themselves are
+// compared, which order as the scores do.
 //
 // A token takes L lanes (64 / L tokens a wave). Its E experts lie in index order over the lanes, each group over lanes of its
-// own, so that among equal keys the lowest lane's lowest place is the lowest index. A pick is the maximum of the lanes' best keys:
-// first of the keys' upper 32 bits, then, where two lanes share those, of the lower.
+// own, so that among equal keys the lowest lane's lowest place is the lowest index.
 #include "gfl_device.hpp"
 #include "gfl_internal.hpp"
+
+#include <type_traits>
+#include <utility>
 
 namespace gfl {
 
@@ -40,38 +44,91 @@ __device__ __forceinline__ uint64_t rt_key(double x)
     return x > -(double)INFINITY ? (b >> 63 ? ~b : b | 1ull << 63) : 0ull;
 }
 
-template <int W>
-__device__ __forceinline__ uint32_t rt_xor(uint32_t v)
+// What a token's lanes hold, joined by `op` (which is associative, commutative and, in a softmax's sum, the same in any lane): within rows of
+// 16 by DPP (quads, then mirrored half rows and rows, whose quads are all equal by then), across rows by gfx950's swaps, which leave a
+// lane both its own value and the other's.
+template <int L, typename V, typename Op>
+__device__ __forceinline__ V rt_all(V v, Op op)
 {
-    return __float_as_uint(lane_xor<W>(__uint_as_float(v)));
-}
-template <int W>
-__device__ __forceinline__ double rt_xor(double v)
-{
-    const uint64_t b = (uint64_t)__double_as_longlong(v);
-    return __longlong_as_double((long long)((uint64_t)rt_xor<W>((uint32_t)(b >> 32)) << 32 | rt_xor<W>((uint32_t)b)));
+    constexpr int N = sizeof(V) / 4;
+    struct Words { uint32_t w[N]; };
+    auto dpp = [&](auto ctrl) {
+        Words a = __builtin_bit_cast(Words, v), b;
+#pragma unroll
+        for (int i = 0; i < N; ++i) b.w[i] = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)a.w[i], decltype(ctrl)::value, 0xF, 0xF, true);
+        v = op(v, __builtin_bit_cast(V, b));
+    };
+    dpp(std::integral_constant<int, 0xB1>{});    // quad_perm 1, 0, 3, 2
+    dpp(std::integral_constant<int, 0x4E>{});    // quad_perm 2, 3, 0, 1
+    dpp(std::integral_constant<int, 0x141>{});   // row_half_mirror
+    dpp(std::integral_constant<int, 0x140>{});   // row_mirror
+    if constexpr (L >= 32)
+    {
+        const Words a = __builtin_bit_cast(Words, v);
+        Words b, c;
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+        {
+            const auto r = __builtin_amdgcn_permlane16_swap(a.w[i], a.w[i], false, false);
+            b.w[i] = r[0], c.w[i] = r[1];
+        }
+        v = op(__builtin_bit_cast(V, b), __builtin_bit_cast(V, c));
+    }
+    if constexpr (L >= 64)
+    {
+        const Words a = __builtin_bit_cast(Words, v);
+        Words b, c;
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+        {
+            const auto r = __builtin_amdgcn_permlane32_swap(a.w[i], a.w[i], false, false);
+            b.w[i] = r[0], c.w[i] = r[1];
+        }
+        v = op(__builtin_bit_cast(V, b), __builtin_bit_cast(V, c));
+    }
+    return v;
 }
 template <int L>
-__device__ __forceinline__ uint32_t rt_max(uint32_t v)   // over a token's lanes
+__device__ __forceinline__ uint32_t rt_max(uint32_t v)
 {
-    v = max(v, rt_xor<1>(v));
-    v = max(v, rt_xor<2>(v));
-    v = max(v, rt_xor<4>(v));
-    v = max(v, rt_xor<8>(v));
-    if constexpr (L >= 32) v = max(v, rt_xor<16>(v));
-    if constexpr (L >= 64) v = max(v, rt_xor<32>(v));
-    return v;
+    return rt_all<L>(v, [](uint32_t a, uint32_t b) { return max(a, b); });
 }
 template <int L>
 __device__ __forceinline__ double rt_sum(double v)
 {
-    v += rt_xor<1>(v);
-    v += rt_xor<2>(v);
-    v += rt_xor<4>(v);
-    v += rt_xor<8>(v);
-    if constexpr (L >= 32) v += rt_xor<16>(v);
-    if constexpr (L >= 64) v += rt_xor<32>(v);
-    return v;
+    return rt_all<L>(v, [](double a, double b) { return a + b; });
+}
+
+// keys[0..N) into descending order by a merge exchange network (any N)
+template <int N>
+struct RtNet
+{
+    int a[N * 6 + 1] = {}, b[N * 6 + 1] = {}, n = 0;
+    constexpr RtNet()
+    {
+        for (int p = 1; p < N; p *= 2)
+            for (int k = p; k >= 1; k /= 2)
+                for (int j = k % p; j + k < N; j += 2 * k)
+                    for (int i = 0; i < k && i + j + k < N; ++i)
+                        if ((i + j) / (2 * p) == (i + j + k) / (2 * p)) a[n] = i + j, b[n] = i + j + k, ++n;
+    }
+};
+template <int N, size_t... I>
+__device__ __forceinline__ void rt_sort(uint32_t (&key)[N], std::index_sequence<I...>)
+{
+    constexpr RtNet<N> net;
+    auto swap = [&](auto at) {
+        constexpr int x = net.a[decltype(at)::value], y = net.b[decltype(at)::value];
+        const uint32_t hi = max(key[x], key[y]), lo = min(key[x], key[y]);
+        key[x] = hi, key[y] = lo;
+    };
+    (swap(std::integral_constant<size_t, I>{}), ...);
+}
+template <int N>
+__device__ __forceinline__ void rt_sort(uint32_t (&key)[N])
+{
+    constexpr RtNet<N> net;
+    rt_sort(key, std::make_index_sequence<net.n>{});
 }
 
 // exp(x - top) of a softmax: experts at the maximum weigh 1 (also where it is +inf), those that are not there 0
@@ -85,34 +142,174 @@ __device__ __forceinline__ float rt_unkey(uint32_t k)
     return k == 0 ? -INFINITY : __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k);
 }
 
-// NI: experts of a lane. FULL: the keys are scores + bias (a bias, or groups); else the logits.
-template <int L, int NI, bool FULL>
-__global__ __launch_bounds__(RT_T) void route_experts_kernel(RouteArgs a)
+__device__ __forceinline__ float rt_exp(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504f); }
+
+// the lanes of a token in a ballot
+template <int L>
+__device__ __forceinline__ uint64_t rt_lanes(uint64_t all, int lane)
 {
-    constexpr int TOK = RT_T / L;
-    __shared__ int pick[TOK][64];
-    const int lane = threadIdx.x % 64, sub = threadIdx.x % L, tok = threadIdx.x / L;
-    const int64_t t = (int64_t)blockIdx.x * TOK + tok, row = min(t, (int64_t)a.M - 1) * a.ld;
-    // the lane's experts: e0 .. e0 + n - 1 of group g
-    const int g = sub / a.lpg, gs = a.E / a.groups, per = (gs + a.lpg - 1) / a.lpg, s0 = sub % a.lpg * per;
-    const int e0 = g * gs + s0, n = g < a.groups ? min(per, gs - s0) : 0;
+    if constexpr (L == 64) return all;
+    else return all >> (lane / L * L) & ((1ull << L) - 1);
+}
 
-    float x[NI];
+template <typename X, int NI>
+__device__ __forceinline__ void rt_row(const X* p, int n, float (&x)[NI])   // n of NI neighbouring elements, -inf past them
+{
+    X e[NI] = {};
+    if (n == NI) __builtin_memcpy(e, p, sizeof e);
+    else if (n > 0)
 #pragma unroll
-    for (int i = 0; i < NI; ++i) x[i] = -INFINITY;
+        for (int i = 0; i < NI; ++i) e[i] = p[min(i, n - 1)];   // (all loads at once: behind a condition each waits for the one before)
 #pragma unroll
-    for (int i = 0; i < NI; ++i)
-        if (i < n) x[i] = rt_load(a.logits, a.dtype, row + e0 + i);
+    for (int i = 0; i < NI; ++i) x[i] = i < n ? static_cast<float>(e[i]) : -INFINITY;
+}
 
-    float top = 0.f;
-    double norm = 1.0;
-    if (a.softmax)
+// Which groups a lane's group is among the kept ones, by their worth (the sum of the one or two largest keys, given as v1 >= v2; -inf:
+// none): how many come before it.
+template <int L, typename V>
+__device__ __forceinline__ int rt_group(const RouteArgs& a, int lpg, int lane, int g, V v1, V v2, V& worth)
+{
+    for (int w = 1; w < lpg; w *= 2)
     {
-        uint32_t k = 0;
-#pragma unroll
-        for (int i = 0; i < NI; ++i) k = max(k, rt_key(x[i]));
-        top = rt_unkey(rt_max<L>(k));
+        const V o1 = __shfl_xor(v1, w), o2 = __shfl_xor(v2, w);
+        v2 = fmax(fmax(v2, o2), fmin(v1, o1));
+        v1 = fmax(v1, o1);
     }
+    worth = a.group_best == 2 && v2 > -(V)INFINITY ? v1 + v2 : v1;
+    int before = 0;
+    for (int h = 0; h < a.groups; ++h)
+    {
+        const V o = __shfl(worth, lane / L * L + h * lpg);
+        before += o > worth || (o == worth && h < g);
+    }
+    return before;
+}
+
+constexpr int RT_MORE = 6;   // candidates past the picks
+
+enum
+{
+    RT_SURE = 0,
+    RT_ORDER = 1,   // the candidates' order is to be looked at again
+    RT_WIDE = 2,    // what fp32 says is not enough
+};
+
+// The choice in fp32: picks, and as many candidates more as lie within the margin of the last (`count` in all). Keys hold a place in the
+// lane in their last bits and compare by the rest; a lane's are sorted once, so that its best is its first, and a pick moves
+// the rest up. exact_keys: the places take no bits of the logits.
+// Margins. Sigmoid: the argument's rounding and v_exp_f32 make 1.5 |x| 2^-24 + 2^-23 of exp(-x), which counts s (1 - s) times, 1 + exp
+// and v_rcp_f32 1.5 2^-23 of s: below 2^-22. Softmax: the same of an exponential, 32 additions and a reciprocal of the sum: below 2^-18.
+// Adding the bias takes 2^-24 of the key, the places up to PLACE 2^-23. Two keys, twice each; 2^-20 leaves as much again.
+template <int L, int NI, bool FULL>
+__device__ __forceinline__ int rt_choose(const RouteArgs& a, int lane, int sub, int g, int e0, const float (&x)[NI], const float (&bias)[NI],
+                                         float top, int* pick, bool exact_keys, int& count)
+{
+    constexpr uint32_t PLACE = NI > 16 ? 31 : NI > 8 ? 15 : NI > 4 ? 7 : NI > 2 ? 3 : NI > 1 ? 1 : 0;
+    const float margin = a.softmax ? 0x1p-16f : 0x1p-20f;
+    constexpr float STEP = (PLACE + 3) * 0x1p-23f;
+    int state = RT_SURE;
+    uint32_t key[NI];
+    if constexpr (FULL)
+    {
+        float s[NI], sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NI; ++i)
+        {
+            const float t = a.softmax ? (x[i] == top ? 1.0f : rt_exp(x[i] - top)) : rt_exp(-x[i]);
+            s[i] = a.softmax ? t : __builtin_amdgcn_rcpf(1.0f + t);
+            sum += x[i] > -INFINITY ? t : 0.0f;
+        }
+        if (a.softmax)
+        {
+            const float r = __builtin_amdgcn_rcpf((float)rt_sum<L>((double)sum));
+#pragma unroll
+            for (int i = 0; i < NI; ++i) s[i] *= r;
+        }
+#pragma unroll
+        for (int i = 0; i < NI; ++i)
+        {
+            s[i] += bias[i];
+            s[i] = x[i] > -INFINITY && s[i] == s[i] ? s[i] : -INFINITY;
+        }
+        bool kept = true;
+        if (a.groups > 1)
+        {
+            float v1 = -INFINITY, v2 = -INFINITY, worth;
+#pragma unroll
+            for (int i = 0; i < NI; ++i)
+            {
+                v2 = fmaxf(v2, fminf(s[i], v1));
+                v1 = fmaxf(v1, s[i]);
+            }
+            kept = rt_group<L, float>(a, a.lpg, lane, g, v1, v2, worth) < a.top_groups;
+            const bool mine = g < a.groups;
+            const float in = -rt_unkey(rt_max<L>(mine && kept ? rt_key(-worth) : 0)), out = rt_unkey(rt_max<L>(mine && !kept ? rt_key(worth) : 0));
+            // (a group that has nothing is worth -inf, and no key of it is compared)
+            if (out > -INFINITY && !(in - out > 2.0f * margin + fabsf(out) * 0x1p-20f)) state = RT_WIDE;
+        }
+#pragma unroll
+        for (int i = 0; i < NI; ++i) key[i] = kept ? rt_key(s[i]) : 0;
+    }
+    else
+#pragma unroll
+        for (int i = 0; i < NI; ++i) key[i] = rt_key(x[i]);
+#pragma unroll
+    for (int i = 0; i < NI; ++i) key[i] = key[i] ? (key[i] & ~PLACE) | (PLACE - i) : 0;
+    rt_sort(key);
+    const int most = min(a.topk + RT_MORE, L);
+    uint32_t least = 0, mine = 0;   // the last pick's key; lane i: candidate i's
+    auto close = [&](uint32_t above, uint32_t m) {
+        if constexpr (!FULL) return m != 0 && above == m;
+        const float u = rt_unkey(above), v = rt_unkey(m);
+        return m != 0 && !(u - v > margin + fmaxf(fabsf(u), fabsf(v)) * STEP);
+    };
+    for (count = 0;; ++count)
+    {
+        const uint32_t best = key[0] & ~PLACE, m = rt_max<L>(best);
+        if (count >= a.topk)
+        {
+            const bool border = !exact_keys && close(least, m);
+            if (!__any(border)) break;
+            if (count >= most)
+            {
+                if (border) state = RT_WIDE;
+                break;
+            }
+        }
+        if (count < a.topk) least = m;
+        mine = sub == count ? m : mine;
+        bool win = best == m;
+        const uint64_t all = __ballot(win);
+        if (__popcll(all) != 64 / L || __any(m == 0))
+        {
+            // two lanes have it (the lower one counts), or a token has none left
+            win = win && m != 0 && (rt_lanes<L>(all, lane) & ((1ull << sub) - 1)) == 0;
+            if (m == 0 && sub == 0) pick[count] = -1;
+        }
+        if (win) pick[count] = e0 + (int)(PLACE - (key[0] & PLACE));
+        // (by masks: of a select between two elements the compiler makes an index, and of that a chain of selects)
+        const uint32_t gone = win ? ~0u : 0u;
+#pragma unroll
+        for (int i = 0; i + 1 < NI; ++i) key[i] = (key[i + 1] & gone) | (key[i] & ~gone);
+        key[NI - 1] &= ~gone;
+    }
+    if (!exact_keys)
+    {
+        const uint32_t above = __shfl_up(mine, 1);
+        const bool c = sub > 0 && sub < count && close(above, mine);
+        if (rt_lanes<L>(__ballot(c), lane)) state |= RT_ORDER;
+    }
+    return state & RT_WIDE || (state && FULL && a.softmax) ? RT_WIDE : state;
+}
+
+// The choice in fp64. A pick is the maximum of the lanes' best keys: first of the upper 32 bits, then, where two lanes share those, of
+// the lower.
+template <int NI, bool FULL>
+__device__ __forceinline__ void rt_choose_wide(const RouteArgs& a, int lpg, int lane, int g, int e0, int n, const float (&x)[NI], float top,
+                                               int* pick)
+{
+    constexpr int L = 64;
+    const int sub = lane;
     uint32_t hi[NI], lo[FULL ? NI : 1];
     if constexpr (FULL)
     {
@@ -124,45 +321,26 @@ __global__ __launch_bounds__(RT_T) void route_experts_kernel(RouteArgs a)
             double part = 0.0;
 #pragma unroll
             for (int i = 0; i < NI; ++i) part += s[i];
-            norm = rt_sum<L>(part);
+            const double norm = rt_sum<L>(part);
 #pragma unroll
             for (int i = 0; i < NI; ++i) s[i] /= norm;
         }
-#pragma unroll
-        for (int i = 0; i < NI; ++i)
-            if (a.bias && i < n) s[i] += (double)a.bias[e0 + i];
+        constexpr double NONE = -(double)INFINITY;
+        double v1 = NONE, v2 = NONE;
 #pragma unroll
         for (int i = 0; i < NI; ++i)
         {
+            if (a.bias && i < n) s[i] += (double)a.bias[e0 + i];
             const uint64_t k = x[i] > -INFINITY ? rt_key(s[i]) : 0;
             hi[i] = (uint32_t)(k >> 32), lo[i] = (uint32_t)k;
+            const double v = k ? s[i] : NONE;
+            v2 = fmax(v2, fmin(v, v1));
+            v1 = fmax(v1, v);
         }
         if (a.groups > 1)
         {
-            // a group is worth the sum of its one or two largest keys
-            constexpr double NONE = -(double)INFINITY;
-            double v1 = NONE, v2 = NONE;
-#pragma unroll
-            for (int i = 0; i < NI; ++i)
-            {
-                const double v = hi[i] | lo[i] ? s[i] : NONE;
-                v2 = fmax(v2, fmin(v, v1));
-                v1 = fmax(v1, v);
-            }
-            for (int w = 1; w < a.lpg; w *= 2)
-            {
-                const double o1 = __shfl_xor(v1, w), o2 = __shfl_xor(v2, w);
-                v2 = fmax(fmax(v2, o2), fmin(v1, o1));
-                v1 = fmax(v1, o1);
-            }
-            const double worth = a.group_best == 2 && v2 > NONE ? v1 + v2 : v1;
-            int before = 0;
-            for (int h = 0; h < a.groups; ++h)
-            {
-                const double o = __shfl(worth, lane / L * L + h * a.lpg);
-                before += o > worth || (o == worth && h < g);
-            }
-            if (before >= a.top_groups)
+            double worth;
+            if (rt_group<L, double>(a, lpg, lane, g, v1, v2, worth) >= a.top_groups)
             {
 #pragma unroll
                 for (int i = 0; i < NI; ++i) hi[i] = lo[i] = 0;
@@ -170,18 +348,8 @@ __global__ __launch_bounds__(RT_T) void route_experts_kernel(RouteArgs a)
         }
     }
     else
-    {
 #pragma unroll
         for (int i = 0; i < NI; ++i) hi[i] = rt_key(x[i]);
-        if (a.softmax && !a.renorm)
-        {
-            double part = 0.0;
-#pragma unroll
-            for (int i = 0; i < NI; ++i) part += rt_soft(x[i], top);
-            norm = rt_sum<L>(part);
-        }
-    }
-
     for (int j = 0; j < a.topk; ++j)
     {
         uint32_t bh = hi[0], bl = FULL ? lo[0] : 0;
@@ -197,18 +365,17 @@ __global__ __launch_bounds__(RT_T) void route_experts_kernel(RouteArgs a)
         }
         const uint32_t m = rt_max<L>(bh);
         bool best = bh == m && m != 0;
-        constexpr uint64_t MASK = L == 64 ? ~0ull : (1ull << (L % 64)) - 1;
-        uint64_t all = __ballot(best) >> (lane / L * L) & MASK;
+        uint64_t all = rt_lanes<L>(__ballot(best), lane);
         if constexpr (FULL)
             if (__any((all & (all - 1)) != 0))
             {
                 const uint32_t ml = rt_max<L>(best ? bl : 0);
                 best = best && bl == ml;
-                all = __ballot(best) >> (lane / L * L) & MASK;
+                all = rt_lanes<L>(__ballot(best), lane);
             }
         if (all == 0 ? sub == 0 : best && (all & ((1ull << sub) - 1)) == 0)
         {
-            pick[tok][j] = all ? e0 + at : -1;
+            pick[j] = all ? e0 + at : -1;
 #pragma unroll
             for (int i = 0; i < NI; ++i)
                 if (i == at)
@@ -218,31 +385,118 @@ __global__ __launch_bounds__(RT_T) void route_experts_kernel(RouteArgs a)
                 }
         }
     }
+}
+
+// NI: experts of a lane. FULL: the keys are scores + bias (a bias, or groups); else the logits.
+template <typename X, int L, int NI, bool FULL>
+__global__ __launch_bounds__(RT_T) void route_experts_kernel(RouteArgs a)
+{
+    constexpr int TOK = RT_T / L;
+    __shared__ int picks[TOK][MAX_ROUTE_K];
+    __shared__ uint64_t keys[TOK][L];
+    const int lane = threadIdx.x % 64, sub = threadIdx.x % L, tok = threadIdx.x / L;
+    const int64_t t = (int64_t)blockIdx.x * TOK + tok;
+    const X* row = static_cast<const X*>(a.logits) + min(t, (int64_t)a.M - 1) * a.ld;
+    // the lane's experts: e0 .. e0 + n - 1 of group g
+    const int gs = a.E / a.groups;
+    auto mine = [&](int l, int lpg, int per, int& g, int& e0, int& n) {
+        const int s0 = l % lpg * per;
+        g = l / lpg;
+        e0 = min(g * gs + s0, a.E);
+        n = g < a.groups ? min(per, max(gs - s0, 0)) : 0;
+    };
+    int g, e0, n;
+    mine(sub, a.lpg, a.per, g, e0, n);
+    float x[NI], bias[NI], top = 0.f;
+    rt_row(row + e0, n, x);
+#pragma unroll
+    for (int i = 0; i < NI; ++i) bias[i] = 0.f;
+    if (FULL && a.bias)
+#pragma unroll
+        for (int i = 0; i < NI; ++i) bias[i] = a.bias[min(e0 + i, a.E - 1)];   // (past the lane's experts there is no logit)
+    if (a.softmax)
+    {
+        uint32_t k = 0;
+#pragma unroll
+        for (int i = 0; i < NI; ++i) k = max(k, rt_key(x[i]));
+        top = rt_unkey(rt_max<L>(k));
+    }
+    int* pick = picks[tok];
+    int count;
+    const int state = rt_choose<L, NI, FULL>(a, lane, sub, g, e0, x, bias, top, pick, !FULL && sizeof(X) == 2, count);
+    if (__any(state == RT_ORDER))
+    {
+        asm volatile("" ::: "memory");   // (LDS is read and written in order within a wave)
+        const int e = sub < count ? pick[sub] : -1;
+        uint64_t key = 0;
+        if (e >= 0)
+        {
+            const float v = static_cast<float>(row[e]);
+            if constexpr (FULL) key = rt_key(rt_sigmoid(v) + (a.bias ? (double)a.bias[e] : 0.0));
+            else key = rt_key((double)v);
+        }
+        keys[tok][sub] = key;
+        asm volatile("" ::: "memory");
+        int before = 0;
+        for (int c = 0; c < count; ++c)
+        {
+            const uint64_t k = keys[tok][c];
+            before += k > key || (k == key && pick[c] < e);
+        }
+        asm volatile("" ::: "memory");
+        if (state == RT_ORDER && e >= 0 && before < a.topk) pick[before] = e;
+    }
+    for (uint64_t left = __ballot(state == RT_WIDE && sub == 0); left; left &= left - 1)
+    {
+        constexpr int NW = (NI * L + 63) / 64;
+        const int first = __builtin_ctzll(left), lpg = a.lpg * (64 / L);
+        const int64_t tw = (int64_t)blockIdx.x * TOK + threadIdx.x / 64 * (64 / L) + first / L;
+        const X* rw = static_cast<const X*>(a.logits) + min(tw, (int64_t)a.M - 1) * a.ld;
+        int gw, ew, nw;
+        mine(lane, lpg, (gs + lpg - 1) / lpg, gw, ew, nw);
+        float xw[NW], topw = 0.f;
+        rt_row(rw + ew, nw, xw);
+        uint32_t k = 0;
+#pragma unroll
+        for (int i = 0; i < NW; ++i) k = max(k, rt_key(xw[i]));
+        if (a.softmax) topw = rt_unkey(rt_max<64>(k));
+        rt_choose_wide<NW, FULL>(a, lpg, lane, gw, ew, nw, xw, topw, picks[threadIdx.x / 64 * (64 / L) + first / L]);
+    }
     __syncthreads();
 
+    double norm = 1.0;
+    if (a.softmax && !a.renorm)
+    {
+        double part = 0.0;
+#pragma unroll
+        for (int i = 0; i < NI; ++i) part += rt_soft(x[i], top);
+        norm = rt_sum<L>(part);
+    }
+    // (renormalised, a softmax's own sum cancels)
     double w[64 / L], sum = 0.0;
 #pragma unroll
     for (int r = 0; r < 64 / L; ++r)
     {
-        const int j = r * L + sub, e = j < a.topk ? pick[tok][j] : -1;
         w[r] = 0.0;
+        if (r * L >= a.topk) continue;
+        const int j = r * L + sub, e = j < a.topk ? pick[j] : -1;
         if (e >= 0)
         {
-            const float v = rt_load(a.logits, a.dtype, row + e);
-            w[r] = a.softmax ? rt_soft(v, top) / norm : rt_sigmoid(v);
+            const float v = static_cast<float>(row[e]);
+            w[r] = a.softmax ? rt_soft(v, top) : rt_sigmoid(v);
         }
         sum += w[r];
     }
     if (a.renorm) norm = rt_sum<L>(sum);
-    else norm = 1.0;
     if (t >= a.M) return;
+    norm = norm > 0.0 ? (double)a.scale / norm : 0.0;
 #pragma unroll
     for (int r = 0; r < 64 / L; ++r)
     {
         const int j = r * L + sub;
         if (j >= a.topk) continue;
-        a.sel[t * a.topk + j] = pick[tok][j];
-        rt_store(a.w, a.wdtype, t * a.topk + j, norm > 0.0 ? (double)a.scale * w[r] / norm : 0.0);
+        a.sel[t * a.topk + j] = pick[j];
+        rt_store(a.w, a.wdtype, t * a.topk + j, w[r] * norm);
     }
 }
 
@@ -251,107 +505,166 @@ __global__ __launch_bounds__(RT_T) void route_experts_kernel(RouteArgs a)
 //   sigmoid: dx = ds s (1 - s) at the picks, 0 elsewhere;
 //   softmax p: dx = p (ds - sum_i ds_i p_i) everywhere; with renormalisation that sum is 0 and only ratios of the picks' exponentials
 //   enter, so the row is not read.
-template <int L>
-__global__ __launch_bounds__(RT_T) void route_backward_kernel(RouteArgs a, const void* dw, const int64_t* sel, void* dx, int64_t ldx)
+template <typename X, int L, int NI>
+__global__ __launch_bounds__(RT_T) void route_backward_kernel(RouteArgs a, const void* dw, const int64_t* sel, X* dx, int64_t ldx)
 {
     constexpr int TOK = RT_T / L;
-    __shared__ int pick[TOK][64];
-    __shared__ float grad[TOK][64];
+    __shared__ int picks[TOK][MAX_ROUTE_K];
+    __shared__ float grads[TOK][MAX_ROUTE_K];
     const int sub = threadIdx.x % L, tok = threadIdx.x / L;
-    const int64_t t = (int64_t)blockIdx.x * TOK + tok, tc = min(t, (int64_t)a.M - 1), row = tc * a.ld;
+    const int64_t t = (int64_t)blockIdx.x * TOK + tok, tc = min(t, (int64_t)a.M - 1);
+    const X* row = static_cast<const X*>(a.logits) + tc * a.ld;
     const bool dense = a.softmax && !a.renorm;
+    const int e0 = min(sub * a.per, a.E), n = min(a.per, a.E - e0);
 
-    float top = -INFINITY, xs[64 / L];
+    float top = -INFINITY, xs[64 / L], up[64 / L];
     int es[64 / L];
     uint32_t k = 0;
+    double p[NI], norm = 1.0;
+    float x[NI];
+    if (dense) rt_row(row + e0, n, x);
 #pragma unroll
     for (int r = 0; r < 64 / L; ++r)
     {
+        es[r] = -1, xs[r] = -INFINITY, up[r] = 0.f;
+        if (r * L >= a.topk) continue;
         const int j = r * L + sub;
         const int64_t e = j < a.topk ? sel[tc * a.topk + j] : -1;
+        if (j < a.topk) up[r] = rt_load(dw, a.wdtype, tc * a.topk + j);
         es[r] = e >= 0 && e < a.E ? (int)e : -1;
-        xs[r] = es[r] >= 0 ? rt_load(a.logits, a.dtype, row + es[r]) : -INFINITY;
+        if (es[r] >= 0) xs[r] = static_cast<float>(row[es[r]]);
         k = max(k, rt_key(xs[r]));
     }
-    double norm = 1.0;
     if (dense)
-        for (int e = sub; e < a.E; e += L) k = max(k, rt_key(rt_load(a.logits, a.dtype, row + e)));
+#pragma unroll
+        for (int i = 0; i < NI; ++i) k = max(k, rt_key(x[i]));
     if (a.softmax) top = rt_unkey(rt_max<L>(k));
     if (dense)
     {
-        double part = 0.0;
-        for (int e = sub; e < a.E; e += L) part += rt_soft(rt_load(a.logits, a.dtype, row + e), top);
-        norm = rt_sum<L>(part);
+        norm = 0.0;
+#pragma unroll
+        for (int i = 0; i < NI; ++i) norm += p[i] = rt_soft(x[i], top);
+        norm = 1.0 / rt_sum<L>(norm);
     }
-    double s[64 / L], d[64 / L], total = 0.0, dot = 0.0;
+    double s[64 / L], total = 0.0, dot = 0.0;
 #pragma unroll
     for (int r = 0; r < 64 / L; ++r)
     {
-        const int j = r * L + sub;
-        s[r] = d[r] = 0.0;
-        if (es[r] >= 0)
-        {
-            s[r] = a.softmax ? rt_soft(xs[r], top) / norm : rt_sigmoid(xs[r]);
-            d[r] = (double)a.scale * rt_load(dw, a.wdtype, tc * a.topk + j);
-        }
+        s[r] = 0.0;
+        if (r * L >= a.topk) continue;
+        if (es[r] >= 0) s[r] = a.softmax ? rt_soft(xs[r], top) * norm : rt_sigmoid(xs[r]);
         total += s[r];
-        dot += s[r] * d[r];
+        dot += s[r] * ((double)a.scale * up[r]);
     }
     total = rt_sum<L>(total);
     dot = rt_sum<L>(dot);
+    const double by = total > 0.0 ? 1.0 / total : 0.0;
 #pragma unroll
     for (int r = 0; r < 64 / L; ++r)
     {
         const int j = r * L + sub;
-        double ds = d[r];
-        if (a.renorm) ds = total > 0.0 ? (ds - dot / total) / total : 0.0;
-        if (j < a.topk)
-        {
-            pick[tok][j] = es[r];
-            // softmax: what is added to -p dot; sigmoid: s (1 - s) = s sigmoid(-x)
-            grad[tok][j] = es[r] < 0 ? 0.f : (float)(ds * s[r] * (a.softmax ? 1.0 : rt_sigmoid(-xs[r])));
-        }
+        if (j >= a.topk) continue;
+        double ds = (double)a.scale * up[r];
+        if (a.renorm) ds = (ds - dot * by) * by;
+        picks[tok][j] = es[r];
+        // softmax: what is added to -p dot; sigmoid: s (1 - s) = s sigmoid(-x)
+        grads[tok][j] = es[r] < 0 ? 0.f : (float)(ds * s[r] * (a.softmax ? 1.0 : rt_sigmoid(-xs[r])));
     }
     __syncthreads();
     if (t >= a.M) return;
-    for (int e = sub; e < a.E; e += L)
+    float v[NI];
+#pragma unroll
+    for (int i = 0; i < NI; ++i) v[i] = dense ? (float)(-dot * (p[i] * norm)) : 0.f;
+    for (int j = 0; j < a.topk; ++j)
     {
-        float v = 0.f;
-        if (dense) v = (float)(-dot * rt_soft(rt_load(a.logits, a.dtype, row + e), top) / norm);
-        for (int j = 0; j < a.topk; ++j)
-            if (pick[tok][j] == e) v += grad[tok][j];
-        rt_store(dx, a.dtype, t * ldx + e, v);
+        const int e = picks[tok][j] - e0;
+        const float d = grads[tok][j];
+#pragma unroll
+        for (int i = 0; i < NI; ++i) v[i] += e == i && i < n ? d : 0.f;
     }
+    X o[NI];
+#pragma unroll
+    for (int i = 0; i < NI; ++i) o[i] = static_cast<X>(v[i]);
+    X* out = dx + t * ldx + e0;
+    if (n == NI) __builtin_memcpy(out, o, sizeof o);
+    else
+#pragma unroll
+        for (int i = 0; i < NI; ++i)
+            if (i < n) out[i] = o[i];
 }
 
-template <int L, bool FULL>
-static int route_go(const RouteArgs& a, int per, hipStream_t st)
+// Experts of a lane that kernels are made for, of each number of lanes.
+template <int L>
+constexpr auto rt_sizes()
+{
+    if constexpr (L == 16) return std::integer_sequence<int, 1, 2, 4, 8, 16>{};
+    else if constexpr (L == 32) return std::integer_sequence<int, 2, 4, 8, 12, 16, 32>{};
+    else return std::integer_sequence<int, 1, 2, 4, 5, 8, 16, 32>{};
+}
+// calls f with the first that holds `per`
+template <typename F, int... N>
+static bool rt_sized(int per, std::integer_sequence<int, N...>, F f)
+{
+    return ((per <= N ? (f(std::integral_constant<int, N>{}), true) : false) || ...);
+}
+
+template <typename X, int L>
+static int route_go(const RouteArgs& a, hipStream_t st)
 {
     const dim3 grid((unsigned)(((int64_t)a.M + RT_T / L - 1) / (RT_T / L))), block(RT_T);
-#define GFL_RT(N)                                                                                   \
-    if (per <= N)                                                                                   \
-    {                                                                                               \
-        hipLaunchKernelGGL((route_experts_kernel<L, N, FULL>), grid, block, 0, st, a);              \
-        return 0;                                                                                   \
-    }
-    GFL_RT(1) GFL_RT(2) GFL_RT(4) GFL_RT(5) GFL_RT(8) GFL_RT(16) GFL_RT(32)
-#undef GFL_RT
-    return -1;
+    const bool done = rt_sized(a.per, rt_sizes<L>(), [&](auto n) {
+        constexpr int N = decltype(n)::value;
+        if (a.bias || a.groups > 1) hipLaunchKernelGGL((route_experts_kernel<X, L, N, true>), grid, block, 0, st, a);
+        else hipLaunchKernelGGL((route_experts_kernel<X, L, N, false>), grid, block, 0, st, a);
+    });
+    return done ? 0 : -1;
+}
+
+template <typename X, int L>
+static void route_back(const RouteArgs& a, const void* dw, const int64_t* sel, void* dx, int64_t ldx, hipStream_t st)
+{
+    const dim3 grid((unsigned)(((int64_t)a.M + RT_T / L - 1) / (RT_T / L))), block(RT_T);
+    rt_sized(a.per, rt_sizes<L>(), [&](auto n) {
+        hipLaunchKernelGGL((route_backward_kernel<X, L, decltype(n)::value>), grid, block, 0, st, a, dw, sel, static_cast<X*>(dx), ldx);
+    });
+}
+
+// Lanes a token. 16 or 32 do the steps of a pick for 4 or 2 tokens at once, 64 hold fewer experts each and are done sooner: us by 64, 32
+// and 16 lanes, sigmoid with a bias, 288 experts, 1 token 4.7, 6.1, 8.2, 4096 8.3, 9.4, 10.2, 8192 13.3, 12.8, 13.3; softmax of 128 experts,
+// 16384 tokens 14.2, 10.0, 8.4.
+template <typename X>
+static int route_of(RouteArgs& a, hipStream_t st)
+{
+    int lanes = 1;   // for each group
+    while (lanes < a.groups) lanes *= 2;
+    const int size = a.E / a.groups;
+    auto per = [&](int L) { return (size + L / lanes - 1) / (L / lanes); };
+    int L = a.M < 6144 ? 64 : a.M < 12288 ? 32 : 16;
+    while (L < 64 && (lanes > L || per(L) > L || a.topk + 1 > L)) L *= 2;
+    a.lpg = L / lanes;
+    a.per = per(L);
+    return L == 16 ? route_go<X, 16>(a, st) : L == 32 ? route_go<X, 32>(a, st) : route_go<X, 64>(a, st);
 }
 
 int launch_route_experts(RouteArgs& a, hipStream_t st)
 {
-    int lanes = 1;   // for each group, of 64
-    while (lanes < a.groups) lanes *= 2;
-    a.lpg = 64 / lanes;
-    const int size = a.E / a.groups, per = (size + a.lpg - 1) / a.lpg;
-    return a.bias || a.groups > 1 ? route_go<64, true>(a, per, st) : route_go<64, false>(a, per, st);
+    return a.dtype == 2 ? route_of<float>(a, st) : a.dtype == 1 ? route_of<__bf16>(a, st) : route_of<_Float16>(a, st);
 }
 
-void launch_route_backward(const RouteArgs& a, const void* dw, const int64_t* sel, void* dx, int64_t ldx, hipStream_t st)
+// 16 lanes a token where each then has a power of two of experts, which it stores as one vector: us by 64 and 16, 16384 tokens of 128
+// experts 14.8 and 9.3, 8192 of 288 8.9 and 16.9.
+template <typename X>
+static void route_back_of(RouteArgs& a, const void* dw, const int64_t* sel, void* dx, int64_t ldx, hipStream_t st)
 {
-    const dim3 grid((unsigned)(((int64_t)a.M + 3) / 4));
-    hipLaunchKernelGGL(route_backward_kernel<64>, grid, dim3(RT_T), 0, st, a, dw, sel, dx, ldx);
+    a.per = (a.E + 15) / 16;
+    if (a.M >= 8192 && a.E % 16 == 0 && (a.per & (a.per - 1)) == 0 && a.per <= 16) return route_back<X, 16>(a, dw, sel, dx, ldx, st);
+    a.per = (a.E + 63) / 64;
+    route_back<X, 64>(a, dw, sel, dx, ldx, st);
+}
+
+void launch_route_backward(RouteArgs& a, const void* dw, const int64_t* sel, void* dx, int64_t ldx, hipStream_t st)
+{
+    (a.dtype == 2 ? &route_back_of<float> : a.dtype == 1 ? &route_back_of<__bf16> : &route_back_of<_Float16>)(a, dw, sel, dx, ldx, st);
 }
 
 }  // namespace gfl

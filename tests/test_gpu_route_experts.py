@@ -52,6 +52,54 @@ def test_groups(gpu, M, E, groups, top, topk, score):
             _check(x, topk, bias=bias, score=score, groups=groups, top_groups=top, group_best=best, dtype=F32)
 
 
+@pytest.mark.parametrize("dt,score,bias", [(F32, "sigmoid", True), (F32, "softmax", True), (F32, "softmax", False), (BF16, "sigmoid", False),
+                                           (F16, "sigmoid", True)])
+@pytest.mark.parametrize("M,E,groups,top,topk", [(6200, 72, 1, 1, 8), (6200, 256, 8, 4, 8), (6200, 1024, 32, 9, 30), (12300, 16, 1, 1, 2),
+                                                 (12300, 128, 4, 2, 6), (12300, 250, 1, 1, 15), (12300, 40, 5, 3, 8)])
+def test_many_tokens(gpu, M, E, groups, top, topk, dt, score, bias):
+    """Batches whose tokens share a wave, two or four to one; a part of them by the definition, all of them as in a smaller batch."""
+    import _native
+    x, b = _logits(M, E, dt, M + E)
+    x[::7] = x[::7].round() if dt == F32 else x[::7]          # rows with ties
+    kw = dict(bias=b if bias else None, score=score, groups=groups, top_groups=top, dtype=F32)
+    sel, w = _native.route_experts(x, topk, **kw)
+    for i in range(0, M, 1000):
+        s2, w2 = _native.route_experts(x[i:i + 1000], topk, **kw)
+        assert torch.equal(sel[i:i + 1000], s2) and torch.equal(w[i:i + 1000], w2)
+    rows = torch.arange(0, M, 61, device="cuda")
+    want_s, want_w = S.route(x[rows], topk, bias=b.cpu() if bias else None, score=score, groups=groups, top_groups=top)
+    assert torch.equal(sel[rows].cpu(), want_s)
+    S.same(w[rows], want_w, (half_step(F32) + 2.0 ** -48) * want_w.abs(), "w")
+
+
+def test_many_tokens_gradient(gpu):
+    import _native
+    for E, topk in ((64, 4), (16, 2), (288, 8)):
+        x, b = _logits(8200, E, BF16, E)
+        dw = torch.randn((8200, topk), generator=torch.Generator().manual_seed(1)).cuda()
+        for score, renorm in (("softmax", False), ("sigmoid", True)):
+            sel, _ = _native.route_experts(x, topk, bias=b, score=score, renorm=renorm)
+            got = _native.route_experts_backward(dw, x, sel, score=score, renorm=renorm)
+            rows = torch.arange(0, 8200, 37, device="cuda")
+            S.same(got[rows], *S.route_gradient(x[rows], sel[rows], dw[rows], score, renorm), "dlogits")
+
+
+def test_crowded_borders(gpu):
+    """Rows of few distinct keys: more candidates at the border than fp32 can order, in every lane layout."""
+    import _native
+    for M in (5, 6200, 12300):
+        g = torch.Generator().manual_seed(M)
+        x = torch.randint(0, 3, (M, 96), generator=g).float()
+        b = torch.randint(0, 2, (96,), generator=g).float() * 3e-8 + 0.125
+        x[1::2] += torch.randint(0, 4, (len(x[1::2]), 96), generator=g) * 2.0 ** -20
+        x = x.cuda()
+        for kw in (dict(), dict(bias=b.cuda()), dict(groups=6, top_groups=2), dict(bias=b.cuda(), score="softmax")):
+            sel, w = _native.route_experts(x, 7, dtype=F32, **kw)
+            rows = torch.arange(0, M, max(1, M // 97), device="cuda")
+            want_s, want_w = S.route(x[rows], 7, **{k: v.cpu() if k == "bias" else v for k, v in kw.items()})
+            assert torch.equal(sel[rows].cpu(), want_s), kw
+
+
 def test_ties_go_to_the_lower_index(gpu):
     x = torch.zeros((4, 96))
     x[1, 40:50] = 3.0
