@@ -178,10 +178,8 @@ def adjust(logits, history=None, lengths=None, prompt=None, repetition=None, fre
                 mag[b, i] += 2 * abs(v)
                 value[b, i] += v
         if allowed is not None:
-            words = allowed[b].tolist()
-            for v in range(V):
-                if not words[v // 32] >> (v % 32) & 1:
-                    value[b, v] = -INF
+            bits = (allowed[b].long()[:, None] >> torch.arange(32) & 1).view(-1)[:V]
+            value[b][bits == 0] = -INF
     dt = logits.dtype
     err = torch.where(torch.isfinite(value), 4 * 2.0 ** -24 * mag, 0.0)
     return value, torch.where(torch.isfinite(value), err + half_step(dt) * (value.abs() + err) + tiny(dt), 0.0)

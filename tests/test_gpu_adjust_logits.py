@@ -162,6 +162,13 @@ def test_strided_lists(gpu):
     assert torch.equal(_check(x, kw), _check(x, wide))
 
 
+@pytest.mark.parametrize("dt", [F32, BF16])
+@pytest.mark.parametrize("B,V,L,n_bias,masked", [(67, 5000, 300, 4, 0.5), (64, 33000, 100, 0, None), (129, 2050, 2050, None, 0.1),
+                                                 (3, 131072, 40000, 2047, 0.8), (2, 262147, 900, 2047, None), (70, 129, 33000, 300, None)])
+def test_many_rows_and_large_vocabularies(gpu, B, V, L, n_bias, masked, dt):
+    _check(*_inputs(B, V, L, n_bias, masked, B + V, dt, pad=5))
+
+
 def test_streams_and_captured(gpu):
     import _native
     x, kw = _inputs(3, 5000, 200, 12, 0.5, 10)

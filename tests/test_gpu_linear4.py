@@ -199,6 +199,23 @@ def test_not_finite(gpu, M):
     assert bool(torch.isnan(y[1]).all()) and not bool(torch.isfinite(y[3]).any()) and bool(torch.isnan(y[:, 5]).all())
 
 
+@pytest.mark.parametrize("dt", [F16, BF16])
+@pytest.mark.parametrize("M,N,K,group,zeros", [(3, 20500, 200, 32, True), (16, 20500, 72, 128, False), (5, 10300, 300, 64, False),
+                                               (2, 10300, 1200, 128, True), (16, 40, 5000, 128, True), (12, 300, 9001, 32, False),
+                                               (33, 40, 5120, 64, True), (17, 700, 5130, 32, True), (512, 2048, 2050, 128, False),
+                                               (700, 1030, 4104, 32, True), (1025, 2100, 2056, 64, True), (64, 5120, 2056, 128, False)])
+def test_forms(gpu, M, N, K, group, zeros, dt):
+    """Few tokens by many channels (a wave, two or four sharing a tile's inputs), few tokens of more inputs than fit in LDS, tiles
+    of one to four times 16 tokens by 128 or 256 channels, with and without parts of the sums, many tiles of rows."""
+    import _native
+    _, q, scale, zero = _weight(N, K, group, zeros, dt, M + N + K)
+    for whole, pad in ((True, 0), (False, 3)):
+        x = _tokens(M, K, dt, N + K, whole, pad)
+        print("linear_i4", M, N, K, group, zeros, dt, pad, flush=True)
+        got = _native.linear_i4(x, q, scale, zero=zero, group=group, dtype=F32)
+        S.same(got, *S.linear(x, q, scale, zero, K, group, F32, True, whole), "y")
+
+
 def test_streams_and_captured(gpu):
     import _native
     _, q, scale, zero = _weight(300, 520, 32, True, F16, 8)
