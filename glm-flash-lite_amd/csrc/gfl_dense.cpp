@@ -404,7 +404,11 @@ int gfl_i4_workspace(int dtype, int out_dtype, int M, int N, int K, int group, s
     if (int rc = i4_check(M, N, K, group)) return rc;
     const size_t w = up256((size_t)N * i4_ldw(K) * 2);
     if (forward) *forward = i4_exact(M, N, K, group, dtype, out_dtype) ? up256(gfl::q4_plan(M, N, K).part_bytes) : w + i4_part(gfl::GM_NT, M, N, K);
-    if (backward) *backward = M ? w + i4_part(gfl::GM_NN, M, K, N) : 0;
+    if (backward)
+    {
+        const gfl::Q4DxPlan p = gfl::q4_dx_plan(M, N, K);
+        *backward = M == 0 ? 0 : p.direct ? up256(p.part_bytes) : w + i4_part(gfl::GM_NN, M, K, N);
+    }
     return GFL_OK;
 }
 
@@ -503,9 +507,20 @@ int gfl_linear_i4_dx(const void* dy, int64_t lddy, int dtype, const uint8_t* q, 
         return api_fail(GFL_EINVAL, "gfl_linear_i4_dx: row strides must be at least the width and below GFL_MAX_LD");
     size_t need = 0;
     gfl_i4_workspace(dtype, dtype, M, N, K, group, nullptr, &need);
-    if (!ws || ws_bytes < need || reinterpret_cast<uintptr_t>(ws) % 16)
+    if (need && (!ws || ws_bytes < need || reinterpret_cast<uintptr_t>(ws) % 16))
         return api_fail(GFL_EINVAL, "gfl_linear_i4_dx: workspace missing, too small or not 16-byte aligned");
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+    if (gfl::q4_dx_plan(M, N, K).direct)
+    {
+        a.x = static_cast<const char*>(dy);
+        a.ldx = lddy * 2;
+        a.M = M;
+        a.out = dx;
+        a.ldo = lddx;
+        a.odt = dtype;
+        gfl::launch_linear_i4_dx(a, dtype == GFL_BF16, ws, st);
+        return check_launch("gfl_linear_i4_dx");
+    }
     const int64_t ldw = i4_ldw(K);
     const size_t wb = up256((size_t)N * ldw * 2);
     gfl::launch_dequant_i4(a, dtype == GFL_BF16, ws, ldw, st);

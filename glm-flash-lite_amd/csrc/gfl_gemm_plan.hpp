@@ -136,4 +136,33 @@ inline bool q4_exact(int M, int N, int K, int group)
     return own <= 3 + 2.5 * N * K / 4.2e6 + gm_plan(GM_NT, EP_OUT, 0, 1, M, N, K, 1).time;
 }
 
+// Its gradient with respect to the input: straight from the packed weights, by tiles of 16 tt tokens and 128 columns over `parts` of the
+// weight's rows, or (direct 0) from weights unpacked to 16 bits first, by the tile GEMM. By estimated time: a step of 256 rows takes a
+// tile 0.8, 1.1 or 1.6 us, the launch 5, a join 5 and the parts' bytes written and read at 4 TB/s; unpacking moves 2.5 bytes a weight at
+// 4.2 TB/s. Measured, us, direct and otherwise, 11008 -> 4096: 1 token 14 and 45, 24 17 and 45, 64 22 and 47, 100 28 and 49, 300 62 and 65,
+// 1001 142 and 147; 5120 -> 12288, 4096 tokens 758 and 471. 256 workgroups, not 512: 8 tokens 14 and 18.
+struct Q4DxPlan
+{
+    int direct, tt, parts;
+    int64_t ldp;
+    size_t part_bytes;
+};
+
+inline Q4DxPlan q4_dx_plan(int M, int N, int K)
+{
+    Q4DxPlan p = {};
+    if (N < 8 || M == 0) return p;   // (a lane loads 8 neighbouring rows)
+    const int blocks = (K + 127) / 128, steps = (N + 31) / 32;
+    p.tt = M <= 16 ? 1 : M <= 32 ? 2 : 4;
+    const int64_t wg = (int64_t)((M + 16 * p.tt - 1) / (16 * p.tt)) * blocks;
+    p.parts = (int)std::max<int64_t>(1, std::min<int64_t>(std::min(steps / 16, 16), 256 / wg));
+    p.ldp = ((int64_t)K + 3) / 4 * 4;
+    p.part_bytes = p.parts > 1 ? (size_t)p.parts * M * p.ldp * 4 : 0;
+    const int64_t each = ((steps + p.parts - 1) / p.parts + 7) / 8;   // a wave's
+    const double own = 5 + (double)((wg * p.parts + 255) / 256) * each * (p.tt == 1 ? 0.8 : p.tt == 2 ? 1.1 : 1.6) +
+                       (p.parts > 1 ? 5 + (double)p.part_bytes * 2 / 4e6 : 0);
+    p.direct = wg * p.parts < 1 << 22 && own <= 3 + 2.5 * N * K / 4.2e6 + gm_plan(GM_NN, EP_OUT, 0, 1, M, K, N, 1).time;
+    return p;
+}
+
 }  // namespace gfl

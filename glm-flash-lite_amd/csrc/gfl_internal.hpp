@@ -258,6 +258,8 @@ void launch_pack_i4(const uint8_t* v, int64_t ld, int N, int K, uint8_t* q, hipS
 void launch_dequant_i4(const Q4Args& a, int bf16, void* w, int64_t ldw, hipStream_t st);   // w [N][ldw], ldw a multiple of 8
 void launch_linear_i4(Q4Args& a, int bf16, void* ws, hipStream_t st);   // ws: q4_plan's part_bytes
 
+void launch_linear_i4_dx(Q4Args& a, int bf16, void* ws, hipStream_t st);   // x: dy; ws: q4_dx_plan's part_bytes
+
 // choice of experts (k_route.hip)
 constexpr int MAX_ROUTE_K = 64;   // picks, groups
 struct RouteArgs

@@ -359,6 +359,7 @@ __global__ __launch_bounds__(512, TT * NT >= 8 ? 2 : 4) void q4_tile_kernel(Q4Ar
         scales(next);
         fetch(next);
         weights(next);
+        __builtin_amdgcn_sched_barrier(0);
         float sf[NS], zf[NS];
 #pragma unroll
         for (int l = 0; l < NS; ++l)

@@ -178,7 +178,7 @@ def adjust(logits, history=None, lengths=None, prompt=None, repetition=None, fre
                 mag[b, i] += 2 * abs(v)
                 value[b, i] += v
         if allowed is not None:
-            bits = (allowed[b].long()[:, None] >> torch.arange(32) & 1).view(-1)[:V]
+            bits = (allowed[b].cpu().long()[:, None] >> torch.arange(32) & 1).view(-1)[:V]
             value[b][bits == 0] = -INF
     dt = logits.dtype
     err = torch.where(torch.isfinite(value), 4 * 2.0 ** -24 * mag, 0.0)

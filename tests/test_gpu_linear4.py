@@ -114,7 +114,9 @@ def test_many_tokens(gpu, M, N, K, group, zeros, dt):
 @pytest.mark.parametrize("dt", [F16, BF16])
 @pytest.mark.parametrize("M,N,K,group,zeros", [(1, 128, 256, 128, False), (7, 264, 1000, 64, True), (20, 33, 131, 32, False),
                                                (70, 500, 264, 128, True), (300, 1032, 520, 32, True), (1030, 2048, 2056, 128, False),
-                                               (3, 1, 1, 32, True)])
+                                               (3, 1, 1, 32, True), (1, 8, 300, 32, True), (16, 777, 384, 64, True), (24, 3001, 130, 128, True),
+                                               (33, 9000, 264, 64, False), (130, 2048, 2056, 128, False), (260, 4104, 1030, 32, True),
+                                               (400, 4096, 512, 128, False), (2, 9, 5, 128, False), (1, 7, 128, 64, True)])
 def test_gradient(gpu, M, N, K, group, zeros, dt):
     import _native
     _, q, scale, zero = _weight(N, K, group, zeros, dt, M + N)

