@@ -47,6 +47,9 @@ __device__ __forceinline__ gm_i4 q4_ones(GmF16) { return gm_i4{ 0x3C003C00, 0x3C
 // U blocks of them while it is at the U before. GB: groups of a block.
 //
 // Loads return in order, and what is loaded first is needed first: the tokens, then scales, then weights.
+//
+// Bound by the weights' bytes from 65536 channels on (9 tokens of 4096 31 us, 4.5 TB/s); one token of 5120 -> 5120 takes 6.4 us, 2.2 of
+// them a launch's, 2.8 its bytes.
 template <typename T, int GB, bool ZERO, int U, int KS, int NW>
 __global__ __launch_bounds__(NW * 64) void q4_few_kernel(Q4Args a)
 {
@@ -208,24 +211,20 @@ static void q4_few_go(Q4Args a, hipStream_t st)
                        dim3(NW * 64), lds, st, a);
 }
 
+// Two blocks on their way while a wave is at two, one where a share of few blocks would be padded: us, U = 1, 2, 3 and 4, 5120 -> 5120 1
+// token (shares of 10) 6.7, 6.4, 7.1 and 7.3, 4072 -> 11007 5 tokens (16) 10.5, 9.9, 11.4 and 10.6, 4096 -> 65536 9 tokens (32) 39.9,
+// 34.7, 36.5 and 35.0; shares of 3, 3000 -> 3000 3 tokens, 4.3 and 4.9 by 1 and 2.
 template <typename T, int GB, bool ZERO, int KS>
 static void q4_few_u(const Q4Args& a, hipStream_t st)
 {
     const int share = (a.blocks + KS - 1) / KS;
-    int best = 1;
-    for (int u = 2; u <= 6; ++u)
-        if ((share + u - 1) / u * (u + 1) <= (share + best - 1) / best * (best + 1)) best = u;   // padding, and a batch's ends
-    switch (best)
-    {
-        case 1: return q4_few_go<T, GB, ZERO, 1, KS>(a, st);
-        case 2: return q4_few_go<T, GB, ZERO, 2, KS>(a, st);
-        case 3: return q4_few_go<T, GB, ZERO, 3, KS>(a, st);
-        case 4: return q4_few_go<T, GB, ZERO, 4, KS>(a, st);
-        case 5: return q4_few_go<T, GB, ZERO, 5, KS>(a, st);
-        default: return q4_few_go<T, GB, ZERO, 6, KS>(a, st);
-    }
+    if (share % 2 == 0 || share > 6) q4_few_go<T, GB, ZERO, 2, KS>(a, st);
+    else q4_few_go<T, GB, ZERO, 1, KS>(a, st);
 }
 
+// As many waves to a tile as leave the card's 2048 or more something each: us by 1, 2, 4 and 8 waves, 4096 -> 65536 (4096 tiles) 9 tokens
+// 34, 39, 39, 40; 4096 -> 10240 (640) 16 tokens 15.5, 11.4, 11.6, 11.2; 5120 -> 5120 (320) 1 token 14.5, 9.2, 6.4, 7.4; 4096 -> 2048 (128) 2
+// tokens 11.8, 7.8, 5.4, 4.0.
 template <typename T, int GB, bool ZERO>
 static void q4_few(const Q4Args& a, hipStream_t st)
 {
@@ -239,6 +238,11 @@ static void q4_few(const Q4Args& a, hipStream_t st)
 // to registers like the wave's weights, which go from memory into its MFMAs. The sums of the tokens' inputs by groups, without
 // which a group's 16 and zero point cannot leave its sums, are formed where the tokens are put into LDS, once for all channels, and
 // enter as the MFMAs' first accumulators: a group then costs one multiply-add a result.
+//
+// A step of 64 tokens and 256 channels takes 2.0 us without its loads and the tokens' way to LDS, 2.7 with them (256 tokens of 5120 ->
+// 12288 57 us): MFMAs, LDS reads and VALU take some 0.85 each, and two waves a SIMD overlap them little. Loads two steps ahead
+// instead of one changed nothing. In 50 tokens of 12288 -> 5120 (23 us and 5 to join 12 parts) most is the ends of 4 steps: 6 parts
+// 36 us, tiles of 128 channels in 6 parts 30.
 template <typename T, int GB, bool ZERO, int TT, int NT>
 __global__ __launch_bounds__(512, TT * NT >= 8 ? 2 : 4) void q4_tile_kernel(Q4Args a)
 {
@@ -359,7 +363,7 @@ __global__ __launch_bounds__(512, TT * NT >= 8 ? 2 : 4) void q4_tile_kernel(Q4Ar
         scales(next);
         fetch(next);
         weights(next);
-        __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_sched_barrier(0);   // the compiler would issue them half a step later (2% of 16 to 64 tokens)
         float sf[NS], zf[NS];
 #pragma unroll
         for (int l = 0; l < NS; ++l)

@@ -4,11 +4,16 @@
 // The choice is that of fp64 scores: in fp32 some token in every few thousand has two experts beside the border that fp32 cannot tell
 // apart (or ties, which then go by index). It is made in fp32 first, whose keys are known to within a margin; where two picks, or the
 // last and what comes after it, lie closer, the candidates are ordered again by their fp64 keys, and where that does not settle it (a
-// border between groups, a softmax with a bias, a crowd at the border) the token is chosen for in fp64 by the whole wave. Without a bias and groups the logits themselves are
-// compared, which order as the scores do.
+// border between groups, a softmax with a bias, a crowd at the border) the token is chosen for in fp64 by the whole wave. Without a
+// bias and groups the logits themselves are compared, which order as the scores do.
 //
 // A token takes L lanes (64 / L tokens a wave). Its E experts lie in index order over the lanes, each group over lanes of its
-// own, so that among equal keys the lowest lane's lowest place is the lowest index.
+// own, so that among equal keys the lowest lane's lowest place is the lowest index. A lane sorts its keys once; a pick is then the
+// largest of the lanes' first ones, found by DPP, and a step down in one lane.
+//
+// Bound by the picks' chains of dependent instructions, not by bytes: 8192 tokens of 256 experts in 8 groups 13.3 us (bytes 1.9; some 870
+// instructions a wave, 6.5 us of issue), of which a choice in fp64 throughout made 15.9; 16384 tokens of 128 8.4 and their gradient
+// 9.3 (bytes 2.2); one token 5.0, 2.2 of them a launch's.
 #include "gfl_device.hpp"
 #include "gfl_internal.hpp"
 
