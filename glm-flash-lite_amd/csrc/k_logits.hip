@@ -115,8 +115,7 @@ __global__ __launch_bounds__(LG_T, 4) void logits_kernel(LogitsArgs a)
     if (allowed)
 #pragma unroll
         for (int k = 0; k < 2; ++k) m[k] = (uint32_t)allowed[v0 / 32 + min(tid + k * LG_T, (nv - 1) / 32)];
-    const bool early = a.early && a.L >= 4;
-    if (early) ids_at(tid * 4);   // as many as the row has room for; which of them count is seen later
+    if (a.L >= 4) ids_at(tid * 4);   // as many as the row has room for; which of them count is seen later
     // Four logits from i on, or where fewer are left the slice's last four, without a branch around the load, which would wait for the
     // loads before it (256 rows of 131,072 87 us instead of 80); the thread at the end loads its own one by one when it comes to them.
     E y[NB][4] = {};
@@ -197,7 +196,7 @@ __global__ __launch_bounds__(LG_T, 4) void logits_kernel(LogitsArgs a)
         // slice, an atomic
         for (int at = tid * 4; at < len; at += U * LG_UNIT)
         {
-            if (a.L >= 4 && !(early && at == tid * 4)) ids_at(at);
+            if (a.L >= 4 && at != tid * 4) ids_at(at);
 #pragma unroll
             for (int u = 0; u < U; ++u)
             {
@@ -294,8 +293,9 @@ static void logits_go(LogitsArgs a, hipStream_t st)
     // as many slices as fill the card, no smaller than they must be: 24 rows of 100,003 by 2,048 tokens 14.8 us, 4,096 11.6, 8,192 13.8
     const int largest = a.L ? most / 4 * LgWord<HALF>::PER : 4 * LG_UNIT;
     a.slice = (int)std::min<int64_t>(std::max<int64_t>((units + 1023) / 1024, 1) * LG_UNIT, largest);
-    a.early = a.B < 64;
     a.slices = (a.V + a.slice - 1) / a.slice;
+    // A row's slices on one XCD read its history once from memory: us with and without, 256 rows of 30,000 81 and 84, 128 52 and 57, 64 26.5 and
+    // 27.1; 16 rows, of which an XCD then has two, 18.1 and 17.8.
     a.by_xcd = a.B >= 64;
 
     const unsigned grid = (unsigned)(a.by_xcd ? (a.B + 7) / 8 * 8 : a.B) * a.slices;
