@@ -291,7 +291,7 @@ static void logits_go(LogitsArgs a, hipStream_t st)
     gm_open(reinterpret_cast<const void*>(kern), LDS_LIMIT, opened);
     const int64_t units = (int64_t)a.B * ((a.V + LG_UNIT - 1) / LG_UNIT);
     // as many slices as fill the card, no smaller than they must be: 24 rows of 100,003 by 2,048 tokens 14.8 us, 4,096 11.6, 8,192 13.8
-    const int largest = a.L ? most / 4 * LgWord<HALF>::PER : 4 * LG_UNIT;
+    const int largest = a.L ? most / 4 * LgWord<HALF>::PER : a.B < 32768 ? 4 * LG_UNIT : 8 * LG_UNIT;   // (a launch has fewer than 2^32 threads)
     a.slice = (int)std::min<int64_t>(std::max<int64_t>((units + 1023) / 1024, 1) * LG_UNIT, largest);
     a.slices = (a.V + a.slice - 1) / a.slice;
     // A row's slices on one XCD read its history once from memory: us with and without, 256 rows of 30,000 81 and 84, 128 52 and 57, 64 26.5 and

@@ -241,3 +241,27 @@ def test_streams_and_captured(gpu):
             again = _native.linear_i4(x, q, scale, zero=zero, group=32)
             assert torch.equal(y, again)
             assert torch.equal(dx, _native.linear_i4_dx(again, q, scale, 520, zero=zero, group=32))
+
+
+@pytest.mark.parametrize("M", [3, 40, 700])
+def test_gradient_captured_and_on_a_stream(gpu, M):
+    """Straight from the packed weights, in parts and not, and through weights of 16 bits; new gradients between the replays."""
+    import _native
+    N, K = (1040, 520) if M < 700 else (2056, 2048)
+    _, q, scale, zero = _weight(N, K, 64, True, BF16, 9)
+    dy = _tokens(M, N, BF16, M)
+    f = lambda: _native.linear_i4_dx(dy, q, scale, K, zero=zero, group=64)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = f()
+    s.synchronize()
+    assert torch.equal(got, f())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = f()
+    for i in range(3):
+        dy.copy_(_tokens(M, N, BF16, M + i + 1))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, f())

@@ -90,6 +90,34 @@ def test_tokens_of_long_rows(gpu):
         assert torch.equal(dx, _native.linear_i4_dx(out[:, :N].contiguous(), q, scale, K, group=group))
 
 
+@pytest.mark.parametrize("M,N,K", [(100003, 3, 5), ((1 << 22) + 5000, 40, 130)])
+def test_more_rows_than_a_launch_takes(gpu, M, N, K):
+    import _native
+    q = _native.pack_i4(_rand(N, K, dtype=torch.uint8))
+    scale = torch.full(((K + 63) // 64, N), 0.125, dtype=F16, device="cuda")
+    x = _rand(M, K, dtype=F16)
+    print("linear_i4", M, N, K, flush=True)
+    y = _native.linear_i4(x, q, scale, group=64, dtype=F32)
+    for a in (0, M // 2, M - 64):      # one part each: the same sums
+        assert torch.equal(y[a:a + 64], _native.linear_i4(x[a:a + 64], q, scale, group=64, dtype=F32))
+
+
+def test_adjust_logits_of_the_most_rows(gpu):
+    import _native
+    B, V = 65535, 1 << 20
+    if torch.cuda.mem_get_info()[0] < 170 << 30:
+        pytest.skip("less than 170 GiB free")
+    x = torch.empty((B, V), dtype=BF16, device="cuda")
+    part = torch.empty((3, V), dtype=BF16, device="cuda").normal_()
+    x[:3], x[-3:] = part, part
+    ids = torch.randint(0, V, (B, 4), dtype=torch.int32, device="cuda")
+    bias = torch.randn((B, 4), device="cuda")
+    print("adjust_logits", B, V, flush=True)
+    _native.adjust_logits(x, bias_ids=ids, bias=bias, out=x)
+    for a in (0, B - 3):
+        assert torch.equal(x[a:a + 3], _native.adjust_logits(part, bias_ids=ids[a:a + 3], bias=bias[a:a + 3]))
+
+
 def test_adjust_logits(gpu):
     """Logits and histories past 2^31 elements, rows with and without tokens."""
     import _native
