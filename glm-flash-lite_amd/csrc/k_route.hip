@@ -12,8 +12,8 @@
 // largest of the lanes' first ones, found by DPP, and a step down in one lane.
 //
 // Bound by the picks' chains of dependent instructions, not by bytes: 8192 tokens of 256 experts in 8 groups 13.3 us (bytes 1.9; some 870
-// instructions a wave, 6.5 us of issue), of which a choice in fp64 throughout made 15.9; 16384 tokens of 128 8.4 and their gradient
-// 9.3 (bytes 2.2); one token 5.0, 2.2 of them a launch's.
+// instructions a wave, 6.5 us of issue), of which a choice in fp64 throughout made 15.9; 16384 tokens of 128 7.6 and their gradient
+// 8.2 (bytes 2.2), 17.7 together with a row's weights by the library's exponentials; one token 4.8, 2.2 of them a launch's.
 #include "gfl_device.hpp"
 #include "gfl_internal.hpp"
 
@@ -140,6 +140,17 @@ __device__ __forceinline__ void rt_sort(uint32_t (&key)[N])
 __device__ __forceinline__ double rt_soft(float x, float top)
 {
     return x == top ? 1.0 : x > -INFINITY ? exp((double)x - (double)top) : 0.0;
+}
+// The same within 2^-35, for what decides nothing: a whole row's weights and their sum. Taylor's series of degree 9 over |r| <= ln 2 / 2; an
+// expert that is not there (NaN) goes to the lower end, which is 0.
+__device__ __forceinline__ double rt_soft_near(float x, float top)
+{
+    const double d = fmax((double)x - (double)top, -750.0), n = rint(d * 1.4426950408889634), r = fma(n, -0.6931471805599453, d);
+    double e = 1.0 / 362880;
+    const double c[9] = { 1.0 / 40320, 1.0 / 5040, 1.0 / 720, 1.0 / 120, 1.0 / 24, 1.0 / 6, 0.5, 1.0, 1.0 };
+#pragma unroll
+    for (int i = 0; i < 9; ++i) e = fma(e, r, c[i]);
+    return x == top ? 1.0 : ldexp(e, (int)n);
 }
 __device__ __forceinline__ double rt_sigmoid(float x) { return 1.0 / (1.0 + exp(-(double)x)); }
 __device__ __forceinline__ float rt_unkey(uint32_t k)
@@ -474,7 +485,7 @@ __global__ __launch_bounds__(RT_T) void route_experts_kernel(RouteArgs a)
     {
         double part = 0.0;
 #pragma unroll
-        for (int i = 0; i < NI; ++i) part += rt_soft(x[i], top);
+        for (int i = 0; i < NI; ++i) part += rt_soft_near(x[i], top);
         norm = rt_sum<L>(part);
     }
     // (renormalised, a softmax's own sum cancels)
@@ -548,7 +559,7 @@ __global__ __launch_bounds__(RT_T) void route_backward_kernel(RouteArgs a, const
     {
         norm = 0.0;
 #pragma unroll
-        for (int i = 0; i < NI; ++i) norm += p[i] = rt_soft(x[i], top);
+        for (int i = 0; i < NI; ++i) norm += p[i] = rt_soft_near(x[i], top);
         norm = 1.0 / rt_sum<L>(norm);
     }
     double s[64 / L], total = 0.0, dot = 0.0;
@@ -635,8 +646,8 @@ static void route_back(const RouteArgs& a, const void* dw, const int64_t* sel, v
 }
 
 // Lanes a token. 16 or 32 do the steps of a pick for 4 or 2 tokens at once, 64 hold fewer experts each and are done sooner: us by 64, 32
-// and 16 lanes, sigmoid with a bias, 288 experts, 1 token 4.7, 6.1, 8.2, 4096 8.3, 9.4, 10.2, 8192 13.3, 12.8, 13.3; softmax of 128 experts,
-// 16384 tokens 14.2, 10.0, 8.4.
+// and 16 lanes, sigmoid with a bias, 288 experts, 4096 tokens 8.0, 9.4, 9.3, 8192 12.9, 12.7, 12.7; 256 in 8 groups, 8192 tokens 14.5,
+// 12.2, 13.1; softmax of 128 experts, 16384 tokens 13.9, 9.4, 7.6.
 template <typename X>
 static int route_of(RouteArgs& a, hipStream_t st)
 {
@@ -656,8 +667,8 @@ int launch_route_experts(RouteArgs& a, hipStream_t st)
     return a.dtype == 2 ? route_of<float>(a, st) : a.dtype == 1 ? route_of<__bf16>(a, st) : route_of<_Float16>(a, st);
 }
 
-// 16 lanes a token where each then has a power of two of experts, which it stores as one vector: us by 64 and 16, 16384 tokens of 128
-// experts 14.8 and 9.3, 8192 of 288 8.9 and 16.9.
+// 16 lanes a token where each then has a power of two of experts, which it stores as one vector: us by 64 and 16, softmax, 16384 tokens of
+// 128 experts 14.0 and 8.2, sigmoid, 8192 of 256 7.8 and 8.1.
 template <typename X>
 static void route_back_of(RouteArgs& a, const void* dw, const int64_t* sel, void* dx, int64_t ldx, hipStream_t st)
 {
