@@ -9,38 +9,61 @@ namespace gfl {
 
 constexpr int Q4_T = 256;
 
-// The word of 8 values from the 4 lanes that hold two each (lane t: values 2 t and 2 t + 1): every lane gets it.
-__device__ __forceinline__ uint32_t q4_word(uint32_t even, uint32_t odd, int lane)
+// A thread per word: the row, the block and the first of its 8 inputs, in the inputs' order (so that a group's threads are neighbours),
+// and where the word lies. N * blocks * 16 is at most 2^29.
+struct Q4Place
 {
-    const int t = lane & 3;
-    uint32_t w = even << (4 * t) | odd << (16 + 4 * t);
-    w |= (uint32_t)__shfl_xor((int)w, 1);
-    w |= (uint32_t)__shfl_xor((int)w, 2);
+    uint32_t n;
+    int k;
+    int64_t at;   // bytes
+    __device__ __forceinline__ Q4Place(uint32_t id, uint32_t words)
+    {
+        n = id / words;
+        const int in = (int)(id - n * words), t = in % 16;
+        k = in * 8;
+        at = (int64_t)n * words * 4 + in / 16 * 64 + t % 4 * 16 + t / 4 * 4;
+    }
+};
+// values 0, 2, 4, 6, 1, 3, 5, 7 from the lowest bits on
+__device__ __forceinline__ uint32_t q4_word(const uint32_t (&u)[8])
+{
+    uint32_t w = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w |= u[i] << (i / 2 * 4 + i % 2 * 16);
     return w;
 }
-// byte offset in a block of the word with inputs 8 * (lane / 4) ..: j = lane / 16, g = lane / 4 % 4
-__device__ __forceinline__ int q4_at(int lane) { return lane / 4 % 4 * 16 + lane / 16 * 4; }
 
-// A wave per block of 128 inputs of a row, two inputs a lane. Symmetric: scale = max |w| / 7, value = w / scale rounded + 8. With
-// zero points: scale = (max - min) / 15 with 0 in the range, zero = -min / scale rounded, value = w / scale rounded + zero. The
-// scale is rounded to w's type first. A group that is all zeros, or whose scale rounds to zero, has scale 0; one that holds an infinity
-// or a NaN a scale of NaN: both have values of 8.
+// Symmetric: scale = max |w| / 7, value = w / scale rounded + 8. With zero points: scale = (max - min) / 15 with 0 in the range, zero =
+// -min / scale rounded, value = w / scale rounded + zero. The scale is rounded to w's type first. A group that is all zeros, or
+// whose scale rounds to zero, has scale 0; one that holds an infinity or a NaN a scale of NaN: both have values of 8. Past K there are zeros,
+// which are in every range.
+// 12288 x 5120 bf16 68 us, bound by eight divisions a thread (bytes 31; a wave a block, two inputs a lane and words joined by shuffles,
+// took 190); pack_i4 20 (bytes 19; 72).
 template <typename E>
 __global__ __launch_bounds__(Q4_T) void quant_i4_kernel(const E* w, int64_t ld, int N, int K, int group, int blocks, uint8_t* q,
                                                         E* scale, uint8_t* zero)
 {
-    const int lane = threadIdx.x % 64;
-    const int64_t at = (int64_t)blockIdx.x * (Q4_T / 64) + threadIdx.x / 64;
-    if (at >= (int64_t)N * blocks) return;
-    const int64_t n = at / blocks;
-    const int block = (int)(at % blocks), k = block * 128 + lane * 2;
-    const E* row = w + n * ld;
-    float v[2];
+    const uint32_t words = blocks * 16, id = blockIdx.x * Q4_T + threadIdx.x;
+    if (id >= N * words) return;   // (16 threads together)
+    const Q4Place p(id, words);
+    const E* row = w + p.n * ld;
+    E e[8] = {};
+    if (p.k + 8 <= K) __builtin_memcpy(e, row + p.k, sizeof e);
+    else
 #pragma unroll
-    for (int i = 0; i < 2; ++i) v[i] = k + i < K ? static_cast<float>(row[k + i]) : 0.0f;
-    uint32_t bad = !(fabsf(v[0]) < INFINITY) || !(fabsf(v[1]) < INFINITY);
-    float lo = fminf(fminf(v[0], v[1]), 0.0f), hi = fmaxf(fmaxf(v[0], v[1]), 0.0f);
-    for (int o = 1; o < group / 2; o *= 2)
+        for (int i = 0; i < 8; ++i)
+            if (p.k + i < K) e[i] = row[p.k + i];
+    float v[8], lo = 0.0f, hi = 0.0f;
+    uint32_t bad = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+    {
+        v[i] = static_cast<float>(e[i]);
+        bad |= !(fabsf(v[i]) < INFINITY);
+        lo = fminf(lo, v[i]);
+        hi = fmaxf(hi, v[i]);
+    }
+    for (int o = 1; o < group / 8; o *= 2)
     {
         lo = fminf(lo, __shfl_xor(lo, o));
         hi = fmaxf(hi, __shfl_xor(hi, o));
@@ -51,14 +74,13 @@ __global__ __launch_bounds__(Q4_T) void quant_i4_kernel(const E* w, int64_t ld, 
     const float s = static_cast<float>(se);
     const bool some = s > 0.0f && !bad;
     const float z = zero && some ? fminf(rintf(-lo / s), 15.0f) : 8.0f;
-    uint32_t u[2];
+    uint32_t u[8];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) u[i] = k + i >= K ? 0 : some ? (uint32_t)fminf(fmaxf(rintf(v[i] / s) + z, 0.0f), 15.0f) : 8;
-    const uint32_t word = q4_word(u[0], u[1], lane);
-    if (lane % 4 == 0) *reinterpret_cast<uint32_t*>(q + n * blocks * 64 + block * 64 + q4_at(lane)) = word;
-    if (lane % (group / 2) == 0 && k < K)
+    for (int i = 0; i < 8; ++i) u[i] = p.k + i >= K ? 0 : some ? (uint32_t)fminf(fmaxf(rintf(v[i] / s) + z, 0.0f), 15.0f) : 8;
+    *reinterpret_cast<uint32_t*>(q + p.at) = q4_word(u);
+    if (p.k % group == 0 && p.k < K)
     {
-        const int64_t g = (int64_t)(k / group) * N + n;
+        const int64_t g = (int64_t)(p.k / group) * N + p.n;
         scale[g] = se;
         if (zero) zero[g] = (uint8_t)z;
     }
@@ -66,24 +88,29 @@ __global__ __launch_bounds__(Q4_T) void quant_i4_kernel(const E* w, int64_t ld, 
 
 __global__ __launch_bounds__(Q4_T) void pack_i4_kernel(const uint8_t* v, int64_t ld, int N, int K, int blocks, uint8_t* q)
 {
-    const int lane = threadIdx.x % 64;
-    const int64_t at = (int64_t)blockIdx.x * (Q4_T / 64) + threadIdx.x / 64;
-    if (at >= (int64_t)N * blocks) return;
-    const int64_t n = at / blocks;
-    const int block = (int)(at % blocks), k = block * 128 + lane * 2;
-    const uint8_t* row = v + n * ld;
-    const uint32_t word = q4_word(k < K ? row[k] & 15 : 0, k + 1 < K ? row[k + 1] & 15 : 0, lane);
-    if (lane % 4 == 0) *reinterpret_cast<uint32_t*>(q + n * blocks * 64 + block * 64 + q4_at(lane)) = word;
+    const uint32_t words = blocks * 16, id = blockIdx.x * Q4_T + threadIdx.x;
+    if (id >= N * words) return;
+    const Q4Place p(id, words);
+    const uint8_t* row = v + p.n * ld;
+    uint8_t e[8] = {};
+    if (p.k + 8 <= K) __builtin_memcpy(e, row + p.k, sizeof e);
+    else
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (p.k + i < K) e[i] = row[p.k + i];
+    uint32_t u[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) u[i] = e[i] & 15;
+    *reinterpret_cast<uint32_t*>(q + p.at) = q4_word(u);
 }
 
 // (value - zero) * scale, rounded to E once, as rows of ldw elements (K up to a multiple of 8): what the
-// large products read as their weights. A thread per word.
+// large products read as their weights. A thread per word: 12288 x 5120 35 us, 4.5 TB/s.
 template <typename E>
 __global__ __launch_bounds__(Q4_T) void dequant_i4_kernel(Q4Args a, E* w, int64_t ldw)
 {
-    const int words = a.blocks * 16;
-    const int64_t at = (int64_t)blockIdx.x * Q4_T + threadIdx.x;
-    if (at >= (int64_t)a.N * words) return;
+    const uint32_t words = a.blocks * 16, at = blockIdx.x * Q4_T + threadIdx.x;   // (at most 2^29)
+    if (at >= a.N * words) return;
     const int64_t n = at / words;
     const int in = (int)(at % words), k = in / 16 * 128 + in % 4 * 32 + in / 4 % 4 * 8;
     if (k >= a.K) return;
@@ -107,7 +134,7 @@ void launch_quant_i4(const void* w, int64_t ld, int bf16, int N, int K, int grou
                      hipStream_t st)
 {
     const int blocks = (K + 127) / 128;
-    const dim3 grid(q4_grid((int64_t)N * blocks, Q4_T / 64)), block(Q4_T);
+    const dim3 grid(q4_grid((int64_t)N * blocks * 16, Q4_T)), block(Q4_T);
     if (bf16)
         hipLaunchKernelGGL(quant_i4_kernel<__bf16>, grid, block, 0, st, static_cast<const __bf16*>(w), ld, N, K, group, blocks, q,
                            static_cast<__bf16*>(scale), zero);
@@ -119,7 +146,7 @@ void launch_quant_i4(const void* w, int64_t ld, int bf16, int N, int K, int grou
 void launch_pack_i4(const uint8_t* v, int64_t ld, int N, int K, uint8_t* q, hipStream_t st)
 {
     const int blocks = (K + 127) / 128;
-    hipLaunchKernelGGL(pack_i4_kernel, dim3(q4_grid((int64_t)N * blocks, Q4_T / 64)), dim3(Q4_T), 0, st, v, ld, N, K, blocks, q);
+    hipLaunchKernelGGL(pack_i4_kernel, dim3(q4_grid((int64_t)N * blocks * 16, Q4_T)), dim3(Q4_T), 0, st, v, ld, N, K, blocks, q);
 }
 
 void launch_dequant_i4(const Q4Args& a, int bf16, void* w, int64_t ldw, hipStream_t st)
