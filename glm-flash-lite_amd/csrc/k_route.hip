@@ -180,10 +180,10 @@ __device__ __forceinline__ void rt_row(const X* p, int n, float (&x)[NI])   // n
     for (int i = 0; i < NI; ++i) x[i] = i < n ? static_cast<float>(e[i]) : -INFINITY;
 }
 
-// Which groups a lane's group is among the kept ones, by their worth (the sum of the one or two largest keys, given as v1 >= v2; -inf:
-// none): how many come before it.
+// Which groups a lane's group is among the kept ones, by their worth (the sum of the one or two largest keys, given as v1 >= v2 of the
+// lane's experts and left as the group's; -inf: none): how many come before it.
 template <int L, typename V>
-__device__ __forceinline__ int rt_group(const RouteArgs& a, int lpg, int lane, int g, V v1, V v2, V& worth)
+__device__ __forceinline__ int rt_group(const RouteArgs& a, int lpg, int lane, int g, V& v1, V& v2, V& worth)
 {
     for (int w = 1; w < lpg; w *= 2)
     {
@@ -216,6 +216,8 @@ enum
 // Margins. Sigmoid: the argument's rounding and v_exp_f32 make 1.5 |x| 2^-24 + 2^-23 of exp(-x), which counts s (1 - s) times, 1 + exp
 // and v_rcp_f32 1.5 2^-23 of s: below 2^-22. Softmax: the same of an exponential, 32 additions and a reciprocal of the sum: below 2^-18.
 // Adding the bias takes 2^-24 of the key, the places up to PLACE 2^-23. Two keys, twice each; 2^-20 leaves as much again.
+// A group's worth is off by its keys' errors, and their sum's rounding is at most 2^-24 of |v1| + |v2|, beside which the worth itself may be
+// small (one expert forced by its bias, the others held off): margin + 2^-22 (|v1| + |v2|) is twice that.
 template <int L, int NI, bool FULL>
 __device__ __forceinline__ int rt_choose(const RouteArgs& a, int lane, int sub, int g, int e0, const float (&x)[NI], const float (&bias)[NI],
                                          float top, int* pick, bool exact_keys, int& count)
@@ -259,9 +261,12 @@ __device__ __forceinline__ int rt_choose(const RouteArgs& a, int lane, int sub, 
             }
             kept = rt_group<L, float>(a, a.lpg, lane, g, v1, v2, worth) < a.top_groups;
             const bool mine = g < a.groups;
-            const float in = -rt_unkey(rt_max<L>(mine && kept ? rt_key(-worth) : 0)), out = rt_unkey(rt_max<L>(mine && !kept ? rt_key(worth) : 0));
-            // (a group that has nothing is worth -inf, and no key of it is compared)
-            if (out > -INFINITY && !(in - out > 2.0f * margin + fabsf(out) * 0x1p-20f)) state = RT_WIDE;
+            // (a group that has nothing is worth -inf, and no key of it is compared; of infinite sums nothing is known)
+            const float off = v1 > -INFINITY ? margin + (fabsf(v1) + (a.group_best == 2 && v2 > -INFINITY ? fabsf(v2) : 0.0f)) * 0x1p-22f : 0.0f;
+            const float least = worth - off, most = worth + off;
+            const float in = -rt_unkey(rt_max<L>(mine && kept ? rt_key(least == least ? -least : INFINITY) : 0)),
+                        out = rt_unkey(rt_max<L>(mine && !kept ? rt_key(most == most ? most : INFINITY) : 0));
+            if (out > -INFINITY && !(in > out)) state = RT_WIDE;
         }
 #pragma unroll
         for (int i = 0; i < NI; ++i) key[i] = kept ? rt_key(s[i]) : 0;

@@ -1,0 +1,51 @@
+"""The general router where its choice is close or its logits are extreme, against the 64-bit definition by whole tensors."""
+import pytest
+
+import serving_ref as S
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+F16, BF16, F32 = torch.float16, torch.bfloat16, torch.float32
+INF, NAN = float("inf"), float("nan")
+
+
+def _gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def _first(v, n):
+    """Indices of the n largest along the last dimension, equal ones by index."""
+    return torch.sort(v, dim=-1, descending=True, stable=True)[1][..., :n]
+
+
+def _kept(key, groups, top_groups, group_best):
+    """Which experts belong to the kept groups, by fp64 keys without -inf."""
+    k = key.view(key.shape[0], groups, -1)
+    worth = torch.sort(k, dim=2, descending=True)[0][:, :, :group_best].sum(2)
+    kept = torch.zeros_like(worth, dtype=torch.bool).scatter_(1, _first(worth, top_groups), True)
+    return kept[:, :, None].expand_as(k).reshape(key.shape)
+
+
+@pytest.mark.parametrize("score", ["sigmoid", "softmax"])
+@pytest.mark.parametrize("group_best", [1, 2])
+@pytest.mark.parametrize("M", [300, 6200, 12300])
+@pytest.mark.parametrize("forced", [0.1, 16.0, 64.0, 1000.0, 10000.0, 3e38])
+def test_close_groups_with_large_biases(gpu, M, forced, group_best, score):
+    """Groups of nearly the same keys in which one expert is forced by its bias and the rest are held off, so that a group's worth is a
+    small difference of large keys: fp32 orders some of them otherwise than fp64."""
+    import _native
+    E, groups, top, topk = 32, 4, 2, 4
+    g = _gen(M + int(min(forced, 1e6)))
+    step = max(min(forced, 1e4) * 2.0 ** -20, 2.0 ** -18)
+    x = torch.randn((M, 8), generator=g).repeat(1, groups) + step * torch.randn((M, E), generator=g)
+    b = torch.full((E,), -forced)
+    b[::8] = forced
+    if forced > 1e30:
+        b[::8] *= -1.0           # both of a group's best: their fp32 sum is not finite
+    p = torch.sigmoid(x.double()) if score == "sigmoid" else torch.softmax(x.double(), 1)
+    key = p + b.double()
+    kept = _kept(key, groups, top, group_best)
+    want = _first(torch.where(kept, key, -INF), topk)
+    sel, _ = _native.route_experts(x.cuda(), topk, bias=b.cuda(), score=score, groups=groups, top_groups=top, group_best=group_best)
+    wrong = (sel.cpu() != want).any(1)
+    assert not wrong.any(), f"{int(wrong.sum())} of {M}"
