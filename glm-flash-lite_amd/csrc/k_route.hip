@@ -526,12 +526,14 @@ __global__ __launch_bounds__(RT_T) void route_experts_kernel(RouteArgs a)
 //   sigmoid: dx = ds s (1 - s) at the picks, 0 elsewhere;
 //   softmax p: dx = p (ds - sum_i ds_i p_i) everywhere; with renormalisation that sum is 0 and only ratios of the picks' exponentials
 //   enter, so the row is not read.
+// Where one expert has nearly the whole row, ds and the sum agree in all but a few bits of its own dx: they stay in fp64 up to the result, and
+// the picks' p are those of the row's pass (near exponentials are still a softmax's, so that what cancels is the same on both sides).
 template <typename X, int L, int NI>
 __global__ __launch_bounds__(RT_T) void route_backward_kernel(RouteArgs a, const void* dw, const int64_t* sel, X* dx, int64_t ldx)
 {
     constexpr int TOK = RT_T / L;
     __shared__ int picks[TOK][MAX_ROUTE_K];
-    __shared__ float grads[TOK][MAX_ROUTE_K];
+    __shared__ double grads[TOK][MAX_ROUTE_K];
     const int sub = threadIdx.x % L, tok = threadIdx.x / L;
     const int64_t t = (int64_t)blockIdx.x * TOK + tok, tc = min(t, (int64_t)a.M - 1);
     const X* row = static_cast<const X*>(a.logits) + tc * a.ld;
@@ -573,7 +575,7 @@ __global__ __launch_bounds__(RT_T) void route_backward_kernel(RouteArgs a, const
     {
         s[r] = 0.0;
         if (r * L >= a.topk) continue;
-        if (es[r] >= 0) s[r] = a.softmax ? rt_soft(xs[r], top) * norm : rt_sigmoid(xs[r]);
+        if (es[r] >= 0) s[r] = dense ? rt_soft_near(xs[r], top) * norm : a.softmax ? rt_soft(xs[r], top) : rt_sigmoid(xs[r]);
         total += s[r];
         dot += s[r] * ((double)a.scale * up[r]);
     }
@@ -588,24 +590,22 @@ __global__ __launch_bounds__(RT_T) void route_backward_kernel(RouteArgs a, const
         double ds = (double)a.scale * up[r];
         if (a.renorm) ds = (ds - dot * by) * by;
         picks[tok][j] = es[r];
-        // softmax: what is added to -p dot; sigmoid: s (1 - s) = s sigmoid(-x)
-        grads[tok][j] = es[r] < 0 ? 0.f : (float)(ds * s[r] * (a.softmax ? 1.0 : rt_sigmoid(-xs[r])));
+        // dense: ds, of the whole row's p (ds - dot); else the pick's dx (sigmoid: s (1 - s) = s sigmoid(-x))
+        grads[tok][j] = es[r] < 0 ? 0.0 : dense ? ds : ds * s[r] * (a.softmax ? 1.0 : rt_sigmoid(-xs[r]));
     }
     __syncthreads();
     if (t >= a.M) return;
-    float v[NI];
-#pragma unroll
-    for (int i = 0; i < NI; ++i) v[i] = dense ? (float)(-dot * (p[i] * norm)) : 0.f;
+    double v[NI] = {};
     for (int j = 0; j < a.topk; ++j)
     {
         const int e = picks[tok][j] - e0;
-        const float d = grads[tok][j];
+        const double d = grads[tok][j];
 #pragma unroll
-        for (int i = 0; i < NI; ++i) v[i] += e == i && i < n ? d : 0.f;
+        for (int i = 0; i < NI; ++i) v[i] += e == i && i < n ? d : 0.0;
     }
     X o[NI];
 #pragma unroll
-    for (int i = 0; i < NI; ++i) o[i] = static_cast<X>(v[i]);
+    for (int i = 0; i < NI; ++i) o[i] = static_cast<X>((float)(dense ? p[i] * norm * (v[i] - dot) : v[i]));
     X* out = dx + t * ldx + e0;
     if (n == NI) __builtin_memcpy(out, o, sizeof o);
     else

@@ -49,3 +49,31 @@ def test_close_groups_with_large_biases(gpu, M, forced, group_best, score):
     sel, _ = _native.route_experts(x.cuda(), topk, bias=b.cuda(), score=score, groups=groups, top_groups=top, group_best=group_best)
     wrong = (sel.cpu() != want).any(1)
     assert not wrong.any(), f"{int(wrong.sum())} of {M}"
+
+
+@pytest.mark.parametrize("dt,wt", [(F32, F32), (BF16, F32), (F16, BF16)])
+@pytest.mark.parametrize("lead", [0.0, 12.0, 16.0, 20.0, 25.0, 40.0])
+@pytest.mark.parametrize("M,E,topk", [(70, 128, 8), (8200, 128, 8), (5, 1000, 64)])
+def test_gradient_of_rows_that_few_experts_lead(gpu, M, E, topk, lead, dt, wt):
+    """Softmax without renormalisation: dx = p (ds - sum p ds) = p_i sum_j p_j (ds_i - ds_j), the second form without cancellation. Of
+    every three rows, one is led by one expert, one by all the picks, whose dw are then equal."""
+    import _native
+    g = _gen(M + E)
+    x = torch.randn((M, E), generator=g)
+    x[::3, 17] += lead
+    x[1::3, 3:3 + topk] += lead
+    x = x.to(dt)
+    dw = torch.randn((M, topk), generator=g)
+    dw[1::3] = dw[1::3, :1]
+    dw = dw.to(wt)
+    sel, _ = _native.route_experts(x.cuda(), topk, score="softmax", renorm=False, scale=16.0)
+    got = _native.route_experts_backward(dw.cuda(), x.cuda(), sel, score="softmax", renorm=False, scale=16.0)
+    rows = torch.arange(0, M, max(1, M // 100))
+    sel, got, dw = sel.cpu()[rows], got.cpu()[rows], dw.double()[rows] * 16
+    p = torch.softmax(x[rows].double(), 1)
+    ds = torch.zeros_like(p).scatter_(1, sel, dw)
+    diff = ds[:, :, None] - ds[:, None, :]
+    value, spread = p * (diff * p[:, None, :]).sum(2), p * (diff.abs() * p[:, None, :]).sum(2)
+    # a softmax of exponentials within 2^-35 of theirs, its sum and the weighted one in fp64; then fp32, then the type
+    err = 2.0 ** -32 * spread + (E + topk + 10) * 2.0 ** -53 * p * ((p * ds.abs()).sum(1, keepdim=True) + ds.abs())
+    S.same(got, value, err + (S.half_step(dt) + 2.0 ** -24) * (value.abs() + err) + S.tiny(dt) + 2.0 ** -150, "dlogits")
