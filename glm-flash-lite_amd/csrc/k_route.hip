@@ -556,6 +556,7 @@ __global__ __launch_bounds__(RT_T) void route_backward_kernel(RouteArgs a, const
         if (j < a.topk) up[r] = rt_load(dw, a.wdtype, tc * a.topk + j);
         es[r] = e >= 0 && e < a.E ? (int)e : -1;
         if (es[r] >= 0) xs[r] = static_cast<float>(row[es[r]]);
+        else up[r] = 0.f;   // (a missing pick's may be anything)
         k = max(k, rt_key(xs[r]));
     }
     if (dense)

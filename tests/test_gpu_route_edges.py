@@ -77,3 +77,24 @@ def test_gradient_of_rows_that_few_experts_lead(gpu, M, E, topk, lead, dt, wt):
     # a softmax of exponentials within 2^-35 of theirs, its sum and the weighted one in fp64; then fp32, then the type
     err = 2.0 ** -32 * spread + (E + topk + 10) * 2.0 ** -53 * p * ((p * ds.abs()).sum(1, keepdim=True) + ds.abs())
     S.same(got, value, err + (S.half_step(dt) + 2.0 ** -24) * (value.abs() + err) + S.tiny(dt) + 2.0 ** -150, "dlogits")
+
+
+@pytest.mark.parametrize("score", ["sigmoid", "softmax"])
+@pytest.mark.parametrize("renorm", [True, False])
+@pytest.mark.parametrize("M", [5, 8200])
+def test_gradient_does_not_read_the_weights_of_missing_picks(gpu, M, score, renorm):
+    """NaN and infinities in dw where sel is -1 or an id that no expert has: as if they were 0."""
+    import _native
+    g = _gen(M)
+    x = torch.randn((M, 32), generator=g)
+    x[::2, 3:] = -INF
+    x, dw = x.cuda(), torch.randn((M, 6), generator=g).cuda()
+    sel, _ = _native.route_experts(x, 6, score=score, renorm=renorm)
+    assert bool((sel[::2, 3:] == -1).all())
+    odd = sel.clone()
+    odd[1, 2], odd[1, 4] = 32, -9
+    zero = torch.where((odd < 0) | (odd > 31), 0.0, dw)
+    bad = zero.clone()
+    bad[::2, 3], bad[::2, 4], bad[::2, 5], bad[1, 2], bad[1, 4] = NAN, INF, -INF, NAN, INF
+    a, b = (_native.route_experts_backward(t, x, odd, score=score, renorm=renorm) for t in (zero, bad))
+    assert bool(torch.isfinite(a).all()) and torch.equal(a, b)
