@@ -5,7 +5,7 @@
 // apart (or ties, which then go by index). It is made in fp32 first, whose keys are known to within a margin; where two picks, or the
 // last and what comes after it, lie closer, the candidates are ordered again by their fp64 keys, and where that does not settle it (a
 // border between groups, a softmax with a bias, a crowd at the border) the token is chosen for in fp64 by the whole wave. Without a
-// bias and groups the logits themselves are compared, which order as the scores do.
+// bias the logits themselves are compared, which order as the scores do and stay apart where those saturate; groups go by the scores.
 //
 // A token takes L lanes (64 / L tokens a wave). Its E experts lie in index order over the lanes, each group over lanes of its
 // own, so that among equal keys the lowest lane's lowest place is the lowest index. A lane sorts its keys once; a pick is then the
@@ -158,6 +158,12 @@ __device__ __forceinline__ float rt_unkey(uint32_t k)
     return k == 0 ? -INFINITY : __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k);
 }
 
+// What experts of the kept groups are compared by without a bias: the logit. Beside a softmax's +inf the others' scores are all 0.
+__device__ __forceinline__ float rt_rank(const RouteArgs& a, float x, float top)
+{
+    return a.softmax && top == INFINITY && x > -INFINITY ? (x == top ? 1.0f : 0.0f) : x;
+}
+
 __device__ __forceinline__ float rt_exp(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504f); }
 
 // the lanes of a token in a ballot
@@ -226,6 +232,7 @@ __device__ __forceinline__ int rt_choose(const RouteArgs& a, int lane, int sub, 
     const float margin = a.softmax ? 0x1p-16f : 0x1p-20f;
     constexpr float STEP = (PLACE + 3) * 0x1p-23f;
     int state = RT_SURE;
+    const bool by_score = FULL && a.bias;
     uint32_t key[NI];
     if constexpr (FULL)
     {
@@ -269,7 +276,7 @@ __device__ __forceinline__ int rt_choose(const RouteArgs& a, int lane, int sub, 
             if (out > -INFINITY && !(in > out)) state = RT_WIDE;
         }
 #pragma unroll
-        for (int i = 0; i < NI; ++i) key[i] = kept ? rt_key(s[i]) : 0;
+        for (int i = 0; i < NI; ++i) key[i] = kept ? rt_key(by_score ? s[i] : rt_rank(a, x[i], top)) : 0;
     }
     else
 #pragma unroll
@@ -280,7 +287,7 @@ __device__ __forceinline__ int rt_choose(const RouteArgs& a, int lane, int sub, 
     const int most = min(a.topk + RT_MORE, L);
     uint32_t least = 0, mine = 0;   // the last pick's key; lane i: candidate i's
     auto close = [&](uint32_t above, uint32_t m) {
-        if constexpr (!FULL) return m != 0 && above == m;
+        if (!by_score) return m != 0 && above == m;
         const float u = rt_unkey(above), v = rt_unkey(m);
         return m != 0 && !(u - v > margin + fmaxf(fabsf(u), fabsf(v)) * STEP);
     };
@@ -320,7 +327,7 @@ __device__ __forceinline__ int rt_choose(const RouteArgs& a, int lane, int sub, 
         const bool c = sub > 0 && sub < count && close(above, mine);
         if (rt_lanes<L>(__ballot(c), lane)) state |= RT_ORDER;
     }
-    return state & RT_WIDE || (state && FULL && a.softmax) ? RT_WIDE : state;
+    return state & RT_WIDE || (state && by_score && a.softmax) ? RT_WIDE : state;
 }
 
 // The choice in fp64. A pick is the maximum of the lanes' best keys: first of the upper 32 bits, then, where two lanes share those, of
@@ -353,7 +360,7 @@ __device__ __forceinline__ void rt_choose_wide(const RouteArgs& a, int lpg, int 
         {
             if (a.bias && i < n) s[i] += (double)a.bias[e0 + i];
             const uint64_t k = x[i] > -INFINITY ? rt_key(s[i]) : 0;
-            hi[i] = (uint32_t)(k >> 32), lo[i] = (uint32_t)k;
+            hi[i] = a.bias ? (uint32_t)(k >> 32) : rt_key(rt_rank(a, x[i], top)), lo[i] = a.bias ? (uint32_t)k : 0;
             const double v = k ? s[i] : NONE;
             v2 = fmax(v2, fmin(v, v1));
             v1 = fmax(v1, v);
@@ -408,7 +415,7 @@ __device__ __forceinline__ void rt_choose_wide(const RouteArgs& a, int lpg, int 
     }
 }
 
-// NI: experts of a lane. FULL: the keys are scores + bias (a bias, or groups); else the logits.
+// NI: experts of a lane. FULL: scores are formed (for a bias, or groups).
 template <typename X, int L, int NI, bool FULL>
 __global__ __launch_bounds__(RT_T) void route_experts_kernel(RouteArgs a)
 {
@@ -444,7 +451,7 @@ __global__ __launch_bounds__(RT_T) void route_experts_kernel(RouteArgs a)
     }
     int* pick = picks[tok];
     int count;
-    const int state = rt_choose<L, NI, FULL>(a, lane, sub, g, e0, x, bias, top, pick, !FULL && sizeof(X) == 2, count);
+    const int state = rt_choose<L, NI, FULL>(a, lane, sub, g, e0, x, bias, top, pick, (!FULL || !a.bias) && sizeof(X) == 2, count);
     if (__any(state == RT_ORDER))
     {
         asm volatile("" ::: "memory");   // (LDS is read and written in order within a wave)
@@ -453,8 +460,8 @@ __global__ __launch_bounds__(RT_T) void route_experts_kernel(RouteArgs a)
         if (e >= 0)
         {
             const float v = static_cast<float>(row[e]);
-            if constexpr (FULL) key = rt_key(rt_sigmoid(v) + (a.bias ? (double)a.bias[e] : 0.0));
-            else key = rt_key((double)v);
+            if (FULL && a.bias) key = rt_key(rt_sigmoid(v) + (double)a.bias[e]);
+            else key = rt_key((double)(FULL ? rt_rank(a, v, top) : v));
         }
         keys[tok][sub] = key;
         asm volatile("" ::: "memory");

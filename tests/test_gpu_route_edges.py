@@ -98,3 +98,31 @@ def test_gradient_does_not_read_the_weights_of_missing_picks(gpu, M, score, reno
     bad[::2, 3], bad[::2, 4], bad[::2, 5], bad[1, 2], bad[1, 4] = NAN, INF, -INF, NAN, INF
     a, b = (_native.route_experts_backward(t, x, odd, score=score, renorm=renorm) for t in (zero, bad))
     assert bool(torch.isfinite(a).all()) and torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dt", [F32, F16])
+@pytest.mark.parametrize("score", ["sigmoid", "softmax"])
+@pytest.mark.parametrize("M", [9, 6200, 12300])
+def test_saturated_scores_go_by_the_logit_with_and_without_groups(gpu, M, score, dt):
+    """Logits whose fp64 scores are equal (sigmoid 1 from 37 on, softmax 0 some 745 below the largest) are still in order. The first
+    group has the largest and is kept, so that its choice is that of a router of its experts alone."""
+    import _native
+    g = _gen(M)
+    x = torch.randn((M, 32), generator=g)
+    if score == "sigmoid":
+        x[:, :16] = x[:, :16] * 3 + 60
+    else:
+        x[:, 1:16] = x[:, 1:16] * 30 - 2000
+        x[:, 16:] -= 4000
+        x[:, 0] = 0
+    x[::3, 2], x[::3, 9], x[1::3, 4], x[2::3, 5] = x[::3, 11], x[::3, 11], -INF, NAN
+    x = x.to(dt)
+    v = torch.where(x > -INF, x.double(), -INF)[:, :16]
+    for topk in (1, 4, 12):
+        sel, _ = _native.route_experts(x.cuda(), topk, score=score, groups=2, top_groups=1)
+        assert torch.equal(sel.cpu(), _first(v, topk))
+        whole, _ = _native.route_experts(x.cuda(), topk, score=score)
+        assert torch.equal(whole, sel)
+    one = torch.full((1, 8), -9.0)
+    one[0, 0], one[0, 1] = 40.0, 60.0
+    assert _native.route_experts(one.cuda(), 1, groups=2, top_groups=1)[0].tolist() == [[1]]
