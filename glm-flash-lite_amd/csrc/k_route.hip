@@ -500,19 +500,25 @@ __global__ __launch_bounds__(RT_T) void route_experts_kernel(RouteArgs a)
         for (int i = 0; i < NI; ++i) part += rt_soft_near(x[i], top);
         norm = rt_sum<L>(part);
     }
-    // (renormalised, a softmax's own sum cancels)
     double w[64 / L], sum = 0.0;
+    float xs[64 / L];
+    uint32_t k = 0;
 #pragma unroll
     for (int r = 0; r < 64 / L; ++r)
     {
-        w[r] = 0.0;
+        xs[r] = -INFINITY;
         if (r * L >= a.topk) continue;
         const int j = r * L + sub, e = j < a.topk ? pick[j] : -1;
-        if (e >= 0)
-        {
-            const float v = static_cast<float>(row[e]);
-            w[r] = a.softmax ? rt_soft(v, top) : rt_sigmoid(v);
-        }
+        if (e >= 0) xs[r] = static_cast<float>(row[e]);
+        k = max(k, rt_key(xs[r]));
+    }
+    // Renormalised, a softmax's own sum cancels: its exponentials are taken from the picks' largest logit, as the gradient's are, so that picks
+    // far below the row's (a bias can choose them) have weights too.
+    if (a.softmax && a.renorm) top = rt_unkey(rt_max<L>(k));
+#pragma unroll
+    for (int r = 0; r < 64 / L; ++r)
+    {
+        w[r] = xs[r] > -INFINITY ? a.softmax ? rt_soft(xs[r], top) : rt_sigmoid(xs[r]) : 0.0;
         sum += w[r];
     }
     if (a.renorm) norm = rt_sum<L>(sum);

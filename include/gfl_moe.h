@@ -349,7 +349,8 @@ int gfl_i4_workspace(int dtype, int out_dtype, int M, int N, int K, int group, s
  *   groups    the E experts in `groups` equal parts, in order; a part is worth the sum of its group_best (1 or 2) largest keys,
  *             and only the top_groups worthiest are chosen from (1 group: all)
  *   sel       the topk largest keys, in descending order
- *   w         scale * s, with renorm divided by the sum of the picks' s (0 where that is 0); fp16, bf16 or fp32
+ *   w         scale * s, with renorm divided by the sum of the picks' s (a softmax's: only ratios of the picks; 0 where
+ *             nothing is picked or fp64 sigmoids are all 0); fp16, bf16 or fp32
  * Scores, keys and sums are fp64; equal keys go to the lower index. Without a bias experts are compared by their logits, which differ
  * where fp64 scores no longer do (with groups, beside +inf in a softmax, the others are equal); groups go by the keys. Experts whose logit is -inf or NaN, or whose bias is, are never picked: where fewer than topk are left, the rest
  * of sel is -1 with weight 0, which the expert calls skip. In a softmax with logits of +inf those share the row.

@@ -126,3 +126,26 @@ def test_saturated_scores_go_by_the_logit_with_and_without_groups(gpu, M, score,
     one = torch.full((1, 8), -9.0)
     one[0, 0], one[0, 1] = 40.0, 60.0
     assert _native.route_experts(one.cuda(), 1, groups=2, top_groups=1)[0].tolist() == [[1]]
+
+
+@pytest.mark.parametrize("M", [4, 6200, 12300])
+def test_renormalised_softmax_of_picks_far_below_the_largest(gpu, M):
+    """A bias that holds off the experts that lead by 2000: weights and gradients are those of a softmax of the picks alone."""
+    import _native
+    g = _gen(M)
+    x = torch.randn((M, 40), generator=g)
+    x[:, 30:] += 2000
+    b = torch.zeros(40)
+    b[30:], b[:30] = -5.0, torch.arange(30) * 1e-3
+    dw = torch.randn((M, 6), generator=g)
+    sel, w = _native.route_experts(x.cuda(), 6, bias=b.cuda(), score="softmax", dtype=F32)
+    dx = _native.route_experts_backward(dw.cuda(), x.cuda(), sel, score="softmax")
+    assert torch.equal(sel.cpu(), torch.arange(29, 23, -1).expand(M, -1))
+    p = torch.softmax(x[:, 24:30].double().flip(1), 1)
+    S.same(w, p, (2.0 ** -24 + 2.0 ** -48) * p, "w")
+    d = dw.double()
+    want = torch.zeros((M, 40), dtype=torch.float64)
+    want[:, 24:30] = (p * (d - (p * d).sum(1, keepdim=True))).flip(1)
+    err = torch.zeros_like(want)
+    err[:, 24:30] = (2.0 ** -48 * p * (d.abs() + (p * d.abs()).sum(1, keepdim=True))).flip(1)
+    S.same(dx, want, err + 2.0 ** -24 * (want.abs() + err) + 2.0 ** -150, "dlogits")
