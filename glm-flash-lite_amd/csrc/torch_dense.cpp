@@ -71,6 +71,12 @@ T* addr(const OptTensor& t)
     return t ? static_cast<T*>(t->data_ptr()) : nullptr;
 }
 
+// The caller's own output has other values now: a backward pass that saved the old ones is refused.
+void written(const OptTensor& out)
+{
+    if (out && !out->is_inference()) out->unsafeGetTensorImpl()->bump_version();
+}
+
 Tensor workspace(size_t bytes, const Tensor& ref)
 {
     return bytes ? at::empty({ static_cast<int64_t>(bytes) }, ref.options().dtype(at::kByte)) : Tensor();
@@ -119,6 +125,7 @@ std::tuple<Tensor, Tensor, Tensor> ffn_forward(const Tensor& x, const Tensor& wg
     check_rc(gfl_ffn_forward(x.data_ptr(), r.ld, wg.data_ptr(), wu.data_ptr(), wd.data_ptr(), f.code, r.n, f.H, f.I,
                              static_cast<float>(act_limit), static_cast<float*>(addr(g)), static_cast<float*>(addr(u)),
                              y.data_ptr(), o.ld, code_of(y.scalar_type()), accumulate, addr(ws), need, on.stream));
+    written(out);
     return { y, g, u };
 }
 
@@ -215,6 +222,7 @@ Tensor gemm_i8(const Tensor& a, const Tensor& sa, const Tensor& b, const Tensor&
     const Tensor ws = workspace(need, a);
     check_rc(gfl_gemm_i8(a.data_ptr<int8_t>(), r.ld, sa.data_ptr<float>(), b.data_ptr<int8_t>(), w.ld, sb.data_ptr<float>(),
                          r.n, w.n, K, y.data_ptr(), o.ld, code_of(y.scalar_type()), addr(ws), need, on.stream));
+    written(out);
     return y;
 }
 
@@ -231,6 +239,7 @@ Tensor linear_i8(const Tensor& x, const Tensor& b, const Tensor& sb, const OptTe
     const Tensor ws = workspace(need, x);
     check_rc(gfl_linear_i8(x.data_ptr(), r.ld, code, b.data_ptr<int8_t>(), w.ld, sb.data_ptr<float>(), r.n, w.n, K, y.data_ptr(),
                            o.ld, code_of(y.scalar_type()), addr(ws), need, on.stream));
+    written(out);
     return y;
 }
 
@@ -311,6 +320,7 @@ Tensor linear_i4(const Tensor& x, const Tensor& q, const Tensor& scale, const Op
     const Tensor ws = workspace(need, x);
     check_rc(gfl_linear_i4(x.data_ptr(), r.ld, code, q.data_ptr<uint8_t>(), scale.data_ptr(), w.scale_code, addr<uint8_t>(zero), r.n,
                            w.N, w.K, w.group, y.data_ptr(), o.ld, ycode, addr(ws), need, on.stream));
+    written(out);
     return y;
 }
 
@@ -423,6 +433,7 @@ Tensor adjust_logits(const Tensor& logits, const OptTensor& history, const OptTe
                                L ? addr<float>(repetition) : nullptr, L ? addr<float>(frequency) : nullptr,
                                L ? addr<float>(presence) : nullptr, addr<int32_t>(bias_ids), bi.ld, addr<float>(bias), bv.ld,
                                size_of(what, n), addr<int32_t>(allowed), m.ld, y.data_ptr(), o.ld, on.stream));
+    written(out);
     return y;
 }
 
