@@ -19,6 +19,40 @@ bool words(const void* p, int64_t ld_bytes)
     return reinterpret_cast<uintptr_t>(p) % 4 == 0 && ld_bytes % 4 == 0 && ld_bytes >= 16;
 }
 
+// rows of a matrix in memory: n of them, `bytes` long, ld (elements of `size` bytes) apart
+struct Span
+{
+    uintptr_t at;
+    int64_t n, bytes, step;
+    Span(const void* p, int64_t rows, int64_t cols, int64_t ld, int size)
+        : at(reinterpret_cast<uintptr_t>(p)), n(rows), bytes(cols * size), step(ld * size)
+    {
+    }
+    uintptr_t row(int64_t i) const { return at + i * step; }
+    uintptr_t end() const { return row(n - 1) + bytes; }
+};
+
+// Whether two matrices (of one row or more, whose own rows do not overlap) share a byte. Matrices beside each other in rows of one buffer
+// do not.
+bool overlap(const Span& a, const Span& b)
+{
+    if (a.end() <= b.at || b.end() <= a.at) return false;
+    if (a.step == b.step && a.step > 0)
+    {
+        const int64_t d = (int64_t)(b.at - a.at), r = (d % a.step + a.step) % a.step;
+        if (r >= a.bytes && r + b.bytes <= a.step) return false;
+    }
+    for (int64_t i = 0, j = 0; i < a.n && j < b.n;)
+    {
+        if (a.row(i) + a.bytes <= b.row(j)) ++i;
+        else if (b.row(j) + b.bytes <= a.row(i)) ++j;
+        else return true;
+    }
+    return false;
+}
+
+int size_of(int dtype) { return dtype == GFL_F32 ? 4 : 2; }
+
 int check_launch(const char* what)
 {
     const hipError_t e = hipGetLastError();
@@ -465,6 +499,7 @@ int gfl_linear_i4(const void* x, int64_t ldx, int dtype, const uint8_t* q, const
     gfl_i4_workspace(dtype, out_dtype, M, N, K, group, &need, nullptr);
     if (need && (!ws || ws_bytes < need || reinterpret_cast<uintptr_t>(ws) % 16))
         return api_fail(GFL_EINVAL, "gfl_linear_i4: workspace missing, too small or not 16-byte aligned");
+    if (overlap(Span(x, M, K, ldx, 2), Span(out, M, N, ldo, size_of(out_dtype)))) return api_fail(GFL_EINVAL, "gfl_linear_i4: out overlaps x");
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     if (i4_exact(M, N, K, group, dtype, out_dtype))
     {
@@ -509,6 +544,7 @@ int gfl_linear_i4_dx(const void* dy, int64_t lddy, int dtype, const uint8_t* q, 
     gfl_i4_workspace(dtype, dtype, M, N, K, group, nullptr, &need);
     if (need && (!ws || ws_bytes < need || reinterpret_cast<uintptr_t>(ws) % 16))
         return api_fail(GFL_EINVAL, "gfl_linear_i4_dx: workspace missing, too small or not 16-byte aligned");
+    if (overlap(Span(dy, M, N, lddy, 2), Span(dx, M, K, lddx, 2))) return api_fail(GFL_EINVAL, "gfl_linear_i4_dx: dx overlaps dy");
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     if (gfl::q4_dx_plan(M, N, K).direct)
     {
@@ -621,6 +657,8 @@ int gfl_adjust_logits(const void* logits, int64_t ld, int dtype, int B, int V, c
     if (ld < V || ldo < V || (history && ldh < L) || (n_bias && (ldb < n_bias || ldv < n_bias)) || (allowed && lda < (V + 31) / 32))
         return api_fail(GFL_EINVAL, "gfl_adjust_logits: row strides must be at least the width");
     if (logits == out && ld != ldo && B > 1) return api_fail(GFL_EINVAL, "gfl_adjust_logits: in place, with one row stride");
+    if (logits != out && overlap(Span(logits, B, V, ld, size_of(dtype)), Span(out, B, V, ldo, size_of(dtype))))
+        return api_fail(GFL_EINVAL, "gfl_adjust_logits: out overlaps the logits without being them");
     gfl::LogitsArgs a;
     a.logits = logits; a.ld = ld; a.out = out; a.ldo = ldo;
     a.dtype = dtype; a.B = B; a.V = V;

@@ -371,7 +371,7 @@ int gfl_route_experts_backward(const void* dw, int w_dtype, const void* logits, 
                                gfl_stream stream);
 
 /* Logits [B, V] (fp32, fp16 or bf16) as each request's settings change them before gfl_sample draws; out of the same type, which may
- * be logits itself. Per row, each array [B] (NULL: off for every row):
+ * be logits itself (an out that overlaps them otherwise is refused). Per row, each array [B] (NULL: off for every row):
  *   history     int32 [B, L], of which the first lengths[b] (NULL: L) count, the first prompt[b] (NULL: 0) of those being the prompt
  *   repetition  a logit of a token that occurs in the history, above 0 divided by it, else multiplied; not above 0: off
  *   frequency   subtracted once for each time the token occurs after the prompt
