@@ -69,7 +69,9 @@ __global__ __launch_bounds__(Q4_T) void quant_i4_kernel(const E* w, int64_t ld, 
         hi = fmaxf(hi, __shfl_xor(hi, o));
         bad |= (uint32_t)__shfl_xor((int)bad, o);
     }
-    const float wide = zero ? (hi - lo) / 15.0f : fmaxf(-lo, hi) / 7.0f;
+    // (a range past the largest number is halved first, which is exact there)
+    const float half = fmaxf(-lo, hi) > 0x1p126f ? 0.5f : 1.0f;
+    const float wide = zero ? (hi * half - lo * half) / (15.0f * half) : fmaxf(-lo, hi) / 7.0f;
     const E se = bad ? static_cast<E>(NAN) : static_cast<E>(wide);
     const float s = static_cast<float>(se);
     const bool some = s > 0.0f && !bad;
