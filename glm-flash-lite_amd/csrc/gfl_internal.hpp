@@ -302,7 +302,7 @@ struct LogitsArgs
     int n_bias = 0;
     const int32_t* allowed = nullptr;   // [B][(V + 31) / 32] bits
     int64_t lda = 0;
-    int slice = 0, slices = 0, by_xcd = 0;   // of the launch
+    int slice = 0, slices = 0, by_xcd = 0, lazy = 0;   // of the launch
 };
 void launch_logits(const LogitsArgs& a, hipStream_t st);
 

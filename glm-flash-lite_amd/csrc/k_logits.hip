@@ -102,7 +102,7 @@ __global__ __launch_bounds__(LG_T, 4) void logits_kernel(LogitsArgs a)
     E* out = static_cast<E*>(a.out) + b * a.ldo + v0;
     const int32_t* allowed = a.allowed ? a.allowed + b * a.lda : nullptr;
     // The mask goes to LDS with the first loads. Read a word a thread beside the logits, it costs 256 rows of 131,072 98 us instead of 87.
-    const bool lazy = a.out == a.logits && !allowed;   // only what the lists name is read and written
+    const bool lazy = a.lazy;   // only what the lists name is read and written
 
     constexpr int U = 4, NB = 2;   // loads of 4 ids, of 4 logits under way
     const int32_t* h = a.L ? a.history + b * a.ldh : nullptr;
@@ -297,6 +297,11 @@ static void logits_go(LogitsArgs a, hipStream_t st)
     // A row's slices on one XCD read its history once from memory: us with and without, 256 rows of 30,000 81 and 84, 128 52 and 57, 64 26.5 and
     // 27.1; 16 rows, of which an XCD then has two, 18.1 and 17.8.
     a.by_xcd = a.B >= 64;
+    // In place without a mask, short lists leave most logits unread; what longer ones name lies in most lines, and is slower one by one than
+    // the whole row in order. us, lists alone and the whole row, 256 rows of 131,072 fp32 with 100, 2,000, 4,000, 8,000 and 30,000 ids 30 and
+    // 69, 52 and 71, 57 and 72, 76 and 73, 95 and 81; bf16 with 100, 500, 2,000, 30,000 28 and 34, 39 and 38, 44 and 41, 63 and 58; 24 rows
+    // of 100,003 fp32 with 100 and 4,000 9.0 and 10.8, 10.9 and 11.8.
+    a.lazy = a.out == a.logits && !a.allowed && ((int64_t)a.L + a.n_bias) * 128 <= (int64_t)a.V * (int)sizeof(E);
 
     const unsigned grid = (unsigned)(a.by_xcd ? (a.B + 7) / 8 * 8 : a.B) * a.slices;
     const size_t lds = (a.L ? a.slice / LgWord<HALF>::PER : 0) * 4 + (a.n_bias ? a.slice / 4 + LG_T / 16 + a.n_bias * 8 : 0) + (a.allowed ? a.slice / 8 : 0);
