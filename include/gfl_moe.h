@@ -351,7 +351,7 @@ int gfl_i4_workspace(int dtype, int out_dtype, int M, int N, int K, int group, s
  *   sel       the topk largest keys, in descending order
  *   w         scale * s, with renorm divided by the sum of the picks' s (a softmax's: only ratios of the picks; 0 where
  *             nothing is picked or fp64 sigmoids are all 0); fp16, bf16 or fp32
- * Scores, keys and sums are fp64; equal keys go to the lower index. Without a bias experts are compared by their logits, which differ
+ * Scores, keys and sums are fp64 (the sum over a softmax's row that its weights are divided by, within 2^-35); equal keys go to the lower index. Without a bias experts are compared by their logits, which differ
  * where fp64 scores no longer do (with groups, beside +inf in a softmax, the others are equal); groups go by the keys. Experts whose logit is -inf or NaN, or whose bias is, are never picked: where fewer than topk are left, the rest
  * of sel is -1 with weight 0, which the expert calls skip. In a softmax with logits of +inf those share the row.
  * E <= 1024, topk <= min(64, E / groups * top_groups), groups <= 64 dividing E. */

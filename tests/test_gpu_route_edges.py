@@ -149,3 +149,17 @@ def test_renormalised_softmax_of_picks_far_below_the_largest(gpu, M):
     err = torch.zeros_like(want)
     err[:, 24:30] = (2.0 ** -48 * p * (d.abs() + (p * d.abs()).sum(1, keepdim=True))).flip(1)
     S.same(dx, want, err + 2.0 ** -24 * (want.abs() + err) + 2.0 ** -150, "dlogits")
+
+
+@pytest.mark.parametrize("dt", [F32, BF16])
+@pytest.mark.parametrize("M,E,topk", [(1, 288, 8), (65, 128, 8), (3, 1024, 64), (6200, 64, 6), (12300, 128, 8)])
+def test_softmax_weights_of_the_whole_row_in_fp32(gpu, M, E, topk, dt):
+    """Not renormalised: a row's sum is of exponentials within 2^-35, the weight's own rounded once."""
+    import _native
+    x = (torch.randn((M, E), generator=_gen(E)) * 3).to(dt)
+    sel, w = _native.route_experts(x.cuda(), topk, score="softmax", renorm=False, scale=2.5, dtype=F32)
+    v = x.double()
+    want = _first(v, topk)
+    assert torch.equal(sel.cpu(), want)
+    p = 2.5 * torch.softmax(v, 1).gather(1, want)
+    S.same(w, p, (2.0 ** -24 + 2.0 ** -34) * p + 2.0 ** -150, "w")
