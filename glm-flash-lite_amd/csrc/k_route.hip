@@ -581,7 +581,8 @@ __global__ __launch_bounds__(RT_T) void route_backward_kernel(RouteArgs a, const
         norm = 0.0;
 #pragma unroll
         for (int i = 0; i < NI; ++i) norm += p[i] = rt_soft_near(x[i], top);
-        norm = 1.0 / rt_sum<L>(norm);
+        norm = rt_sum<L>(norm);
+        norm = norm > 0.0 ? 1.0 / norm : 0.0;   // (a row of NaN has no experts)
     }
     double s[64 / L], total = 0.0, dot = 0.0;
 #pragma unroll

@@ -163,3 +163,21 @@ def test_softmax_weights_of_the_whole_row_in_fp32(gpu, M, E, topk, dt):
     assert torch.equal(sel.cpu(), want)
     p = 2.5 * torch.softmax(v, 1).gather(1, want)
     S.same(w, p, (2.0 ** -24 + 2.0 ** -34) * p + 2.0 ** -150, "w")
+
+
+@pytest.mark.parametrize("E", [64, 100, 128, 1024])
+@pytest.mark.parametrize("M", [3, 8200])
+def test_rows_without_experts_have_no_gradient(gpu, M, E):
+    """All logits NaN, or -inf, or some of each: nothing is picked, and dx is 0."""
+    import _native
+    x = torch.randn((M, E), generator=_gen(E))
+    x[::3], x[1::3] = NAN, -INF
+    x[1::6, ::2] = NAN
+    dw = torch.randn((M, 4), generator=_gen(1)).cuda()
+    for score in ("sigmoid", "softmax"):
+        for renorm in (True, False):
+            sel, w = _native.route_experts(x.cuda(), 4, score=score, renorm=renorm)
+            dx = _native.route_experts_backward(dw, x.cuda(), sel, score=score, renorm=renorm)
+            for i in (0, 1):
+                assert bool((sel[i::3] == -1).all()) and bool((w[i::3] == 0).all()) and bool((dx[i::3] == 0).all())
+            assert bool((sel[2::3] >= 0).all()) and bool(torch.isfinite(dx).all())
