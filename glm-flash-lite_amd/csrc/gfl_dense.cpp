@@ -413,7 +413,7 @@ static int i4_check(int64_t M, int N, int K, int group)
 {
     if (M < 0 || M >= GFL_MAX_ROWS || N < 1 || N >= GFL_MAX_LD || K < 1 || K >= GFL_MAX_LD)
         return api_fail(GFL_EINVAL, "gfl_i4: need 0 <= M < GFL_MAX_ROWS (M >= 0) and 1 <= N, K < GFL_MAX_LD");
-    if (((int64_t)K + 127) / 128 * 128 * N > (int64_t)1 << 32)   // a launch of 64 threads a block of 128 has fewer than 2^32
+    if (((int64_t)K + 127) / 128 * 128 * N > (int64_t)1 << 32)   // 32-bit byte offsets in the products: 2^31 bytes of values, 2^28 of scales
         return api_fail(GFL_EINVAL, "gfl_i4: N * K (K up to a multiple of 128) must be at most 2^32");
     if (group != 32 && group != 64 && group != 128) return api_fail(GFL_EINVAL, "gfl_i4: group must be 32, 64 or 128");
     return GFL_OK;
@@ -639,6 +639,8 @@ int gfl_route_experts_backward(const void* dw, int w_dtype, const void* logits, 
 }
 
 // ---- logits before the draw ----
+
+static_assert(gfl::MAX_BIASES == GFL_MAX_BIASES && GFL_MAX_HISTORY < 1 << 30);   // (a history's count has 31 bits)
 
 int gfl_adjust_logits(const void* logits, int64_t ld, int dtype, int B, int V, const int32_t* history, int64_t ldh, int L,
                       const int32_t* lengths, const int32_t* prompt, const float* repetition, const float* frequency,

@@ -279,7 +279,7 @@ int launch_route_experts(RouteArgs& a, hipStream_t st);
 void launch_route_backward(RouteArgs& a, const void* dw, const int64_t* sel, void* dx, int64_t ldx, hipStream_t st);
 
 // logits before the draw (k_logits.hip)
-constexpr int MAX_HISTORY = (1 << 20) - 1, MAX_BIASES = 2047;
+constexpr int MAX_BIASES = 2047;   // a thread's share of them is a register each
 struct LogitsArgs
 {
     const void* logits = nullptr;

@@ -94,8 +94,7 @@ __global__ __launch_bounds__(512, TT >= 2 ? 2 : 4) void q4_dx_kernel(Q4Args a)
             const uint16_t bits = (uint16_t)(o.s[i / 2] >> (i % 2 * 16));
             sc[i] = a.scale_bf ? q_val<true>(bits) : q_val<false>(bits);
             off[i] = (ZERO ? -(float)(o.z[i / 4] >> (i % 4 * 8) & 255) : -8.0f) * sc[i];
-            // (opaque: a byte is then one conversion, and not cut out first)
-            asm volatile("" : "+v"(half[0][i]), "+v"(half[1][i]), "+v"(off[i]));
+            asm volatile("" : "+v"(off[i]));   // (and z s is kept for the row)
         }
         if (s * 32 + 32 > a.N)
         {

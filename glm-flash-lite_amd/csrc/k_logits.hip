@@ -220,7 +220,7 @@ __global__ __launch_bounds__(LG_T, 4) void logits_kernel(LogitsArgs a)
     }
     if (penal || a.n_bias || allowed) __syncthreads();
 
-    auto change = [&](int i, float (&v)[4]) {   // tokens i .. i + 3 of the slice; true: something changed
+    auto change = [&](int i, float (&v)[4]) {   // tokens i .. i + 3 of the slice
         uint32_t w[4] = {};
         const bool any = penal && W::four(word, i, w);
         if (any)
