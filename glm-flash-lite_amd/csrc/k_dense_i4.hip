@@ -48,7 +48,7 @@ __device__ __forceinline__ gm_i4 q4_ones(GmF16) { return gm_i4{ 0x3C003C00, 0x3C
 //
 // Loads return in order, and what is loaded first is needed first: the tokens, then scales, then weights.
 //
-// Bound by the weights' bytes from 65536 channels on (9 tokens of 4096 31 us, 4.5 TB/s); one token of 5120 -> 5120 takes 6.4 us, 2.2 of
+// Bound by the weights' bytes from 65536 channels on (9 tokens of 4096 29 us, 4.8 TB/s); one token of 5120 -> 5120 takes 6.0 us, 2.2 of
 // them a launch's, 2.8 its bytes.
 template <typename T, int GB, bool ZERO, int U, int KS, int NW>
 __global__ __launch_bounds__(NW * 64) void q4_few_kernel(Q4Args a)
@@ -222,9 +222,13 @@ static void q4_few_u(const Q4Args& a, hipStream_t st)
     else q4_few_go<T, GB, ZERO, 1, KS>(a, st);
 }
 
-// As many waves to a tile as leave the card's 2048 or more something each: us by 1, 2, 4 and 8 waves, 4096 -> 65536 (4096 tiles) 9 tokens
-// 34, 39, 39, 40; 4096 -> 10240 (640) 16 tokens 15.5, 11.4, 11.6, 11.2; 5120 -> 5120 (320) 1 token 14.5, 9.2, 6.4, 7.4; 4096 -> 2048 (128) 2
-// tokens 11.8, 7.8, 5.4, 4.0.
+// Waves to a tile: the fewer, the longer a wave's own chain; the more, the more workgroups beyond a CU's. us by 1, 2, 4 and 8 waves, 1 and 8
+// tokens of 5120:
+//    256 tiles  14.3 9.0 6.3 5.0, 16.0 10.6 7.7 6.6     319  14.5 9.1 6.5 6.7, 16.1 10.7 7.9 8.8     320  14.5 9.2 6.4 6.8, 16.1 10.7 7.8 8.9
+//    512        14.5 9.3 6.7 7.2, 16.1 10.8 8.3 9.3     639  14.6 9.3 9.0 8.8, 16.4 11.2 11.6 11.3   640  14.6 9.3 9.1 8.7, 16.3 11.1 11.7 11.5
+//   1024        14.6 9.6 9.3 10.3, 16.6 11.6 11.8 14.0  1280  14.7 14.2 12.5 12.3, 16.8 18.1 15.1 16.2  2048  16.9 15.7 16.5 19.6, 18.9 19.3 19.8 25.6
+// and 4096 -> 65536 (4096 tiles) 9 tokens 34, 39, 39, 40. Of 2048 inputs the order is the same: 256 tiles 7.0 5.0 3.9 3.4, 1280 7.6 7.6 7.2
+// 6.9. Between the edges the best is missed by up to 10% from 257 to 319 tiles, and by 15% from 1280 to some 2000.
 template <typename T, int GB, bool ZERO>
 static void q4_few(const Q4Args& a, hipStream_t st)
 {

@@ -4,8 +4,8 @@
 // atomics (the same in any order), then the slice is read, changed and written once.
 //
 // Large batches are bound by the logits' way through memory and by what cannot overlap it, a slice's search of its row's history: 256
-// rows of 131,072 with 30,000 tokens each 80 us, 52 without lists (a copy 50), 57 without histories (bytes 60 us). Small ones by
-// latency: a row of 131,072 4.8 us, 24 of 100,003 11.6 (5 without lists: a launch, two trips to memory).
+// rows of 131,072 with 30,000 tokens each 84 us (in place without a mask 78), 52 without lists (a copy 50), 57 without histories (bytes
+// 60 us). Small ones by latency: a row of 131,072 5.0 us, 24 of 100,003 10.7 (5 without lists: a launch, two trips to memory).
 #include "gfl_internal.hpp"
 #include "gfl_open.hpp"
 

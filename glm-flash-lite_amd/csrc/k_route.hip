@@ -11,9 +11,11 @@
 // own, so that among equal keys the lowest lane's lowest place is the lowest index. A lane sorts its keys once; a pick is then the
 // largest of the lanes' first ones, found by DPP, and a step down in one lane.
 //
-// Bound by the picks' chains of dependent instructions, not by bytes: 8192 tokens of 256 experts in 8 groups 13.3 us (bytes 1.9; some 870
-// instructions a wave, 6.5 us of issue), of which a choice in fp64 throughout made 15.9; 16384 tokens of 128 7.6 and their gradient
-// 8.2 (bytes 2.2), 17.7 together with a row's weights by the library's exponentials; one token 4.8, 2.2 of them a launch's.
+// Bound by the picks' chains of dependent instructions, not by bytes: 8192 tokens of 256 experts in 8 groups 11.9 us (bytes 1.9; some 920
+// instructions a wave, 7.0 us of issue; 15.9 with a choice in fp64 throughout); 16384 tokens of 128, softmax without renormalisation in
+// bf16, and their gradient 16.7 (7.6 and 9.3 by the tracer, bytes 2.2, issue 5.6 and 6.5); one token 5.0, 2.2 of them a launch's. What
+// falls back to fp64 costs more: 8192 tokens of 256 experts, softmax 7.2, with a bias 16.5, with 8 groups 14.6, with both 18.8; sigmoid with
+// 8 groups in fp32, fp16 and bf16, whose groups' worths tie more often, 10.0, 11.4 and 13.0.
 #include "gfl_device.hpp"
 #include "gfl_internal.hpp"
 
@@ -665,9 +667,12 @@ static void route_back(const RouteArgs& a, const void* dw, const int64_t* sel, v
     });
 }
 
-// Lanes a token. 16 or 32 do the steps of a pick for 4 or 2 tokens at once, 64 hold fewer experts each and are done sooner: us by 64, 32
-// and 16 lanes, sigmoid with a bias, 288 experts, 4096 tokens 8.0, 9.4, 9.3, 8192 12.9, 12.7, 12.7; 256 in 8 groups, 8192 tokens 14.5,
-// 12.2, 13.1; softmax of 128 experts, 16384 tokens 13.9, 9.4, 7.6.
+// Lanes a token. 16 or 32 do the steps of a pick for 4 or 2 tokens at once, 64 hold fewer experts each and are done sooner. us by 64, 32
+// and 16 lanes (16 are 32 where a lane would hold more than 16 experts), 1024, 2048, 4096, 6144, 8192, 12288 and 16384 tokens:
+//   288 experts, sigmoid and bias  6.1 7.7 -, 6.8 8.1 -, 8.5 9.9 -, 11.1 11.4 -, 13.3 12.6 -, 17.6 16.8 -, 22.4 20.3 -
+//   256 in 8 groups, the same      7.6 8.6 10.4, 7.4 7.9 9.7, 10.4 11.1 11.6, 13.0 12.6 14.2, 14.8 13.2 13.7, 19.2 15.9 15.7, 24.8 20.0 19.0
+//   128 experts, softmax           4.6 4.5 4.8, 4.9 4.6 4.8, 6.1 4.8 5.1, 7.4 5.2 5.0, 8.9 5.8 5.3, 11.7 7.3 5.7, 14.6 8.7 6.5
+// The edges are those of the larger routers; 128 experts and fewer would take 32 lanes from 1024 tokens on and 16 from 6144 (1.3 us of 6).
 template <typename X>
 static int route_of(RouteArgs& a, hipStream_t st)
 {
@@ -687,8 +692,10 @@ int launch_route_experts(RouteArgs& a, hipStream_t st)
     return a.dtype == 2 ? route_of<float>(a, st) : a.dtype == 1 ? route_of<__bf16>(a, st) : route_of<_Float16>(a, st);
 }
 
-// 16 lanes a token where each then has a power of two of experts, which it stores as one vector: us by 64 and 16, softmax, 16384 tokens of
-// 128 experts 14.0 and 8.2, sigmoid, 8192 of 256 7.8 and 8.1.
+// 16 lanes a token where each then has a power of two of experts, which it stores as one vector. us by 64 and 16 lanes, sigmoid renormalised in
+// fp32 and softmax not renormalised in bf16: 128 experts 4096 tokens 5.0 4.5, 5.9 5.4, 8192 7.6 5.4, 8.9 6.2, 16384 13.4 8.3, 15.5 8.9;
+// 256 experts 4096 tokens 5.9 7.3, 7.0 7.5, 8192 9.3 9.1, 11.1 9.2, 16384 16.5 14.2, 20.3 15.0; 160 (10 a lane) 8192 8.9 9.5, 11.3 10.2, 16384
+// 16.0 14.8, 20.3 15.3. 288 and 384 experts, more than 16 a lane, 8192 tokens by 64 lanes 10.5 and 13.1, 13.0 and 16.8.
 template <typename X>
 static void route_back_of(RouteArgs& a, const void* dw, const int64_t* sel, void* dx, int64_t ldx, hipStream_t st)
 {

@@ -328,14 +328,17 @@ int gfl_pack_i4(const uint8_t* v, int64_t ldv, int N, int K, uint8_t* q, gfl_str
 
 /* out[m][n] = sum_k x[m][k] * w[n][k] for x [M, K] fp16 or bf16 (dtype); out fp16, bf16 or fp32. Sums are fp32. Up to 64 tokens,
  * in larger calls as long as that is quicker (some hundred tokens), and wherever out is not of x's type, the weights enter
- * exactly, as whole numbers; else they are rounded to x's type. An infinity in a token's x makes its outputs not finite (NaN in the
- * exact form). q 16-byte aligned. */
+ * exactly, as whole numbers; else they are rounded to x's type (a result of x's type from exact weights, whatever the number of
+ * tokens: ask for fp32 and round it). In the exact form a group is s (sum x (16 + v) - (16 + z) sum x): an fp32 result is off by some
+ * 2^-24 of s (32 + z) sum |x|, which counts where inputs of one sign cancel (K = 4096, inputs of mean 1: 2e-6 of the result in bf16,
+ * 5e-6 in fp16, of mean 0 2e-7 and 5e-7), and tokens of 2^112 and more (bf16) overflow. An infinity in a token's x makes its outputs not finite (NaN in the exact
+ * form). q 16-byte aligned. */
 int gfl_linear_i4(const void* x, int64_t ldx, int dtype, const uint8_t* q, const void* scale, int scale_dtype, const uint8_t* zero,
                   int M, int N, int K, int group, void* out, int64_t ldo, int out_dtype, void* ws, size_t ws_bytes,
                   gfl_stream stream);
 
 /* Its gradient with respect to x (the weight is frozen): dx[m][k] = sum_n dy[m][n] * w[n][k], both of dtype, the weights rounded to
- * it. */
+ * it (scales below 2^119). */
 int gfl_linear_i4_dx(const void* dy, int64_t lddy, int dtype, const uint8_t* q, const void* scale, int scale_dtype,
                      const uint8_t* zero, int M, int N, int K, int group, void* dx, int64_t lddx, void* ws, size_t ws_bytes,
                      gfl_stream stream);
@@ -351,9 +354,11 @@ int gfl_i4_workspace(int dtype, int out_dtype, int M, int N, int K, int group, s
  *   sel       the topk largest keys, in descending order
  *   w         scale * s, with renorm divided by the sum of the picks' s (a softmax's: only ratios of the picks; 0 where
  *             nothing is picked or fp64 sigmoids are all 0); fp16, bf16 or fp32
- * Scores, keys and sums are fp64 (the sum over a softmax's row that its weights are divided by, within 2^-35); equal keys go to the lower index. Without a bias experts are compared by their logits, which differ
- * where fp64 scores no longer do (with groups, beside +inf in a softmax, the others are equal); groups go by the keys. Experts whose logit is -inf or NaN, or whose bias is, are never picked: where fewer than topk are left, the rest
- * of sel is -1 with weight 0, which the expert calls skip. In a softmax with logits of +inf those share the row.
+ * Scores, keys and sums are fp64 (a softmax row's sum, by which weights are divided without renorm, within 2^-35); equal keys go to
+ * the lower index. Without a bias experts are compared by their logits, which differ where fp64 scores no longer do (with groups,
+ * beside +inf in a softmax, the others are equal); groups go by the keys. Experts whose logit is -inf or NaN, or whose bias is,
+ * are never picked: where fewer than topk are left, the rest of sel is -1 with weight 0, which the expert calls skip. In a
+ * softmax with logits of +inf those share the row.
  * E <= 1024, topk <= min(64, E / groups * top_groups), groups <= 64 dividing E. */
 enum
 {
@@ -365,7 +370,8 @@ int gfl_route_experts(const void* logits, int64_t ld, int dtype, const float* bi
                       gfl_stream stream);
 
 /* Gradient of the logits (dlogits [M, E] of dtype) for a gradient dw [M, topk] of the weights (of w_dtype), sel as the forward call
- * wrote it (ids outside [0, E) are skipped). The choice itself and the bias have none. */
+ * wrote it (ids outside [0, E) are skipped, and so is their dw). The choice itself and the bias have none. Formed in fp64 (a
+ * softmax row's exponentials, without renorm, within 2^-35) and rounded to fp32 and dtype at the end. */
 int gfl_route_experts_backward(const void* dw, int w_dtype, const void* logits, int64_t ld, int dtype, const int64_t* sel, int M,
                                int E, int topk, int score, int renorm, float scale, void* dlogits, int64_t ldd,
                                gfl_stream stream);
