@@ -5,7 +5,7 @@
 // MFMAs' fragments for 8 neighbouring columns: 16 lanes take a block of 128 columns, and no weight goes through LDS or memory. A weight
 // costs a conversion, a multiply-add (z s, kept for a row, is finite up to scales of 2^119) and half a rounding of two; up to 64 tokens share
 // it. That is what bounds 64 tokens (1.6 us a step, of which 0.8 are these and 0.4 the MFMAs), and few tokens the weight's way from memory:
-// 11008 -> 4096 1 token 13.6 us, 24 16.7, 64 22.6; through weights of 16 bits in memory 45, 45 and 47.
+// 11008 -> 4096 1 token 13.0 us, 24 16.0, 64 21.3; through weights of 16 bits in memory 45, 45 and 47.
 #include "gfl_device.hpp"
 #include "gfl_gemm.hpp"
 #include "gfl_gemm_plan.hpp"

@@ -11,9 +11,9 @@
 // own, so that among equal keys the lowest lane's lowest place is the lowest index. A lane sorts its keys once; a pick is then the
 // largest of the lanes' first ones, found by DPP, and a step down in one lane.
 //
-// Bound by the picks' chains of dependent instructions, not by bytes: 8192 tokens of 256 experts in 8 groups 11.9 us (bytes 1.9; some 920
+// Bound by the picks' chains of dependent instructions, not by bytes: 8192 tokens of 256 experts in 8 groups 11.9 to 14.5 us (bytes 1.9; some 920
 // instructions a wave, 7.0 us of issue; 15.9 with a choice in fp64 throughout); 16384 tokens of 128, softmax without renormalisation in
-// bf16, and their gradient 16.7 (7.6 and 9.3 by the tracer, bytes 2.2, issue 5.6 and 6.5); one token 5.0, 2.2 of them a launch's. What
+// bf16, and their gradient 16.6 (7.6 and 9.3 by the tracer, bytes 2.2, issue 5.6 and 6.5); one token 5.0, 2.2 of them a launch's. What
 // falls back to fp64 costs more: 8192 tokens of 256 experts, softmax 7.2, with a bias 16.5, with 8 groups 14.6, with both 18.8; sigmoid with
 // 8 groups in fp32, fp16 and bf16, whose groups' worths tie more often, 10.0, 11.4 and 13.0.
 #include "gfl_device.hpp"
@@ -615,10 +615,10 @@ __global__ __launch_bounds__(RT_T) void route_backward_kernel(RouteArgs a, const
     double v[NI] = {};
     for (int j = 0; j < a.topk; ++j)
     {
-        const int e = picks[tok][j] - e0;
+        const int at = picks[tok][j] - e0, e = at < n ? at : -1;
         const double d = grads[tok][j];
 #pragma unroll
-        for (int i = 0; i < NI; ++i) v[i] += e == i && i < n ? d : 0.0;
+        for (int i = 0; i < NI; ++i) v[i] += e == i ? d : 0.0;
     }
     X o[NI];
 #pragma unroll
