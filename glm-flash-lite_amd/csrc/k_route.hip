@@ -13,7 +13,7 @@
 //
 // Bound by the picks' chains of dependent instructions, not by bytes: 8192 tokens of 256 experts in 8 groups 11.9 to 14.5 us (bytes 1.9; some 920
 // instructions a wave, 7.0 us of issue; 15.9 with a choice in fp64 throughout); 16384 tokens of 128, softmax without renormalisation in
-// bf16, and their gradient 16.6 (7.6 and 9.3 by the tracer, bytes 2.2, issue 5.6 and 6.5); one token 5.0, 2.2 of them a launch's. What
+// bf16, and their gradient 16.6 (7.6 and 9.2 by the tracer, bytes 2.2, issue 5.6 and 6.5); one token 5.0, 2.2 of them a launch's. What
 // falls back to fp64 costs more: 8192 tokens of 256 experts, softmax 7.2, with a bias 16.5, with 8 groups 14.6, with both 18.8; sigmoid with
 // 8 groups in fp32, fp16 and bf16, whose groups' worths tie more often, 10.0, 11.4 and 13.0.
 #include "gfl_device.hpp"
